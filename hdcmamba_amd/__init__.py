@@ -13,6 +13,8 @@ from .model import (
     set_fused_step_front,
 )
 from .lm import DecodeGraph, ForwardGraph, HdcMambaLM
+from .quant4 import Weight4Bit, linear_4bit
+from .sampling import append_tokens, fill_token_history, new_token_history, process_logits, select_tokens
 
 __all__ = [
     "HdcMamba9v3Block",
@@ -26,4 +28,11 @@ __all__ = [
     "set_differentiable_mixer",
     "set_fused_out_proj",
     "set_fused_step_front",
+    "Weight4Bit",
+    "linear_4bit",
+    "process_logits",
+    "select_tokens",
+    "new_token_history",
+    "fill_token_history",
+    "append_tokens",
 ]

@@ -20,6 +20,15 @@ ABI_VERSION = 2
 HDCM_F32, HDCM_BF16 = 0, 1
 _DTYPES = {torch.float32: HDCM_F32, torch.bfloat16: HDCM_BF16}
 
+
+class LogitsControls(ctypes.Structure):
+    """hdcm_logits_controls of include/hdcm.h."""
+    _fields_ = [("history", c_void_p), ("history_row_stride", c_int64), ("repetition", c_void_p), ("frequency", c_void_p),
+                ("presence", c_void_p), ("repetition_all", c_float), ("frequency_all", c_float), ("presence_all", c_float),
+                ("bias", c_void_p), ("bias_row_stride", c_int64), ("bias_dtype", c_int), ("mask", c_void_p),
+                ("mask_row_stride", c_int64)]
+
+
 # name -> (restype, argtypes); mirrors include/hdcm.h
 _PROTOS = {
     "hdcm_abi_version": (c_int, []),
@@ -113,6 +122,23 @@ _PROTOS = {
                                        c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int64, c_int64, c_int64,
                                        c_float, c_int, c_void_p]),
+    "hdcm_w4_packed_bytes": (c_size_t, [c_int64, c_int64]),
+    "hdcm_w4_pack": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "hdcm_w4_quantize": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                 c_void_p]),
+    "hdcm_w4_dequant": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                c_void_p]),
+    "hdcm_w4_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                                   c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "hdcm_logits_process": (c_int, [c_void_p, c_int64, ctypes.POINTER(LogitsControls), c_void_p, c_int64, c_int64, c_int64,
+                                    c_int, c_void_p]),
+    "hdcm_token_select_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "hdcm_token_select": (c_int, [c_void_p, c_int64, ctypes.POINTER(LogitsControls), c_void_p, c_float, c_void_p, c_int64,
+                                  c_void_p, c_void_p, c_void_p, c_size_t, c_int64, c_int64, c_int, c_void_p]),
+    "hdcm_token_history_fill": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_int64, c_int64, c_void_p]),
+    "hdcm_token_history_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                          c_void_p]),
 }
 
 _lib = None

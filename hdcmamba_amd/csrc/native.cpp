@@ -4,10 +4,12 @@
 // library products.  A block forward is 7-9 launches; issued one by one through ctypes they cost
 // about 190 us of Python per block, more than the kernels take below ~8192 rows.  Nothing is kept
 // between calls: workspaces that outlive a call are passed in.
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 #include <optional>
 #include <tuple>
+#include <variant>
 #include <vector>
 
 #include "../../include/hdcm.h"
@@ -574,6 +576,296 @@ std::vector<OptTensor> block_backward(const Tensor& x, const Tensor& dy, const s
   return out;
 }
 
+// ------------------------------------------------------------------------ 4-bit products
+// The operators below are inference only: one that autograd would have to differentiate is refused.
+void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), op, " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+const Tensor& or_none(const OptTensor& t) {
+  static const Tensor none;
+  return t ? *t : none;
+}
+const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+void same_device(const Tensor& t, const Tensor& ref, const char* name) {
+  TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
+}
+
+// Whether the rows of a 2-D tensor are what the kernels address: unit inner stride, a row at least its width apart.
+bool plain_rows(const Tensor& t) {
+  return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+// [..., W] as such rows, copied where the layout is another
+Tensor rows(const Tensor& t) {
+  const Tensor r = t.dim() == 2 ? t : t.reshape({t.size(-1) ? t.numel() / t.size(-1) : 0, t.size(-1)});
+  return plain_rows(r) ? r : r.contiguous();
+}
+
+// Whether two row layouts share an element (or may: rows of different pitch whose ranges meet).
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || a.numel() == 0 || b.numel() == 0) return false;
+  const auto lo = [](const Tensor& t) { return (uintptr_t)t.const_data_ptr(); };
+  const auto span = [](const Tensor& t) { return (uintptr_t)(((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size()); };
+  if (lo(a) + span(a) <= lo(b) || lo(b) + span(b) <= lo(a)) return false;
+  const int64_t e = a.element_size(), pitch = a.stride(0) * e;
+  if (a.size(0) > 1 && b.size(0) > 1 && pitch == b.stride(0) * (int64_t)b.element_size()) {  // column blocks of one buffer
+    const int64_t d = (((int64_t)lo(b) - (int64_t)lo(a)) % pitch + pitch) % pitch;
+    return d < a.size(1) * e || d + b.size(1) * (int64_t)b.element_size() > pitch;
+  }
+  return true;
+}
+bool same_place(const Tensor& a, const Tensor& b) {
+  return a.const_data_ptr() == b.const_data_ptr() && (a.size(0) <= 1 || a.stride(0) == b.stride(0));
+}
+
+using WeightArgs = std::tuple<Tensor, Tensor, OptTensor, int64_t, int64_t, int64_t>;  // packed, scales, zeros, N, K, group
+struct Weight4 {
+  Tensor packed, scales, zeros;
+  int64_t N, K, group;
+};
+Weight4 weight4_of(const WeightArgs& a) {
+  Weight4 w{std::get<0>(a), std::get<1>(a), or_none(std::get<2>(a)), std::get<3>(a), std::get<4>(a), std::get<5>(a)};
+  TORCH_CHECK(w.N > 0 && w.K > 0 && (w.group == 32 || w.group == 64 || w.group == 128), "a 4-bit weight [", w.N, ", ", w.K,
+              "] in groups of ", w.group);
+  const int64_t per = (w.K + 127) / 128 * 128 / w.group * ((w.N + 15) / 16 * 16);
+  on_gpu(w.packed);
+  same_device(w.scales, w.packed, "scales");
+  TORCH_CHECK(w.packed.scalar_type() == at::kByte && w.packed.is_contiguous() &&
+                  (size_t)w.packed.numel() == hdcm_w4_packed_bytes(w.N, w.K) && w.scales.is_contiguous() &&
+                  w.scales.numel() == per,
+              "the packed weight's buffers do not hold [", w.N, ", ", w.K, "] in groups of ", w.group);
+  if (w.zeros.defined()) {
+    same_device(w.zeros, w.packed, "zeros");
+    TORCH_CHECK(w.zeros.scalar_type() == at::kByte && w.zeros.is_contiguous() && w.zeros.numel() == per,
+                "zeros must hold one byte per scale");
+  }
+  return w;
+}
+
+Tensor linear_4bit(const Tensor& x, const WeightArgs& weight, const OptTensor& bias_, const OptTensor& residual_,
+                   const OptTensor& out_, int64_t stream) {
+  const Tensor &bias = or_none(bias_), &residual = or_none(residual_), &given = or_none(out_);
+  on_gpu(x);
+  no_gradient("linear_4bit", {&x, &bias, &residual, &given});
+  Entry entry;
+  const c10::DeviceGuard guard(x.device());
+  const Weight4 w = weight4_of(weight);
+  const int dt = dtype_of(x);
+  same_device(w.packed, x, "the weight");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == w.K, "linear_4bit: x ", x.sizes(), " does not end in the weight's ", w.K, " columns");
+  auto shape = x.sizes().vec();
+  shape.back() = w.N;
+  const Tensor xr = rows(x);
+  Tensor out = given;
+  if (out.defined()) {
+    same_device(out, x, "out");
+    TORCH_CHECK(out.scalar_type() == x.scalar_type() && out.sizes() == shape, "linear_4bit: out must be ", shape, " of x's type");
+  } else {
+    out = at::empty(shape, x.options());
+  }
+  const Tensor o = out.dim() == 2 ? out : out.view({xr.size(0), w.N});  // a view, never a copy
+  TORCH_CHECK(plain_rows(o), "linear_4bit: out's rows must be contiguous and apart");
+  Tensor b, r;
+  if (bias.defined()) {
+    TORCH_CHECK(bias.dim() == 1 && bias.size(0) == w.N, "linear_4bit: bias must be [", w.N, "]");
+    b = same(bias, x, "bias");
+  }
+  if (residual.defined()) {
+    same_device(residual, x, "residual");
+    TORCH_CHECK(residual.scalar_type() == x.scalar_type() && residual.sizes() == shape, "linear_4bit: residual must be ", shape,
+                " of x's type");
+    r = rows(residual);
+  }
+  if (given.defined())
+    TORCH_CHECK(!overlap(o, xr) && (!r.defined() || same_place(o, r) || !overlap(o, r)),
+                "linear_4bit: out may be the residual itself but share no other memory with x or the residual");
+  check("hdcm_w4_linear_fwd",
+        hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), w.packed.const_data_ptr(), w.scales.const_data_ptr(),
+                           dtype_of(w.scales), (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
+                           r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, w.K, dt,
+                           (void*)stream));
+  return out;
+}
+
+// ------------------------------------------------------------------------ logits and tokens
+using Penalty = std::optional<std::variant<double, Tensor>>;
+// The controls of B rows of V logits, and what has to stay alive for the call.
+struct Controls {
+  hdcm_logits_controls c{};
+  std::vector<Tensor> held;
+};
+const float* per_row(const Penalty& p, double dflt, int64_t B, const Tensor& ref, const char* name, float& all,
+                     std::vector<Tensor>& held) {
+  all = (float)dflt;
+  if (!p) return nullptr;
+  if (const double* v = std::get_if<double>(&*p)) {
+    all = (float)*v;
+    return nullptr;
+  }
+  const Tensor& t = std::get<Tensor>(*p);
+  same_device(t, ref, name);
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == B, name, " must be a number or a tensor of ", B, " values");
+  held.push_back(t.to(at::kFloat).contiguous());
+  return held.back().const_data_ptr<float>();
+}
+// [n], [1, n] or [B, n] as (pointer, row stride), 0 for a shared row
+std::pair<const void*, int64_t> shared_rows(const Tensor& t, int64_t B, int64_t n, const Tensor& ref, const char* name,
+                                            std::vector<Tensor>& held) {
+  same_device(t, ref, name);
+  TORCH_CHECK((t.dim() == 1 || (t.dim() == 2 && (t.size(0) == 1 || t.size(0) == B))) && t.size(-1) == n, name, " ", t.sizes(),
+              " must be [", n, "] or [", B, ", ", n, "]");
+  const bool shared = t.dim() == 1 || t.size(0) == 1 || t.stride(0) == 0;
+  Tensor r = t.dim() == 1 ? t.unsqueeze(0) : shared ? t.narrow(0, 0, std::min<int64_t>(t.size(0), 1)) : t;
+  if (!plain_rows(r)) r = r.contiguous();
+  held.push_back(r);
+  return {r.const_data_ptr(), shared ? 0 : r.stride(0)};
+}
+using ControlArgs = std::tuple<OptTensor, Penalty, Penalty, Penalty, OptTensor, OptTensor>;
+Controls controls_of(const ControlArgs& a, const Tensor& logits) {
+  const auto& [history, repetition, frequency, presence, bias, mask] = a;
+  const int64_t B = logits.size(0), V = logits.size(1);
+  Controls k;
+  hdcm_logits_controls& c = k.c;
+  c.repetition = per_row(repetition, 1.0, B, logits, "repetition", c.repetition_all, k.held);
+  c.frequency = per_row(frequency, 0.0, B, logits, "frequency", c.frequency_all, k.held);
+  c.presence = per_row(presence, 0.0, B, logits, "presence", c.presence_all, k.held);
+  TORCH_CHECK(c.repetition || c.repetition_all > 0.f, "repetition must be above 0");
+  TORCH_CHECK(history || !(repetition || frequency || presence), "penalties need the token history");
+  if (history) {
+    same_device(*history, logits, "history");
+    TORCH_CHECK(history->scalar_type() == at::kShort && history->dim() == 2 && history->size(0) == B && history->size(1) == V &&
+                    plain_rows(*history),
+                "history must be an int16 table [", B, ", ", V, "] with contiguous rows");
+    c.history = history->const_data_ptr<int16_t>();
+    c.history_row_stride = history->stride(0);
+  }
+  if (bias) {
+    std::tie(c.bias, c.bias_row_stride) = shared_rows(*bias, B, V, logits, "bias", k.held);
+    c.bias_dtype = dtype_of(*bias);
+  }
+  if (mask) {
+    TORCH_CHECK(mask->scalar_type() == at::kInt, "mask must be int32 words of 32 tokens");
+    const auto m = shared_rows(*mask, B, (V + 31) / 32, logits, "mask", k.held);
+    c.mask = (const uint32_t*)m.first, c.mask_row_stride = m.second;
+  }
+  return k;
+}
+void logits_shape(const Tensor& logits, const char* op) {
+  on_gpu(logits);
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, op, ": logits must be [sequences, vocabulary], got ", logits.sizes());
+}
+
+Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTensor& out_, int64_t stream) {
+  logits_shape(logits, "process_logits");
+  no_gradient("process_logits", {&logits, &or_none(std::get<4>(args)), &or_none(out_)});
+  Entry entry;
+  const c10::DeviceGuard guard(logits.device());
+  const int dt = dtype_of(logits);
+  const Controls k = controls_of(args, logits);
+  const Tensor l = rows(logits);
+  Tensor out;
+  if (out_) {
+    out = *out_;
+    same_device(out, logits, "out");
+    TORCH_CHECK(out.scalar_type() == logits.scalar_type() && out.sizes() == logits.sizes() && plain_rows(out),
+                "process_logits: out must match the logits, with contiguous rows");
+    TORCH_CHECK(same_place(out, l) || !overlap(out, l),
+                "process_logits: out may be the logits themselves but share no other memory with them");
+    for (const Tensor& t : k.held)
+      TORCH_CHECK(t.dim() != 2 || !overlap(out, t), "process_logits: out shares memory with the bias or the mask");
+  } else {
+    out = at::empty(logits.sizes(), logits.options());
+  }
+  check("hdcm_logits_process",
+        hdcm_logits_process(l.const_data_ptr(), l.stride(0), &k.c, out.mutable_data_ptr(), out.stride(0), l.size(0), l.size(1), dt,
+                            (void*)stream));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> select_tokens(const Tensor& logits, const ControlArgs& args, const Penalty& temperature,
+                                         const OptTensor& noise_, int64_t stream) {
+  logits_shape(logits, "select_tokens");
+  no_gradient("select_tokens", {&logits, &or_none(std::get<4>(args)), &or_none(noise_)});
+  Entry entry;
+  const c10::DeviceGuard guard(logits.device());
+  const int dt = dtype_of(logits);
+  const int64_t B = logits.size(0), V = logits.size(1);
+  Controls k = controls_of(args, logits);
+  const Tensor l = rows(logits);
+  float temp_all;
+  const float* temp = per_row(temperature, 1.0, B, logits, "temperature", temp_all, k.held);
+  Tensor noise;
+  if (noise_) {
+    same_device(*noise_, logits, "noise");
+    TORCH_CHECK(noise_->scalar_type() == at::kFloat && noise_->sizes() == logits.sizes(), "noise must be float32 ", logits.sizes());
+    noise = rows(*noise_);
+  }
+  Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong)), logprobs = fp32({B}, logits);
+  const size_t n = hdcm_token_select_workspace_bytes(B, V);
+  const Tensor ws = n ? bytes(n, logits) : Tensor();
+  check("hdcm_token_select",
+        hdcm_token_select(l.const_data_ptr(), l.stride(0), &k.c, temp, temp_all, (const float*)pointer(noise),
+                          noise.defined() ? noise.stride(0) : 0, tokens.mutable_data_ptr<int64_t>(),
+                          logprobs.mutable_data_ptr<float>(), n ? ws.mutable_data_ptr() : nullptr, n, B, V, dt, (void*)stream));
+  return {tokens, logprobs};
+}
+
+void table_shape(const Tensor& table, const char* op) {
+  on_gpu(table);
+  TORCH_CHECK(table.scalar_type() == at::kShort && table.dim() == 2 && plain_rows(table), op,
+              ": the table must be int16 [sequences, vocabulary] with contiguous rows");
+}
+// Token ids as int64 rows of the table's sequences, and how many of each count
+struct Ids {
+  Tensor ids, lengths;
+  const int64_t *p = nullptr, *n = nullptr;
+  int64_t stride = 0, width = 0;
+};
+Ids ids_of(const OptTensor& ids, const OptTensor& lengths, const Tensor& table, const char* name) {
+  Ids r;
+  TORCH_CHECK(ids || !lengths, name, "_lengths without ", name);
+  if (!ids) return r;
+  const auto whole = [](const Tensor& t) { return at::isIntegralType(t.scalar_type(), false); };
+  same_device(*ids, table, name);
+  TORCH_CHECK(whole(*ids) && ids->dim() == 2 && ids->size(0) == table.size(0), name, " ", ids->sizes(), " must be token ids [",
+              table.size(0), ", any]");
+  r.ids = rows(ids->to(at::kLong));
+  r.p = r.ids.const_data_ptr<int64_t>(), r.stride = r.ids.stride(0), r.width = r.ids.size(1);
+  if (lengths) {
+    same_device(*lengths, table, "lengths");
+    TORCH_CHECK(whole(*lengths) && lengths->dim() == 1 && lengths->size(0) == table.size(0), name, "_lengths must be [",
+                table.size(0), "] whole numbers");
+    r.lengths = lengths->to(at::kLong).contiguous();
+    r.n = r.lengths.const_data_ptr<int64_t>();
+  }
+  return r;
+}
+
+Tensor fill_token_history(Tensor table, const OptTensor& prompt, const OptTensor& prompt_lengths, const OptTensor& output,
+                          const OptTensor& output_lengths, int64_t stream) {
+  Entry entry;
+  table_shape(table, "fill_token_history");
+  const c10::DeviceGuard guard(table.device());
+  const Ids p = ids_of(prompt, prompt_lengths, table, "prompt"), o = ids_of(output, output_lengths, table, "output");
+  check("hdcm_token_history_fill",
+        hdcm_token_history_fill(table.mutable_data_ptr<int16_t>(), table.stride(0), p.p, p.stride, p.n, p.width, o.p, o.stride,
+                                o.n, o.width, table.size(0), table.size(1), (void*)stream));
+  return table;
+}
+
+Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& lengths, int64_t stream) {
+  Entry entry;
+  table_shape(table, "append_tokens");
+  const c10::DeviceGuard guard(table.device());
+  const Ids t = ids_of(tokens.dim() == 1 ? tokens.unsqueeze(1) : tokens, lengths, table, "tokens");
+  check("hdcm_token_history_append",
+        hdcm_token_history_append(table.mutable_data_ptr<int16_t>(), table.stride(0), t.p, t.stride, t.n, t.width, table.size(0),
+                                  table.size(1), (void*)stream));
+  return table;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -597,4 +889,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mixer_backward", &mixer_backward);
   m.def("norm_conv_forward", &norm_conv_forward);
   m.def("norm_conv_backward", &norm_conv_backward);
+  m.def("linear_4bit", &linear_4bit);
+  m.def("process_logits", &process_logits);
+  m.def("select_tokens", &select_tokens);
+  m.def("fill_token_history", &fill_token_history);
+  m.def("append_tokens", &append_tokens);
 }

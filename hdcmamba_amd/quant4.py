@@ -1,0 +1,134 @@
+"""4-bit weights with group scales for the decode step's products (csrc/linear4.hip).
+
+A weight [N, K] is held as codes 0..15 with a scale, and optionally a zero point, per row and group of
+32, 64 or 128 columns: w[n, k] = scales[n, g] * (codes[n, k] - zeros[n, g]), zeros 8 where there are
+none.  Inference only, on the GPU only, as every operator of this package.  The reference holds its
+weights in the activation type (hdcmamba/model.py:313,325; train_fineweb.py:55); 4-bit weights have no
+counterpart there.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _ops
+
+__all__ = ["Weight4Bit", "linear_4bit"]
+
+GROUP_SIZES = (32, 64, 128)
+
+
+class Weight4Bit:
+    """A packed 4-bit weight: made once from codes (``from_codes``) or by rounding a weight
+    (``quantize``), then passed to linear_4bit.  Not changed after that.
+
+    ``shape`` (N, K), ``group_size``; ``packed`` uint8, ``scales`` (float32 or bfloat16) and ``zeros``
+    (uint8 or None) in the layout of hdcm_w4_linear_fwd (include/hdcm.h)."""
+
+    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "_args")
+
+    def __init__(self, packed, scales, zeros, shape, group_size):
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.shape, self.group_size = tuple(int(n) for n in shape), int(group_size)
+        self._args = (packed, scales, zeros, *self.shape, self.group_size)
+
+    @staticmethod
+    def _groups(N, K, group_size):
+        """(padded groups, padded rows) of the scale layout."""
+        if group_size not in GROUP_SIZES:
+            raise ValueError(f"group_size must be one of {GROUP_SIZES}, got {group_size}")
+        if N < 1 or K < 1:
+            raise ValueError(f"a 4-bit weight needs rows and columns, got [{N}, {K}]")
+        return -(-K // 128) * 128 // group_size, -(-N // 16) * 16
+
+    @classmethod
+    def from_codes(cls, codes, scales, zeros=None, group_size=128):
+        """codes [N, K] uint8 in 0..15, one per byte; scales [N, ceil(K / group_size)] float32 or
+        bfloat16; zeros (zero points, 0..15) uint8 of the scales' shape, or None for 8."""
+        _ops._on_gpu(codes, scales, zeros)
+        if codes.dim() != 2 or codes.dtype != torch.uint8:
+            raise TypeError(f"codes must be a uint8 [N, K] tensor, got {codes.dtype} {tuple(codes.shape)}")
+        N, K = codes.shape
+        G, Np = cls._groups(N, K, group_size)
+        _ops._dtype(scales)
+        shape = (N, -(-K // group_size))
+        for name, t in (("scales", scales), ("zeros", zeros)):
+            if t is not None and (tuple(t.shape) != shape or t.device != codes.device):
+                raise ValueError(f"{name} must be {shape} on {codes.device}, got {tuple(t.shape)} on {t.device}")
+        if zeros is not None and zeros.dtype != torch.uint8:
+            raise TypeError(f"zeros must be uint8, got {zeros.dtype}")
+        for name, t in (("codes", codes), ("zeros", zeros)):
+            if t is not None and int(t.max()) > 15:
+                raise ValueError(f"{name} must be in 0..15, got {int(t.max())}")
+        with torch.cuda.device(codes.device):
+            codes = codes.contiguous()
+            packed = torch.empty(int(_ops.lib().hdcm_w4_packed_bytes(N, K)), dtype=torch.uint8, device=codes.device)
+            _ops._check("hdcm_w4_pack", _ops.lib().hdcm_w4_pack(codes.data_ptr(), codes.stride(0), N, K, packed.data_ptr(),
+                                                                _ops._stream(codes)))
+
+            def by_group(t, fill):
+                full = torch.full((G, Np), fill, dtype=t.dtype, device=t.device)
+                full[:shape[1], :N] = t.detach().t()
+                return full
+
+            return cls(packed, by_group(scales, 0), None if zeros is None else by_group(zeros, 8), (N, K), group_size)
+
+    @classmethod
+    def quantize(cls, weight, group_size=128, zero_points=False, scale_dtype=None):
+        """weight [N, K] (float32 or bfloat16, finite) rounded to 4 bits per group of a row: without
+        zero points to -7..7 times the group's largest magnitude / 7, with them to the 16 steps from
+        the group's smallest to its largest value (0 among them).  ``scale_dtype``: the weight's by
+        default."""
+        _ops._on_gpu(weight)
+        dtype = _ops._dtype(weight)
+        if weight.dim() != 2:
+            raise ValueError(f"a weight [N, K] is expected, got {tuple(weight.shape)}")
+        weight = weight.detach()
+        scale_dtype = weight.dtype if scale_dtype is None else scale_dtype
+        if scale_dtype not in _ops._DTYPES:
+            raise TypeError(f"scale_dtype must be float32 or bfloat16, got {scale_dtype}")
+        N, K = weight.shape
+        G, Np = cls._groups(N, K, group_size)
+        if not bool(torch.isfinite(weight).all()):
+            raise ValueError("a weight with infinities or NaN cannot be rounded to 4 bits")
+        dev = weight.device
+        with torch.cuda.device(dev):
+            weight = weight.contiguous()
+            packed = torch.empty(int(_ops.lib().hdcm_w4_packed_bytes(N, K)), dtype=torch.uint8, device=dev)
+            scales = torch.empty(G, Np, dtype=scale_dtype, device=dev)
+            zeros = torch.empty(G, Np, dtype=torch.uint8, device=dev) if zero_points else None
+            _ops._check("hdcm_w4_quantize", _ops.lib().hdcm_w4_quantize(
+                weight.data_ptr(), weight.stride(0), N, K, group_size, packed.data_ptr(), scales.data_ptr(),
+                _ops._DTYPES[scale_dtype], None if zeros is None else zeros.data_ptr(), dtype, _ops._stream(weight)))
+        return cls(packed, scales, zeros, (N, K), group_size)
+
+    def dequantize(self, dtype=torch.bfloat16):
+        """The weight [N, K] it stands for, rounded once to ``dtype`` (float32 or bfloat16)."""
+        if dtype not in _ops._DTYPES:
+            raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
+        _ops._on_gpu(self.packed)
+        N, K = self.shape
+        with torch.cuda.device(self.packed.device):
+            out = torch.empty(N, K, dtype=dtype, device=self.packed.device)
+            _ops._check("hdcm_w4_dequant", _ops.lib().hdcm_w4_dequant(
+                self.packed.data_ptr(), self.scales.data_ptr(), _ops._dtype(self.scales),
+                None if self.zeros is None else self.zeros.data_ptr(), self.group_size, out.data_ptr(), K, N, K,
+                _ops._DTYPES[dtype], _ops._stream(out)))
+        return out
+
+    def to(self, device):
+        """The same weight on another device."""
+        move = lambda t: None if t is None else t.to(device)  # noqa: E731
+        return Weight4Bit(move(self.packed), move(self.scales), move(self.zeros), self.shape, self.group_size)
+
+    def __repr__(self):
+        return (f"Weight4Bit({self.shape[0]}x{self.shape[1]}, group_size={self.group_size}, "
+                f"zero_points={self.zeros is not None}, scales={self.scales.dtype}, device={self.packed.device})")
+
+
+def linear_4bit(x, weight, bias=None, residual=None, out=None):
+    """x [..., K] times a Weight4Bit [N, K], transposed, (+ bias [N]) (+ residual [..., N]) -> [..., N] in
+    x's type (float32 or bfloat16): fp32 sums of exact code products, the scales applied to the groups'
+    sums, one rounding.  ``out`` may be ``residual``.  No gradient: refused where one would be
+    recorded."""
+    _ops._on_gpu(x)
+    return _ops.native().linear_4bit(x, weight._args, bias, residual, out, _ops._stream(x))

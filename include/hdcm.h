@@ -533,6 +533,97 @@ int hdcm_rowln_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t
                    const void* w, void* dx, int64_t dx_row_stride, float* dw, float* db, void* ws,
                    size_t ws_bytes, int64_t rows, int64_t width, float eps, int dtype, void* stream);
 
+/*
+ * 4-bit weights with group scales (csrc/linear4.hip): w[n,k] = s[n,g] (c[n,k] - z[n,g]) with codes c
+ * in 0..15, g = k / group, group 32, 64 or 128.  Held as
+ *   packed  hdcm_w4_packed_bytes(N, K) bytes, 16-byte aligned: tiles of 16 rows x 128 columns, written
+ *           by hdcm_w4_pack or hdcm_w4_quantize;
+ *   scales  [G][Np] of scale_dtype, G = ceil(K / 128) * 128 / group, Np = N rounded up to 16: the
+ *           scales of one group of all rows adjacent; groups and rows past the weight hold 0;
+ *   zeros   [G][Np] zero points in 0..15, or NULL: 8 everywhere.
+ * hdcm_w4_pack packs codes [N, K] (one per byte; bits above the low four are dropped).
+ * hdcm_w4_quantize rounds a weight [N, K] of `dtype` to packed, scales and (non-NULL zeros)
+ * zero points: without zero points s = max |w| / 7 per group, c = round(w / s) + 8; with them s =
+ * (max - min) / 15 over the group and 0, z = round(-min / s), c = round(w / s) + z.  The weight has to be
+ * finite.  hdcm_w4_dequant writes s (c - z), rounded once, to out [N, K] of `dtype`.
+ * hdcm_w4_linear_fwd: out[m,n] = sum_k x[m,k] w[n,k] (+ bias[n]) (+ res[m,n]) for x [M, K] of
+ * `dtype`, fp32 accumulation of exact code products, the scales applied to the groups' sums, one
+ * rounding.  bias and res may be NULL; res may be out itself.  x, bias, res and out need only
+ * their type's alignment; rows may have any stride of at least their width.  x's columns past K (row
+ * padding) are not read.  For the decode step's rows (it reads every weight once per 64 rows).
+ * Replaces, in a decode step with 4-bit weights, the nn.Linear in_proj, out_proj and tied head
+ * (hdcmamba/model.py:313,325,340,383; train_fineweb.py:55,94), which the reference holds in the
+ * activation type.
+ */
+size_t hdcm_w4_packed_bytes(int64_t N, int64_t K);
+int hdcm_w4_pack(const uint8_t* codes, int64_t codes_row_stride, int64_t N, int64_t K, void* packed, void* stream);
+int hdcm_w4_quantize(const void* w, int64_t w_row_stride, int64_t N, int64_t K, int64_t group, void* packed,
+                     void* scales, int scale_dtype, uint8_t* zeros, int dtype, void* stream);
+int hdcm_w4_dequant(const void* packed, const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group,
+                    void* out, int64_t out_row_stride, int64_t N, int64_t K, int dtype, void* stream);
+int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const void* packed, const void* scales,
+                       int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias, const void* res,
+                       int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N,
+                       int64_t K, int dtype, void* stream);
+
+/*
+ * From logits to tokens (csrc/logits.hip; the reference's generate, train.py:139-151, samples in torch
+ * and has none of the controls).
+ *
+ * Controls of a batch of B rows of V logits.  A NULL pointer leaves that control out, a row stride of
+ * 0 shares one row between all sequences, and a penalty is per row ([B] fp32) or, where its pointer is
+ * NULL, the `_all` value.  For logit l of token v of a row, in fp32, each step rounded once:
+ *   seen (its history entry is not 0):  l > 0 ? l / repetition : l * repetition
+ *   l - frequency * count;  l - presence if count > 0;  l + bias;  -inf unless bit v % 32 of mask
+ *   word v / 32 is set.
+ * history is an int16 table: the sign bit marks tokens of the prompt, the low 15 bits count the
+ * token in the output.  A row with repetition 1 and frequency and presence 0 does not read it.
+ */
+typedef struct {
+  const int16_t* history;
+  int64_t history_row_stride;
+  const float *repetition, *frequency, *presence;
+  float repetition_all, frequency_all, presence_all;
+  const void* bias; /* bias_dtype */
+  int64_t bias_row_stride;
+  int bias_dtype;
+  const uint32_t* mask; /* [.., ceil(V / 32)] */
+  int64_t mask_row_stride;
+} hdcm_logits_controls;
+
+/*
+ * hdcm_logits_process writes the processed logits (out may be logits itself).  hdcm_token_select
+ * processes them without writing: t = processed / temperature, token = the lowest index of the
+ * largest t + noise, logprob = t[token] - log(sum exp t).  A row's temperature that is not above 0
+ * (temperature [B], or temperature_all) is a greedy choice: t = processed, no noise.  noise [B, V]
+ * fp32 or NULL.  -inf and NaN are never chosen; a row with nothing else gives token -1 and logprob
+ * -inf, and a row with an allowed NaN or +inf a NaN logprob.  ws:
+ * hdcm_token_select_workspace_bytes(B, V) bytes (may be 0), 4-byte aligned, not kept between calls.
+ * Logits, bias, noise and out need only their type's alignment.  V <= 2^30, B <= 65535 (select).
+ */
+int hdcm_logits_process(const void* logits, int64_t logits_row_stride, const hdcm_logits_controls* controls,
+                        void* out, int64_t out_row_stride, int64_t B, int64_t V, int dtype, void* stream);
+size_t hdcm_token_select_workspace_bytes(int64_t B, int64_t V);
+int hdcm_token_select(const void* logits, int64_t logits_row_stride, const hdcm_logits_controls* controls,
+                      const float* temperature, float temperature_all, const float* noise,
+                      int64_t noise_row_stride, int64_t* tokens, float* logprobs, void* ws, size_t ws_bytes,
+                      int64_t B, int64_t V, int dtype, void* stream);
+
+/*
+ * The int16 history table [B, V] of hdcm_logits_controls.  hdcm_token_history_fill writes all of
+ * it from prompt [B, P] and output [B, O] token ids (either may be NULL with a width of 0; lengths [B] or
+ * NULL: how many of a row's ids count, taken into 0..P and 0..O).  hdcm_token_history_append adds the
+ * output tokens [B, T] (lengths as above) to what the table holds.  Counts stop at 32767; ids outside
+ * 0..V-1 are passed over; columns past V of a wider table are left as they are.  B <= 65535.
+ */
+int hdcm_token_history_fill(int16_t* table, int64_t table_row_stride, const int64_t* prompt,
+                            int64_t prompt_row_stride, const int64_t* prompt_lengths, int64_t P,
+                            const int64_t* output, int64_t output_row_stride, const int64_t* output_lengths,
+                            int64_t O, int64_t B, int64_t V, void* stream);
+int hdcm_token_history_append(int16_t* table, int64_t table_row_stride, const int64_t* tokens,
+                              int64_t tokens_row_stride, const int64_t* lengths, int64_t T, int64_t B, int64_t V,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif
