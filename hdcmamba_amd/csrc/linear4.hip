@@ -7,12 +7,16 @@
 //
 // Packed weight: tiles of 16 rows x 128 columns, 1 KB each, tile (n / 16, k / 128) at index
 // (n / 16) * ceil(K / 128) + k / 128.  Inside a tile lane l = 16 g + n % 16 of a wave owns 16
-// bytes, four dwords j = 0..3, dword j holding the codes of columns 32 j + 8 g + 0..7 from its lowest
-// nibble up: one 16-byte load per lane is a whole tile, dword j is the lane's B operand of the
-// tile's j-th v_mfma_f32_16x16x32_bf16, and a wave reads 1 KB that is contiguous.  A code is stored
-// as c ^ 8, the two's complement of c - 8, which v_cvt_off_f32_i4 turns into (c - 8) / 16; a zero
-// point other than 8 is subtracted there.  (c - z) / 16 is exact in bf16, so a product's only
-// roundings are those of the fp32 sums: the scale multiplies a group's sum, not the weights.
+// bytes, four dwords j = 0..3, dword j holding the codes of columns 32 j + 8 g + 0..7: one 16-byte
+// load per lane is a whole tile, dword j is the lane's B operand of the tile's j-th
+// v_mfma_f32_16x16x32_bf16, and a wave reads 1 KB that is contiguous.  In a dword the codes of columns
+// 2 p and 2 p + 1 lie at bits 3 and 19, rotated left by 4 p: rotated back, masked and or-ed with
+// 0x41804180 they are the bf16 values 16 + c of both (the exponent of 16, the code in the top
+// mantissa bits), 7 instructions for 8 codes.
+// bf16 x: a group's sum is formed as sum x (16 + c) - (16 + z) sum x, the second term started with:
+// all products are exact, so the roundings are those of the fp32 sums and the last one; the scale
+// multiplies the group's sum, not the weights.  (An infinity in x meets its negative there: that
+// row becomes NaN.)  fp32 x, whose sums have no bits to spare for that: c - z is formed per weight.
 #include "hdcm_common.h"
 
 using namespace hdcm;
@@ -22,8 +26,8 @@ namespace {
 constexpr int kTileN = 16, kTileK = 128;
 constexpr int kTileBytes = kTileN * kTileK / 2;
 
-// 16-byte loads at the type's own alignment (the row start of a matrix with an odd width)
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// 16-byte loads at the type's own alignment (the row start of a matrix with an odd width)
 __device__ __forceinline__ u32x4_t ldu16(const bf16_t* p) {
   typedef u32x4_t run_t __attribute__((aligned(2)));
   return *reinterpret_cast<const run_t*>(p);
@@ -33,55 +37,92 @@ __device__ __forceinline__ u32x4_t ldu16(const float* p) {
   return *reinterpret_cast<const run_t*>(p);
 }
 
-// Eight activations of a row from column k on; past the row's K columns zero, whatever lies there.
-template <typename T> __device__ __forceinline__ void load_x(Frag<T>& f, const T* row, int k, int K);
-template <> __device__ __forceinline__ void load_x<bf16_t>(Frag<bf16_t>& f, const bf16_t* row, int k, int K) {
-  if (k + 8 <= K) {
-    f.v = __builtin_bit_cast(bf16x8_t, ldu16(row + k));
-  } else {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < K) w[e / 2] |= (uint32_t)row[k + e] << (16 * (e & 1));
-    f.v = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0], w[1], w[2], w[3]});
-  }
+// The 16 bytes of a row of K >= E columns from column k on, zero past its K columns (nothing there is
+// read), in two steps, so that the loads of many need no branch between them: the load (from K - E
+// on where k lies behind it) and, after all loads, the columns moved into place.
+template <typename T> __device__ __forceinline__ u32x4_t load_run(const T* row, int k, int K) {
+  constexpr int E = 16 / sizeof(T);
+  return ldu16(row + min(k, K - E));
 }
-template <> __device__ __forceinline__ void load_x<float>(Frag<float>& f, const float* row, int k, int K) {
-  if (k + 8 <= K) {
-    const u32x4_t a = ldu16(row + k), b = ldu16(row + k + 4);
+template <typename T> __device__ __forceinline__ u32x4_t place_run(u32x4_t v, int k, int K) {
+  constexpr int E = 16 / sizeof(T);
+  if (k >= K) return u32x4_t{0, 0, 0, 0};
+  const int by = k > K - E ? (k - (K - E)) * (int)sizeof(T) : 0;
+  if (by & 8) v = u32x4_t{v[2], v[3], 0, 0};
+  if (by & 4) v = u32x4_t{v[1], v[2], v[3], 0};
+  if (by & 2)
+    v = u32x4_t{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16),
+                __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+  return v;
+}
+
+// 16 + c of a dword's codes as eight bf16.  The mask is kept in a scalar and the exponent in a vector
+// register: with two literals the and and the or would not become one v_and_or_b32.
+struct Decode {
+  uint32_t mask, expo;
+  __device__ __forceinline__ Decode() : mask(0x00780078u), expo(0x41804180u) {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(expo));
+  }
+  __device__ __forceinline__ u32x4_t operator()(uint32_t d) const {
+    return u32x4_t{(d & mask) | expo, ((d >> 4) & mask) | expo, ((d >> 8) & mask) | expo,
+                   (__builtin_amdgcn_alignbit(d, d, 12) & mask) | expo};
+  }
+};
+// The eight values of (16 + c) - z16 as fp32 (exact).
+__device__ __forceinline__ void less_zero(u32x4_t v, float z16, float* c) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f.v[e] = __uint_as_float(a[e]), f.v[4 + e] = __uint_as_float(b[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = k + e < K ? row[k + e] : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    c[2 * i] = __uint_as_float(v[i] << 16) - z16;
+    c[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u) - z16;
   }
 }
 
-// (c - z) / 16 of the eight codes of a dword; z16 = (z - 8) / 16.
-template <bool ZERO> __device__ __forceinline__ void decode8(uint32_t d, float z16, float* w) {
-  const uint32_t h = d >> 4;
-  w[0] = __builtin_amdgcn_cvt_off_f32_i4(d);
-  w[1] = __builtin_amdgcn_cvt_off_f32_i4(h);
-  w[2] = __builtin_amdgcn_cvt_off_f32_i4((d >> 8) & 255);
-  w[3] = __builtin_amdgcn_cvt_off_f32_i4((h >> 8) & 255);
-  w[4] = __builtin_amdgcn_cvt_off_f32_i4((d >> 16) & 255);
-  w[5] = __builtin_amdgcn_cvt_off_f32_i4((h >> 16) & 255);
-  w[6] = __builtin_amdgcn_cvt_off_f32_i4(d >> 24);
-  w[7] = __builtin_amdgcn_cvt_off_f32_i4(h >> 24);
-  if constexpr (ZERO) {
+// Eight columns of a row as A operands: bf16 as they are; an fp32 value as the sum of three bf16 (its
+// leading, middle and last eight mantissa bits, cut off exactly), whose three products on the bf16
+// MFMA take a fifth of the eight v_mfma_f32_16x16x4_f32 that fp32 operands would.
+template <typename T> struct Rows;
+template <> struct Rows<bf16_t> {
+  Frag<bf16_t> x;
+  __device__ __forceinline__ void set(const u32x4_t* v) { x.v = __builtin_bit_cast(bf16x8_t, v[0]); }
+};
+template <> struct Rows<float> {
+  Frag<bf16_t> hi, mid, lo;
+  __device__ __forceinline__ void set(const u32x4_t* v) {
+    uint32_t h[8], m[8], l[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] -= z16;
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = v[e / 4][e & 3];
+      const float f = __uint_as_float(u);
+      const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+      h[e] = f != f ? 0x7fc00000u : u & 0xffff0000u;
+      const float rest = finite ? f - __uint_as_float(h[e]) : 0.f;
+      m[e] = __float_as_uint(rest) & 0xffff0000u;
+      l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
+    }
+    u32x4_t ph, pm, pl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ph[i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
+      pm[i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
+      pl[i] = __builtin_amdgcn_perm(l[2 * i + 1], l[2 * i], 0x07060302u);
+    }
+    hi.v = __builtin_bit_cast(bf16x8_t, ph), mid.v = __builtin_bit_cast(bf16x8_t, pm), lo.v = __builtin_bit_cast(bf16x8_t, pl);
   }
+};
+__device__ __forceinline__ f32x4_t mma(const Rows<bf16_t>& a, const Frag<bf16_t>& b, f32x4_t c) { return hdcm::mma(a.x, b, c); }
+__device__ __forceinline__ f32x4_t mma(const Rows<float>& a, const Frag<bf16_t>& b, f32x4_t c) {
+  return hdcm::mma(a.hi, b, hdcm::mma(a.mid, b, hdcm::mma(a.lo, b, c)));
 }
-
-__device__ __forceinline__ float load_scale(const void* s, bool f32, int64_t i) {
-  return f32 ? reinterpret_cast<const float*>(s)[i] : bf2f(reinterpret_cast<const bf16_t*>(s)[i]);
+__device__ __forceinline__ Frag<bf16_t> fill(uint32_t v) {
+  Frag<bf16_t> f;
+  f.v = __builtin_bit_cast(bf16x8_t, u32x4_t{v, v, v, v});
+  return f;
 }
 
 struct Linear4Args {
   const void* x;
-  const uint4* codes;
-  const void* scales;
+  const char *codes, *scales;
   const uint8_t* zeros;
   const void *bias, *res;
   void* out;
@@ -90,94 +131,350 @@ struct Linear4Args {
   bool s_f32;
 };
 
-// A workgroup of W waves computes MT row tiles of 16 by NT column tiles of 16, the waves taking the
-// 128-column tiles of K in turn; their partial sums are added in wave order through LDS.
-template <typename T, int MT, int NT, int W, int GS, bool ZERO>
-__global__ __launch_bounds__(W* kWave) void linear4_kernel(Linear4Args p) {
-  constexpr int ROWS = 16 * MT, COLS = 16 * NT, PITCH = COLS + 1;
-  constexpr int GPT = 4 / GS;  // groups per tile
-  __shared__ float part[W][ROWS * PITCH];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
-  const int l16 = lane & 15, g = lane >> 4;
-  const int t0 = blockIdx.x * NT, m0 = blockIdx.y * ROWS;
-  const T* x = reinterpret_cast<const T*>(p.x);
-  const T* xr[MT];  // rows past M read row M-1 (their outputs are not stored)
-#pragma unroll
-  for (int r = 0; r < MT; ++r) xr[r] = x + (int64_t)min(m0 + 16 * r + l16, p.M - 1) * p.x_rs;
-  f32x4_t acc[MT][NT];
-#pragma unroll
-  for (int r = 0; r < MT; ++r)
-#pragma unroll
-    for (int c = 0; c < NT; ++c) acc[r][c] = {0.f, 0.f, 0.f, 0.f};
+// A lane's scale of a row of a tile: the loads take a uniform address and a 32-bit lane offset, and of
+// bf16 scales the dword that holds two, so that no branch on the type stands between them.
+struct Scales {
+  const char* p;
+  int log;
+  uint32_t off, shift, mask;
+  __device__ __forceinline__ Scales(const char* s, bool f32, int n)
+      : p(s), log(f32 ? 2 : 1), off(f32 ? 4 * n : 2 * n & ~3), shift(f32 || (n & 1) ? 0 : 16), mask(f32 ? ~0u : 0xffff0000u) {}
+  // at: the index of the scale of row 0 of the lane's sixteen (even)
+  __device__ __forceinline__ uint32_t raw(int64_t at) const { return *reinterpret_cast<const uint32_t*>(p + (at << log) + off); }
+  __device__ __forceinline__ float value(uint32_t raw) const { return __uint_as_float((raw << shift) & mask); }
+};
+__device__ __forceinline__ uint4 load_tile(const Linear4Args& p, int t, int kt, int lane) {
+  const char* at = p.codes + ((int64_t)t * p.tiles_k + kt) * kTileBytes;
+  return *reinterpret_cast<const uint4*>(at + (uint32_t)(lane * 16));
+}
 
-  for (int kt = w; kt < p.tiles_k; kt += W) {
-    uint4 q[NT];
-    float s[NT][GPT], z[NT][GPT];
+__device__ __forceinline__ void lds_barrier() {  // orders LDS only: loads in flight stay in flight
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// What a wave does with one tile: acc += scale (sum x (16 + c) - (16 + z) sum x) per group.  q: the
+// tile's dwords; xa: the rows' fragments; xsum: with one group per tile the rows' sums (or -24 times
+// them without zero points), else unused.
+template <typename T, int MT, int GS, bool ZERO>
+__device__ __forceinline__ void tile_mma(uint4 q, const uint32_t (&sr)[4 / GS], const int (&zr)[4 / GS], const Scales& sc,
+                                         const Decode& decode, const Rows<T> (&xa)[4][MT], const f32x4_t (&xsum)[MT],
+                                         f32x4_t (&acc)[MT]) {
+  constexpr bool BF = sizeof(T) == 2;
+  f32x4_t sum[MT];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {  // column tiles past the last re-read it
-      const int t = min(t0 + c, p.tiles_n - 1);
-      q[c] = p.codes[((int64_t)t * p.tiles_k + kt) * kWave + lane];
+  for (int u = 0; u < 4 / GS; ++u) {
+    const float z16 = ZERO ? (float)(zr[u] + 16) : 24.f;
+    if constexpr (!BF) {
 #pragma unroll
-      for (int i = 0; i < GPT; ++i) {
-        const int64_t at = (int64_t)(kt * GPT + i) * p.np + 16 * t + l16;
-        s[c][i] = 16.f * load_scale(p.scales, p.s_f32, at);
-        z[c][i] = ZERO ? ((int)p.zeros[at] - 8) * 0.0625f : 0.f;
+      for (int r = 0; r < MT; ++r) sum[r] = {0.f, 0.f, 0.f, 0.f};
+    } else if constexpr (GS == 4) {
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[r][e] = ZERO ? -z16 * xsum[r][e] : xsum[r][e];
+    } else {
+      // smaller groups: -(16 + z) as a constant operand (bf16 0xc180 + 8 z), one MFMA a step instead of
+      // four multiplications and the registers of the sums
+      uint32_t c = 0xc1c0c1c0u;
+      if constexpr (ZERO) {
+        c = 0xc180u + 8u * (uint32_t)zr[u];
+        c |= c << 16;
+      }
+      const Frag<bf16_t> k = fill(c);
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        sum[r] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GS; ++j) sum[r] = mma(xa[u * GS + j][r], k, sum[r]);
       }
     }
-    f32x4_t sum[MT][NT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      Frag<T> a[MT];
-#pragma unroll
-      for (int r = 0; r < MT; ++r) load_x<T>(a[r], xr[r], kt * kTileK + 32 * j + 8 * g, p.K);
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const uint32_t d = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
-        float v[8];
-        decode8<ZERO>(d, z[c][j / GS], v);
-        Frag<T> b;
-        frag_from_f32(b, v);
-#pragma unroll
-        for (int r = 0; r < MT; ++r) {
-          const f32x4_t none = {0.f, 0.f, 0.f, 0.f};
-          sum[r][c] = mma(a[r], b, j % GS == 0 ? none : sum[r][c]);
-          if ((j + 1) % GS == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][c][e] = fmaf(s[c][j / GS], sum[r][c][e], acc[r][c][e]);
-          }
-        }
+    for (int j = 0; j < GS; ++j) {
+      const int i = u * GS + j;
+      const u32x4_t v = decode(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w);
+      Frag<bf16_t> b;
+      if constexpr (BF) {
+        b.v = __builtin_bit_cast(bf16x8_t, v);
+      } else {
+        float c[8];
+        less_zero(v, z16, c);
+        frag_from_f32(b, c);
       }
+#pragma unroll
+      for (int r = 0; r < MT; ++r) sum[r] = mma(xa[i][r], b, sum[r]);
     }
-  }
-  // D layout: lane holds D[4 g + e][l16]
+    const float s = sc.value(sr[u]);
 #pragma unroll
-  for (int r = 0; r < MT; ++r)
+    for (int r = 0; r < MT; ++r)
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[w][(16 * r + 4 * g + e) * PITCH + 16 * c + l16] = acc[r][c][e];
-  __syncthreads();
-  for (int i = tid; i < ROWS * COLS; i += W * kWave) {
-    const int m = i / COLS, c = i % COLS, row = m0 + m, n = 16 * t0 + c;
-    if (row >= p.M || n >= p.N) continue;
-    float v = 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) v += part[k][m * PITCH + c];
-    if (p.bias) v += to_f<T>(reinterpret_cast<const T*>(p.bias)[n]);
-    if (p.res) v += to_f<T>(reinterpret_cast<const T*>(p.res)[(int64_t)row * p.r_rs + n]);
-    reinterpret_cast<T*>(p.out)[(int64_t)row * p.o_rs + n] = from_f<T>(v);
+      for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(s, sum[r][e], acc[r][e]);
   }
 }
 
-template <typename T, int MT, int NT, int GS, bool ZERO> void launch_linear4(const Linear4Args& a, hipStream_t s) {
-  constexpr int W = 8;
-  const dim3 grid((unsigned)((a.tiles_n + NT - 1) / NT), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  HDCM_LAUNCH((linear4_kernel<T, MT, NT, W, GS, ZERO>), grid, dim3(W * kWave), 0, s, a);
+// The sums of the rows over a tile's columns (times -24 without zero points), in the MFMA's D layout.
+template <typename T, int MT, bool ZERO>
+__device__ __forceinline__ void row_sums(const Rows<T> (&xa)[4][MT], f32x4_t (&xsum)[MT]) {
+  const Frag<bf16_t> k = fill(ZERO ? 0x3f803f80u : 0xc1c0c1c0u);
+#pragma unroll
+  for (int r = 0; r < MT; ++r) {
+    xsum[r] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xsum[r] = mma(xa[j][r], k, xsum[r]);
+  }
+}
+
+// The end of four rows (row0 + 0..3) of one column n: what is added is loaded ahead of the products (at
+// clamped places, without a branch per lane, and converted only here), then one rounding and the store.
+template <typename T> struct Ending {
+  T bias, res[4];
+  __device__ __forceinline__ void load(const Linear4Args& p, int row0, int rows_end, int n) {
+    n = min(n, p.N - 1);
+    if (p.bias) bias = reinterpret_cast<const T*>(p.bias)[n];
+    if (p.res) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) res[e] = reinterpret_cast<const T*>(p.res)[(int64_t)min(row0 + e, rows_end - 1) * p.r_rs + n];
+    }
+  }
+  __device__ __forceinline__ void store(const Linear4Args& p, f32x4_t v, int row0, int rows_end, int n) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float y = v[e];
+      if (p.bias) y += to_f<T>(bias);
+      if (p.res) y += to_f<T>(res[e]);
+      if (row0 + e < rows_end && n < p.N) reinterpret_cast<T*>(p.out)[(int64_t)(row0 + e) * p.o_rs + n] = from_f<T>(y);
+    }
+  }
+};
+
+// Rows held in registers.  The W waves of a workgroup split K, two 128-column tiles each, and keep
+// the fragments of up to 16 MT rows of x for their columns while the workgroup walks over column
+// tiles of the output; the next tile's codes are in flight while one is multiplied.  Per output tile
+// each wave leaves its partial sums in LDS (two buffers, so one barrier a tile) and the waves take
+// turns in adding them up.  x is read once per workgroup, a quarter row per load instruction (whole
+// lines; fragments read straight from the rows, 16 rows x 64 bytes an instruction, took 1.4 us
+// longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS.
+// What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
+// instructions per wave and tile.
+template <typename T, int MT, int GS, bool ZERO, int MAXW>
+__global__ __launch_bounds__(MAXW* kWave) void linear4_kernel(Linear4Args p) {
+  constexpr int P = 2, GPT = 4 / GS;
+  constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
+  extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [2][MAXW][MT][64]; at first the waves' slabs of x
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int W = blockDim.x / kWave;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.y * 16 * MT;
+  const int rows = min(16 * MT, p.M - m0);
+  const int k0 = w * P;  // the wave's first column tile
+  const Decode decode;
+  const Scales scales(p.scales, p.s_f32, l16);
+
+  // x: 16 rows x 128 columns in NLD loads
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.x_rs;
+  u32x4_t raw[MT][P][NLD];
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int n = 0; n < NLD; ++n) {
+        // rows past M re-read the last; a whole load of them is left out (their fragments hold what LDS held:
+        // every row of a product depends on its own row of x alone, and theirs are not stored)
+        if (n * kWave / CPR + 16 * r >= rows) continue;
+        const int at = n * kWave + lane, row = min(16 * r + at / CPR, rows - 1);
+        raw[r][i][n] = load_run<T>(x + (int64_t)row * p.x_rs, (k0 + i) * kTileK + at % CPR * E, p.K);
+      }
+  uint4 q[P];
+  uint32_t sr[P][GPT];
+  int zr[P][GPT];
+  auto fetch = [&](int t) {  // tiles past the last re-read it
+    t = min(t, p.tiles_n - 1);
+#pragma unroll
+    for (int i = 0; i < P; ++i) q[i] = load_tile(p, t, min(k0 + i, p.tiles_k - 1), lane);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int u = 0; u < GPT; ++u) {
+        const int64_t at = (int64_t)(min(k0 + i, p.tiles_k - 1) * GPT + u) * p.np + kTileN * t;
+        sr[i][u] = scales.raw(at);
+        if constexpr (ZERO) zr[i][u] = (p.zeros + at)[(uint32_t)l16];
+      }
+  };
+  fetch(blockIdx.x);
+
+  T* slab = reinterpret_cast<T*>(part) + w * 16 * PITCH;  // the wave's own: no barrier
+  Rows<T> xa[P][4][MT];
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      asm volatile("" ::: "memory");  // a wave's LDS accesses complete in order; they stay in this one
+#pragma unroll
+      for (int n = 0; n < NLD; ++n) {
+        if (n * kWave / CPR + 16 * r >= rows) continue;
+        const int at = n * kWave + lane, k = (k0 + i) * kTileK + at % CPR * E;
+        u32x4_t v = raw[r][i][n];
+        if ((k0 + i + 1) * kTileK > p.K) v = place_run<T>(v, k, p.K);  // (uniform)
+        *reinterpret_cast<u32x4_t*>(slab + at / CPR * PITCH + at % CPR * E) = v;
+      }
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4_t v[8 / E];
+#pragma unroll
+        for (int h = 0; h < 8 / E; ++h) v[h] = *reinterpret_cast<const u32x4_t*>(slab + l16 * PITCH + 32 * j + 8 * g + E * h);
+        xa[i][j][r].set(v);
+      }
+      asm volatile("" ::: "memory");
+    }
+  f32x4_t xsum[P][MT];
+  if constexpr (GS == 4 && sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) row_sums<T, MT, ZERO>(xa[i], xsum[i]);
+  }
+  __syncthreads();  // the slabs become the partial sums' buffers
+  for (int k = W + w; k < MAXW; k += W)  // waves that are not there add nothing
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) part[(i / MT * MAXW + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  int buf = 0, turn = 0;
+  for (int t = blockIdx.x; t < p.tiles_n; t += gridDim.x) {
+    Ending<T> end;
+    const int own = w >= turn ? w - turn : w + W - turn;  // the row tile that this wave adds up (none past MT)
+    if (own < MT) end.load(p, m0 + 16 * own + 4 * g, m0 + rows, kTileN * t + l16);
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r) acc[r] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (i == 0 || k0 + i < p.tiles_k)
+        tile_mma<T, MT, GS, ZERO>(q[i], sr[i], zr[i], scales, decode, xa[i], xsum[i], acc);
+    fetch(t + gridDim.x);
+    f32x4_t* mine = part + (buf * MAXW + w) * MT * kWave + lane;
+#pragma unroll
+    for (int r = 0; r < MT; ++r) mine[r * kWave] = acc[r];
+    lds_barrier();
+    for (int r = own; r < MT; r += W) {  // (fewer waves than row tiles: the others follow)
+      if (r != own) end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+      const f32x4_t* from = part + buf * MAXW * MT * kWave + r * kWave + lane;
+      f32x4_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = from[k * MT * kWave];
+      f32x4_t sum = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+      for (int b = 4; b < MAXW; b += 4)
+        if (W > b) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = from[(b + k) * MT * kWave];
+          sum += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+      end.store(p, sum, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+    }
+    turn += MT;
+    while (turn >= W) turn -= W;
+    buf ^= 1;
+  }
+}
+
+// Any K: a workgroup of W waves computes MT row tiles by one column tile, the waves taking the 128-column
+// tiles of K in turn and reading x's fragments as they go; the partial sums are added through LDS.
+template <typename T, int MT, int GS, bool ZERO>
+__global__ __launch_bounds__(8 * kWave) void linear4_long_kernel(Linear4Args p) {
+  constexpr int W = 8, GPT = 4 / GS, E = 16 / sizeof(T);
+  __shared__ f32x4_t part[W][MT][kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int l16 = lane & 15, g = lane >> 4;
+  const int t = blockIdx.x, m0 = blockIdx.y * 16 * MT;
+  const int rows = min(16 * MT, p.M - m0);
+  const Decode decode;
+  const Scales scales(p.scales, p.s_f32, l16);
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.x_rs;
+  f32x4_t acc[MT];
+#pragma unroll
+  for (int r = 0; r < MT; ++r) acc[r] = {0.f, 0.f, 0.f, 0.f};
+  for (int kt = w; kt < p.tiles_k; kt += W) {
+    const uint4 q = load_tile(p, t, kt, lane);
+    uint32_t sr[GPT];
+    int zr[GPT];
+#pragma unroll
+    for (int u = 0; u < GPT; ++u) {
+      const int64_t at = (int64_t)(kt * GPT + u) * p.np + kTileN * t;
+      sr[u] = scales.raw(at);
+      if constexpr (ZERO) zr[u] = (p.zeros + at)[(uint32_t)l16];
+    }
+    u32x4_t raw[4][MT][8 / E];
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 8 / E; ++h)
+          raw[j][r][h] = load_run<T>(x + (int64_t)min(16 * r + l16, rows - 1) * p.x_rs, kt * kTileK + 32 * j + 8 * g + E * h, p.K);
+    Rows<T> xa[4][MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+      {
+        if ((kt + 1) * kTileK > p.K)  // (uniform)
+#pragma unroll
+          for (int h = 0; h < 8 / E; ++h) raw[j][r][h] = place_run<T>(raw[j][r][h], kt * kTileK + 32 * j + 8 * g + E * h, p.K);
+        xa[j][r].set(raw[j][r]);
+      }
+    f32x4_t xsum[MT];
+    if constexpr (GS == 4 && sizeof(T) == 2) row_sums<T, MT, ZERO>(xa, xsum);
+    tile_mma<T, MT, GS, ZERO>(q, sr, zr, scales, decode, xa, xsum, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < MT; ++r) part[w][r][lane] = acc[r];
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < MT; ++r)
+    if (w == r) {
+      Ending<T> end;
+      end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+      f32x4_t v = part[0][r][lane];
+#pragma unroll
+      for (int k = 1; k < W; ++k) v += part[k][r][lane];
+      end.store(p, v, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+    }
+}
+
+// The registers hold up to 64 bf16 rows of 16 column tiles (2048 columns) in 8 waves, or 32 rows of 24
+// in 12; of fp32 rows, whose three parts take three times as many, 16.  More rows run as row blocks of equal height, which read the
+// weight again (out of the caches); longer rows run on linear4_long_kernel.
+constexpr int kWidest = 24, kWide = 16;
+
+template <typename T, int MT, int GS, bool ZERO, int MAXW> void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
+  const int W = (a.tiles_k + 1) / 2;
+  // waves per CU: 16 with one row tile, 8 with more (their registers): whole workgroups
+  const int per_cu = (MT == 1 ? 16 : 8) / W;
+  const int most = 256 * (per_cu > 1 ? per_cu : 1);
+  const size_t slabs = (size_t)W * 16 * (kTileK * sizeof(T) + 16), parts = (size_t)2 * MAXW * MT * kWave * 16;
+  HDCM_LAUNCH((linear4_kernel<T, MT, GS, ZERO, MAXW>), dim3((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m),
+              dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+}
+template <typename T, int MT, int GS, bool ZERO> void launch_long(const Linear4Args& a, hipStream_t s) {
+  HDCM_LAUNCH((linear4_long_kernel<T, MT, GS, ZERO>), dim3((unsigned)a.tiles_n, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+              dim3(8 * kWave), 0, s, a);
 }
 template <typename T, int GS, bool ZERO> void pick_rows(const Linear4Args& a, hipStream_t s) {
-  if (a.M <= 16) launch_linear4<T, 1, 2, GS, ZERO>(a, s);
-  else if (a.M <= 32) launch_linear4<T, 2, 2, GS, ZERO>(a, s);
-  else launch_linear4<T, 4, 2, GS, ZERO>(a, s);
+  const int tiles_m = (a.M + 15) / 16;
+  if (a.tiles_k > kWidest) {
+    tiles_m == 1 ? launch_long<T, 1, GS, ZERO>(a, s) : launch_long<T, 2, GS, ZERO>(a, s);
+    return;
+  }
+  const bool wide = a.tiles_k > kWide;
+  const int most = sizeof(T) == 4 ? 1 : wide ? 2 : 4;
+  const int blocks = (tiles_m + most - 1) / most, mt = (tiles_m + blocks - 1) / blocks;
+  if (mt == 1) launch_linear4<T, 1, GS, ZERO, 12>(a, blocks, s);
+  if constexpr (sizeof(T) == 2) {
+    if (mt == 2) launch_linear4<T, 2, GS, ZERO, 12>(a, blocks, s);
+    if (mt == 3) launch_linear4<T, 3, GS, ZERO, 8>(a, blocks, s);
+    if (mt == 4) launch_linear4<T, 4, GS, ZERO, 8>(a, blocks, s);
+  }
 }
 template <typename T, int GS> void pick_zero(const Linear4Args& a, hipStream_t s) {
   a.zeros ? pick_rows<T, GS, true>(a, s) : pick_rows<T, GS, false>(a, s);
@@ -189,6 +486,11 @@ template <typename T> void pick_group(const Linear4Args& a, int group, hipStream
 }
 
 // ------------------------------------------------------------ packing and unpacking
+// The bits of code c of column e of a dword's eight.
+__device__ __forceinline__ uint32_t code_bits(uint32_t c, int e) {
+  const uint32_t v = c << (e & 1 ? 19 : 3);
+  return __builtin_amdgcn_alignbit(v, v, (32 - 4 * (e / 2)) & 31);  // rotated left by 4 (e / 2)
+}
 __device__ __forceinline__ int64_t dword_at(int n, int k8, int tiles_k) {  // columns 8 k8 .. +8 of row n
   const int kt = k8 / 16, j = (k8 % 16) / 4, g = k8 % 4;
   return (((int64_t)(n / kTileN) * tiles_k + kt) * kWave + 16 * g + n % kTileN) * 4 + j;
@@ -205,7 +507,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict_
   for (int e = 0; e < 8; ++e) {
     const int k = 8 * k8 + e;
     const uint32_t c = n < N && k < K ? codes[(int64_t)n * rs + k] & 15u : 8u;
-    d |= (c ^ 8u) << (4 * e);
+    d |= code_bits(c, e);
   }
   packed[dword_at(n, k8, tiles_k)] = d;
 }
@@ -240,7 +542,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const T* __restrict__ 
     for (int e = 0; e < 8; ++e) {
       const int k = 8 * k8 + e;
       const float c = k >= k1 ? 8.f : s > 0.f ? fminf(fmaxf(rintf(to_f<T>(row[k]) / s) + z, 0.f), 15.f) : z;
-      d |= ((uint32_t)c ^ 8u) << (4 * e);
+      d |= code_bits((uint32_t)c, e);
     }
     packed[dword_at(n, k8, tiles_k)] = d;
   }
@@ -256,13 +558,14 @@ __global__ __launch_bounds__(256) void w4_dequant_kernel(const uint32_t* __restr
   if (i >= (int64_t)N * k8s) return;
   const int k8 = (int)(i % k8s), n = (int)(i / k8s);
   const int64_t at = (int64_t)(8 * k8 / group) * np + n;
-  const float s = 16.f * load_scale(scales, s_f32, at);
-  float v[8];
-  decode8<true>(packed[dword_at(n, k8, tiles_k)], zeros ? ((int)zeros[at] - 8) * 0.0625f : 0.f, v);
+  const Scales sc((const char*)scales, s_f32, n % kTileN);
+  const float s = sc.value(sc.raw(at - n % kTileN));
+  float c[8];
+  less_zero(Decode()(packed[dword_at(n, k8, tiles_k)]), zeros ? (float)(zeros[at] + 16) : 24.f, c);
   T* o = out + (int64_t)n * o_rs + 8 * k8;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (8 * k8 + e < K) o[e] = from_f<T>(s * v[e]);
+    if (8 * k8 + e < K) o[e] = from_f<T>(s * c[e]);
 }
 
 bool sizes_ok(int64_t N, int64_t K, int64_t group) {
@@ -332,7 +635,7 @@ extern "C" int hdcm_w4_dequant(const void* packed, const void* scales, int scale
   HDCM_CHECK_ARG((packed && scales && out) || N == 0, HDCM_EINVAL);
   HDCM_CHECK_ARG(out_row_stride >= K || N <= 1, HDCM_EINVAL);
   HDCM_CHECK_ARG(sizes_ok(N, K, group), HDCM_EUNSUPPORTED);
-  HDCM_CHECK_ARG(hdcm_aligned16(packed), HDCM_EALIGN);
+  HDCM_CHECK_ARG(hdcm_aligned16(packed) && ((uintptr_t)scales & 3u) == 0, HDCM_EALIGN);
   if (N == 0) return HDCM_OK;
   const int tk = tiles_of(K, kTileK), np = tiles_of(N, kTileN) * kTileN, g = (int)group, n = (int)N, k = (int)K;
   const int64_t total = N * ((K + 7) / 8);
@@ -359,11 +662,11 @@ extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const voi
   HDCM_CHECK_ARG(M >= 0 && N >= 0 && K > 0, HDCM_EINVAL);
   HDCM_CHECK_ARG(M == 0 || N == 0 || (x && packed && scales && out), HDCM_EINVAL);
   HDCM_CHECK_ARG(M <= 1 || (x_row_stride >= K && out_row_stride >= N && (!res || res_row_stride >= N)), HDCM_EINVAL);
-  HDCM_CHECK_ARG(sizes_ok(N, K, group) && M <= 64 * 65535, HDCM_EUNSUPPORTED);
-  HDCM_CHECK_ARG(hdcm_aligned16(packed), HDCM_EALIGN);
+  HDCM_CHECK_ARG(sizes_ok(N, K, group) && K >= (dtype == HDCM_F32 ? 4 : 8) && M <= 16 * 65535, HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(hdcm_aligned16(packed) && ((uintptr_t)scales & 3u) == 0, HDCM_EALIGN);
   if (M == 0 || N == 0) return HDCM_OK;
   Linear4Args a;
-  a.x = x, a.codes = (const uint4*)packed, a.scales = scales, a.zeros = zeros, a.bias = bias, a.res = res, a.out = out;
+  a.x = x, a.codes = (const char*)packed, a.scales = (const char*)scales, a.zeros = zeros, a.bias = bias, a.res = res, a.out = out;
   a.x_rs = x_row_stride, a.r_rs = res_row_stride, a.o_rs = out_row_stride;
   a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.tiles_n = tiles_of(N, kTileN), a.tiles_k = tiles_of(K, kTileK), a.np = a.tiles_n * kTileN;

@@ -657,7 +657,7 @@ Tensor linear_4bit(const Tensor& x, const WeightArgs& weight, const OptTensor& b
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) == w.K, "linear_4bit: x ", x.sizes(), " does not end in the weight's ", w.K, " columns");
   auto shape = x.sizes().vec();
   shape.back() = w.N;
-  const Tensor xr = rows(x);
+  Tensor xr = rows(x);
   Tensor out = given;
   if (out.defined()) {
     same_device(out, x, "out");
@@ -681,10 +681,15 @@ Tensor linear_4bit(const Tensor& x, const WeightArgs& weight, const OptTensor& b
   if (given.defined())
     TORCH_CHECK(!overlap(o, xr) && (!r.defined() || same_place(o, r) || !overlap(o, r)),
                 "linear_4bit: out may be the residual itself but share no other memory with x or the residual");
+  int64_t K = w.K;
+  if (K < 8) {  // shorter than a load of the kernel's: columns of zeros, which the packed weight holds too
+    xr = at::constant_pad_nd(xr, {0, 8 - K});
+    K = 8;
+  }
   check("hdcm_w4_linear_fwd",
         hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), w.packed.const_data_ptr(), w.scales.const_data_ptr(),
                            dtype_of(w.scales), (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
-                           r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, w.K, dt,
+                           r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, K, dt,
                            (void*)stream));
   return out;
 }

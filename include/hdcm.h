@@ -538,7 +538,7 @@ int hdcm_rowln_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t
  * in 0..15, g = k / group, group 32, 64 or 128.  Held as
  *   packed  hdcm_w4_packed_bytes(N, K) bytes, 16-byte aligned: tiles of 16 rows x 128 columns, written
  *           by hdcm_w4_pack or hdcm_w4_quantize;
- *   scales  [G][Np] of scale_dtype, G = ceil(K / 128) * 128 / group, Np = N rounded up to 16: the
+ *   scales  [G][Np] of scale_dtype, 4-byte aligned, G = ceil(K / 128) * 128 / group, Np = N rounded up to 16: the
  *           scales of one group of all rows adjacent; groups and rows past the weight hold 0;
  *   zeros   [G][Np] zero points in 0..15, or NULL: 8 everywhere.
  * hdcm_w4_pack packs codes [N, K] (one per byte; bits above the low four are dropped).
@@ -550,7 +550,8 @@ int hdcm_rowln_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t
  * `dtype`, fp32 accumulation of exact code products, the scales applied to the groups' sums, one
  * rounding.  bias and res may be NULL; res may be out itself.  x, bias, res and out need only
  * their type's alignment; rows may have any stride of at least their width.  x's columns past K (row
- * padding) are not read.  For the decode step's rows (it reads every weight once per 64 rows).
+ * padding) are not read.  K >= 8 (bf16) or 4 (fp32).  bf16 x: an infinity makes its row NaN.  For the decode step's rows: the
+ * weight is read once per 64 bf16 rows of up to 2048 columns (less for longer and fp32 rows).
  * Replaces, in a decode step with 4-bit weights, the nn.Linear in_proj, out_proj and tied head
  * (hdcmamba/model.py:313,325,340,383; train_fineweb.py:55,94), which the reference holds in the
  * activation type.

@@ -36,6 +36,7 @@ def test_w4_linear_validation():
     assert f(*with_(base, _4=2)) == EUNSUPPORTED
     assert f(*with_(base, _6=16)) == EUNSUPPORTED
     assert f(*with_(base, _6=256)) == EUNSUPPORTED
+    assert f(*with_(base, _14=7)) == EUNSUPPORTED  # shorter than one load
     assert f(*with_(base, _0=None)) == EINVAL
     assert f(*with_(base, _3=None)) == EINVAL
     assert f(*with_(base, _14=0)) == EINVAL
@@ -43,6 +44,7 @@ def test_w4_linear_validation():
     assert f(*with_(base, _11=8575)) == EINVAL
     assert f(*with_(base, _8=P16, _9=100)) == EINVAL
     assert f(*with_(base, _2=P18)) == EALIGN
+    assert f(*with_(base, _3=P18)) == EALIGN
     assert f(*with_(base, _12=-1)) == EINVAL
     assert f(*with_(base, _12=0, _0=None, _10=None)) == OK
     assert f(*with_(base, _13=0, _2=None, _3=None, _10=None)) == OK

@@ -1,8 +1,8 @@
 """4-bit products, logits processing, token choice and token history against plain implementations.
 
-Products: every output within the rounding of its type plus what fp32 sums of K exact products may
-lose, (K + 8) 2^-23 of the sum of magnitudes (a step of 2^-23 per addition covers an accumulator
-that truncates).  Processed logits: bit for bit the fp32 formula, operation by operation.
+Products: every output within the rounding of its type plus what fp32 sums of exact products may lose.
+fp32 rows sum K products x (c - z), bf16 rows the 2 K products x (16 + c) and -x (16 + z): a step of
+2^-23 per addition (covers an accumulator that truncates) of the sum of their magnitudes.  Processed logits: bit for bit the fp32 formula, operation by operation.
 """
 import pytest
 import torch
@@ -38,14 +38,20 @@ def _dense(codes, scales, z, group):
     return (codes.double() - (wide(z) if z is not None else 8.0)) * wide(scales)
 
 
-def _check_linear(got, x, w, bias, res):
+def _check_linear(got, x, codes, scales, z, group, bias, res):
     """got against x w^T + bias + res in 64 bits, elementwise."""
-    x, w = x.double(), w.double()
-    ref, mag = x @ w.t(), x.abs() @ w.abs().t()
+    N, K = codes.shape
+    w, x = _dense(codes, scales, z, group), x.double()
+    ref = x @ w.t()
+    if got.dtype == F32:
+        mag, n = x.abs() @ w.abs().t(), K
+    else:
+        wide = lambda t: t.double().repeat_interleave(group, 1)[:, :K]  # noqa: E731
+        mag, n = x.abs() @ ((32 + codes.double() + (wide(z) if z is not None else 8.0)) * wide(scales)).t(), 2 * K
     for t in (bias, res):
         if t is not None:
             ref, mag = ref + t.double(), mag + t.double().abs()
-    tol = torch.finfo(got.dtype).eps / 2 * ref.abs() + (x.shape[1] + 8) * 2.0**-23 * mag
+    tol = torch.finfo(got.dtype).eps / 2 * ref.abs() + (n + 8) * 2.0**-23 * mag
     err = (got.cpu().double() - ref).abs()
     worst = float((err / tol.clamp_min(1e-300)).max()) if err.numel() else 0.0
     _say("  worst error / tolerance", worst)
@@ -67,6 +73,16 @@ LINEAR = [
     (200, 130, 40, 64, True, F32, F32),
     (7, 4224, 96, 128, False, BF, BF),     # more column tiles than waves take at once
     (31, 96, 1, 32, False, BF, F32),
+    (40, 2048, 100, 128, True, BF, BF),    # three row tiles
+    (16, 2176, 2048, 128, False, BF, BF),  # seventeen column tiles
+    (50, 3000, 70, 32, True, F32, BF),     # too many column tiles for three
+    (20, 2500, 33, 64, False, BF, F32),
+    (70, 3200, 50, 32, True, BF, BF),      # longer rows than the registers take
+    (3, 5001, 40, 64, False, F32, F32),
+    (2, 7, 20, 32, False, BF, BF),         # rows shorter than a 16-byte load
+    (2, 3, 20, 32, True, BF, F32),
+    (4, 9, 17, 64, True, F32, BF),
+    (129, 128, 4200, 64, False, BF, BF),   # more output tiles than workgroups
 ]
 
 
@@ -83,7 +99,7 @@ def test_linear_4bit(dev, M, K, N, group, zeros, sdt, dtype, extra):
     w = hm.Weight4Bit.from_codes(to(codes), to(scales), to(z), group)
     got = hm.linear_4bit(to(x), w, bias=to(bias), residual=to(res))
     assert got.shape == (M, N) and got.dtype == dtype
-    _check_linear(got, x, _dense(codes, scales, z, group), bias, res)
+    _check_linear(got, x, codes, scales, z, group, bias, res)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -114,20 +130,19 @@ def test_linear_4bit_layouts(dev, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_linear_4bit_infinities(dev, dtype):
-    """A row's infinity or NaN stays in its row and has the sign that the weights give it."""
+    """A row's infinity or NaN stays in its row: a bf16 row becomes NaN, an fp32 row what the weights give."""
     N, K = 32, 256
     codes, scales, _ = _weight(N, K, 128, False, F32, 5)
-    codes[0] = 15
-    codes[1] = 1
     w = hm.Weight4Bit.from_codes(codes.to(dev), scales.to(dev), None, 128)
     x = torch.randn(4, K, generator=_gen(1)).to(dtype)
     x[1, 7], x[2, 9] = float("inf"), float("nan")
     got = hm.linear_4bit(x.to(dev), w).cpu()
     assert got[0].isfinite().all() and got[3].isfinite().all() and got[2].isnan().all()
-    assert got[1, 0] == float("inf") and got[1, 1] == float("-inf")
-    dense = _dense(codes, scales, None, 128)
-    ref = x[1].double() * dense  # an infinity times a weight of 0 is NaN
-    assert torch.equal(got[1].isnan(), ref.sum(1).isnan())
+    if dtype == BF:
+        assert got[1].isnan().all()
+    else:  # an infinity times a weight of 0 is NaN
+        want = (x[1].double() * _dense(codes, scales, None, 128)).sum(1)
+        assert torch.equal(torch.nan_to_num(got[1].double()), torch.nan_to_num(want.float().double()))
 
 
 @pytest.mark.parametrize("N,K,group,zeros,sdt,dtype", [
@@ -165,7 +180,7 @@ def test_quantize_and_dequantize(dev, N, K, group, zeros, sdt, dtype):
     assert torch.equal(again.packed, q.packed)
     assert torch.equal(again.dequantize(BF), q.dequantize(F32).to(BF))
     x = torch.randn(3, K, generator=_gen(9)).to(dtype)
-    _check_linear(hm.linear_4bit(x.to(dev), q), x, d, None, None)
+    _check_linear(hm.linear_4bit(x.to(dev), q), x, codes, s, z if zeros else None, group, None, None)
 
 
 def test_weight_refusals(dev):
