@@ -53,9 +53,10 @@ def _compile_native() -> str:
 
     from torch.utils import cpp_extension
 
-    inc = [str(PKG.parent / "include"), *cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    rocm = Path(_hipcc()).resolve().parent.parent / "include"
+    inc = [str(PKG.parent / "include"), *cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(rocm)]
     return _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-DTORCH_EXTENSION_NAME=_native",
-                 "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{p}" for p in inc], "-c", str(CSRC / "native.cpp"), "-o",
+                 "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1", *[f"-I{p}" for p in inc], "-c", str(CSRC / "native.cpp"), "-o",
                  str(BUILD / "native.o")])
 
 
@@ -65,7 +66,7 @@ def _link_native() -> None:
     lib = str(Path(torch.__file__).parent / "lib")
     tmp = NATIVE.with_suffix(".so.tmp")
     _run(["g++", "-shared", str(BUILD / "native.o"), "-o", str(tmp), f"-L{PKG}", "-l:libhdcmamba_hip.so", f"-L{lib}",
-          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"])
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"])
     os.replace(tmp, NATIVE)
 
 

@@ -5,6 +5,7 @@
 // about 190 us of Python per block, more than the kernels take below ~8192 rows.  Nothing is kept
 // between calls: workspaces that outlive a call are passed in.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -589,6 +590,9 @@ const Tensor& or_none(const OptTensor& t) {
 }
 const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
+// torch's current stream on t's device (asked here: a call through Python costs 1.8 us)
+void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
 void same_device(const Tensor& t, const Tensor& ref, const char* name) {
   TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
 }
@@ -620,38 +624,37 @@ bool same_place(const Tensor& a, const Tensor& b) {
   return a.const_data_ptr() == b.const_data_ptr() && (a.size(0) <= 1 || a.stride(0) == b.stride(0));
 }
 
-using WeightArgs = std::tuple<Tensor, Tensor, OptTensor, int64_t, int64_t, int64_t>;  // packed, scales, zeros, N, K, group
+// A packed weight, checked once (the handle of a Weight4Bit)
 struct Weight4 {
   Tensor packed, scales, zeros;
   int64_t N, K, group;
+  int scale_dtype;
 };
-Weight4 weight4_of(const WeightArgs& a) {
-  Weight4 w{std::get<0>(a), std::get<1>(a), or_none(std::get<2>(a)), std::get<3>(a), std::get<4>(a), std::get<5>(a)};
-  TORCH_CHECK(w.N > 0 && w.K > 0 && (w.group == 32 || w.group == 64 || w.group == 128), "a 4-bit weight [", w.N, ", ", w.K,
-              "] in groups of ", w.group);
-  const int64_t per = (w.K + 127) / 128 * 128 / w.group * ((w.N + 15) / 16 * 16);
-  on_gpu(w.packed);
-  same_device(w.scales, w.packed, "scales");
-  TORCH_CHECK(w.packed.scalar_type() == at::kByte && w.packed.is_contiguous() &&
-                  (size_t)w.packed.numel() == hdcm_w4_packed_bytes(w.N, w.K) && w.scales.is_contiguous() &&
-                  w.scales.numel() == per,
-              "the packed weight's buffers do not hold [", w.N, ", ", w.K, "] in groups of ", w.group);
+Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor& zeros, int64_t N, int64_t K, int64_t group) {
+  on_gpu(packed);
+  Weight4 w{packed, scales, or_none(zeros), N, K, group, dtype_of(scales)};
+  TORCH_CHECK(N > 0 && K > 0 && (group == 32 || group == 64 || group == 128), "a 4-bit weight [", N, ", ", K, "] in groups of ",
+              group);
+  const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
+  same_device(scales, packed, "scales");
+  TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() &&
+                  (size_t)packed.numel() == hdcm_w4_packed_bytes(N, K) && scales.is_contiguous() && scales.numel() == per,
+              "the packed weight's buffers do not hold [", N, ", ", K, "] in groups of ", group);
   if (w.zeros.defined()) {
-    same_device(w.zeros, w.packed, "zeros");
+    same_device(w.zeros, packed, "zeros");
     TORCH_CHECK(w.zeros.scalar_type() == at::kByte && w.zeros.is_contiguous() && w.zeros.numel() == per,
                 "zeros must hold one byte per scale");
   }
   return w;
 }
 
-Tensor linear_4bit(const Tensor& x, const WeightArgs& weight, const OptTensor& bias_, const OptTensor& residual_,
-                   const OptTensor& out_, int64_t stream) {
+Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, const OptTensor& residual_,
+                   const OptTensor& out_) {
   const Tensor &bias = or_none(bias_), &residual = or_none(residual_), &given = or_none(out_);
   on_gpu(x);
   no_gradient("linear_4bit", {&x, &bias, &residual, &given});
   Entry entry;
   const c10::DeviceGuard guard(x.device());
-  const Weight4 w = weight4_of(weight);
   const int dt = dtype_of(x);
   same_device(w.packed, x, "the weight");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) == w.K, "linear_4bit: x ", x.sizes(), " does not end in the weight's ", w.K, " columns");
@@ -688,9 +691,9 @@ Tensor linear_4bit(const Tensor& x, const WeightArgs& weight, const OptTensor& b
   }
   check("hdcm_w4_linear_fwd",
         hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), w.packed.const_data_ptr(), w.scales.const_data_ptr(),
-                           dtype_of(w.scales), (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
+                           w.scale_dtype, (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
                            r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, K, dt,
-                           (void*)stream));
+                           stream_of(x)));
   return out;
 }
 
@@ -762,7 +765,7 @@ void logits_shape(const Tensor& logits, const char* op) {
   TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, op, ": logits must be [sequences, vocabulary], got ", logits.sizes());
 }
 
-Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTensor& out_, int64_t stream) {
+Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTensor& out_) {
   logits_shape(logits, "process_logits");
   no_gradient("process_logits", {&logits, &or_none(std::get<4>(args)), &or_none(out_)});
   Entry entry;
@@ -785,12 +788,12 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
   }
   check("hdcm_logits_process",
         hdcm_logits_process(l.const_data_ptr(), l.stride(0), &k.c, out.mutable_data_ptr(), out.stride(0), l.size(0), l.size(1), dt,
-                            (void*)stream));
+                            stream_of(l)));
   return out;
 }
 
 std::tuple<Tensor, Tensor> select_tokens(const Tensor& logits, const ControlArgs& args, const Penalty& temperature,
-                                         const OptTensor& noise_, int64_t stream) {
+                                         const OptTensor& noise_) {
   logits_shape(logits, "select_tokens");
   no_gradient("select_tokens", {&logits, &or_none(std::get<4>(args)), &or_none(noise_)});
   Entry entry;
@@ -813,7 +816,7 @@ std::tuple<Tensor, Tensor> select_tokens(const Tensor& logits, const ControlArgs
   check("hdcm_token_select",
         hdcm_token_select(l.const_data_ptr(), l.stride(0), &k.c, temp, temp_all, (const float*)pointer(noise),
                           noise.defined() ? noise.stride(0) : 0, tokens.mutable_data_ptr<int64_t>(),
-                          logprobs.mutable_data_ptr<float>(), n ? ws.mutable_data_ptr() : nullptr, n, B, V, dt, (void*)stream));
+                          logprobs.mutable_data_ptr<float>(), n ? ws.mutable_data_ptr() : nullptr, n, B, V, dt, stream_of(l)));
   return {tokens, logprobs};
 }
 
@@ -849,25 +852,25 @@ Ids ids_of(const OptTensor& ids, const OptTensor& lengths, const Tensor& table, 
 }
 
 Tensor fill_token_history(Tensor table, const OptTensor& prompt, const OptTensor& prompt_lengths, const OptTensor& output,
-                          const OptTensor& output_lengths, int64_t stream) {
+                          const OptTensor& output_lengths) {
   Entry entry;
   table_shape(table, "fill_token_history");
   const c10::DeviceGuard guard(table.device());
   const Ids p = ids_of(prompt, prompt_lengths, table, "prompt"), o = ids_of(output, output_lengths, table, "output");
   check("hdcm_token_history_fill",
         hdcm_token_history_fill(table.mutable_data_ptr<int16_t>(), table.stride(0), p.p, p.stride, p.n, p.width, o.p, o.stride,
-                                o.n, o.width, table.size(0), table.size(1), (void*)stream));
+                                o.n, o.width, table.size(0), table.size(1), stream_of(table)));
   return table;
 }
 
-Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& lengths, int64_t stream) {
+Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& lengths) {
   Entry entry;
   table_shape(table, "append_tokens");
   const c10::DeviceGuard guard(table.device());
   const Ids t = ids_of(tokens.dim() == 1 ? tokens.unsqueeze(1) : tokens, lengths, table, "tokens");
   check("hdcm_token_history_append",
         hdcm_token_history_append(table.mutable_data_ptr<int16_t>(), table.stride(0), t.p, t.stride, t.n, t.width, table.size(0),
-                                  table.size(1), (void*)stream));
+                                  table.size(1), stream_of(table)));
   return table;
 }
 
@@ -894,6 +897,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mixer_backward", &mixer_backward);
   m.def("norm_conv_forward", &norm_conv_forward);
   m.def("norm_conv_backward", &norm_conv_backward);
+  pybind11::class_<Weight4>(m, "Weight4").def(pybind11::init(&make_weight4));
   m.def("linear_4bit", &linear_4bit);
   m.def("process_logits", &process_logits);
   m.def("select_tokens", &select_tokens);

@@ -24,12 +24,15 @@ class Weight4Bit:
     ``shape`` (N, K), ``group_size``; ``packed`` uint8, ``scales`` (float32 or bfloat16) and ``zeros``
     (uint8 or None) in the layout of hdcm_w4_linear_fwd (include/hdcm.h)."""
 
-    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "_args")
+    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "_handle")
 
     def __init__(self, packed, scales, zeros, shape, group_size):
         self.packed, self.scales, self.zeros = packed, scales, zeros
         self.shape, self.group_size = tuple(int(n) for n in shape), int(group_size)
-        self._args = (packed, scales, zeros, *self.shape, self.group_size)
+        self._handle = _ops.native().Weight4(packed, scales, zeros, *self.shape, self.group_size)
+
+    def __reduce__(self):  # copies and pickles are made from the buffers
+        return Weight4Bit, (self.packed, self.scales, self.zeros, self.shape, self.group_size)
 
     @staticmethod
     def _groups(N, K, group_size):
@@ -130,5 +133,4 @@ def linear_4bit(x, weight, bias=None, residual=None, out=None):
     x's type (float32 or bfloat16): fp32 sums of exact code products, the scales applied to the groups'
     sums, one rounding.  ``out`` may be ``residual``.  No gradient: refused where one would be
     recorded."""
-    _ops._on_gpu(x)
-    return _ops.native().linear_4bit(x, weight._args, bias, residual, out, _ops._stream(x))
+    return _ops.native().linear_4bit(x, weight._handle, bias, residual, out)

@@ -28,9 +28,7 @@ __all__ = ["process_logits", "select_tokens", "new_token_history", "fill_token_h
 def process_logits(logits, history=None, repetition=None, frequency=None, presence=None, bias=None, mask=None, out=None):
     """logits [B, V] (float32 or bfloat16) under the controls, rounded once to their type; ``out`` may be
     ``logits``.  No gradient."""
-    _ops._on_gpu(logits)
-    return _ops.native().process_logits(logits, (history, repetition, frequency, presence, bias, mask), out,
-                                        _ops._stream(logits))
+    return _ops.native().process_logits(logits, (history, repetition, frequency, presence, bias, mask), out)
 
 
 def select_tokens(logits, history=None, repetition=None, frequency=None, presence=None, bias=None, mask=None,
@@ -44,9 +42,7 @@ def select_tokens(logits, history=None, repetition=None, frequency=None, presenc
     number or one per sequence (1 by default); one that is not above 0 makes a greedy choice, without
     noise, from t = processed.  -inf and NaN are never chosen: a sequence with nothing else gets token -1
     and -inf.  A NaN or +inf among the allowed logits makes the log-probability NaN.  No gradient."""
-    _ops._on_gpu(logits)
-    return _ops.native().select_tokens(logits, (history, repetition, frequency, presence, bias, mask), temperature, noise,
-                                       _ops._stream(logits))
+    return _ops.native().select_tokens(logits, (history, repetition, frequency, presence, bias, mask), temperature, noise)
 
 
 def new_token_history(batch, vocab, device="cuda"):
@@ -58,12 +54,10 @@ def fill_token_history(table, prompt=None, prompt_lengths=None, output=None, out
     """Write all of ``table`` [B, V] from the token ids of prompts [B, P] and outputs [B, O]; ``*_lengths``
     [B]: how many of a row's ids count (right-padded batches).  Ids outside 0..V-1 are passed over.
     Returns the table."""
-    _ops._on_gpu(table)
-    return _ops.native().fill_token_history(table, prompt, prompt_lengths, output, output_lengths, _ops._stream(table))
+    return _ops.native().fill_token_history(table, prompt, prompt_lengths, output, output_lengths)
 
 
 def append_tokens(table, tokens, lengths=None):
     """Count output tokens [B] or [B, T] (``lengths`` [B]: how many of a row) in ``table``, in place; ids
     outside 0..V-1 (a token -1 of select_tokens) are passed over.  Returns the table."""
-    _ops._on_gpu(table)
-    return _ops.native().append_tokens(table, tokens, lengths, _ops._stream(table))
+    return _ops.native().append_tokens(table, tokens, lengths)

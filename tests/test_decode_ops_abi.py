@@ -137,7 +137,6 @@ def test_token_history_validation():
 @pytest.mark.parametrize("call", [
     lambda: hm.Weight4Bit.quantize(torch.zeros(16, 128)),
     lambda: hm.Weight4Bit.from_codes(torch.zeros(16, 128, dtype=torch.uint8), torch.ones(16, 1)),
-    lambda: hm.linear_4bit(torch.zeros(1, 128), None),
     lambda: hm.process_logits(torch.zeros(1, 8)),
     lambda: hm.select_tokens(torch.zeros(1, 8)),
     lambda: hm.fill_token_history(torch.zeros(1, 8, dtype=torch.int16)),

@@ -4,6 +4,9 @@ Products: every output within the rounding of its type plus what fp32 sums of ex
 fp32 rows sum K products x (c - z), bf16 rows the 2 K products x (16 + c) and -x (16 + z): a step of
 2^-23 per addition (covers an accumulator that truncates) of the sum of their magnitudes.  Processed logits: bit for bit the fp32 formula, operation by operation.
 """
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -209,7 +212,13 @@ def test_weight_refusals(dev):
     with pytest.raises(TypeError):
         hm.Weight4Bit.quantize(bad.half())
     w = make(codes, scales, z, 64)
+    with pytest.raises(RuntimeError, match="do not hold"):
+        hm.Weight4Bit(w.packed, w.scales, w.zeros, (33, 128), 64)
     x = torch.randn(4, 128, device=dev, dtype=BF)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w)), w.to(dev)):
+        assert torch.equal(hm.linear_4bit(x, other), hm.linear_4bit(x, w)) and "32x128" in repr(other)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        hm.linear_4bit(x.cpu(), w)
     with pytest.raises(RuntimeError, match="128 columns"):
         hm.linear_4bit(x[:, :64], w)
     with pytest.raises(TypeError):
