@@ -17,33 +17,43 @@ namespace {
 constexpr float kInf = __builtin_inff();
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// Eight values of a row from column v on at the type's own alignment (rows of an odd vocabulary start
-// anywhere); `pad` past the row's V columns.
-template <typename T> __device__ __forceinline__ void load8(const T* row, int v, int V, float pad, float* z);
-template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* row, int v, int V, float pad, float* z) {
-  typedef u32x4_t run_t __attribute__((aligned(2)));
-  if (v + 8 <= V) {
-    const u32x4_t a = *reinterpret_cast<const run_t*>(row + v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      z[2 * e] = __uint_as_float(a[e] << 16);
-      z[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u);
-    }
+// Eight consecutive values of a row as they lie in memory, at the type's own alignment (rows of an odd
+// vocabulary start anywhere).
+template <typename T> struct Run {
+  u32x4_t v[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ Run<T> load_run(const T* p) {
+  typedef u32x4_t run2_t __attribute__((aligned(2)));
+  typedef u32x4_t run4_t __attribute__((aligned(4)));
+  Run<T> r;
+  if constexpr (sizeof(T) == 2) {
+    r.v[0] = *reinterpret_cast<const run2_t*>(p);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = v + e < V ? bf2f(row[v + e]) : pad;
+    r.v[0] = *reinterpret_cast<const run4_t*>(p);
+    r.v[1] = *reinterpret_cast<const run4_t*>(p + 4);
   }
+  return r;
 }
-template <> __device__ __forceinline__ void load8<float>(const float* row, int v, int V, float pad, float* z) {
-  typedef u32x4_t run_t __attribute__((aligned(4)));
-  if (v + 8 <= V) {
-    const u32x4_t a = *reinterpret_cast<const run_t*>(row + v), b = *reinterpret_cast<const run_t*>(row + v + 4);
+// The end of a row: n < 8 values, zero bits behind them.
+template <typename T> __device__ __forceinline__ Run<T> load_end(const T* p, int n) {
+  Run<T> r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = __uint_as_float(a[e]), z[4 + e] = __uint_as_float(b[e]);
-  } else {
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = u32x4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = v + e < V ? row[v + e] : pad;
-  }
+  for (int e = 0; e < 8; ++e)
+    if (e < n) {
+      if constexpr (sizeof(T) == 2) r.v[0][e / 2] |= (uint32_t)(uint16_t)p[e] << (16 * (e & 1));
+      else r.v[e / 4][e & 3] = __float_as_uint(p[e]);
+    }
+  return r;
+}
+__device__ __forceinline__ void values(const Run<bf16_t>& r, float* z) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[2 * e] = __uint_as_float(r.v[0][e] << 16), z[2 * e + 1] = __uint_as_float(r.v[0][e] & 0xffff0000u);
+}
+__device__ __forceinline__ void values(const Run<float>& r, float* z) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = __uint_as_float(r.v[0][e]), z[4 + e] = __uint_as_float(r.v[1][e]);
 }
 template <typename T> __device__ __forceinline__ void store8(T* row, int v, int V, const float* z);
 template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* row, int v, int V, const float* z) {
@@ -96,44 +106,57 @@ __device__ __forceinline__ RowControls row_controls(const hdcm_logits_controls& 
   return o;
 }
 
-// z of eight logits from column v (a multiple of 8) on; columns past V become -inf.
-template <typename T>
-__device__ __forceinline__ void process8(const T* row, const RowControls& c, int v, int V, float* z) {
-#pragma clang fp contract(off)
-  load8<T>(row, v, V, -kInf, z);
-  if (c.history) {
-    typedef u32x4_t run_t __attribute__((aligned(2)));
-    u32x4_t h = {0, 0, 0, 0};
-    if (v + 8 <= V) {
-      h = *reinterpret_cast<const run_t*>(c.history + v);
+// Eight logits from column v (a multiple of 8) on and what their controls hold: all loads first, converted
+// only in z(), so that none waits for another.
+template <typename T> struct Eight {
+  Run<T> l;
+  Run<int16_t> h;
+  Run<bf16_t> b16;
+  Run<float> b32, noise;
+  uint32_t mask;
+  int n;  // columns inside the row
+  __device__ __forceinline__ void load(const T* row, const RowControls& c, const float* nrow, int v, int V) {
+    n = min(8, V - v);
+    if (n == 8) {
+      l = load_run(row + v);
+      if (c.history) h = load_run(c.history + v);
+      if (c.bias && c.bias_f32) b32 = load_run((const float*)c.bias + v);
+      if (c.bias && !c.bias_f32) b16 = load_run((const bf16_t*)c.bias + v);
+      if (nrow) noise = load_run(nrow + v);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v + e < V) h[e / 2] |= (uint32_t)(uint16_t)c.history[v + e] << (16 * (e & 1));
+      l = load_end(row + v, n);
+      if (c.history) h = load_end(c.history + v, n);
+      if (c.bias && c.bias_f32) b32 = load_end((const float*)c.bias + v, n);
+      if (c.bias && !c.bias_f32) b16 = load_end((const bf16_t*)c.bias + v, n);
+      if (nrow) noise = load_end(nrow + v, n);
     }
-    if (h[0] | h[1] | h[2] | h[3]) {  // most tokens were never seen
+    if (c.mask) mask = c.mask[v / 8];  // bit v % 32 of word v / 32, little endian
+  }
+  // the processed logits; -inf behind the row's end
+  __device__ __forceinline__ void z(const RowControls& c, float* z) const {
+#pragma clang fp contract(off)
+    values(l, z);
+    if (c.history && (h.v[0][0] | h.v[0][1] | h.v[0][2] | h.v[0][3])) {  // most tokens were never seen
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t t = (h[e / 2] >> (16 * (e & 1))) & 0xffffu, count = t & 0x7fffu;
+        const uint32_t t = (h.v[0][e / 2] >> (16 * (e & 1))) & 0xffffu, count = t & 0x7fffu;
         if (t) z[e] = z[e] > 0.f ? z[e] / c.r : z[e] * c.r;
         z[e] = z[e] - c.f * (float)count;
         z[e] = z[e] - (count ? c.p : 0.f);
       }
     }
-  }
-  if (c.bias) {
-    float b[8];
-    if (c.bias_f32) load8<float>((const float*)c.bias, v, V, 0.f, b);
-    else load8<bf16_t>((const bf16_t*)c.bias, v, V, 0.f, b);
+    if (c.bias) {
+      float b[8];
+      if (c.bias_f32) values(b32, b);
+      else values(b16, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = z[e] + b[e];
-  }
-  if (c.mask) {
-    const uint32_t m = c.mask[v / 8];  // bit v % 32 of word v / 32, little endian
+      for (int e = 0; e < 8; ++e) z[e] = z[e] + b[e];
+    }
+    const uint32_t allowed = (c.mask ? mask : 0xffu) & (n < 8 ? (1u << n) - 1 : 0xffu);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = (m >> e) & 1 ? z[e] : -kInf;
+    for (int e = 0; e < 8; ++e) z[e] = (allowed >> e) & 1 ? z[e] : -kInf;
   }
-}
+};
 
 constexpr int kProcThreads = 256;
 
@@ -144,8 +167,10 @@ __global__ __launch_bounds__(kProcThreads) void logits_process_kernel(const T* l
   if (v >= V) return;
   for (int64_t b = blockIdx.y; b < B; b += gridDim.y) {
     const RowControls c = row_controls(ctl, b);
+    Eight<T> x;
+    x.load(logits + b * l_rs, c, nullptr, v, V);
     float z[8];
-    process8<T>(logits + b * l_rs, c, v, V, z);
+    x.z(c, z);
     store8<T>(out + b * o_rs, v, V, z);
   }
 }
@@ -156,25 +181,39 @@ struct Pick {
   float best, t, max, sum;
   int at;
 };
-__device__ __forceinline__ Pick no_pick() { return {-kInf, -kInf, -kInf, 0.f, 0x7fffffff}; }
-__device__ __forceinline__ void merge(Pick& a, const Pick& b) {
-  if (b.best > a.best || (b.best == a.best && b.at < a.at)) a.best = b.best, a.at = b.at, a.t = b.t;
-  const float m = fmaxf(a.max, b.max), ref = m == -kInf ? 0.f : m;
-  a.sum = a.sum * fexp(a.max - ref) + b.sum * fexp(b.max - ref);
-  a.max = m;
+constexpr int kNoToken = 0x7fffffff;
+__device__ __forceinline__ Pick no_pick() { return {-kInf, -kInf, -kInf, 0.f, kNoToken}; }
+
+// Maximum and minimum over the 64 lanes on DPP lane moves (the steps of wave_total; a lane without a
+// source keeps its own value), read into a wave-uniform scalar.
+__device__ __forceinline__ float wave_max(float v) {
+#define HDCM_STEP(CTRL, ROWS)                                                                                         \
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)));
+  HDCM_STEP(0xB1, 0xf) HDCM_STEP(0x4E, 0xf) HDCM_STEP(0x141, 0xf) HDCM_STEP(0x140, 0xf) HDCM_STEP(0x142, 0xa) HDCM_STEP(0x143, 0xc)
+#undef HDCM_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
-__device__ __forceinline__ Pick merge_lanes(Pick a) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const Pick b = {__shfl_xor(a.best, o, kWave), __shfl_xor(a.t, o, kWave), __shfl_xor(a.max, o, kWave),
-                    __shfl_xor(a.sum, o, kWave), __shfl_xor(a.at, o, kWave)};
-    merge(a, b);
-  }
-  return a;
+__device__ __forceinline__ int wave_min(int v) {
+#define HDCM_STEP(CTRL, ROWS) v = min(v, __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xf, false));
+  HDCM_STEP(0xB1, 0xf) HDCM_STEP(0x4E, 0xf) HDCM_STEP(0x141, 0xf) HDCM_STEP(0x140, 0xf) HDCM_STEP(0x142, 0xa) HDCM_STEP(0x143, 0xc)
+#undef HDCM_STEP
+  return __builtin_amdgcn_readlane(v, 63);
+}
+// The lanes' picks as one (in every lane): ties of `best` go to the lowest index.
+__device__ __forceinline__ Pick merge_lanes(const Pick& a) {
+  Pick o;
+  o.max = wave_max(a.max);
+  const float ref = o.max == -kInf ? 0.f : o.max;
+  o.sum = wave_total(a.sum * fexp(a.max - ref));
+  o.best = wave_max(a.best);
+  o.at = wave_min(a.best == o.best ? a.at : kNoToken);
+  const uint64_t owner = __ballot(a.best == o.best && a.at == o.at);  // one lane, or (no token) all
+  o.t = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a.t), owner ? __builtin_ctzll(owner) : 0));
+  return o;
 }
 __device__ __forceinline__ void write_pick(const Pick& a, int64_t* token, float* logprob) {
   // nothing allowed (or only NaN): no token
-  const bool none = a.at == 0x7fffffff;
+  const bool none = a.at == kNoToken;
   *token = none ? -1 : a.at;
   *logprob = none ? -kInf : a.t - (a.max + logf(a.sum));
 }
@@ -182,7 +221,9 @@ __device__ __forceinline__ void write_pick(const Pick& a, int64_t* token, float*
 constexpr int kPickThreads = 512;
 constexpr int kPickWaves = kPickThreads / kWave;
 
-// Workgroup (s, b) takes part s of gridDim.x of row b, in whole groups of eight columns.
+// Workgroup (s, b) takes part s of gridDim.x of row b, in whole groups of eight columns.  One pass: the
+// eight values' maximum moves the running one, and only a maximum above the best so far is looked
+// up.
 template <typename T>
 __global__ __launch_bounds__(kPickThreads) void token_select_kernel(const T* logits, int64_t l_rs, hdcm_logits_controls ctl,
                                                                     const float* temperature, float temperature_all,
@@ -199,82 +240,125 @@ __global__ __launch_bounds__(kPickThreads) void token_select_kernel(const T* log
   const int v0 = blockIdx.x * part, v1 = min(v0 + part, V);
   Pick a = no_pick();
   for (int v = v0 + 8 * threadIdx.x; v < v1; v += 8 * kPickThreads) {
+    Eight<T> x;
+    x.load(row, c, nrow, v, V);
     float t[8], n[8];
-    process8<T>(row, c, v, V, t);
+    x.z(c, t);
     if (!greedy && temp != 1.f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] = t[e] / temp;
     }
-    if (nrow) load8<float>(nrow, v, V, 0.f, n);
-    float m = a.max;
+    const float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+    float best = top;
+    if (nrow) {
+      values(x.noise, n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = nrow ? t[e] + n[e] : t[e];
-      // a thread's columns ascend, so a tie keeps the lower one; -inf and NaN are no candidates
-      if (x > a.best) a.best = x, a.at = v + e, a.t = t[e];
-      m = fmaxf(m, t[e]);
+      for (int e = 0; e < 8; ++e) n[e] = t[e] + n[e];
+      best = fmaxf(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])), fmaxf(fmaxf(n[4], n[5]), fmaxf(n[6], n[7])));
     }
-    const float ref = m == -kInf ? 0.f : m;
+    if (best > a.best) {  // a thread's columns ascend, so a tie keeps the lower one; -inf and NaN are no candidates
+      a.best = best;
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if ((nrow ? n[e] : t[e]) == best) a.at = v + e, a.t = t[e];
+    }
+    const float m = fmaxf(a.max, top), ref = m == -kInf ? 0.f : m;
     float s = a.sum * fexp(a.max - ref);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += fexp(t[e] - ref);
     a.sum = s, a.max = m;
   }
   a = merge_lanes(a);
-  if (threadIdx.x % kWave == 0) picks[threadIdx.x / kWave] = a;
+  const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  if (lane == 0) picks[w] = a;
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < kPickWaves; ++w) merge(a, picks[w]);
+  if (w != 0) return;
+  a = merge_lanes(lane < kPickWaves ? picks[lane] : no_pick());
+  if (lane != 0) return;
   if (gridDim.x == 1) write_pick(a, tokens + b, logprobs + b);
   else ws[b * gridDim.x + blockIdx.x] = a;
 }
 
-// The parts of a row in order, one wave per row.
+// The parts of a row, at most a wave's lanes.
 __global__ __launch_bounds__(kWave) void token_select_join_kernel(const Pick* ws, int parts, int64_t* tokens, float* logprobs) {
   const int64_t b = blockIdx.x;
-  Pick a = no_pick();
-  for (int s = threadIdx.x; s < parts; s += kWave) merge(a, ws[b * parts + s]);
-  a = merge_lanes(a);
+  const Pick a = merge_lanes((int)threadIdx.x < parts ? ws[b * parts + threadIdx.x] : no_pick());
   if (threadIdx.x == 0) write_pick(a, tokens + b, logprobs + b);
 }
 
+// Parts of a row: enough workgroups for the CUs, each with a full pass of its threads at least.
 int select_parts(int64_t B, int64_t V) {
-  const int64_t most = (V + 8191) / 8192;
-  return B >= 256 ? 1 : (int)most;
+  const int64_t full = (V + 8 * kPickThreads - 1) / (8 * kPickThreads), want = (1024 + B - 1) / B;
+  const int64_t n = full < want ? full : want;
+  return (int)(n < kWave ? n : kWave);
 }
 
 // ------------------------------------------------------------------ token history
-constexpr int kHistThreads = 256;
-constexpr int kHistSlice = 4096;  // tokens of a row per workgroup
+constexpr int kHistThreads = 512;
+constexpr int kHistSlice = 8 * kHistThreads;  // tokens of a row per workgroup
 
-// Workgroup (s, b) counts slice s of row b in LDS from all of the row's ids, then writes the slice: no
-// atomics on the table, every entry written once.  keep: on top of what the table holds.
+// Calls f with the ids[0..n) that lie in [v0, v0 + size), less v0; eight loads of a thread in flight.
+template <typename F>
+__device__ __forceinline__ void each_id(const int64_t* ids, int64_t n, int v0, int size, F f) {
+  constexpr int U = 8;
+  for (int64_t i0 = 0; i0 < n; i0 += U * kHistThreads) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * kHistThreads + threadIdx.x;
+      id[u] = ids[i < n ? i : n - 1];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t at = (uint64_t)(id[u] - v0);
+      if (i0 + u * kHistThreads + threadIdx.x < n && at < (uint64_t)size) f((int)at);
+    }
+  }
+}
+
+// Workgroup (s, b) counts slice s of row b in LDS from all of the row's ids, then writes the slice, eight
+// entries a thread: no atomics on the table, every entry written once.  keep: on top of what the
+// table holds.
 __global__ __launch_bounds__(kHistThreads) void token_history_kernel(int16_t* table, int64_t rs, const int64_t* prompt,
                                                                      int64_t p_rs, const int64_t* p_len, int64_t P,
                                                                      const int64_t* output, int64_t o_rs,
                                                                      const int64_t* o_len, int64_t O, int V, bool keep) {
-  __shared__ uint32_t cell[kHistSlice];  // bit 31: in the prompt; below: the count
+  typedef u32x4_t run_t __attribute__((aligned(2)));
+  __shared__ __attribute__((aligned(16))) uint32_t cell[kHistSlice];  // bit 31: in the prompt; below: the count
   const int64_t b = blockIdx.y;
-  const int v0 = blockIdx.x * kHistSlice, n = min(kHistSlice, V - v0);
+  const int v0 = blockIdx.x * kHistSlice, n = min(kHistSlice, V - v0), i0 = 8 * threadIdx.x;
   int16_t* row = table + b * rs + v0;
-  for (int i = threadIdx.x; i < n; i += kHistThreads) {
-    const uint32_t h = keep ? (uint16_t)row[i] : 0u;
-    cell[i] = (h & 0x7fffu) | (h >> 15) << 31;
+  uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (keep) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t t = i0 + e < n ? (uint16_t)row[i0 + e] : 0u;
+      h[e] = (t & 0x7fffu) | (t >> 15) << 31;
+    }
   }
+  u32x4_t* mine = reinterpret_cast<u32x4_t*>(cell + i0);
+  mine[0] = u32x4_t{h[0], h[1], h[2], h[3]};
+  mine[1] = u32x4_t{h[4], h[5], h[6], h[7]};
   __syncthreads();
   const int64_t np = p_len ? min(max(p_len[b], (int64_t)0), P) : P, no = o_len ? min(max(o_len[b], (int64_t)0), O) : O;
-  for (int64_t i = threadIdx.x; i < np; i += kHistThreads) {
-    const uint64_t at = (uint64_t)(prompt[b * p_rs + i] - v0);
-    if (at < (uint64_t)n) atomicOr(&cell[at], 0x80000000u);
-  }
-  for (int64_t i = threadIdx.x; i < no; i += kHistThreads) {
-    const uint64_t at = (uint64_t)(output[b * o_rs + i] - v0);
-    if (at < (uint64_t)n) atomicAdd(&cell[at], 1u);
-  }
+  each_id(prompt + b * p_rs, np, v0, n, [&](int at) { atomicOr(&cell[at], 0x80000000u); });
+  each_id(output + b * o_rs, no, v0, n, [&](int at) { atomicAdd(&cell[at], 1u); });
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kHistThreads) {
-    const uint32_t h = cell[i];
-    row[i] = (int16_t)(min(h & 0x7fffffffu, 0x7fffu) | (h >> 31) << 15);
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4_t c = mine[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[4 * i + e] = min(c[e] & 0x7fffffffu, 0x7fffu) | (c[e] >> 31) << 15;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = h[2 * e] | h[2 * e + 1] << 16;
+  if (i0 + 8 <= n) {
+    *reinterpret_cast<run_t*>(row + i0) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i0 + e < n) row[i0 + e] = (int16_t)h[e];
   }
 }
 
