@@ -8,12 +8,13 @@ from .model import (
     HdcMamba9v3Block,
     HdcMamba9v3Model,
     fused_norm_conv1d_trainable,
+    quantize_4bit,
     set_differentiable_mixer,
     set_fused_out_proj,
     set_fused_step_front,
 )
 from .lm import DecodeGraph, ForwardGraph, HdcMambaLM
-from .quant4 import Weight4Bit, linear_4bit
+from .quant4 import Linear4Bit, Weight4Bit, linear_4bit
 from .sampling import append_tokens, fill_token_history, new_token_history, process_logits, select_tokens
 
 __all__ = [
@@ -29,6 +30,8 @@ __all__ = [
     "set_fused_out_proj",
     "set_fused_step_front",
     "Weight4Bit",
+    "Linear4Bit",
+    "quantize_4bit",
     "linear_4bit",
     "process_logits",
     "select_tokens",

@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from . import _ops
 from .model import BlockState, HdcMamba9v3Model, layer_norm
+from .sampling import append_tokens, fill_token_history, new_token_history, select_tokens
 
 __all__ = ["HdcMambaLM", "DecodeGraph", "ForwardGraph", "SIZES"]
 
@@ -87,9 +88,52 @@ class HdcMambaLM(nn.Module):
             x = self.embedding.weight[input_ids]
             return self.lm_head(self.backbone.step(x, states, pos_dev, then=self.norm_f))
 
-    def capture_decode(self, states):
-        """A DecodeGraph stepping ``states`` (as returned by prefill) from replays."""
-        return DecodeGraph(self, states)
+    def capture_decode(self, states, controls=None):
+        """A DecodeGraph stepping ``states`` (as returned by prefill) from replays; with ``controls`` (the
+        keyword arguments of select_tokens) it also chooses each next token."""
+        return DecodeGraph(self, states, controls)
+
+    def generate(self, input_ids, max_new_tokens, temperature=0.0, repetition=None, frequency=None, presence=None, bias=None,
+                 mask=None, generator=None):
+        """Continue input_ids [B,L] by max_new_tokens tokens: (tokens [B,n], their log-probabilities [B,n]).
+
+        A prefill, then one replay of a recorded decode step per token, the choice (select_tokens, whose
+        controls these are) and the token history included, so that nothing waits for the host.
+        ``temperature`` (a number, or one per sequence) above 0 samples, with ``generator`` (a GPU
+        torch.Generator) or the default one; 0 is greedy.  The reference's generate re-runs the whole
+        forward for every token (train.py:139-151)."""
+        _ops._on_gpu(input_ids)
+        B, n = input_ids.shape[0], int(max_new_tokens)
+        dev = input_ids.device
+        with torch.no_grad():
+            tokens = torch.empty(B, n, dtype=torch.long, device=dev)
+            logprobs = torch.empty(B, n, dtype=torch.float32, device=dev)
+            if n < 1 or B == 0:
+                return tokens, logprobs
+            last, states = self.prefill(input_ids)
+            logits = last[:, -1]
+            controls = dict(repetition=repetition, frequency=frequency, presence=presence, bias=bias, mask=mask,
+                            temperature=temperature)
+            if any(p is not None for p in (repetition, frequency, presence)):
+                controls["history"] = fill_token_history(new_token_history(B, logits.shape[1], dev), input_ids)
+            if isinstance(temperature, torch.Tensor) or temperature > 0:
+                controls["noise"] = torch.empty(logits.shape, dtype=torch.float32, device=dev)
+
+            def draw():  # the negative logarithm of an exponential variate has the Gumbel distribution
+                if "noise" in controls:
+                    controls["noise"].exponential_(generator=generator).log_().neg_()
+
+            draw()
+            tokens[:, 0], logprobs[:, 0] = token, _ = select_tokens(logits, **controls)
+            if "history" in controls:
+                append_tokens(controls["history"], token)
+            if n > 1:
+                graph = self.capture_decode(states, controls)
+                graph.ids.copy_(token)
+                for i in range(1, n):
+                    draw()
+                    tokens[:, i], logprobs[:, i] = graph.next()
+            return tokens, logprobs
 
     def capture_forward(self, input_ids):
         """A ForwardGraph replaying this model's inference forward at input_ids' shape."""
@@ -112,15 +156,22 @@ class DecodeGraph:
     of launching each from Python.  The states passed in are the ones the replays
     update; ``step`` keeps their host-side ``pos`` in sync.  Replays of one DecodeGraph must
     not overlap with other work on the same states.
+
+    With ``controls`` (the keyword arguments of sampling.select_tokens but for the logits) the recording goes on
+    to choose the next token of every sequence, counts it in controls["history"] where there is one and
+    leaves it as the next input: ``next`` replays from there.  Tensors among the controls are read at
+    replay time: noise, masks and penalties are changed in place between replays.
     """
 
-    def __init__(self, lm, states):
+    def __init__(self, lm, states, controls=None):
         chunks = {layer.chunk_size for layer in lm.backbone.layers}
         pos = {st.pos for st in states}
         if len(chunks) != 1 or len(pos) != 1 or len(states) != len(lm.backbone.layers):
             raise RuntimeError("capture_decode needs one chunk size and states at one position")
         (self.chunk,) = chunks
         self.lm, self.states = lm, states
+        self.controls = None if controls is None else dict(controls)
+        self.tokens = self.logprobs = None
         dev = states[0].h.device
         B = states[0].h.shape[0]
         self.ids = torch.zeros(B, dtype=torch.long, device=dev)
@@ -128,17 +179,23 @@ class DecodeGraph:
         # warm up on scratch copies (library handles, allocator pools), then record
         scratch = [_clone_state(st) for st in states]
         scratch_pos = self.pos.clone()
+        scratch_controls = None
+        if self.controls is not None:
+            history = self.controls.get("history")
+            scratch_controls = dict(self.controls, history=None if history is None else history.clone())
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
             for _ in range(2):
-                self._run(scratch, scratch_pos)
+                self._choose(self._run(scratch, scratch_pos), scratch_controls)
+                self.ids.zero_()
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
-        del scratch, scratch_pos
+        del scratch, scratch_pos, scratch_controls
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = self._run(self.states, self.pos)
+            self.tokens, self.logprobs = self._choose(self.logits, self.controls)
 
     def _run(self, states, pos):
         with torch.no_grad():
@@ -146,13 +203,35 @@ class DecodeGraph:
             _ops.chunk_pos_advance(pos, self.chunk)
         return logits
 
+    def _choose(self, logits, controls):
+        if controls is None:
+            return None, None
+        with torch.no_grad():
+            tokens, logprobs = select_tokens(logits, **controls)
+            if controls.get("history") is not None:
+                append_tokens(controls["history"], tokens)
+            self.ids.copy_(tokens)
+        return tokens, logprobs
+
     def step(self, input_ids):
         """input_ids [B] -> logits [B,V] (a static buffer, overwritten by the next step)."""
         self.ids.copy_(input_ids)
+        self._replay()
+        return self.logits
+
+    def next(self):
+        """One token further from the tokens chosen last (at first those that ``ids`` was given): (tokens [B],
+        log-probabilities [B]), static buffers that the next replay overwrites.  A sequence without an
+        allowed token has -1, which as the next input reads the embedding's last row."""
+        if self.controls is None:
+            raise RuntimeError("next needs a DecodeGraph captured with controls")
+        self._replay()
+        return self.tokens, self.logprobs
+
+    def _replay(self):
         self.graph.replay()
         for st in self.states:
             st.pos = (st.pos + 1) % self.chunk
-        return self.logits
 
 
 class ForwardGraph:

@@ -33,10 +33,11 @@ from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from . import _ops
+from .quant4 import Linear4Bit, linear_4bit
 
 __all__ = ["HdcMamba9v3Block", "HdcMamba9v3Model", "FusedNormConv1dFunction",
            "fused_norm_conv1d_trainable", "RowLayerNormFunction", "layer_norm", "SlotSsmMixerFunction",
-           "set_differentiable_mixer", "set_fused_out_proj", "set_fused_step_front", "BlockState"]
+           "set_differentiable_mixer", "set_fused_out_proj", "set_fused_step_front", "quantize_4bit", "BlockState"]
 
 
 @dataclass
@@ -301,7 +302,7 @@ class HdcMamba9v3Block(nn.Module):
         ds, H, C = self.d_state, self.num_heads, self.chunk_size
         dtype = x.dtype
         x_conv = fused_norm_conv1d_trainable(x, self.norm, self.conv1d)
-        w_in, b_in = self.in_proj.weight.to(dtype), self.in_proj.bias.to(dtype)
+        w_in, b_in = self._weights(dtype)[0].to(dtype), self.in_proj.bias.to(dtype)
         # the SSM and slot kernels are constants for autograd, so projs needs no graph either
         if _ops.gemm_preferred(x_conv, w_in, b_in):
             projs = _ops.gemm(x_conv, w_in, b_in)
@@ -396,11 +397,23 @@ class HdcMamba9v3Block(nn.Module):
                 and not _ops.timer.active and forward_ad._current_level < 0 and self.ssm_overlap in ("auto", "none", "state", "gate", "after_state")
                 and (not torch.is_autocast_enabled("cuda") or torch.get_autocast_dtype("cuda") == x.dtype))
 
-    def _params(self):
+    @property
+    def weights_4bit(self):
+        """Whether in_proj and out_proj hold 4-bit weights (quantize_4bit): inference only."""
+        return isinstance(self.in_proj, Linear4Bit)
+
+    def _weights(self, dtype):
+        """in_proj's and out_proj's weights; 4-bit ones brought back to ``dtype`` for products of many rows."""
+        if self.weights_4bit:
+            return self.in_proj.weight4.dequantize(dtype), self.out_proj.weight4.dequantize(dtype)
+        return self.in_proj.weight, self.out_proj.weight
+
+    def _params(self, weights=None):
         """The parameters in the order the native host path takes them."""
-        return [self.norm.weight, self.norm.bias, self.conv1d.weight, self.conv1d.bias, self.in_proj.weight,
+        w_in, w_out = (self.in_proj.weight, self.out_proj.weight) if weights is None else weights
+        return [self.norm.weight, self.norm.bias, self.conv1d.weight, self.conv1d.bias, w_in,
                 self.in_proj.bias, self.A_log, self.gamma_buf, self.group_norm.weight, self.group_norm.bias,
-                self.out_proj.weight]
+                w_out]
 
     def _grad_params(self, mixer=None):
         """Those that receive a gradient (``mixer``: with the differentiable mixer)."""
@@ -418,9 +431,12 @@ class HdcMamba9v3Block(nn.Module):
         (two-pass variance, the weight as it is now: the folded form reads row sums kept until the
         weight's version changes, which a write through ``.data`` or a flat buffer does not do)."""
         fused = not train and self._fused_out(x)
-        sums = self._out_weight_sums(x.dtype) if fused and _ops.rowln_stats_ok(x, self.d_model) else None
+        weights = self._weights(x.dtype)
+        sums = None
+        if fused and _ops.rowln_stats_ok(x, self.d_model):
+            sums = _ops.row_sums(weights[1]) if self.weights_4bit else self._out_weight_sums(x.dtype)
         return _ops.native().block_forward(
-            x, self._params(), self.norm.eps, (self.d_state, self.num_heads, self.chunk_size), self._native_streams(x),
+            x, self._params(weights), self.norm.eps, (self.d_state, self.num_heads, self.chunk_size), self._native_streams(x),
             out, fused, sums, torch.cuda.tunable.is_enabled(), None if state is None else state.h,
             None if state is None else state.S_prev)
 
@@ -430,6 +446,10 @@ class HdcMamba9v3Block(nn.Module):
             return self._native_forward(x.contiguous(), train=train)
         xp = _ops.native().pad_rows(x, pad, _ops._stream(x))
         return self._native_forward(xp, out=xp, train=train)[:, pad:, :]
+
+    def _no_grad_4bit(self):
+        if self.weights_4bit and (self.training or torch.is_grad_enabled()):
+            raise RuntimeError("a block with 4-bit weights is for inference: call eval() and run under torch.no_grad()")
 
     def _fused_out(self, x):
         """Whether out_proj runs as the GEMM with the LayerNorm folded in (bf16, no autograd).
@@ -465,6 +485,8 @@ class HdcMamba9v3Block(nn.Module):
         unchanged)."""
         if getattr(self, "_wsum_key", None) is None:
             return
+        if self.weights_4bit:
+            return
         p = self.out_proj.weight
         if (p.data_ptr(), p._version) != self._wsum_key[:2]:
             self._out_weight_sums(self._wsum_key[2])
@@ -475,14 +497,15 @@ class HdcMamba9v3Block(nn.Module):
         row statistics to the GEMM (hdcm_rowln_gemm_stats_fwd); otherwise the GEMM takes them
         from its operands (hdcm_rowln_gemm_fwd)."""
         B, L, dm = x.shape
-        w = self.out_proj.weight.to(x.dtype)
+        w = self._weights(x.dtype)[1].to(x.dtype)
         x2 = x.reshape(B * L, dm)
         o2 = None if out is None else out.view(B * L, dm)
         if _ops.rowln_stats_ok(x2, dm):
             parts = _ops.ssm_stats_parts(self.d_state) + self.num_heads
             stats = torch.empty(parts, B * L, 2, device=x.device, dtype=torch.float32)
             c = self._mixer(x, state, normalize=False, row_stats=stats)
-            y = _ops.rowln_gemm_stats(c, w, self._out_weight_sums(w.dtype), stats, x2, out=o2)
+            sums = _ops.row_sums(w) if self.weights_4bit else self._out_weight_sums(w.dtype)
+            y = _ops.rowln_gemm_stats(c, w, sums, stats, x2, out=o2)
         else:
             c = self._mixer(x, state, normalize=False)
             y = _ops.rowln_gemm(c, w, x2, out=o2)
@@ -505,6 +528,7 @@ class HdcMamba9v3Block(nn.Module):
     def _inner_forward(self, x, state=None):
         """Block body on a chunk-aligned [B,L,dm] input; returns x + out_proj(LN(combined))."""
         B, L, dm = x.shape
+        self._no_grad_4bit()
         if not torch.is_grad_enabled() and self._native_ok(x):
             return self._native_forward(x, state)
         if self._fused_out(x):
@@ -519,7 +543,7 @@ class HdcMamba9v3Block(nn.Module):
 
     def _out_proj(self, x, c, out=None):
         """x + c @ out_proj.weight^T of rows x [M, dm], c [M, ds + dm], into ``out`` (which may be x) when given."""
-        w = self.out_proj.weight.to(x.dtype)
+        w = self._weights(x.dtype)[1].to(x.dtype)
         if not torch.is_grad_enabled() and forward_ad._current_level < 0 and _ops.gemm_f32_preferred(x.shape[0], c, w, x):
             return _ops.gemm_f32(c, w, res=x, out=out)
         return torch.addmm(x, c, w.t()) if out is None else out.addmm_(c, w.t())
@@ -581,6 +605,8 @@ class HdcMamba9v3Block(nn.Module):
         state.pos is left to the caller (graph replay)."""
         _ops._on_gpu(x)
         dm, ds, H, C = self.d_model, self.d_state, self.num_heads, self.chunk_size
+        if self.weights_4bit:
+            return self._step_4bit(x, state, pos_dev)
         if not torch.is_grad_enabled() and self._native_ok(x):
             w = self.in_proj.weight
             front = (self.fused_step_front and x.dtype == torch.bfloat16 and w.shape[0] >= 2048
@@ -620,6 +646,24 @@ class HdcMamba9v3Block(nn.Module):
             state.pos = (state.pos + 1) % C
         return y
 
+    def _step_4bit(self, x, state, pos_dev):
+        """step with 4-bit in_proj and out_proj: LayerNorm + conv of the token, in_proj, the mixer step, the row
+        LayerNorm and out_proj with the residual."""
+        self._no_grad_4bit()
+        dm, ds, H, C = self.d_model, self.d_state, self.num_heads, self.chunk_size
+        xc = _ops.norm_conv_step(x, self.norm.weight, self.norm.bias, self.conv1d.weight.squeeze(1), self.conv1d.bias,
+                                 self.norm.eps, state.conv)
+        projs = linear_4bit(xc, self.in_proj.weight4, self.in_proj.bias)
+        combined = torch.empty(x.shape[0], ds + dm, device=x.device, dtype=x.dtype)
+        _ops.mixer_step(projs, self.A_log, ds, 3 * ds, self.gamma_buf.to(x.dtype), self.group_norm.weight,
+                        self.group_norm.bias, 1e-5, state.h, state.S_prev, state.S_intra, state.pos, C, combined, dm, H,
+                        pos_dev=pos_dev)
+        _ops.layer_norm(combined, eps=1e-5, out=combined)
+        y = linear_4bit(combined, self.out_proj.weight4, residual=x)
+        if pos_dev is None:
+            state.pos = (state.pos + 1) % C
+        return y
+
     def _refresh_gamma(self):
         """gamma_buf from decay_log, as the reference does at every training forward (model.py:390)."""
         d, g = self.decay_log, self.gamma_buf
@@ -632,6 +676,7 @@ class HdcMamba9v3Block(nn.Module):
 
     def forward(self, x):
         _ops._on_gpu(x)
+        self._no_grad_4bit()
         B, L_in, _ = x.shape
         pad = (self.chunk_size - (L_in % self.chunk_size)) % self.chunk_size
         if self.training:
@@ -768,4 +813,18 @@ def set_differentiable_mixer(module, enabled=True):
     for m in module.modules():
         if isinstance(m, HdcMamba9v3Block):
             m.differentiable_mixer = bool(enabled)
+    return module
+
+
+def quantize_4bit(module, group_size=128, zero_points=False, head=True):
+    """Round in_proj and out_proj of every HdcMamba9v3Block inside ``module`` to 4 bits with group scales
+    (Weight4Bit.quantize, scales in the weight's type), and with ``head`` an HdcMambaLM's head (the
+    embedding that it shares its weight with keeps it); returns ``module``, on the GPU and for inference
+    only from then on.  A decode step then streams a quarter of the weights' bytes."""
+    for m in module.modules():
+        names = ("in_proj", "out_proj") if isinstance(m, HdcMamba9v3Block) else ("lm_head",) if head else ()
+        for name in names:
+            linear = getattr(m, name, None)
+            if isinstance(linear, nn.Linear):
+                setattr(m, name, Linear4Bit.from_linear(linear, group_size, zero_points))
     return module

@@ -9,10 +9,12 @@ counterpart there.
 from __future__ import annotations
 
 import torch
+import torch.nn as nn
+import torch.nn.functional as F
 
 from . import _ops
 
-__all__ = ["Weight4Bit", "linear_4bit"]
+__all__ = ["Weight4Bit", "linear_4bit", "Linear4Bit"]
 
 GROUP_SIZES = (32, 64, 128)
 
@@ -134,3 +136,47 @@ def linear_4bit(x, weight, bias=None, residual=None, out=None):
     sums, one rounding.  ``out`` may be ``residual``.  No gradient: refused where one would be
     recorded."""
     return _ops.native().linear_4bit(x, weight._handle, bias, residual, out)
+
+
+class Linear4Bit(nn.Module):
+    """nn.Linear with a Weight4Bit in place of its weight, for inference: the packed weight, its scales and
+    zero points are buffers, the bias (or None) a parameter that takes no gradient.
+
+    Up to ``direct_rows`` rows go through linear_4bit; more multiply by the weight brought back to x's
+    type, which rounds it once more (measured: 128 rows of the d_model 2048 in_proj 21 us against
+    27, 256 rows 38 against 35)."""
+
+    direct_rows = 192
+
+    def __init__(self, weight, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self.group_size = weight.group_size
+        self.register_buffer("packed", weight.packed)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("zeros", weight.zeros)
+        self.bias = None if bias is None else nn.Parameter(bias.detach(), requires_grad=False)
+        self._weight4 = weight
+
+    @classmethod
+    def from_linear(cls, linear, group_size=128, zero_points=False, scale_dtype=None):
+        """The nn.Linear's weight rounded to 4 bits (Weight4Bit.quantize); the bias is shared."""
+        return cls(Weight4Bit.quantize(linear.weight, group_size, zero_points, scale_dtype), linear.bias)
+
+    @property
+    def weight4(self) -> Weight4Bit:
+        """The packed weight (made anew after the buffers were moved)."""
+        w = self._weight4
+        if w.packed is not self.packed or w.scales is not self.scales or w.zeros is not self.zeros:
+            w = self._weight4 = Weight4Bit(self.packed, self.scales, self.zeros, w.shape, w.group_size)
+        return w
+
+    def forward(self, x):
+        rows = x.numel() // max(x.shape[-1], 1)
+        if rows > self.direct_rows:
+            return F.linear(x, self.weight4.dequantize(x.dtype), None if self.bias is None else self.bias.to(x.dtype))
+        return linear_4bit(x, self.weight4, self.bias)
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"group_size={self.group_size}, zero_points={self.zeros is not None}")
