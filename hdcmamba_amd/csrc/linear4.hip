@@ -248,7 +248,7 @@ template <typename T> struct Ending {
   }
 };
 
-// Rows held in registers.  The W waves of a workgroup split K, two 128-column tiles each, and keep
+// Rows held in registers.  The W waves of a workgroup split K, P (one or two) 128-column tiles each, and keep
 // the fragments of up to 16 MT rows of x for their columns while the workgroup walks over column
 // tiles of the output; the next tile's codes are in flight while one is multiplied.  Per output tile
 // each wave leaves its partial sums in LDS (two buffers, so one barrier a tile) and the waves take
@@ -257,9 +257,9 @@ template <typename T> struct Ending {
 // longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS.
 // What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
 // instructions per wave and tile.
-template <typename T, int MT, int GS, bool ZERO, int MAXW>
-__global__ __launch_bounds__(MAXW* kWave) void linear4_kernel(Linear4Args p) {
-  constexpr int P = 2, GPT = 4 / GS;
+template <typename T, int MT, int P, int GS, bool ZERO, int MAXW>
+__global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4_kernel(Linear4Args p) {
+  constexpr int GPT = 4 / GS;
   constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
   extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [2][MAXW][MT][64]; at first the waves' slabs of x
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -443,18 +443,32 @@ __global__ __launch_bounds__(8 * kWave) void linear4_long_kernel(Linear4Args p) 
 }
 
 // The registers hold up to 64 bf16 rows of 16 column tiles (2048 columns) in 8 waves, or 32 rows of 24
-// in 12; of fp32 rows, whose three parts take three times as many, 16.  More rows run as row blocks of equal height, which read the
-// weight again (out of the caches); longer rows run on linear4_long_kernel.
-constexpr int kWidest = 24, kWide = 16;
+// in 12; of fp32 rows, whose three parts take three times as many, 16.  More rows run as row blocks of
+// equal height, which read the weight again (out of the caches); longer rows run on linear4_long_kernel.
+//
+// A row block has the CUs that the others leave (128 x 8576 x 2048 with all of them for each block 19.0 us, with half 14.1; 192
+// rows 27.4, 17.9): x is read once per workgroup, 256 KB at 64 rows of 2048.
+//
+// Column tiles a wave: one, where that makes no more waves than a workgroup has, since the rows' way into the fragments, the
+// longest part of a short run, then has twice the waves (us with two and one: 16 x 1024 x 1152 3.9, 3.5; 32 x 3264 x 768
+// 4.6, 4.0; 64 x 3264 x 768 6.7, 5.5; 64 x 50277 x 768 19.9, 18.4; fp32 3 x 3264 x 768 5.9, 5.6, 16 x 25600 x 1500 24.2, 17.9).  Two
+// for one row tile of bf16 and more than two output tiles for every CU: there the sums over the waves count (16 x 8192 x 1152
+// 5.1, 4.6, x 12800 6.3, 6.7, x 25600 7.8, 9.9).
+constexpr int kWidest = 24, kWide = 16, kCUs = 256;
 
-template <typename T, int MT, int GS, bool ZERO, int MAXW> void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
-  const int W = (a.tiles_k + 1) / 2;
-  // waves per CU: 16 with one row tile, 8 with more (their registers): whole workgroups
-  const int per_cu = (MT == 1 ? 16 : 8) / W;
-  const int most = 256 * (per_cu > 1 ? per_cu : 1);
+template <typename T, int MT, int P, int GS, bool ZERO, int MAXW>
+void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
+  const int W = (a.tiles_k + P - 1) / P;
+  // waves per CU: 8 where the registers hold more than one row tile of two column tiles, else 16: whole workgroups
+  const int per_cu = (MT == 1 || P == 1 ? 16 : 8) / W;
+  const int slots = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m, most = slots > 1 ? slots : 1;
   const size_t slabs = (size_t)W * 16 * (kTileK * sizeof(T) + 16), parts = (size_t)2 * MAXW * MT * kWave * 16;
-  HDCM_LAUNCH((linear4_kernel<T, MT, GS, ZERO, MAXW>), dim3((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m),
+  HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW>), dim3((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m),
               dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+}
+template <typename T, int MT, int GS, bool ZERO, int MAXW> void pick_tiles(const Linear4Args& a, int blocks_m, hipStream_t s) {
+  const bool one = a.tiles_k <= MAXW && (MT > 1 || sizeof(T) == 4 || a.tiles_n <= 2 * kCUs);
+  one ? launch_linear4<T, MT, 1, GS, ZERO, MAXW>(a, blocks_m, s) : launch_linear4<T, MT, 2, GS, ZERO, MAXW>(a, blocks_m, s);
 }
 template <typename T, int MT, int GS, bool ZERO> void launch_long(const Linear4Args& a, hipStream_t s) {
   HDCM_LAUNCH((linear4_long_kernel<T, MT, GS, ZERO>), dim3((unsigned)a.tiles_n, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
@@ -469,11 +483,11 @@ template <typename T, int GS, bool ZERO> void pick_rows(const Linear4Args& a, hi
   const bool wide = a.tiles_k > kWide;
   const int most = sizeof(T) == 4 ? 1 : wide ? 2 : 4;
   const int blocks = (tiles_m + most - 1) / most, mt = (tiles_m + blocks - 1) / blocks;
-  if (mt == 1) launch_linear4<T, 1, GS, ZERO, 12>(a, blocks, s);
+  if (mt == 1) pick_tiles<T, 1, GS, ZERO, 12>(a, blocks, s);
   if constexpr (sizeof(T) == 2) {
-    if (mt == 2) launch_linear4<T, 2, GS, ZERO, 12>(a, blocks, s);
-    if (mt == 3) launch_linear4<T, 3, GS, ZERO, 8>(a, blocks, s);
-    if (mt == 4) launch_linear4<T, 4, GS, ZERO, 8>(a, blocks, s);
+    if (mt == 2) pick_tiles<T, 2, GS, ZERO, 12>(a, blocks, s);
+    if (mt == 3) pick_tiles<T, 3, GS, ZERO, 8>(a, blocks, s);
+    if (mt == 4) pick_tiles<T, 4, GS, ZERO, 8>(a, blocks, s);
   }
 }
 template <typename T, int GS> void pick_zero(const Linear4Args& a, hipStream_t s) {
