@@ -129,6 +129,8 @@ struct Linear4Args {
   int64_t x_rs, r_rs, o_rs;
   int M, N, K, tiles_n, tiles_k, np;
   bool s_f32;
+  const float* row_sums;  // of the weight, where x's rows are to be normalised
+  float eps;
 };
 
 // A lane's scale of a row of a tile: the loads take a uniform address and a 32-bit lane offset, and of
@@ -227,20 +229,25 @@ __device__ __forceinline__ void row_sums(const Rows<T> (&xa)[4][MT], f32x4_t (&x
 
 // The end of four rows (row0 + 0..3) of one column n: what is added is loaded ahead of the products (at
 // clamped places, without a branch per lane, and converted only here), then one rounding and the store.
-template <typename T> struct Ending {
+// NORM: stats holds the mean and the reciprocal deviation of the four rows.
+template <typename T, bool NORM = false> struct Ending {
   T bias, res[4];
+  float wsum;
   __device__ __forceinline__ void load(const Linear4Args& p, int row0, int rows_end, int n) {
     n = min(n, p.N - 1);
+    if constexpr (NORM) wsum = p.row_sums[n];
     if (p.bias) bias = reinterpret_cast<const T*>(p.bias)[n];
     if (p.res) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) res[e] = reinterpret_cast<const T*>(p.res)[(int64_t)min(row0 + e, rows_end - 1) * p.r_rs + n];
     }
   }
-  __device__ __forceinline__ void store(const Linear4Args& p, f32x4_t v, int row0, int rows_end, int n) const {
+  __device__ __forceinline__ void store(const Linear4Args& p, f32x4_t v, int row0, int rows_end, int n,
+                                        const float2* stats = nullptr) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float y = v[e];
+      if constexpr (NORM) y = (y - stats[e].x * wsum) * stats[e].y;
       if (p.bias) y += to_f<T>(bias);
       if (p.res) y += to_f<T>(res[e]);
       if (row0 + e < rows_end && n < p.N) reinterpret_cast<T*>(p.out)[(int64_t)(row0 + e) * p.o_rs + n] = from_f<T>(y);
@@ -257,7 +264,11 @@ template <typename T> struct Ending {
 // longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS.
 // What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
 // instructions per wave and tile.
-template <typename T, int MT, int P, int GS, bool ZERO, int MAXW>
+// NORM (bf16): out = rstd (x w - mean sum w) takes the row LayerNorm without affine behind the product.  The rows' sums
+// and sums of squares come from MFMAs on the fragments that are there (squares: the diagonal of x x'), so they cost no pass
+// and no barrier: 0.6 us at 16 x 2048 x 2176 (5.1 us, 4.5 without).  Normalising the rows on their way in, with two
+// sums over the waves before the first product, took 4.2 us, the LayerNorm as a launch of its own 2.6.
+template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool NORM>
 __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4_kernel(Linear4Args p) {
   constexpr int GPT = 4 / GS;
   constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
@@ -334,14 +345,39 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
 #pragma unroll
     for (int i = 0; i < P; ++i) row_sums<T, MT, ZERO>(xa[i], xsum[i]);
   }
+  __shared__ float2 sums[NORM ? MAXW : 1][16 * MT], stats[NORM ? 16 * MT : 1];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int r = 0; r < MT; ++r) {
+      f32x4_t s1 = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s1 = mma(xa[i][j][r], fill(0x3f803f80u), s1);
+          s2 = mma(xa[i][j][r], xa[i][j][r].x, s2);
+        }
+      const int e = l16 & 3;  // row 4 g + e, column l16
+      if (l16 / 4 == g)
+        sums[w][16 * r + l16] = make_float2(e == 0 ? s1[0] : e == 1 ? s1[1] : e == 2 ? s1[2] : s1[3],
+                                            e == 0 ? s2[0] : e == 1 ? s2[1] : e == 2 ? s2[2] : s2[3]);
+    }
+  }
   __syncthreads();  // the slabs become the partial sums' buffers
+  if constexpr (NORM)
+    if (tid < 16 * MT) {  // (seen by the others from the first barrier of the loop on)
+      float s1 = 0.f, s2 = 0.f;
+      for (int k = 0; k < W; ++k) s1 += sums[k][tid].x, s2 += sums[k][tid].y;
+      const float mean = s1 / (float)p.K;
+      stats[tid] = make_float2(mean, rsqrtf(fmaxf(s2 / (float)p.K - mean * mean, 0.f) + p.eps));
+    }
   for (int k = W + w; k < MAXW; k += W)  // waves that are not there add nothing
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) part[(i / MT * MAXW + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   int buf = 0, turn = 0;
   for (int t = blockIdx.x; t < p.tiles_n; t += gridDim.x) {
-    Ending<T> end;
+    Ending<T, NORM> end;
     const int own = w >= turn ? w - turn : w + W - turn;  // the row tile that this wave adds up (none past MT)
     if (own < MT) end.load(p, m0 + 16 * own + 4 * g, m0 + rows, kTileN * t + l16);
     f32x4_t acc[MT];
@@ -370,7 +406,7 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
           for (int k = 0; k < 4; ++k) v[k] = from[(b + k) * MT * kWave];
           sum += (v[0] + v[1]) + (v[2] + v[3]);
         }
-      end.store(p, sum, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+      end.store(p, sum, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16, NORM ? stats + 16 * r + 4 * g : nullptr);
     }
     turn += MT;
     while (turn >= W) turn -= W;
@@ -463,8 +499,13 @@ void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
   const int per_cu = (MT == 1 || P == 1 ? 16 : 8) / W;
   const int slots = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m, most = slots > 1 ? slots : 1;
   const size_t slabs = (size_t)W * 16 * (kTileK * sizeof(T) + 16), parts = (size_t)2 * MAXW * MT * kWave * 16;
-  HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW>), dim3((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m),
-              dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+  const dim3 grid((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m);
+  if constexpr (sizeof(T) == 2)
+    if (a.row_sums) {
+      HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, true>), grid, dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+      return;
+    }
+  HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, false>), grid, dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
 }
 template <typename T, int MT, int GS, bool ZERO, int MAXW> void pick_tiles(const Linear4Args& a, int blocks_m, hipStream_t s) {
   const bool one = a.tiles_k <= MAXW && (MT > 1 || sizeof(T) == 4 || a.tiles_n <= 2 * kCUs);
@@ -689,7 +730,9 @@ extern "C" int hdcm_w4_dequant(const void* packed, const void* scales, int scale
   return hdcm_launch_status();
 }
 
-extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const void* packed, const void* scales,
+extern "C" int64_t hdcm_w4_norm_max_k(void) { return kWidest * kTileK; }
+
+extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sums, float eps, const void* packed, const void* scales,
                                   int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias, const void* res,
                                   int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N, int64_t K,
                                   int dtype, void* stream) {
@@ -698,6 +741,7 @@ extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const voi
   HDCM_CHECK_ARG(M >= 0 && N >= 0 && K > 0, HDCM_EINVAL);
   HDCM_CHECK_ARG(M == 0 || N == 0 || (x && packed && scales && out), HDCM_EINVAL);
   HDCM_CHECK_ARG(M <= 1 || (x_row_stride >= K && out_row_stride >= N && (!res || res_row_stride >= N)), HDCM_EINVAL);
+  HDCM_CHECK_ARG(!row_sums || (dtype == HDCM_BF16 && K <= kWidest * kTileK), HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(sizes_ok(N, K, group) && K >= (dtype == HDCM_F32 ? 4 : 8) && M <= 16 * 65535, HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(hdcm_aligned16(packed) && ((uintptr_t)scales & 3u) == 0, HDCM_EALIGN);
   if (M == 0 || N == 0) return HDCM_OK;
@@ -706,7 +750,7 @@ extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const voi
   a.x_rs = x_row_stride, a.r_rs = res_row_stride, a.o_rs = out_row_stride;
   a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.tiles_n = tiles_of(N, kTileN), a.tiles_k = tiles_of(K, kTileK), a.np = a.tiles_n * kTileN;
-  a.s_f32 = scale_dtype == HDCM_F32;
+  a.s_f32 = scale_dtype == HDCM_F32, a.row_sums = row_sums, a.eps = eps;
   hipStream_t s = (hipStream_t)stream;
   dtype == HDCM_F32 ? pick_group<float>(a, (int)group, s) : pick_group<bf16_t>(a, (int)group, s);
   return hdcm_launch_status();

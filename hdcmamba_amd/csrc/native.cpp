@@ -626,13 +626,15 @@ bool same_place(const Tensor& a, const Tensor& b) {
 
 // A packed weight, checked once (the handle of a Weight4Bit)
 struct Weight4 {
-  Tensor packed, scales, zeros;
+  Tensor packed, scales, zeros, row_sums;  // row_sums: as the products give them
   int64_t N, K, group;
   int scale_dtype;
 };
+Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, const OptTensor& residual_,
+                   const OptTensor& out_, std::optional<double> norm_eps);
 Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor& zeros, int64_t N, int64_t K, int64_t group) {
   on_gpu(packed);
-  Weight4 w{packed, scales, or_none(zeros), N, K, group, dtype_of(scales)};
+  Weight4 w{packed, scales, or_none(zeros), Tensor(), N, K, group, dtype_of(scales)};
   TORCH_CHECK(N > 0 && K > 0 && (group == 32 || group == 64 || group == 128), "a 4-bit weight [", N, ", ", K, "] in groups of ",
               group);
   const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
@@ -645,11 +647,14 @@ Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor
     TORCH_CHECK(w.zeros.scalar_type() == at::kByte && w.zeros.is_contiguous() && w.zeros.numel() == per,
                 "zeros must hold one byte per scale");
   }
+  const at::NoGradGuard guard;
+  w.row_sums = linear_4bit(at::ones({1, K}, packed.options().dtype(at::kFloat)), w, std::nullopt, std::nullopt, std::nullopt,
+                           std::nullopt).view({N});
   return w;
 }
 
 Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, const OptTensor& residual_,
-                   const OptTensor& out_) {
+                   const OptTensor& out_, std::optional<double> norm_eps) {
   const Tensor &bias = or_none(bias_), &residual = or_none(residual_), &given = or_none(out_);
   on_gpu(x);
   no_gradient("linear_4bit", {&x, &bias, &residual, &given});
@@ -685,13 +690,16 @@ Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, co
     TORCH_CHECK(!overlap(o, xr) && (!r.defined() || same_place(o, r) || !overlap(o, r)),
                 "linear_4bit: out may be the residual itself but share no other memory with x or the residual");
   int64_t K = w.K;
+  TORCH_CHECK(!norm_eps || (*norm_eps >= 0 && K >= 8 && dt == HDCM_BF16),
+              "linear_4bit: norm_eps must not be negative, the rows bfloat16 and of 8 columns at least");
   if (K < 8) {  // shorter than a load of the kernel's: columns of zeros, which the packed weight holds too
     xr = at::constant_pad_nd(xr, {0, 8 - K});
     K = 8;
   }
   check("hdcm_w4_linear_fwd",
-        hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), w.packed.const_data_ptr(), w.scales.const_data_ptr(),
-                           w.scale_dtype, (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
+        hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), norm_eps ? (const float*)w.row_sums.const_data_ptr() : nullptr,
+                           norm_eps ? (float)*norm_eps : 0.f, w.packed.const_data_ptr(), w.scales.const_data_ptr(), w.scale_dtype,
+                           (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
                            r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, K, dt,
                            stream_of(x)));
   return out;

@@ -647,8 +647,8 @@ class HdcMamba9v3Block(nn.Module):
         return y
 
     def _step_4bit(self, x, state, pos_dev):
-        """step with 4-bit in_proj and out_proj: LayerNorm + conv of the token, in_proj, the mixer step, the row
-        LayerNorm and out_proj with the residual."""
+        """step with 4-bit in_proj and out_proj: LayerNorm + conv of the token, in_proj, the mixer step, and out_proj
+        with the row LayerNorm before it and the residual."""
         self._no_grad_4bit()
         dm, ds, H, C = self.d_model, self.d_state, self.num_heads, self.chunk_size
         xc = _ops.norm_conv_step(x, self.norm.weight, self.norm.bias, self.conv1d.weight.squeeze(1), self.conv1d.bias,
@@ -658,8 +658,11 @@ class HdcMamba9v3Block(nn.Module):
         _ops.mixer_step(projs, self.A_log, ds, 3 * ds, self.gamma_buf.to(x.dtype), self.group_norm.weight,
                         self.group_norm.bias, 1e-5, state.h, state.S_prev, state.S_intra, state.pos, C, combined, dm, H,
                         pos_dev=pos_dev)
-        _ops.layer_norm(combined, eps=1e-5, out=combined)
-        y = linear_4bit(combined, self.out_proj.weight4, residual=x)
+        eps = 1e-5
+        if x.dtype != torch.bfloat16 or ds + dm > _ops.lib().hdcm_w4_norm_max_k():  # not for the product's own LayerNorm
+            _ops.layer_norm(combined, eps=eps, out=combined)
+            eps = None
+        y = linear_4bit(combined, self.out_proj.weight4, residual=x, norm_eps=eps)
         if pos_dev is None:
             state.pos = (state.pos + 1) % C
         return y

@@ -130,12 +130,14 @@ class Weight4Bit:
                 f"zero_points={self.zeros is not None}, scales={self.scales.dtype}, device={self.packed.device})")
 
 
-def linear_4bit(x, weight, bias=None, residual=None, out=None):
+def linear_4bit(x, weight, bias=None, residual=None, out=None, norm_eps=None):
     """x [..., K] times a Weight4Bit [N, K], transposed, (+ bias [N]) (+ residual [..., N]) -> [..., N] in
     x's type (float32 or bfloat16): fp32 sums of exact code products, the scales applied to the groups'
-    sums, one rounding.  ``out`` may be ``residual``.  No gradient: refused where one would be
-    recorded."""
-    return _ops.native().linear_4bit(x, weight._handle, bias, residual, out)
+    sums, one rounding.  ``out`` may be ``residual``.  ``norm_eps`` (bfloat16 rows of 8 to hdcm_w4_norm_max_k() columns):
+    the product of the rows after a LayerNorm without affine, in the same launch; its variance is the
+    difference of two fp32 sums, for rows whose mean is not far above their deviation.  A bf16 row
+    that holds an infinity becomes NaN.  No gradient: refused where one would be recorded."""
+    return _ops.native().linear_4bit(x, weight._handle, bias, residual, out, norm_eps)
 
 
 class Linear4Bit(nn.Module):

@@ -30,24 +30,27 @@ def test_packed_bytes():
 
 def test_w4_linear_validation():
     f = _ops.lib().hdcm_w4_linear_fwd
-    # x, x_rs, packed, scales, scale_dtype, zeros, group, bias, res, res_rs, out, out_rs, M, N, K, dtype, stream
-    base = [P16, 2048, P16, P16, BF16, None, 128, None, None, 0, P16, 8576, 16, 8576, 2048, BF16, None]
-    assert f(*with_(base, _15=7)) == EUNSUPPORTED
-    assert f(*with_(base, _4=2)) == EUNSUPPORTED
-    assert f(*with_(base, _6=16)) == EUNSUPPORTED
-    assert f(*with_(base, _6=256)) == EUNSUPPORTED
-    assert f(*with_(base, _14=7)) == EUNSUPPORTED  # shorter than one load
+    # x, x_rs, row_sums, eps, packed, scales, scale_dtype, zeros, group, bias, res, res_rs, out, out_rs, M, N, K, dtype, stream
+    base = [P16, 2048, None, 1e-5, P16, P16, BF16, None, 128, None, None, 0, P16, 8576, 16, 8576, 2048, BF16, None]
+    assert f(*with_(base, _17=7)) == EUNSUPPORTED
+    assert f(*with_(base, _6=2)) == EUNSUPPORTED
+    assert f(*with_(base, _8=16)) == EUNSUPPORTED
+    assert f(*with_(base, _8=256)) == EUNSUPPORTED
+    assert f(*with_(base, _16=7)) == EUNSUPPORTED  # shorter than one load
+    most = _ops.lib().hdcm_w4_norm_max_k()
+    assert f(*with_(base, _1=4096, _2=P16, _16=most + 1)) == EUNSUPPORTED  # too long for the LayerNorm
+    assert f(*with_(base, _2=P16, _17=F32)) == EUNSUPPORTED
     assert f(*with_(base, _0=None)) == EINVAL
-    assert f(*with_(base, _3=None)) == EINVAL
-    assert f(*with_(base, _14=0)) == EINVAL
+    assert f(*with_(base, _5=None)) == EINVAL
+    assert f(*with_(base, _16=0)) == EINVAL
     assert f(*with_(base, _1=2047)) == EINVAL    # rows overlap
-    assert f(*with_(base, _11=8575)) == EINVAL
-    assert f(*with_(base, _8=P16, _9=100)) == EINVAL
-    assert f(*with_(base, _2=P18)) == EALIGN
-    assert f(*with_(base, _3=P18)) == EALIGN
-    assert f(*with_(base, _12=-1)) == EINVAL
-    assert f(*with_(base, _12=0, _0=None, _10=None)) == OK
-    assert f(*with_(base, _13=0, _2=None, _3=None, _10=None)) == OK
+    assert f(*with_(base, _13=8575)) == EINVAL
+    assert f(*with_(base, _10=P16, _11=100)) == EINVAL
+    assert f(*with_(base, _4=P18)) == EALIGN
+    assert f(*with_(base, _5=P18)) == EALIGN
+    assert f(*with_(base, _14=-1)) == EINVAL
+    assert f(*with_(base, _14=0, _0=None, _12=None)) == OK
+    assert f(*with_(base, _15=0, _4=None, _5=None, _12=None)) == OK
 
 
 def test_w4_pack_quantize_dequant_validation():

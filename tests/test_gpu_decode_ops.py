@@ -131,6 +131,52 @@ def test_linear_4bit_layouts(dev, dtype):
     assert (out[:, :2] == 7).all() and (out[:, 2 + N:] == 7).all()
 
 
+@pytest.mark.parametrize("M,K,N,group,zeros", [
+    (1, 8, 16, 32, False), (1, 1152, 100, 128, False), (16, 2176, 70, 128, True), (5, 333, 33, 32, True),
+    (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True),
+    (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True)])
+def test_linear_4bit_with_layer_norm(dev, M, K, N, group, zeros):
+    """norm_eps against the LayerNorm and product in 64 bits.
+
+    out = rstd (x w - mean sum w): the two terms in fp32 sums of K exact products each, rounded at most 2 K + 8 times by
+    2^-24 of the sum of magnitudes of code products (|c| <= 31 + 24 scales, as for the product alone), times rstd; row_sums
+    likewise, times mean.  rstd from v = q / K - mean^2, sums of K positive terms: relative error of v up to
+    (K + 4) 2^-24 (q / K + mean^2) / (v + eps), half of that in rstd, times the result without residual."""
+    codes, scales, z = _weight(N, K, group, zeros, BF, seed=K)
+    x = (torch.randn(M, K, generator=_gen(M)) * 2 + 6 * torch.rand(M, 1, generator=_gen(M + 1)) - 3).to(BF)
+    x[0] = 0  # no variance: eps alone
+    res = torch.randn(M, N, generator=_gen(M)).to(BF)
+    w = hm.Weight4Bit.from_codes(codes.to(dev), scales.to(dev), None if z is None else z.to(dev), group)
+    got = hm.linear_4bit(x.to(dev), w, residual=res.to(dev), norm_eps=1e-5).cpu().double()
+    xd = x.double()
+    mean, var = xd.mean(1, keepdim=True), xd.var(1, unbiased=False, keepdim=True)
+    rstd = (var + 1e-5).rsqrt()
+    dense = _dense(codes, scales, z, group)
+    y = ((xd - mean) * rstd) @ dense.t()
+    ref = y + res.double()
+    big = (dense.abs() + 48 * scales.double().max()).t()
+    sums = (xd.abs() @ big + mean.abs() * big.sum(0)) * rstd
+    stat = (K + 4) * 2.0**-24 * ((xd**2).mean(1, keepdim=True) + mean**2) / (var + 1e-5)
+    tol = 2.0**-8 * ref.abs() + (2 * K + 8) * 2.0**-24 * sums + stat * (y.abs() + rstd * mean.abs() * dense.sum(1).abs()) + 1e-6
+    _say("  worst", float(((got - ref).abs() / tol).max()))
+    assert ((got - ref).abs() <= tol).all()
+    assert torch.equal(got[0], res[0].double())  # zero rows stay zero
+    assert hm.linear_4bit(x[:0].to(dev), w, norm_eps=1e-5).shape == (0, N)
+
+
+def test_linear_4bit_layer_norm_rows_apart(dev):
+    """A row's NaN or infinity stays in its row."""
+    w = hm.Weight4Bit.quantize(torch.randn(64, 640, generator=_gen(3)).to(BF).to(dev))
+    x = torch.randn(19, 640, generator=_gen(4)).to(BF).to(dev)
+    plain = hm.linear_4bit(x, w, norm_eps=1e-5)
+    bad = x.clone()
+    bad[4, 17], bad[18, 0] = float("nan"), float("inf")
+    got = hm.linear_4bit(bad, w, norm_eps=1e-5)
+    assert got[4].isnan().all() and got[18].isnan().all()
+    keep = [r for r in range(19) if r not in (4, 18)]
+    assert torch.equal(got[keep], plain[keep])
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_linear_4bit_infinities(dev, dtype):
     """A row's infinity or NaN stays in its row: a bf16 row becomes NaN, an fp32 row what the weights give."""
@@ -233,6 +279,13 @@ def test_weight_refusals(dev):
         hm.linear_4bit(x, w, out=torch.zeros(4, 31, device=dev, dtype=BF))
     with pytest.raises(RuntimeError, match="no gradient"):
         hm.linear_4bit(x.float().requires_grad_(), w)
+    with pytest.raises(RuntimeError, match="norm_eps"):
+        hm.linear_4bit(x, w, norm_eps=-1.0)
+    with pytest.raises(RuntimeError, match="norm_eps"):
+        hm.linear_4bit(x.float(), w, norm_eps=1e-5)
+    long = hm.Weight4Bit.quantize(torch.randn(16, _ops.lib().hdcm_w4_norm_max_k() + 1, device=dev))
+    with pytest.raises(_ops.HdcmError):
+        hm.linear_4bit(torch.zeros(1, long.shape[1], device=dev, dtype=BF), long, norm_eps=1e-5)
     buf = torch.zeros(4, 256, device=dev, dtype=BF)
     with pytest.raises(RuntimeError, match="share no other memory"):
         hm.linear_4bit(buf[:, :128], w, out=buf[:, 100:132])
