@@ -128,7 +128,6 @@ _PROTOS = {
                                  c_void_p]),
     "hdcm_w4_dequant": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int,
                                 c_void_p]),
-    "hdcm_w4_norm_max_k": (c_int64, []),
     "hdcm_w4_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
                                    c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "hdcm_logits_process": (c_int, [c_void_p, c_int64, ctypes.POINTER(LogitsControls), c_void_p, c_int64, c_int64, c_int64,

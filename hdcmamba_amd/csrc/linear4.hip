@@ -127,7 +127,7 @@ struct Linear4Args {
   const void *bias, *res;
   void* out;
   int64_t x_rs, r_rs, o_rs;
-  int M, N, K, tiles_n, tiles_k, np;
+  int M, N, K, tiles_n, tiles_k, np, segs;
   bool s_f32;
   const float* row_sums;  // of the weight, where x's rows are to be normalised
   float eps;
@@ -268,7 +268,7 @@ template <typename T, bool NORM = false> struct Ending {
 // and sums of squares come from MFMAs on the fragments that are there (squares: the diagonal of x x'), so they cost no pass
 // and no barrier: 0.6 us at 16 x 2048 x 2176 (5.1 us, 4.5 without).  Normalising the rows on their way in, with two
 // sums over the waves before the first product, took 4.2 us, the LayerNorm as a launch of its own 2.6.
-template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool NORM>
+template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool NORM, bool SEG>
 __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4_kernel(Linear4Args p) {
   constexpr int GPT = 4 / GS;
   constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
@@ -278,209 +278,172 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
   const int l16 = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * 16 * MT;
   const int rows = min(16 * MT, p.M - m0);
-  const int k0 = w * P;  // the wave's first column tile
-  const Decode decode;
+    const Decode decode;
   const Scales scales(p.scales, p.s_f32, l16);
 
-  // x: 16 rows x 128 columns in NLD loads
-  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.x_rs;
-  u32x4_t raw[MT][P][NLD];
-#pragma unroll
-  for (int r = 0; r < MT; ++r)
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-      for (int n = 0; n < NLD; ++n) {
-        // rows past M re-read the last; a whole load of them is left out (their fragments hold what LDS held:
-        // every row of a product depends on its own row of x alone, and theirs are not stored)
-        if (n * kWave / CPR + 16 * r >= rows) continue;
-        const int at = n * kWave + lane, row = min(16 * r + at / CPR, rows - 1);
-        raw[r][i][n] = load_run<T>(x + (int64_t)row * p.x_rs, (k0 + i) * kTileK + at % CPR * E, p.K);
-      }
-  uint4 q[P];
-  uint32_t sr[P][GPT];
-  int zr[P][GPT];
-  auto fetch = [&](int t) {  // tiles past the last re-read it
-    t = min(t, p.tiles_n - 1);
-#pragma unroll
-    for (int i = 0; i < P; ++i) q[i] = load_tile(p, t, min(k0 + i, p.tiles_k - 1), lane);
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-      for (int u = 0; u < GPT; ++u) {
-        const int64_t at = (int64_t)(min(k0 + i, p.tiles_k - 1) * GPT + u) * p.np + kTileN * t;
-        sr[i][u] = scales.raw(at);
-        if constexpr (ZERO) zr[i][u] = (p.zeros + at)[(uint32_t)l16];
-      }
-  };
-  fetch(blockIdx.x);
-
-  T* slab = reinterpret_cast<T*>(part) + w * 16 * PITCH;  // the wave's own: no barrier
-  Rows<T> xa[P][4][MT];
-#pragma unroll
-  for (int r = 0; r < MT; ++r)
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      asm volatile("" ::: "memory");  // a wave's LDS accesses complete in order; they stay in this one
-#pragma unroll
-      for (int n = 0; n < NLD; ++n) {
-        if (n * kWave / CPR + 16 * r >= rows) continue;
-        const int at = n * kWave + lane, k = (k0 + i) * kTileK + at % CPR * E;
-        u32x4_t v = raw[r][i][n];
-        if ((k0 + i + 1) * kTileK > p.K) v = place_run<T>(v, k, p.K);  // (uniform)
-        *reinterpret_cast<u32x4_t*>(slab + at / CPR * PITCH + at % CPR * E) = v;
-      }
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x4_t v[8 / E];
-#pragma unroll
-        for (int h = 0; h < 8 / E; ++h) v[h] = *reinterpret_cast<const u32x4_t*>(slab + l16 * PITCH + 32 * j + 8 * g + E * h);
-        xa[i][j][r].set(v);
-      }
-      asm volatile("" ::: "memory");
-    }
-  f32x4_t xsum[P][MT];
-  if constexpr (GS == 4 && sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) row_sums<T, MT, ZERO>(xa[i], xsum[i]);
-  }
+  // with more than one segment: the sums of the workgroup's tiles so far, behind the slabs and the partial sums
+  f32x4_t* hold = part + max(2 * MAXW * MT * kWave, W * 16 * PITCH * (int)sizeof(T) / 16) + lane;
   __shared__ float2 sums[NORM ? MAXW : 1][16 * MT], stats[NORM ? 16 * MT : 1];
-  if constexpr (NORM) {
+  const int segs = SEG ? p.segs : 1;
+  for (int seg = 0; seg < segs; ++seg) {
+    int64_t x_rs = p.x_rs;
+    int ln = lane;
+    // with many rows their addresses are formed anew: kept over the products they would spill (64 x 8576 x 4096: 22.6 us, 25.1;
+    // for 16 rows, which have the registers, 11.4 and 10.5)
+    if constexpr (SEG && MT > 2) asm volatile("" : "+s"(x_rs), "+v"(ln));
+    const int k0 = (seg * W + w) * P;  // the wave's first column tile
+
+    // x: 16 rows x 128 columns in NLD loads
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * x_rs;
+    u32x4_t raw[MT][P][NLD];
 #pragma unroll
-    for (int r = 0; r < MT; ++r) {
-      f32x4_t s1 = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < MT; ++r)
 #pragma unroll
       for (int i = 0; i < P; ++i)
 #pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+          // rows past M re-read the last; a whole load of them is left out (their fragments hold what LDS held:
+          // every row of a product depends on its own row of x alone, and theirs are not stored)
+          if (n * kWave / CPR + 16 * r >= rows) {
+            if constexpr (SEG) raw[r][i][n] = u32x4_t{0, 0, 0, 0};  // (else the last segment's stay in registers)
+            continue;
+          }
+          const int at = n * kWave + ln, row = min(16 * r + at / CPR, rows - 1);
+          raw[r][i][n] = load_run<T>(x + (int64_t)row * x_rs, (k0 + i) * kTileK + at % CPR * E, p.K);
+        }
+    uint4 q[P];
+    uint32_t sr[P][GPT];
+    int zr[P][GPT];
+    auto fetch = [&](int t) {  // tiles past the last re-read it
+      t = min(t, p.tiles_n - 1);
+#pragma unroll
+      for (int i = 0; i < P; ++i) q[i] = load_tile(p, t, min(k0 + i, p.tiles_k - 1), lane);
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int u = 0; u < GPT; ++u) {
+          const int64_t at = (int64_t)(min(k0 + i, p.tiles_k - 1) * GPT + u) * p.np + kTileN * t;
+          sr[i][u] = scales.raw(at);
+          if constexpr (ZERO) zr[i][u] = (p.zeros + at)[(uint32_t)l16];
+        }
+    };
+    fetch(blockIdx.x);
+
+    if constexpr (SEG) __syncthreads();  // the partial sums are read
+    T* slab = reinterpret_cast<T*>(part) + w * 16 * PITCH;  // the wave's own: no barrier
+    Rows<T> xa[P][4][MT];
+#pragma unroll
+    for (int r = 0; r < MT; ++r)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        asm volatile("" ::: "memory");  // a wave's LDS accesses complete in order; they stay in this one
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+          if (n * kWave / CPR + 16 * r >= rows) continue;
+          const int at = n * kWave + ln, k = (k0 + i) * kTileK + at % CPR * E;
+          u32x4_t v = raw[r][i][n];
+          if ((k0 + i + 1) * kTileK > p.K) v = place_run<T>(v, k, p.K);  // (uniform)
+          *reinterpret_cast<u32x4_t*>(slab + at / CPR * PITCH + at % CPR * E) = v;
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s1 = mma(xa[i][j][r], fill(0x3f803f80u), s1);
-          s2 = mma(xa[i][j][r], xa[i][j][r].x, s2);
+          u32x4_t v[8 / E];
+#pragma unroll
+          for (int h = 0; h < 8 / E; ++h) v[h] = *reinterpret_cast<const u32x4_t*>(slab + (ln & 15) * PITCH + 32 * j + 8 * (ln >> 4) + E * h);
+          xa[i][j][r].set(v);
         }
-      const int e = l16 & 3;  // row 4 g + e, column l16
-      if (l16 / 4 == g)
-        sums[w][16 * r + l16] = make_float2(e == 0 ? s1[0] : e == 1 ? s1[1] : e == 2 ? s1[2] : s1[3],
-                                            e == 0 ? s2[0] : e == 1 ? s2[1] : e == 2 ? s2[2] : s2[3]);
-    }
-  }
-  __syncthreads();  // the slabs become the partial sums' buffers
-  if constexpr (NORM)
-    if (tid < 16 * MT) {  // (seen by the others from the first barrier of the loop on)
-      float s1 = 0.f, s2 = 0.f;
-      for (int k = 0; k < W; ++k) s1 += sums[k][tid].x, s2 += sums[k][tid].y;
-      const float mean = s1 / (float)p.K;
-      stats[tid] = make_float2(mean, rsqrtf(fmaxf(s2 / (float)p.K - mean * mean, 0.f) + p.eps));
-    }
-  for (int k = W + w; k < MAXW; k += W)  // waves that are not there add nothing
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) part[(i / MT * MAXW + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  int buf = 0, turn = 0;
-  for (int t = blockIdx.x; t < p.tiles_n; t += gridDim.x) {
-    Ending<T, NORM> end;
-    const int own = w >= turn ? w - turn : w + W - turn;  // the row tile that this wave adds up (none past MT)
-    if (own < MT) end.load(p, m0 + 16 * own + 4 * g, m0 + rows, kTileN * t + l16);
-    f32x4_t acc[MT];
-#pragma unroll
-    for (int r = 0; r < MT; ++r) acc[r] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (i == 0 || k0 + i < p.tiles_k)
-        tile_mma<T, MT, GS, ZERO>(q[i], sr[i], zr[i], scales, decode, xa[i], xsum[i], acc);
-    fetch(t + gridDim.x);
-    f32x4_t* mine = part + (buf * MAXW + w) * MT * kWave + lane;
-#pragma unroll
-    for (int r = 0; r < MT; ++r) mine[r * kWave] = acc[r];
-    lds_barrier();
-    for (int r = own; r < MT; r += W) {  // (fewer waves than row tiles: the others follow)
-      if (r != own) end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
-      const f32x4_t* from = part + buf * MAXW * MT * kWave + r * kWave + lane;
-      f32x4_t v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = from[k * MT * kWave];
-      f32x4_t sum = (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-      for (int b = 4; b < MAXW; b += 4)
-        if (W > b) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = from[(b + k) * MT * kWave];
-          sum += (v[0] + v[1]) + (v[2] + v[3]);
-        }
-      end.store(p, sum, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16, NORM ? stats + 16 * r + 4 * g : nullptr);
-    }
-    turn += MT;
-    while (turn >= W) turn -= W;
-    buf ^= 1;
-  }
-}
-
-// Any K: a workgroup of W waves computes MT row tiles by one column tile, the waves taking the 128-column
-// tiles of K in turn and reading x's fragments as they go; the partial sums are added through LDS.
-template <typename T, int MT, int GS, bool ZERO>
-__global__ __launch_bounds__(8 * kWave) void linear4_long_kernel(Linear4Args p) {
-  constexpr int W = 8, GPT = 4 / GS, E = 16 / sizeof(T);
-  __shared__ f32x4_t part[W][MT][kWave];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int l16 = lane & 15, g = lane >> 4;
-  const int t = blockIdx.x, m0 = blockIdx.y * 16 * MT;
-  const int rows = min(16 * MT, p.M - m0);
-  const Decode decode;
-  const Scales scales(p.scales, p.s_f32, l16);
-  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)m0 * p.x_rs;
-  f32x4_t acc[MT];
-#pragma unroll
-  for (int r = 0; r < MT; ++r) acc[r] = {0.f, 0.f, 0.f, 0.f};
-  for (int kt = w; kt < p.tiles_k; kt += W) {
-    const uint4 q = load_tile(p, t, kt, lane);
-    uint32_t sr[GPT];
-    int zr[GPT];
-#pragma unroll
-    for (int u = 0; u < GPT; ++u) {
-      const int64_t at = (int64_t)(kt * GPT + u) * p.np + kTileN * t;
-      sr[u] = scales.raw(at);
-      if constexpr (ZERO) zr[u] = (p.zeros + at)[(uint32_t)l16];
-    }
-    u32x4_t raw[4][MT][8 / E];
-#pragma unroll
-    for (int r = 0; r < MT; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int h = 0; h < 8 / E; ++h)
-          raw[j][r][h] = load_run<T>(x + (int64_t)min(16 * r + l16, rows - 1) * p.x_rs, kt * kTileK + 32 * j + 8 * g + E * h, p.K);
-    Rows<T> xa[4][MT];
-#pragma unroll
-    for (int r = 0; r < MT; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-      {
-        if ((kt + 1) * kTileK > p.K)  // (uniform)
-#pragma unroll
-          for (int h = 0; h < 8 / E; ++h) raw[j][r][h] = place_run<T>(raw[j][r][h], kt * kTileK + 32 * j + 8 * g + E * h, p.K);
-        xa[j][r].set(raw[j][r]);
+        asm volatile("" ::: "memory");
       }
-    f32x4_t xsum[MT];
-    if constexpr (GS == 4 && sizeof(T) == 2) row_sums<T, MT, ZERO>(xa, xsum);
-    tile_mma<T, MT, GS, ZERO>(q, sr, zr, scales, decode, xa, xsum, acc);
-  }
+    f32x4_t xsum[P][MT];
+    if constexpr (GS == 4 && sizeof(T) == 2) {
 #pragma unroll
-  for (int r = 0; r < MT; ++r) part[w][r][lane] = acc[r];
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < MT; ++r)
-    if (w == r) {
-      Ending<T> end;
-      end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
-      f32x4_t v = part[0][r][lane];
-#pragma unroll
-      for (int k = 1; k < W; ++k) v += part[k][r][lane];
-      end.store(p, v, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+      for (int i = 0; i < P; ++i) row_sums<T, MT, ZERO>(xa[i], xsum[i]);
     }
+    if constexpr (NORM) {
+#pragma unroll
+      for (int r = 0; r < MT; ++r) {
+        f32x4_t s1 = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s1 = mma(xa[i][j][r], fill(0x3f803f80u), s1);
+            s2 = mma(xa[i][j][r], xa[i][j][r].x, s2);
+          }
+        const int e = l16 & 3;  // row 4 g + e, column l16
+        if (l16 / 4 == g) {  // (of every segment the same lane)
+          const float2 before = seg ? sums[w][16 * r + l16] : make_float2(0.f, 0.f);
+          sums[w][16 * r + l16] = make_float2(before.x + (e == 0 ? s1[0] : e == 1 ? s1[1] : e == 2 ? s1[2] : s1[3]),
+                                              before.y + (e == 0 ? s2[0] : e == 1 ? s2[1] : e == 2 ? s2[2] : s2[3]));
+        }
+      }
+    }
+    __syncthreads();  // the slabs become the partial sums' buffers
+    if constexpr (NORM)
+      if (seg == segs - 1 && tid < 16 * MT) {  // (seen by the others from the first barrier of the loop on)
+        float s1 = 0.f, s2 = 0.f;
+        for (int k = 0; k < W; ++k) s1 += sums[k][tid].x, s2 += sums[k][tid].y;
+        const float mean = s1 / (float)p.K;
+        stats[tid] = make_float2(mean, rsqrtf(fmaxf(s2 / (float)p.K - mean * mean, 0.f) + p.eps));
+      }
+    for (int k = W + w; k < MAXW; k += W)  // waves that are not there add nothing
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) part[(i / MT * MAXW + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    int buf = 0, turn = 0;
+    f32x4_t* kept = hold;
+    for (int t = blockIdx.x; t < p.tiles_n; t += gridDim.x, kept += MT * kWave) {
+      Ending<T, NORM> end;
+      const int own = w >= turn ? w - turn : w + W - turn;  // the row tile that this wave adds up (none past MT)
+      if (own < MT) end.load(p, m0 + 16 * own + 4 * g, m0 + rows, kTileN * t + l16);
+      f32x4_t acc[MT];
+#pragma unroll
+      for (int r = 0; r < MT; ++r) acc[r] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if ((i == 0 && !SEG) || k0 + i < p.tiles_k)
+          tile_mma<T, MT, GS, ZERO>(q[i], sr[i], zr[i], scales, decode, xa[i], xsum[i], acc);
+      fetch(t + gridDim.x);
+      f32x4_t* mine = part + (buf * MAXW + w) * MT * kWave + lane;
+#pragma unroll
+      for (int r = 0; r < MT; ++r) mine[r * kWave] = acc[r];
+      lds_barrier();
+      for (int r = own; r < MT; r += W) {  // (fewer waves than row tiles: the others follow)
+        if (r != own) end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+        const f32x4_t* from = part + buf * MAXW * MT * kWave + r * kWave + lane;
+        f32x4_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = from[k * MT * kWave];
+        f32x4_t sum = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+        for (int b = 4; b < MAXW; b += 4)
+          if (W > b) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = from[(b + k) * MT * kWave];
+            sum += (v[0] + v[1]) + (v[2] + v[3]);
+          }
+        if (seg > 0) sum += kept[r * kWave];  // the same wave's in every segment
+        if (seg < segs - 1) {
+          kept[r * kWave] = sum;
+          continue;
+        }
+        end.store(p, sum, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16, NORM ? stats + 16 * r + 4 * g : nullptr);
+      }
+      turn += MT;
+      while (turn >= W) turn -= W;
+      buf ^= 1;
+    }
+  }
 }
 
 // The registers hold up to 64 bf16 rows of 16 column tiles (2048 columns) in 8 waves, or 32 rows of 24
 // in 12; of fp32 rows, whose three parts take three times as many, 16.  More rows run as row blocks of
-// equal height, which read the weight again (out of the caches); longer rows run on linear4_long_kernel.
+// equal height, which read the weight again (out of the caches); longer rows in segments of K, whose
+// sums wait in LDS (a workgroup takes no more tiles than fit).  64 rows
+// at once where that takes no more segments than 32 (us with 64 and 32: 64 x 4096 x 4352, three segments or
+// two, 22.9, 14.4; 384 rows 43.1, 36.7; 64 x 50304 x 4096, two both ways, 45.3, 53.5).  Read anew for
+// every output tile, without registers, 64 x 8576 x 4096 took 40 us instead of 23.
 //
 // A row block has the CUs that the others leave (128 x 8576 x 2048 with all of them for each block 19.0 us, with half 14.1; 192
 // rows 27.4, 17.9): x is read once per workgroup, 256 KB at 64 rows of 2048.
@@ -490,40 +453,44 @@ __global__ __launch_bounds__(8 * kWave) void linear4_long_kernel(Linear4Args p) 
 // 4.6, 4.0; 64 x 3264 x 768 6.7, 5.5; 64 x 50277 x 768 19.9, 18.4; fp32 3 x 3264 x 768 5.9, 5.6, 16 x 25600 x 1500 24.2, 17.9).  Two
 // for one row tile of bf16 and more than two output tiles for every CU: there the sums over the waves count (16 x 8192 x 1152
 // 5.1, 4.6, x 12800 6.3, 6.7, x 25600 7.8, 9.9).
-constexpr int kWidest = 24, kWide = 16, kCUs = 256;
+constexpr int kCUs = 256, kHeldBytes = kWave * 16;
+constexpr int kLds = 152 * 1024;  // for the slabs, partial and held sums; NORM's sums take up to 6 KB more
 
-template <typename T, int MT, int P, int GS, bool ZERO, int MAXW>
+template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool SEG>
 void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
-  const int W = (a.tiles_k + P - 1) / P;
+  const int W = ((a.tiles_k + a.segs - 1) / a.segs + P - 1) / P;
   // waves per CU: 8 where the registers hold more than one row tile of two column tiles, else 16: whole workgroups
   const int per_cu = (MT == 1 || P == 1 ? 16 : 8) / W;
-  const int slots = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m, most = slots > 1 ? slots : 1;
-  const size_t slabs = (size_t)W * 16 * (kTileK * sizeof(T) + 16), parts = (size_t)2 * MAXW * MT * kWave * 16;
-  const dim3 grid((unsigned)(a.tiles_n < most ? a.tiles_n : most), (unsigned)blocks_m);
+  int most = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m;
+  const int slabs = W * 16 * (kTileK * (int)sizeof(T) + 16), parts = 2 * MAXW * MT * kHeldBytes;
+  int shmem = slabs > parts ? slabs : parts;
+  if (a.segs > 1) {
+    const int room = (kLds - shmem) / kHeldBytes / MT, least = (a.tiles_n + room - 1) / room;  // column tiles of a workgroup
+    most = most > least ? most : least;
+  }
+  if (most < 1) most = 1;
+  if (most > a.tiles_n) most = a.tiles_n;
+  if (a.segs > 1) shmem += (a.tiles_n + most - 1) / most * MT * kHeldBytes;
+  const dim3 grid((unsigned)most, (unsigned)blocks_m);
   if constexpr (sizeof(T) == 2)
     if (a.row_sums) {
-      HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, true>), grid, dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+      HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, true, SEG>), grid, dim3(W * kWave), shmem, s, a);
       return;
     }
-  HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, false>), grid, dim3(W * kWave), slabs > parts ? slabs : parts, s, a);
+  HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, false, SEG>), grid, dim3(W * kWave), shmem, s, a);
 }
 template <typename T, int MT, int GS, bool ZERO, int MAXW> void pick_tiles(const Linear4Args& a, int blocks_m, hipStream_t s) {
   const bool one = a.tiles_k <= MAXW && (MT > 1 || sizeof(T) == 4 || a.tiles_n <= 2 * kCUs);
-  one ? launch_linear4<T, MT, 1, GS, ZERO, MAXW>(a, blocks_m, s) : launch_linear4<T, MT, 2, GS, ZERO, MAXW>(a, blocks_m, s);
+  if (a.segs > 1) launch_linear4<T, MT, 2, GS, ZERO, MAXW, true>(a, blocks_m, s);
+  else if (one) launch_linear4<T, MT, 1, GS, ZERO, MAXW, false>(a, blocks_m, s);
+  else launch_linear4<T, MT, 2, GS, ZERO, MAXW, false>(a, blocks_m, s);
 }
-template <typename T, int MT, int GS, bool ZERO> void launch_long(const Linear4Args& a, hipStream_t s) {
-  HDCM_LAUNCH((linear4_long_kernel<T, MT, GS, ZERO>), dim3((unsigned)a.tiles_n, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
-              dim3(8 * kWave), 0, s, a);
-}
-template <typename T, int GS, bool ZERO> void pick_rows(const Linear4Args& a, hipStream_t s) {
+template <typename T, int GS, bool ZERO> void pick_rows(Linear4Args a, hipStream_t s) {
   const int tiles_m = (a.M + 15) / 16;
-  if (a.tiles_k > kWidest) {
-    tiles_m == 1 ? launch_long<T, 1, GS, ZERO>(a, s) : launch_long<T, 2, GS, ZERO>(a, s);
-    return;
-  }
-  const bool wide = a.tiles_k > kWide;
-  const int most = sizeof(T) == 4 ? 1 : wide ? 2 : 4;
+  const auto segments = [&](int widest) { return (a.tiles_k + widest - 1) / widest; };
+  const int most = sizeof(T) == 4 ? 1 : segments(24) < segments(16) ? 2 : 4;
   const int blocks = (tiles_m + most - 1) / most, mt = (tiles_m + blocks - 1) / blocks;
+  a.segs = segments(mt > 2 ? 16 : 24);
   if (mt == 1) pick_tiles<T, 1, GS, ZERO, 12>(a, blocks, s);
   if constexpr (sizeof(T) == 2) {
     if (mt == 2) pick_tiles<T, 2, GS, ZERO, 12>(a, blocks, s);
@@ -730,8 +697,6 @@ extern "C" int hdcm_w4_dequant(const void* packed, const void* scales, int scale
   return hdcm_launch_status();
 }
 
-extern "C" int64_t hdcm_w4_norm_max_k(void) { return kWidest * kTileK; }
-
 extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sums, float eps, const void* packed, const void* scales,
                                   int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias, const void* res,
                                   int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N, int64_t K,
@@ -741,7 +706,7 @@ extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const flo
   HDCM_CHECK_ARG(M >= 0 && N >= 0 && K > 0, HDCM_EINVAL);
   HDCM_CHECK_ARG(M == 0 || N == 0 || (x && packed && scales && out), HDCM_EINVAL);
   HDCM_CHECK_ARG(M <= 1 || (x_row_stride >= K && out_row_stride >= N && (!res || res_row_stride >= N)), HDCM_EINVAL);
-  HDCM_CHECK_ARG(!row_sums || (dtype == HDCM_BF16 && K <= kWidest * kTileK), HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(!row_sums || dtype == HDCM_BF16, HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(sizes_ok(N, K, group) && K >= (dtype == HDCM_F32 ? 4 : 8) && M <= 16 * 65535, HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(hdcm_aligned16(packed) && ((uintptr_t)scales & 3u) == 0, HDCM_EALIGN);
   if (M == 0 || N == 0) return HDCM_OK;

@@ -659,7 +659,7 @@ class HdcMamba9v3Block(nn.Module):
                         self.group_norm.bias, 1e-5, state.h, state.S_prev, state.S_intra, state.pos, C, combined, dm, H,
                         pos_dev=pos_dev)
         eps = 1e-5
-        if x.dtype != torch.bfloat16 or ds + dm > _ops.lib().hdcm_w4_norm_max_k():  # not for the product's own LayerNorm
+        if x.dtype != torch.bfloat16:  # the product's own LayerNorm is for bfloat16
             _ops.layer_norm(combined, eps=eps, out=combined)
             eps = None
         y = linear_4bit(combined, self.out_proj.weight4, residual=x, norm_eps=eps)

@@ -86,6 +86,12 @@ LINEAR = [
     (2, 3, 20, 32, True, BF, F32),
     (4, 9, 17, 64, True, F32, BF),
     (129, 128, 4200, 64, False, BF, BF),   # more output tiles than workgroups
+    (64, 4096, 200, 128, False, BF, BF),   # two segments of K
+    (41, 4000, 4200, 64, True, F32, BF),
+    (90, 3300, 150, 32, True, BF, BF),
+    (2, 9000, 8200, 128, True, BF, BF),
+    (1100, 3300, 5200, 128, False, BF, BF),  # more sums to hold than a workgroup has room for
+    (30, 6500, 100, 64, False, BF, F32),
 ]
 
 
@@ -133,7 +139,7 @@ def test_linear_4bit_layouts(dev, dtype):
 
 @pytest.mark.parametrize("M,K,N,group,zeros", [
     (1, 8, 16, 32, False), (1, 1152, 100, 128, False), (16, 2176, 70, 128, True), (5, 333, 33, 32, True),
-    (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True),
+    (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True), (33, 5000, 300, 128, False),
     (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True)])
 def test_linear_4bit_with_layer_norm(dev, M, K, N, group, zeros):
     """norm_eps against the LayerNorm and product in 64 bits.
@@ -283,9 +289,6 @@ def test_weight_refusals(dev):
         hm.linear_4bit(x, w, norm_eps=-1.0)
     with pytest.raises(RuntimeError, match="norm_eps"):
         hm.linear_4bit(x.float(), w, norm_eps=1e-5)
-    long = hm.Weight4Bit.quantize(torch.randn(16, _ops.lib().hdcm_w4_norm_max_k() + 1, device=dev))
-    with pytest.raises(_ops.HdcmError):
-        hm.linear_4bit(torch.zeros(1, long.shape[1], device=dev, dtype=BF), long, norm_eps=1e-5)
     buf = torch.zeros(4, 256, device=dev, dtype=BF)
     with pytest.raises(RuntimeError, match="share no other memory"):
         hm.linear_4bit(buf[:, :128], w, out=buf[:, 100:132])
