@@ -310,7 +310,7 @@ __device__ __forceinline__ void each_id(const int64_t* ids, int64_t n, int v0, i
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint64_t at = (uint64_t)(id[u] - v0);
+      const uint64_t at = (uint64_t)id[u] - (uint64_t)v0;
       if (i0 + u * kHistThreads + threadIdx.x < n && at < (uint64_t)size) f((int)at);
     }
   }
@@ -377,6 +377,7 @@ __global__ __launch_bounds__(kWave) void token_append_kernel(int16_t* table, int
 }
 
 constexpr int64_t kMaxVocab = (int64_t)1 << 30, kMaxRows = 65535;
+constexpr int64_t kMaxIds = (int64_t)1 << 30;  // of a row: a count of them and of what the table holds stays below bit 31
 
 int check_controls(const hdcm_logits_controls* c, int64_t B, int64_t V) {
   HDCM_CHECK_ARG(c, HDCM_EINVAL);
@@ -453,7 +454,7 @@ extern "C" int hdcm_token_history_fill(int16_t* table, int64_t table_row_stride,
   if (B == 0 || V == 0) return HDCM_OK;
   HDCM_CHECK_ARG(table && (prompt || P == 0) && (output || O == 0), HDCM_EINVAL);
   HDCM_CHECK_ARG(B == 1 || (table_row_stride >= V && prompt_row_stride >= P && output_row_stride >= O), HDCM_EINVAL);
-  HDCM_CHECK_ARG(V <= kMaxVocab && B <= kMaxRows && P < ((int64_t)1 << 31) && O < ((int64_t)1 << 31), HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(V <= kMaxVocab && B <= kMaxRows && P <= kMaxIds && O <= kMaxIds, HDCM_EUNSUPPORTED);
   const dim3 grid((unsigned)((V + kHistSlice - 1) / kHistSlice), (unsigned)B);
   HDCM_LAUNCH(token_history_kernel, grid, dim3(kHistThreads), 0, (hipStream_t)stream, table, table_row_stride, prompt,
               prompt_row_stride, prompt_lengths, P, output, output_row_stride, output_lengths, O, (int)V, false);
@@ -467,7 +468,7 @@ extern "C" int hdcm_token_history_append(int16_t* table, int64_t table_row_strid
   if (B == 0 || V == 0 || T == 0) return HDCM_OK;
   HDCM_CHECK_ARG(table && tokens, HDCM_EINVAL);
   HDCM_CHECK_ARG(B == 1 || (table_row_stride >= V && tokens_row_stride >= T), HDCM_EINVAL);
-  HDCM_CHECK_ARG(V <= kMaxVocab && B <= kMaxRows && T < ((int64_t)1 << 31), HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(V <= kMaxVocab && B <= kMaxRows && T <= kMaxIds, HDCM_EUNSUPPORTED);
   hipStream_t s = (hipStream_t)stream;
   // up to 16 tokens a row (a step, or a few accepted drafts) touch single entries; more are counted slice by slice
   if (T <= 16)

@@ -4,6 +4,7 @@
 // library products.  A block forward is 7-9 launches; issued one by one through ctypes they cost
 // about 190 us of Python per block, more than the kernels take below ~8192 rows.  Nothing is kept
 // between calls: workspaces that outlive a call are passed in.
+#include <array>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -624,14 +625,25 @@ bool same_place(const Tensor& a, const Tensor& b) {
   return a.const_data_ptr() == b.const_data_ptr() && (a.size(0) <= 1 || a.stride(0) == b.stride(0));
 }
 
-// A packed weight, checked once (the handle of a Weight4Bit)
+// A packed weight, checked once (the handle of a Weight4Bit), and its row sums as the products give them: for
+// products behind a LayerNorm, formed again where a buffer was written since (load_state_dict)
 struct Weight4 {
-  Tensor packed, scales, zeros, row_sums;  // row_sums: as the products give them
+  Tensor packed, scales, zeros, row_sums;
   int64_t N, K, group;
   int scale_dtype;
+  std::array<uint32_t, 3> versions{};
+  std::array<uint32_t, 3> versions_now() const {
+    const auto of = [](const Tensor& t) { return t.defined() && !t.is_inference() ? (uint32_t)t._version() : 0u; };
+    return {of(packed), of(scales), of(zeros)};
+  }
 };
-Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, const OptTensor& residual_,
-                   const OptTensor& out_, std::optional<double> norm_eps);
+Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const OptTensor& residual_, const OptTensor& out_,
+                   std::optional<double> norm_eps);
+void sum_rows(Weight4& w) {
+  const at::NoGradGuard guard;
+  w.versions = w.versions_now();
+  linear_4bit(at::ones({1, w.K}, w.row_sums.options()), w, std::nullopt, std::nullopt, w.row_sums.unsqueeze(0), std::nullopt);
+}
 Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor& zeros, int64_t N, int64_t K, int64_t group) {
   on_gpu(packed);
   Weight4 w{packed, scales, or_none(zeros), Tensor(), N, K, group, dtype_of(scales)};
@@ -647,14 +659,13 @@ Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor
     TORCH_CHECK(w.zeros.scalar_type() == at::kByte && w.zeros.is_contiguous() && w.zeros.numel() == per,
                 "zeros must hold one byte per scale");
   }
-  const at::NoGradGuard guard;
-  w.row_sums = linear_4bit(at::ones({1, K}, packed.options().dtype(at::kFloat)), w, std::nullopt, std::nullopt, std::nullopt,
-                           std::nullopt).view({N});
+  w.row_sums = fp32({N}, packed);
+  sum_rows(w);
   return w;
 }
 
-Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, const OptTensor& residual_,
-                   const OptTensor& out_, std::optional<double> norm_eps) {
+Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const OptTensor& residual_, const OptTensor& out_,
+                   std::optional<double> norm_eps) {
   const Tensor &bias = or_none(bias_), &residual = or_none(residual_), &given = or_none(out_);
   on_gpu(x);
   no_gradient("linear_4bit", {&x, &bias, &residual, &given});
@@ -687,11 +698,13 @@ Tensor linear_4bit(const Tensor& x, const Weight4& w, const OptTensor& bias_, co
     r = rows(residual);
   }
   if (given.defined())
-    TORCH_CHECK(!overlap(o, xr) && (!r.defined() || same_place(o, r) || !overlap(o, r)),
-                "linear_4bit: out may be the residual itself but share no other memory with x or the residual");
+    TORCH_CHECK(!overlap(o, xr) && (!b.defined() || !overlap(o, b.unsqueeze(0))) &&
+                    (!r.defined() || same_place(o, r) || !overlap(o, r)),
+                "linear_4bit: out may be the residual itself but share no other memory with x, the bias or the residual");
   int64_t K = w.K;
   TORCH_CHECK(!norm_eps || (*norm_eps >= 0 && K >= 8 && dt == HDCM_BF16),
               "linear_4bit: norm_eps must not be negative, the rows bfloat16 and of 8 columns at least");
+  if (norm_eps && w.versions != w.versions_now()) sum_rows(w);
   if (K < 8) {  // shorter than a load of the kernel's: columns of zeros, which the packed weight holds too
     xr = at::constant_pad_nd(xr, {0, 8 - K});
     K = 8;
@@ -756,6 +769,7 @@ Controls controls_of(const ControlArgs& a, const Tensor& logits) {
                 "history must be an int16 table [", B, ", ", V, "] with contiguous rows");
     c.history = history->const_data_ptr<int16_t>();
     c.history_row_stride = history->stride(0);
+    k.held.push_back(*history);
   }
   if (bias) {
     std::tie(c.bias, c.bias_row_stride) = shared_rows(*bias, B, V, logits, "bias", k.held);
@@ -790,7 +804,7 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
     TORCH_CHECK(same_place(out, l) || !overlap(out, l),
                 "process_logits: out may be the logits themselves but share no other memory with them");
     for (const Tensor& t : k.held)
-      TORCH_CHECK(t.dim() != 2 || !overlap(out, t), "process_logits: out shares memory with the bias or the mask");
+      TORCH_CHECK(!overlap(out, t.dim() == 1 ? t.unsqueeze(0) : t), "process_logits: out shares memory with the penalties, the history, the bias or the mask");
   } else {
     out = at::empty(logits.sizes(), logits.options());
   }
@@ -905,7 +919,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mixer_backward", &mixer_backward);
   m.def("norm_conv_forward", &norm_conv_forward);
   m.def("norm_conv_backward", &norm_conv_backward);
-  pybind11::class_<Weight4>(m, "Weight4").def(pybind11::init(&make_weight4));
+  pybind11::class_<Weight4>(m, "Weight4").def(pybind11::init(&make_weight4)).def("refresh", &sum_rows);
   m.def("linear_4bit", &linear_4bit);
   m.def("process_logits", &process_logits);
   m.def("select_tokens", &select_tokens);

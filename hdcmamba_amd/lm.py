@@ -159,8 +159,9 @@ class DecodeGraph:
 
     With ``controls`` (the keyword arguments of sampling.select_tokens but for the logits) the recording goes on
     to choose the next token of every sequence, counts it in controls["history"] where there is one and
-    leaves it as the next input: ``next`` replays from there.  Tensors among the controls are read at
-    replay time: noise, masks and penalties are changed in place between replays.
+    leaves it as the next input: ``next`` replays from there (``step`` replays the same recording, choice and
+    count included).  Tensors among the controls are read at replay time: noise, masks and penalties are
+    changed in place between replays.
     """
 
     def __init__(self, lm, states, controls=None):

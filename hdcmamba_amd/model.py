@@ -821,8 +821,8 @@ def set_differentiable_mixer(module, enabled=True):
 
 def quantize_4bit(module, group_size=128, zero_points=False, head=True):
     """Round in_proj and out_proj of every HdcMamba9v3Block inside ``module`` to 4 bits with group scales
-    (Weight4Bit.quantize, scales in the weight's type), and with ``head`` an HdcMambaLM's head (the
-    embedding that it shares its weight with keeps it); returns ``module``, on the GPU and for inference
+    (Weight4Bit.quantize, scales in the weight's type), and with ``head`` every ``lm_head`` (the embedding
+    that HdcMambaLM's shares its weight with keeps it); returns ``module``, on the GPU and for inference
     only from then on.  A decode step then streams a quarter of the weights' bytes."""
     for m in module.modules():
         names = ("in_proj", "out_proj") if isinstance(m, HdcMamba9v3Block) else ("lm_head",) if head else ()

@@ -21,7 +21,8 @@ GROUP_SIZES = (32, 64, 128)
 
 class Weight4Bit:
     """A packed 4-bit weight: made once from codes (``from_codes``) or by rounding a weight
-    (``quantize``), then passed to linear_4bit.  Not changed after that.
+    (``quantize``), then passed to linear_4bit.  Its buffers may be written in place (load_state_dict); a
+    recorded graph with norm_eps sees that after ``refresh``.
 
     ``shape`` (N, K), ``group_size``; ``packed`` uint8, ``scales`` (float32 or bfloat16) and ``zeros``
     (uint8 or None) in the layout of hdcm_w4_linear_fwd (include/hdcm.h)."""
@@ -125,6 +126,10 @@ class Weight4Bit:
         move = lambda t: None if t is None else t.to(device)  # noqa: E731
         return Weight4Bit(move(self.packed), move(self.scales), move(self.zeros), self.shape, self.group_size)
 
+    def refresh(self):
+        """Bring what the weight keeps beside its buffers (the row sums of norm_eps) in line with them."""
+        self._handle.refresh()
+
     def __repr__(self):
         return (f"Weight4Bit({self.shape[0]}x{self.shape[1]}, group_size={self.group_size}, "
                 f"zero_points={self.zeros is not None}, scales={self.scales.dtype}, device={self.packed.device})")
@@ -174,7 +179,14 @@ class Linear4Bit(nn.Module):
             w = self._weight4 = Weight4Bit(self.packed, self.scales, self.zeros, w.shape, w.group_size)
         return w
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        if self.packed.is_cuda:
+            self.weight4.refresh()
+
     def forward(self, x):
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("a Linear4Bit has no gradient: call it under torch.no_grad() or on detached tensors")
         rows = x.numel() // max(x.shape[-1], 1)
         if rows > self.direct_rows:
             return F.linear(x, self.weight4.dequantize(x.dtype), None if self.bias is None else self.bias.to(x.dtype))

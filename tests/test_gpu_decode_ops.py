@@ -621,3 +621,65 @@ def test_recorded_step_matches_eager(dev):
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
         assert torch.equal(c["history"], eager["history"]), i
+
+
+def test_row_sums_follow_the_weight(dev):
+    """A loaded state dict changes the weight in place: norm_eps uses the new weight's row sums, eagerly and, the module
+    having loaded it, in a graph recorded before."""
+    one, two = (torch.nn.Linear(256, 96, bias=False, device=dev, dtype=BF) for _ in range(2))
+    layer, other = hm.Linear4Bit.from_linear(one, 64), hm.Linear4Bit.from_linear(two, 64)
+    x = (torch.randn(5, 256, generator=_gen(1)) + 2).to(BF).to(dev)
+    with torch.no_grad():
+        want = hm.linear_4bit(x, other.weight4, norm_eps=1e-5)
+        hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+        layer.load_state_dict(other.state_dict())
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+            assert torch.equal(hm.linear_4bit(x, layer.weight4, norm_eps=1e-5), want)
+        w = hm.Weight4Bit.quantize(one.weight, 64)
+        for name in ("packed", "scales"):  # by hand
+            getattr(w, name).copy_(getattr(other.weight4, name))
+        assert torch.equal(hm.linear_4bit(x, w, norm_eps=1e-5), want)
+
+
+def test_shared_memory_is_refused(dev):
+    w = hm.Weight4Bit.quantize(torch.randn(32, 64, generator=_gen(5)).to(dev), 32)
+    out = torch.zeros(3, 32, device=dev)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="memory"):
+        hm.linear_4bit(torch.zeros(3, 64, device=dev), w, bias=out[1], out=out)
+    logits, table = torch.zeros(4, 64, device=dev), torch.zeros(4, 64, device=dev, dtype=torch.int16)
+    out = torch.zeros(4, 64, device=dev)
+    with pytest.raises(RuntimeError, match="memory"):
+        hm.process_logits(logits, history=table, repetition=out[2, :4], out=out)
+    with pytest.raises(RuntimeError, match="memory"):
+        hm.process_logits(logits, history=out.view(torch.int16)[:, :64], presence=1.0, out=out)
+    with pytest.raises(RuntimeError, match="memory"):
+        hm.process_logits(logits, bias=out[0], out=out)
+
+
+@pytest.mark.parametrize("rows", [2, 500])
+def test_linear4bit_module_has_no_gradient(dev, rows):
+    layer = hm.Linear4Bit.from_linear(torch.nn.Linear(64, 32, device=dev), 32)
+    x = torch.randn(rows, 64, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer(x)
+    assert not layer(x.detach()).requires_grad
+
+
+def test_history_passes_over_any_other_id(dev):
+    far = [-(2**63), 2**63 - 1, -1, 40, 2**32 + 3, -(2**32) + 3]
+    table = hm.new_token_history(1, 40, dev)
+    hm.fill_token_history(table, prompt=torch.tensor([far + [3]], device=dev), output=torch.tensor([far + [5, 5]], device=dev))
+    want = torch.zeros(40, dtype=torch.int16)
+    want[3], want[5] = -(2**15), 2
+    assert torch.equal(table[0].cpu(), want)
+    hm.append_tokens(table, torch.tensor([far + [3]], device=dev))
+    hm.append_tokens(table, torch.tensor([far * 3 + [3]], device=dev))
+    want[3] = -(2**15) + 2
+    assert torch.equal(table[0].cpu(), want)
