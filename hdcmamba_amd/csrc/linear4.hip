@@ -272,9 +272,9 @@ template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool NORM, boo
 __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4_kernel(Linear4Args p) {
   constexpr int GPT = 4 / GS;
   constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
-  extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [2][MAXW][MT][64]; at first the waves' slabs of x
+  extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [2][WP][MT][64]; at first the waves' slabs of x
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int W = blockDim.x / kWave;
+  const int W = blockDim.x / kWave, WP = (W + 3) & ~3;
   const int l16 = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * 16 * MT;
   const int rows = min(16 * MT, p.M - m0);
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
   const Scales scales(p.scales, p.s_f32, l16);
 
   // with more than one segment: the sums of the workgroup's tiles so far, behind the slabs and the partial sums
-  f32x4_t* hold = part + max(2 * MAXW * MT * kWave, W * 16 * PITCH * (int)sizeof(T) / 16) + lane;
+  f32x4_t* hold = part + max(2 * WP * MT * kWave, W * 16 * PITCH * (int)sizeof(T) / 16) + lane;
   __shared__ float2 sums[NORM ? MAXW : 1][16 * MT], stats[NORM ? 16 * MT : 1];
   const int segs = SEG ? p.segs : 1;
   for (int seg = 0; seg < segs; ++seg) {
@@ -387,9 +387,9 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
         const float mean = s1 / (float)p.K;
         stats[tid] = make_float2(mean, rsqrtf(fmaxf(s2 / (float)p.K - mean * mean, 0.f) + p.eps));
       }
-    for (int k = W + w; k < MAXW; k += W)  // waves that are not there add nothing
+    for (int k = W + w; k < WP; k += W)  // waves that are not there add nothing
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) part[(i / MT * MAXW + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 2 * MT; ++i) part[(i / MT * WP + k) * MT * kWave + i % MT * kWave + lane] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     int buf = 0, turn = 0;
     f32x4_t* kept = hold;
@@ -405,13 +405,21 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
         if ((i == 0 && !SEG) || k0 + i < p.tiles_k)
           tile_mma<T, MT, GS, ZERO>(q[i], sr[i], zr[i], scales, decode, xa[i], xsum[i], acc);
       fetch(t + gridDim.x);
-      f32x4_t* mine = part + (buf * MAXW + w) * MT * kWave + lane;
+      if (P == 1 && MT <= 2 && W == 1) {  // nothing to add up
+#pragma unroll
+        for (int r = 0; r < MT; ++r) {
+          if (r > 0) end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
+          end.store(p, acc[r], m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16, NORM ? stats + 16 * r + 4 * g : nullptr);
+        }
+        continue;
+      }
+      f32x4_t* mine = part + (buf * WP + w) * MT * kWave + lane;
 #pragma unroll
       for (int r = 0; r < MT; ++r) mine[r * kWave] = acc[r];
       lds_barrier();
       for (int r = own; r < MT; r += W) {  // (fewer waves than row tiles: the others follow)
         if (r != own) end.load(p, m0 + 16 * r + 4 * g, m0 + rows, kTileN * t + l16);
-        const f32x4_t* from = part + buf * MAXW * MT * kWave + r * kWave + lane;
+        const f32x4_t* from = part + buf * WP * MT * kWave + r * kWave + lane;
         f32x4_t v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = from[k * MT * kWave];
@@ -440,19 +448,24 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
 // The registers hold up to 64 bf16 rows of 16 column tiles (2048 columns) in 8 waves, or 32 rows of 24
 // in 12; of fp32 rows, whose three parts take three times as many, 16.  More rows run as row blocks of
 // equal height, which read the weight again (out of the caches); longer rows in segments of K, whose
-// sums wait in LDS (a workgroup takes no more tiles than fit).  64 rows
-// at once where that takes no more segments than 32 (us with 64 and 32: 64 x 4096 x 4352, three segments or
-// two, 22.9, 14.4; 384 rows 43.1, 36.7; 64 x 50304 x 4096, two both ways, 45.3, 53.5).  Read anew for
-// every output tile, without registers, 64 x 8576 x 4096 took 40 us instead of 23.
+// sums wait in LDS (a workgroup takes no more tiles than fit).  Figures below in us, rows x N x K.
 //
-// A row block has the CUs that the others leave (128 x 8576 x 2048 with all of them for each block 19.0 us, with half 14.1; 192
+// Height of a row block: 64 rows where that takes no more segments than 32 (with 64 and 32: 64 x 4096 x 4352, three
+// segments or two, 22.9, 14.4; 384 rows 43.1, 36.7; 64 x 50304 x 4096, two both ways, 45.3, 53.5) and K has more than four
+// tiles, below which the few waves of a workgroup with the registers of 64 rows leave the SIMDs empty (64 x 20000 x 384 10.4,
+// 7.6; 106 x 46400 x 192 21.0, 16.6; but 33 x 50277 x 768 17.1, 22.7); lower where there are so few column tiles that
+// more blocks still make no more than four workgroups for every CU: a block's rows take the longest part of such a run
+// (64 x 1024 x 1152 in one block and four 7.1, 3.9; 64 x 2048 x 2176 in two and four 6.8, 5.7; 128 x 3264 x 768 in
+// two and five 7.3, 6.3; with eight workgroups for every CU 128 x 8576 x 2048 13.6, 14.2).
+//
+// A row block has the CUs that the others leave (128 x 8576 x 2048 with all of them for each block 19.0, with half 14.1; 192
 // rows 27.4, 17.9): x is read once per workgroup, 256 KB at 64 rows of 2048.
 //
-// Column tiles a wave: one, where that makes no more waves than a workgroup has, since the rows' way into the fragments, the
-// longest part of a short run, then has twice the waves (us with two and one: 16 x 1024 x 1152 3.9, 3.5; 32 x 3264 x 768
-// 4.6, 4.0; 64 x 3264 x 768 6.7, 5.5; 64 x 50277 x 768 19.9, 18.4; fp32 3 x 3264 x 768 5.9, 5.6, 16 x 25600 x 1500 24.2, 17.9).  Two
-// for one row tile of bf16 and more than two output tiles for every CU: there the sums over the waves count (16 x 8192 x 1152
-// 5.1, 4.6, x 12800 6.3, 6.7, x 25600 7.8, 9.9).
+// Column tiles a wave: one, where that makes no more than 12 waves (16 of fp32, 8 with more than 32 rows: the registers),
+// since the rows' way into the fragments then has twice the waves (with two and one: 16 x 1024 x 1152 3.9, 3.5; 32 x 3264 x
+// 768 4.6, 4.0; 64 x 3264 x 768 6.7, 5.5; 64 x 50277 x 768 19.9, 18.4; fp32 3 x 3264 x 768 5.9, 5.6, 16 x 8576 x 2048
+// 17.8, 11.5).  Two for one row tile of bf16 and more than two output tiles for every CU: there the sums over the
+// waves count (16 x 8192 x 1152 5.1, 4.6, x 12800 6.3, 6.7, x 25600 7.8, 9.9).
 constexpr int kCUs = 256, kHeldBytes = kWave * 16;
 constexpr int kLds = 152 * 1024;  // for the slabs, partial and held sums; NORM's sums take up to 6 KB more
 
@@ -462,7 +475,7 @@ void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
   // waves per CU: 8 where the registers hold more than one row tile of two column tiles, else 16: whole workgroups
   const int per_cu = (MT == 1 || P == 1 ? 16 : 8) / W;
   int most = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m;
-  const int slabs = W * 16 * (kTileK * (int)sizeof(T) + 16), parts = 2 * MAXW * MT * kHeldBytes;
+  const int slabs = W * 16 * (kTileK * (int)sizeof(T) + 16), parts = 2 * ((W + 3) & ~3) * MT * kHeldBytes;
   int shmem = slabs > parts ? slabs : parts;
   if (a.segs > 1) {
     const int room = (kLds - shmem) / kHeldBytes / MT, least = (a.tiles_n + room - 1) / room;  // column tiles of a workgroup
@@ -480,16 +493,19 @@ void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
   HDCM_LAUNCH((linear4_kernel<T, MT, P, GS, ZERO, MAXW, false, SEG>), grid, dim3(W * kWave), shmem, s, a);
 }
 template <typename T, int MT, int GS, bool ZERO, int MAXW> void pick_tiles(const Linear4Args& a, int blocks_m, hipStream_t s) {
-  const bool one = a.tiles_k <= MAXW && (MT > 1 || sizeof(T) == 4 || a.tiles_n <= 2 * kCUs);
+  constexpr int most1 = MT > 2 ? 8 : sizeof(T) == 4 ? 16 : 12;
+  const bool one = a.tiles_k <= most1 && (MT > 1 || sizeof(T) == 4 || a.tiles_n <= 2 * kCUs);
   if (a.segs > 1) launch_linear4<T, MT, 2, GS, ZERO, MAXW, true>(a, blocks_m, s);
-  else if (one) launch_linear4<T, MT, 1, GS, ZERO, MAXW, false>(a, blocks_m, s);
+  else if (one) launch_linear4<T, MT, 1, GS, ZERO, most1, false>(a, blocks_m, s);
   else launch_linear4<T, MT, 2, GS, ZERO, MAXW, false>(a, blocks_m, s);
 }
 template <typename T, int GS, bool ZERO> void pick_rows(Linear4Args a, hipStream_t s) {
   const int tiles_m = (a.M + 15) / 16;
   const auto segments = [&](int widest) { return (a.tiles_k + widest - 1) / widest; };
-  const int most = sizeof(T) == 4 ? 1 : segments(24) < segments(16) ? 2 : 4;
-  const int blocks = (tiles_m + most - 1) / most, mt = (tiles_m + blocks - 1) / blocks;
+  const int most = sizeof(T) == 4 ? 1 : a.tiles_k <= 4 || segments(24) < segments(16) ? 2 : 4;
+  const int least = (tiles_m + most - 1) / most, room = 4 * kCUs / a.tiles_n, fill = room < tiles_m ? room : tiles_m;
+  const int blocks = least > fill ? least : fill;
+  const int mt = (tiles_m + blocks - 1) / blocks;
   a.segs = segments(mt > 2 ? 16 : 24);
   if (mt == 1) pick_tiles<T, 1, GS, ZERO, 12>(a, blocks, s);
   if constexpr (sizeof(T) == 2) {
