@@ -81,38 +81,25 @@ __device__ __forceinline__ void less_zero(u32x4_t v, float z16, float* c) {
 // Eight columns of a row as A operands: bf16 as they are; an fp32 value as the sum of three bf16 (its
 // leading, middle and last eight mantissa bits, cut off exactly), whose three products on the bf16
 // MFMA take a fifth of the eight v_mfma_f32_16x16x4_f32 that fp32 operands would.
-template <typename T> struct Rows;
-template <> struct Rows<bf16_t> {
-  Frag<bf16_t> x;
-  __device__ __forceinline__ void set(const u32x4_t* v) { x.v = __builtin_bit_cast(bf16x8_t, v[0]); }
+template <typename T> struct Rows {
+  static constexpr int kParts = sizeof(T) == 2 ? 1 : 3;
+  Frag<bf16_t> part[kParts];
 };
-template <> struct Rows<float> {
-  Frag<bf16_t> hi, mid, lo;
-  __device__ __forceinline__ void set(const u32x4_t* v) {
-    uint32_t h[8], m[8], l[8];
+template <typename T> __device__ __forceinline__ f32x4_t mma(const Rows<T>& a, const Frag<bf16_t>& b, f32x4_t c) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = v[e / 4][e & 3];
-      const float f = __uint_as_float(u);
-      const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-      h[e] = f != f ? 0x7fc00000u : u & 0xffff0000u;
-      const float rest = finite ? f - __uint_as_float(h[e]) : 0.f;
-      m[e] = __float_as_uint(rest) & 0xffff0000u;
-      l[e] = __float_as_uint(rest - __uint_as_float(m[e]));
-    }
-    u32x4_t ph, pm, pl;
+  for (int i = Rows<T>::kParts - 1; i >= 0; --i) c = hdcm::mma(a.part[i], b, c);
+  return c;
+}
+// The leading parts of four fp32 values as bf16, and what they leave in the values' place (of an infinity, which only
+// the first part meets, nothing).
+__device__ __forceinline__ uint2 take_part(u32x4_t& v, bool first) {
+  const uint2 o = make_uint2(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ph[i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
-      pm[i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
-      pl[i] = __builtin_amdgcn_perm(l[2 * i + 1], l[2 * i], 0x07060302u);
-    }
-    hi.v = __builtin_bit_cast(bf16x8_t, ph), mid.v = __builtin_bit_cast(bf16x8_t, pm), lo.v = __builtin_bit_cast(bf16x8_t, pl);
+  for (int e = 0; e < 4; ++e) {
+    const float f = __uint_as_float(v[e]), rest = f - __uint_as_float(v[e] & 0xffff0000u);
+    v[e] = first && __builtin_amdgcn_classf(f, 0x204) ? 0u : __float_as_uint(rest);
   }
-};
-__device__ __forceinline__ f32x4_t mma(const Rows<bf16_t>& a, const Frag<bf16_t>& b, f32x4_t c) { return hdcm::mma(a.x, b, c); }
-__device__ __forceinline__ f32x4_t mma(const Rows<float>& a, const Frag<bf16_t>& b, f32x4_t c) {
-  return hdcm::mma(a.hi, b, hdcm::mma(a.mid, b, hdcm::mma(a.lo, b, c)));
+  return o;
 }
 __device__ __forceinline__ Frag<bf16_t> fill(uint32_t v) {
   Frag<bf16_t> f;
@@ -261,7 +248,8 @@ template <typename T, bool NORM = false> struct Ending {
 // each wave leaves its partial sums in LDS (two buffers, so one barrier a tile) and the waves take
 // turns in adding them up.  x is read once per workgroup, a quarter row per load instruction (whole
 // lines; fragments read straight from the rows, 16 rows x 64 bytes an instruction, took 1.4 us
-// longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS.
+// longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS, fp32 part by part (split there a run
+// of four is split once, and rows past M cost nothing: 3 x 3264 x 768 4.6 us, 5.6 with the fragments split).
 // What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
 // instructions per wave and tile.
 // NORM (bf16): out = rstd (x w - mean sum w) takes the row LayerNorm without affine behind the product.  The rows' sums
@@ -271,7 +259,7 @@ template <typename T, bool NORM = false> struct Ending {
 template <typename T, int MT, int P, int GS, bool ZERO, int MAXW, bool NORM, bool SEG>
 __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4_kernel(Linear4Args p) {
   constexpr int GPT = 4 / GS;
-  constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + E;
+  constexpr int E = 16 / sizeof(T), CPR = kTileK / E, NLD = 16 * CPR / kWave, PITCH = kTileK + 8;
   extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [2][WP][MT][64]; at first the waves' slabs of x
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int W = blockDim.x / kWave, WP = (W + 3) & ~3;
@@ -282,7 +270,7 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
   const Scales scales(p.scales, p.s_f32, l16);
 
   // with more than one segment: the sums of the workgroup's tiles so far, behind the slabs and the partial sums
-  f32x4_t* hold = part + max(2 * WP * MT * kWave, W * 16 * PITCH * (int)sizeof(T) / 16) + lane;
+  f32x4_t* hold = part + max(2 * WP * MT * kWave, W * 16 * PITCH * 2 / 16) + lane;
   __shared__ float2 sums[NORM ? MAXW : 1][16 * MT], stats[NORM ? 16 * MT : 1];
   const int segs = SEG ? p.segs : 1;
   for (int seg = 0; seg < segs; ++seg) {
@@ -330,31 +318,31 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
     fetch(blockIdx.x);
 
     if constexpr (SEG) __syncthreads();  // the partial sums are read
-    T* slab = reinterpret_cast<T*>(part) + w * 16 * PITCH;  // the wave's own: no barrier
+    bf16_t* slab = reinterpret_cast<bf16_t*>(part) + w * 16 * PITCH;  // the wave's own: no barrier
     Rows<T> xa[P][4][MT];
 #pragma unroll
     for (int r = 0; r < MT; ++r)
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        asm volatile("" ::: "memory");  // a wave's LDS accesses complete in order; they stay in this one
+      for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int n = 0; n < NLD; ++n) {
-          if (n * kWave / CPR + 16 * r >= rows) continue;
-          const int at = n * kWave + ln, k = (k0 + i) * kTileK + at % CPR * E;
-          u32x4_t v = raw[r][i][n];
-          if ((k0 + i + 1) * kTileK > p.K) v = place_run<T>(v, k, p.K);  // (uniform)
-          *reinterpret_cast<u32x4_t*>(slab + at / CPR * PITCH + at % CPR * E) = v;
+        for (int h = 0; h < Rows<T>::kParts; ++h) {
+          asm volatile("" ::: "memory");  // a wave's LDS accesses complete in order; they stay in this one
+#pragma unroll
+          for (int n = 0; n < NLD; ++n) {
+            if (n * kWave / CPR + 16 * r >= rows) continue;
+            const int at = n * kWave + ln, k = (k0 + i) * kTileK + at % CPR * E;
+            u32x4_t& v = raw[r][i][n];
+            if (h == 0 && (k0 + i + 1) * kTileK > p.K) v = place_run<T>(v, k, p.K);  // (uniform)
+            bf16_t* to = slab + at / CPR * PITCH + at % CPR * E;
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x4_t*>(to) = v;
+            else *reinterpret_cast<uint2*>(to) = take_part(v, h == 0);
+          }
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            xa[i][j][r].part[h].v = *reinterpret_cast<const bf16x8_t*>(slab + (ln & 15) * PITCH + 32 * j + 8 * (ln >> 4));
+          asm volatile("" ::: "memory");
         }
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32x4_t v[8 / E];
-#pragma unroll
-          for (int h = 0; h < 8 / E; ++h) v[h] = *reinterpret_cast<const u32x4_t*>(slab + (ln & 15) * PITCH + 32 * j + 8 * (ln >> 4) + E * h);
-          xa[i][j][r].set(v);
-        }
-        asm volatile("" ::: "memory");
-      }
     f32x4_t xsum[P][MT];
     if constexpr (GS == 4 && sizeof(T) == 2) {
 #pragma unroll
@@ -369,7 +357,7 @@ __global__ __launch_bounds__(MAXW* kWave, P == 1 && MT > 1 ? 4 : 1) void linear4
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             s1 = mma(xa[i][j][r], fill(0x3f803f80u), s1);
-            s2 = mma(xa[i][j][r], xa[i][j][r].x, s2);
+            s2 = mma(xa[i][j][r], xa[i][j][r].part[0], s2);
           }
         const int e = l16 & 3;  // row 4 g + e, column l16
         if (l16 / 4 == g) {  // (of every segment the same lane)
@@ -475,7 +463,7 @@ void launch_linear4(const Linear4Args& a, int blocks_m, hipStream_t s) {
   // waves per CU: 8 where the registers hold more than one row tile of two column tiles, else 16: whole workgroups
   const int per_cu = (MT == 1 || P == 1 ? 16 : 8) / W;
   int most = kCUs * (per_cu > 1 ? per_cu : 1) / blocks_m;
-  const int slabs = W * 16 * (kTileK * (int)sizeof(T) + 16), parts = 2 * ((W + 3) & ~3) * MT * kHeldBytes;
+  const int slabs = W * 16 * (kTileK + 8) * 2, parts = 2 * ((W + 3) & ~3) * MT * kHeldBytes;
   int shmem = slabs > parts ? slabs : parts;
   if (a.segs > 1) {
     const int room = (kLds - shmem) / kHeldBytes / MT, least = (a.tiles_n + room - 1) / room;  // column tiles of a workgroup
