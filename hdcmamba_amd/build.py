@@ -66,7 +66,7 @@ def _link_native() -> None:
     lib = str(Path(torch.__file__).parent / "lib")
     tmp = NATIVE.with_suffix(".so.tmp")
     _run(["g++", "-shared", str(BUILD / "native.o"), "-o", str(tmp), f"-L{PKG}", "-l:libhdcmamba_hip.so", f"-L{lib}",
-          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"])
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"])
     os.replace(tmp, NATIVE)
 
 

@@ -6,7 +6,9 @@
 // between calls: workspaces that outlive a call are passed in.
 #include <array>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -579,6 +581,12 @@ std::vector<OptTensor> block_backward(const Tensor& x, const Tensor& dy, const s
 }
 
 // ------------------------------------------------------------------------ 4-bit products
+// at::empty on ref's device without the dispatcher, half of what a small call spends beside its launch (0.5 us)
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor& ref) {
+  return at::detail::empty_cuda(shape, type, ref.device(), std::nullopt);
+}
+Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+
 // The operators below are inference only: one that autograd would have to differentiate is refused.
 void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return;
@@ -682,7 +690,7 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
     same_device(out, x, "out");
     TORCH_CHECK(out.scalar_type() == x.scalar_type() && out.sizes() == shape, "linear_4bit: out must be ", shape, " of x's type");
   } else {
-    out = at::empty(shape, x.options());
+    out = fresh(shape, x.scalar_type(), x);
   }
   const Tensor o = out.dim() == 2 ? out : out.view({xr.size(0), w.N});  // a view, never a copy
   TORCH_CHECK(plain_rows(o), "linear_4bit: out's rows must be contiguous and apart");
@@ -736,7 +744,7 @@ const float* per_row(const Penalty& p, double dflt, int64_t B, const Tensor& ref
   const Tensor& t = std::get<Tensor>(*p);
   same_device(t, ref, name);
   TORCH_CHECK(t.dim() == 1 && t.size(0) == B, name, " must be a number or a tensor of ", B, " values");
-  held.push_back(t.to(at::kFloat).contiguous());
+  held.push_back(as_type(t, at::kFloat).contiguous());
   return held.back().const_data_ptr<float>();
 }
 // [n], [1, n] or [B, n] as (pointer, row stride), 0 for a shared row
@@ -746,10 +754,9 @@ std::pair<const void*, int64_t> shared_rows(const Tensor& t, int64_t B, int64_t 
   TORCH_CHECK((t.dim() == 1 || (t.dim() == 2 && (t.size(0) == 1 || t.size(0) == B))) && t.size(-1) == n, name, " ", t.sizes(),
               " must be [", n, "] or [", B, ", ", n, "]");
   const bool shared = t.dim() == 1 || t.size(0) == 1 || t.stride(0) == 0;
-  Tensor r = t.dim() == 1 ? t.unsqueeze(0) : shared ? t.narrow(0, 0, std::min<int64_t>(t.size(0), 1)) : t;
-  if (!plain_rows(r)) r = r.contiguous();
-  held.push_back(r);
-  return {r.const_data_ptr(), shared ? 0 : r.stride(0)};
+  const bool plain = shared ? t.size(-1) <= 1 || t.stride(-1) == 1 : plain_rows(t);
+  held.push_back(plain ? t : t.contiguous());
+  return {held.back().const_data_ptr(), shared ? 0 : held.back().stride(0)};
 }
 using ControlArgs = std::tuple<OptTensor, Penalty, Penalty, Penalty, OptTensor, OptTensor>;
 Controls controls_of(const ControlArgs& a, const Tensor& logits) {
@@ -804,9 +811,9 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
     TORCH_CHECK(same_place(out, l) || !overlap(out, l),
                 "process_logits: out may be the logits themselves but share no other memory with them");
     for (const Tensor& t : k.held)
-      TORCH_CHECK(!overlap(out, t.dim() == 1 ? t.unsqueeze(0) : t), "process_logits: out shares memory with the penalties, the history, the bias or the mask");
+      TORCH_CHECK(!overlap(out, t.dim() == 1 ? t.unsqueeze(0) : t.size(0) && !t.stride(0) ? t.narrow(0, 0, 1) : t), "process_logits: out shares memory with the penalties, the history, the bias or the mask");
   } else {
-    out = at::empty(logits.sizes(), logits.options());
+    out = fresh(logits.sizes(), logits.scalar_type(), logits);
   }
   check("hdcm_logits_process",
         hdcm_logits_process(l.const_data_ptr(), l.stride(0), &k.c, out.mutable_data_ptr(), out.stride(0), l.size(0), l.size(1), dt,
@@ -832,13 +839,13 @@ std::tuple<Tensor, Tensor> select_tokens(const Tensor& logits, const ControlArgs
     TORCH_CHECK(noise_->scalar_type() == at::kFloat && noise_->sizes() == logits.sizes(), "noise must be float32 ", logits.sizes());
     noise = rows(*noise_);
   }
-  Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong)), logprobs = fp32({B}, logits);
+  Tensor tokens = fresh({B}, at::kLong, logits), logprobs = fresh({B}, at::kFloat, logits);
   const size_t n = hdcm_token_select_workspace_bytes(B, V);
-  const Tensor ws = n ? bytes(n, logits) : Tensor();
+  const c10::DataPtr ws = n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr();  // on the current stream
   check("hdcm_token_select",
         hdcm_token_select(l.const_data_ptr(), l.stride(0), &k.c, temp, temp_all, (const float*)pointer(noise),
                           noise.defined() ? noise.stride(0) : 0, tokens.mutable_data_ptr<int64_t>(),
-                          logprobs.mutable_data_ptr<float>(), n ? ws.mutable_data_ptr() : nullptr, n, B, V, dt, stream_of(l)));
+                          logprobs.mutable_data_ptr<float>(), ws.get(), n, B, V, dt, stream_of(l)));
   return {tokens, logprobs};
 }
 
@@ -853,21 +860,23 @@ struct Ids {
   const int64_t *p = nullptr, *n = nullptr;
   int64_t stride = 0, width = 0;
 };
-Ids ids_of(const OptTensor& ids, const OptTensor& lengths, const Tensor& table, const char* name) {
+Ids ids_of(const OptTensor& ids, const OptTensor& lengths, const Tensor& table, const char* name, bool one_each = false) {
   Ids r;
   TORCH_CHECK(ids || !lengths, name, "_lengths without ", name);
   if (!ids) return r;
   const auto whole = [](const Tensor& t) { return at::isIntegralType(t.scalar_type(), false); };
   same_device(*ids, table, name);
-  TORCH_CHECK(whole(*ids) && ids->dim() == 2 && ids->size(0) == table.size(0), name, " ", ids->sizes(), " must be token ids [",
-              table.size(0), ", any]");
-  r.ids = rows(ids->to(at::kLong));
-  r.p = r.ids.const_data_ptr<int64_t>(), r.stride = r.ids.stride(0), r.width = r.ids.size(1);
+  TORCH_CHECK(whole(*ids) && (ids->dim() == 2 || (one_each && ids->dim() == 1)) && ids->size(0) == table.size(0), name, " ",
+              ids->sizes(), " must be token ids [", table.size(0), ", any]");
+  r.ids = as_type(*ids, at::kLong);
+  if (ids->dim() == 2) r.ids = rows(r.ids);
+  else if (r.ids.stride(0) < 1) r.ids = r.ids.contiguous();
+  r.p = r.ids.const_data_ptr<int64_t>(), r.stride = r.ids.stride(0), r.width = ids->dim() == 2 ? r.ids.size(1) : 1;
   if (lengths) {
     same_device(*lengths, table, "lengths");
     TORCH_CHECK(whole(*lengths) && lengths->dim() == 1 && lengths->size(0) == table.size(0), name, "_lengths must be [",
                 table.size(0), "] whole numbers");
-    r.lengths = lengths->to(at::kLong).contiguous();
+    r.lengths = as_type(*lengths, at::kLong).contiguous();
     r.n = r.lengths.const_data_ptr<int64_t>();
   }
   return r;
@@ -889,7 +898,7 @@ Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& length
   Entry entry;
   table_shape(table, "append_tokens");
   const c10::DeviceGuard guard(table.device());
-  const Ids t = ids_of(tokens.dim() == 1 ? tokens.unsqueeze(1) : tokens, lengths, table, "tokens");
+  const Ids t = ids_of(tokens, lengths, table, "tokens", true);
   check("hdcm_token_history_append",
         hdcm_token_history_append(table.mutable_data_ptr<int16_t>(), table.stride(0), t.p, t.stride, t.n, t.width, table.size(0),
                                   table.size(1), stream_of(table)));
