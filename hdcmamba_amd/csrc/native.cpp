@@ -811,7 +811,8 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
     TORCH_CHECK(same_place(out, l) || !overlap(out, l),
                 "process_logits: out may be the logits themselves but share no other memory with them");
     for (const Tensor& t : k.held)
-      TORCH_CHECK(!overlap(out, t.dim() == 1 ? t.unsqueeze(0) : t.size(0) && !t.stride(0) ? t.narrow(0, 0, 1) : t), "process_logits: out shares memory with the penalties, the history, the bias or the mask");
+      TORCH_CHECK(!overlap(out, t.dim() == 1 ? t.unsqueeze(0) : t.size(0) && !t.stride(0) ? t.narrow(0, 0, 1) : t),
+                  "process_logits: out shares memory with the penalties, the history, the bias or the mask");
   } else {
     out = fresh(logits.sizes(), logits.scalar_type(), logits);
   }

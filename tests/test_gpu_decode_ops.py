@@ -139,8 +139,8 @@ def test_linear_4bit_layouts(dev, dtype):
 
 @pytest.mark.parametrize("M,K,N,group,zeros", [
     (1, 8, 16, 32, False), (1, 1152, 100, 128, False), (16, 2176, 70, 128, True), (5, 333, 33, 32, True),
-    (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True), (33, 5000, 300, 128, False),
-    (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True)])
+    (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True),
+    (33, 5000, 300, 128, False), (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True)])
 def test_linear_4bit_with_layer_norm(dev, M, K, N, group, zeros):
     """norm_eps against the LayerNorm and product in 64 bits.
 
