@@ -712,6 +712,7 @@ extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const flo
   HDCM_CHECK_ARG(M == 0 || N == 0 || (x && packed && scales && out), HDCM_EINVAL);
   HDCM_CHECK_ARG(M <= 1 || (x_row_stride >= K && out_row_stride >= N && (!res || res_row_stride >= N)), HDCM_EINVAL);
   HDCM_CHECK_ARG(!row_sums || dtype == HDCM_BF16, HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(!row_sums || eps >= 0.f, HDCM_EINVAL);
   HDCM_CHECK_ARG(sizes_ok(N, K, group) && K >= (dtype == HDCM_F32 ? 4 : 8) && M <= 16 * 65535, HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(hdcm_aligned16(packed) && ((uintptr_t)scales & 3u) == 0, HDCM_EALIGN);
   if (M == 0 || N == 0) return HDCM_OK;

@@ -38,6 +38,8 @@ def test_w4_linear_validation():
     assert f(*with_(base, _8=256)) == EUNSUPPORTED
     assert f(*with_(base, _16=7)) == EUNSUPPORTED  # shorter than one load
     assert f(*with_(base, _2=P16, _17=F32)) == EUNSUPPORTED
+    assert f(*with_(base, _2=P16, _3=-1.0)) == EINVAL
+    assert f(*with_(base, _2=P16, _3=float("nan"))) == EINVAL
     assert f(*with_(base, _0=None)) == EINVAL
     assert f(*with_(base, _5=None)) == EINVAL
     assert f(*with_(base, _16=0)) == EINVAL

@@ -683,3 +683,68 @@ def test_history_passes_over_any_other_id(dev):
     hm.append_tokens(table, torch.tensor([far * 3 + [3]], device=dev))
     want[3] = -(2**15) + 2
     assert torch.equal(table[0].cpu(), want)
+
+
+def test_many_rows(dev):
+    """More rows than a grid has blocks in y: process_logits walks them, select_tokens refuses them; a product's are row
+    blocks."""
+    B, V = 70000, 9
+    l = torch.randn(B, V, generator=_gen(1)).to(dev)
+    bias = torch.randn(V, generator=_gen(2)).to(dev)
+    assert torch.equal(hm.process_logits(l, bias=bias), l + bias)
+    with pytest.raises(_ops.HdcmError):
+        hm.select_tokens(l)
+    token, _ = hm.select_tokens(l[:65535])
+    assert torch.equal(token, l[:65535].argmax(1))
+    for dtype in (BF, F32):
+        codes, scales, _ = _weight(16, 40, 32, False, BF, seed=3)
+        w = hm.Weight4Bit.from_codes(codes.to(dev), scales.to(dev), None, 32)
+        x = torch.randn(B, 40, generator=_gen(4)).to(dtype)
+        _check_linear(hm.linear_4bit(x.to(dev), w), x, codes, scales, None, 32, None, None)
+
+
+def test_two_streams_at_once(dev):
+    """Calls in flight on two streams share nothing."""
+    V = 50000
+    w = hm.Weight4Bit.quantize(torch.randn(V // 10, 512, generator=_gen(1)).to(dev), 64)
+    jobs = [(torch.randn(8, V, generator=_gen(s)).to(dev), torch.randn(8, 512, generator=_gen(s)).to(BF).to(dev)) for s in (2, 3)]
+    want = [(hm.select_tokens(l), hm.linear_4bit(x, w, norm_eps=1e-5)) for l, x in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(50):
+        for i, (l, x) in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((hm.select_tokens(l), hm.linear_4bit(x, w, norm_eps=1e-5)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for (token, logprob), y in got[i]:
+            assert torch.equal(token, want[i][0][0]) and torch.equal(logprob, want[i][0][1]) and torch.equal(y, want[i][1])
+
+
+def test_graphs_share_no_workspace(dev):
+    """Two recorded graphs of the same calls, replayed in turn and at once on two streams."""
+    V = 40000
+    w = hm.Weight4Bit.quantize(torch.randn(2000, 640, generator=_gen(1)).to(dev))
+    x = [torch.randn(5, 640, generator=_gen(s)).to(BF).to(dev) for s in (2, 3)]
+    l = [torch.randn(5, V, generator=_gen(s)).to(dev) for s in (4, 5)]
+    want = [(hm.select_tokens(l[i]), hm.linear_4bit(x[i], w, norm_eps=1e-5)) for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append((hm.select_tokens(l[i]), hm.linear_4bit(x[i], w, norm_eps=1e-5)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for n in range(6):
+        for (token, logprob), y in outs:
+            token.zero_(), logprob.zero_(), y.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            if n % 2:
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+            else:
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for ((token, logprob), y), ((t, p), z) in zip(outs, want):
+            assert torch.equal(token, t) and torch.equal(logprob, p) and torch.equal(y, z)

@@ -225,3 +225,15 @@ def test_generate(dev):
     out, _ = lm.generate(ids, 12, temperature=torch.tensor([0.0, 1.0], device=dev), mask=mask, repetition=1.2, presence=5.0)
     assert (out % 7 == 5).all() and all(len(set(row)) > 6 for row in out.tolist())  # the presence penalty spreads them
     assert lm.generate(ids, 0)[0].shape == (B, 0)
+
+
+def test_generate_with_nothing_allowed(dev):
+    """A sequence whose mask leaves nothing goes on with token -1, the other as without it."""
+    V = 300
+    lm = _lm(256, 64, 4, 32, 1, V, BF).to(dev)
+    ids = torch.randint(0, V, (2, 5), generator=torch.Generator().manual_seed(1)).to(dev)
+    mask = torch.full((2, -(-V // 32)), -1, dtype=torch.int32, device=dev)
+    mask[0] = 0
+    tokens, lp = lm.generate(ids, 6, mask=mask, presence=0.5)
+    assert (tokens[0] == -1).all() and (lp[0] == -float("inf")).all()
+    assert torch.equal(tokens[1], lm.generate(ids, 6, presence=0.5)[0][1])
