@@ -248,8 +248,9 @@ template <typename T, bool NORM = false> struct Ending {
 // each wave leaves its partial sums in LDS (two buffers, so one barrier a tile) and the waves take
 // turns in adding them up.  x is read once per workgroup, a quarter row per load instruction (whole
 // lines; fragments read straight from the rows, 16 rows x 64 bytes an instruction, took 1.4 us
-// longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS, fp32 part by part (split there a run
-// of four is split once, and rows past M cost nothing: 3 x 3264 x 768 4.6 us, 5.6 with the fragments split).
+// longer at 16 rows of 2048 and 6.5 us at 64), and brought into fragments through LDS, fp32 part by part
+// (split there a run of four is split once, and rows past M cost nothing: 3 x 3264 x 768 4.6 us, 5.6 with
+// the fragments split).
 // What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
 // instructions per wave and tile.
 // NORM (bf16): out = rstd (x w - mean sum w) takes the row LayerNorm without affine behind the product.  The rows' sums
@@ -492,8 +493,8 @@ template <typename T, int GS, bool ZERO> void pick_rows(Linear4Args a, hipStream
   const auto segments = [&](int widest) { return (a.tiles_k + widest - 1) / widest; };
   const int most = sizeof(T) == 4 ? 1 : a.tiles_k <= 4 || segments(24) < segments(16) ? 2 : 4;
   const int least = (tiles_m + most - 1) / most, room = 4 * kCUs / a.tiles_n, fill = room < tiles_m ? room : tiles_m;
-  const int blocks = least > fill ? least : fill;
-  const int mt = (tiles_m + blocks - 1) / blocks;
+  const int wanted = least > fill ? least : fill, mt = (tiles_m + wanted - 1) / wanted;
+  const int blocks = (tiles_m + mt - 1) / mt;  // none without rows
   a.segs = segments(mt > 2 ? 16 : 24);
   if (mt == 1) pick_tiles<T, 1, GS, ZERO, 12>(a, blocks, s);
   if constexpr (sizeof(T) == 2) {
@@ -703,9 +704,9 @@ extern "C" int hdcm_w4_dequant(const void* packed, const void* scales, int scale
 }
 
 extern "C" int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sums, float eps, const void* packed,
-                                  const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias, const void* res,
-                                  int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N, int64_t K,
-                                  int dtype, void* stream) {
+                                  const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias,
+                                  const void* res, int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M,
+                                  int64_t N, int64_t K, int dtype, void* stream) {
   HDCM_CHECK_ARG((dtype == HDCM_F32 || dtype == HDCM_BF16) && (scale_dtype == HDCM_F32 || scale_dtype == HDCM_BF16),
                  HDCM_EUNSUPPORTED);
   HDCM_CHECK_ARG(M >= 0 && N >= 0 && K > 0, HDCM_EINVAL);

@@ -550,12 +550,13 @@ int hdcm_rowln_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t
  * `dtype`, fp32 accumulation of exact code products, the scales applied to the groups' sums, one
  * rounding.  bias and res may be NULL; res may be out itself.  x, bias, res and out need only
  * their type's alignment; rows may have any stride of at least their width.  x's columns past K (row
- * padding) are not read.  K >= 8 (bf16) or 4 (fp32).  bf16 x: an infinity makes its row NaN.  For the decode step's rows: the
- * weight is read once per 64 bf16 rows of up to 2048 columns (less for longer and fp32 rows).
+ * padding) are not read.  K >= 8 (bf16) or 4 (fp32).  bf16 x: an infinity makes its row NaN.  For the decode
+ * step's rows: the weight is read once per block of up to 64 bf16 rows (16 of fp32), the largest where
+ * the output is wide.
  * row_sums [N] fp32 (sum_k w[n,k]; NULL: x as it is): the product of x's rows after a LayerNorm without
- * affine, rstd (x w - mean row_sums), bf16 only.  Mean and variance are
- * fp32 sums of the row and its squares, the variance their difference: a row whose mean is 100 times its
- * deviation keeps about three digits of it.
+ * affine, rstd (x w - mean row_sums), bf16 only, eps >= 0.  Mean and variance are fp32 sums of the row and its
+ * squares, the variance their difference: a row whose mean is 100 times its deviation keeps about
+ * three digits of it.
  */
 size_t hdcm_w4_packed_bytes(int64_t N, int64_t K);
 int hdcm_w4_pack(const uint8_t* codes, int64_t codes_row_stride, int64_t N, int64_t K, void* packed, void* stream);
@@ -563,9 +564,9 @@ int hdcm_w4_quantize(const void* w, int64_t w_row_stride, int64_t N, int64_t K, 
                      void* scales, int scale_dtype, uint8_t* zeros, int dtype, void* stream);
 int hdcm_w4_dequant(const void* packed, const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group,
                     void* out, int64_t out_row_stride, int64_t N, int64_t K, int dtype, void* stream);
-int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sums, float eps, const void* packed, const void* scales,
-                       int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias, const void* res,
-                       int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N,
+int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sums, float eps, const void* packed,
+                       const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group, const void* bias,
+                       const void* res, int64_t res_row_stride, void* out, int64_t out_row_stride, int64_t M, int64_t N,
                        int64_t K, int dtype, void* stream);
 
 /*

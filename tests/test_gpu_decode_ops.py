@@ -92,6 +92,8 @@ LINEAR = [
     (2, 9000, 8200, 128, True, BF, BF),
     (1100, 3300, 5200, 128, False, BF, BF),  # more sums to hold than a workgroup has room for
     (30, 6500, 100, 64, False, BF, F32),
+    (70, 256, 4096, 128, False, BF, BF),   # five row tiles where four blocks would fill the card
+    (90, 100, 3000, 64, True, BF, BF),     # one wave a workgroup
 ]
 
 
@@ -140,7 +142,8 @@ def test_linear_4bit_layouts(dev, dtype):
 @pytest.mark.parametrize("M,K,N,group,zeros", [
     (1, 8, 16, 32, False), (1, 1152, 100, 128, False), (16, 2176, 70, 128, True), (5, 333, 33, 32, True),
     (40, 2048, 50, 64, False), (64, 832, 60, 128, False), (100, 1000, 20, 128, True), (3, 23 * 128, 64, 64, True),
-    (33, 5000, 300, 128, False), (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True)])
+    (33, 5000, 300, 128, False), (33, 17 * 128 + 1, 48, 32, False), (16, 768, 8500, 128, True),
+    (40, 100, 70, 64, True), (70, 256, 4096, 128, False)])
 def test_linear_4bit_with_layer_norm(dev, M, K, N, group, zeros):
     """norm_eps against the LayerNorm and product in 64 bits.
 
