@@ -7,6 +7,7 @@
 #include <array>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <torch/extension.h>
@@ -634,23 +635,42 @@ bool same_place(const Tensor& a, const Tensor& b) {
 }
 
 // A packed weight, checked once (the handle of a Weight4Bit), and its row sums as the products give them: for
-// products behind a LayerNorm, formed again where a buffer was written since (load_state_dict)
+// products behind a LayerNorm, formed again where a buffer was written since (load_state_dict).  The host
+// waits for them (a weight is made or written once), so a call on any stream, and any recording, reads finished sums.
 struct Weight4 {
   Tensor packed, scales, zeros, row_sums;
   int64_t N, K, group;
   int scale_dtype;
-  std::array<uint32_t, 3> versions{};
-  std::array<uint32_t, 3> versions_now() const {
-    const auto of = [](const Tensor& t) { return t.defined() && !t.is_inference() ? (uint32_t)t._version() : 0u; };
-    return {of(packed), of(scales), of(zeros)};
+  using Versions = std::array<uint32_t, 3>;
+  std::optional<Versions> versions{};  // of the buffers that row_sums belongs to
+  // none where a buffer was made under inference mode: such a tensor does not count its writes
+  std::optional<Versions> versions_now() const {
+    Versions v{};
+    const Tensor* const ts[] = {&packed, &scales, &zeros};
+    for (int i = 0; i < 3; ++i)
+      if (ts[i]->defined()) {
+        if (ts[i]->is_inference()) return std::nullopt;
+        v[i] = (uint32_t)ts[i]->_version();
+      }
+    return v;
   }
 };
 Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const OptTensor& residual_, const OptTensor& out_,
                    std::optional<double> norm_eps);
+void form_row_sums(Weight4& w, const Tensor& out) {
+  linear_4bit(at::ones({1, w.K}, out.options()), w, std::nullopt, std::nullopt, out.unsqueeze(0), std::nullopt);
+}
 void sum_rows(Weight4& w) {
-  const at::NoGradGuard guard;
-  w.versions = w.versions_now();
-  linear_4bit(at::ones({1, w.K}, w.row_sums.options()), w, std::nullopt, std::nullopt, w.row_sums.unsqueeze(0), std::nullopt);
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(w.packed.device());
+  TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+              "the row sums of a 4-bit weight that was made, moved or written since are not formed inside a recording: call "
+              "its refresh(), or a step, before it");
+  w.versions.reset();
+  const auto now = w.versions_now();
+  form_row_sums(w, w.row_sums);
+  c10::hip::getCurrentHIPStream(w.packed.device().index()).synchronize();
+  w.versions = now;
 }
 Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor& zeros, int64_t N, int64_t K, int64_t group) {
   on_gpu(packed);
@@ -712,13 +732,19 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
   int64_t K = w.K;
   TORCH_CHECK(!norm_eps || (*norm_eps >= 0 && K >= 8 && dt == HDCM_BF16),
               "linear_4bit: norm_eps must not be negative, the rows bfloat16 and of 8 columns at least");
-  if (norm_eps && w.versions != w.versions_now()) sum_rows(w);
+  Tensor row_sums;
+  if (norm_eps) {
+    const auto now = w.versions_now();
+    if (now && w.versions != now) sum_rows(w);
+    row_sums = now ? w.row_sums : fresh({w.N}, at::kFloat, x);
+    if (!now) form_row_sums(w, row_sums);
+  }
   if (K < 8) {  // shorter than a load of the kernel's: columns of zeros, which the packed weight holds too
     xr = at::constant_pad_nd(xr, {0, 8 - K});
     K = 8;
   }
   check("hdcm_w4_linear_fwd",
-        hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), norm_eps ? (const float*)w.row_sums.const_data_ptr() : nullptr,
+        hdcm_w4_linear_fwd(xr.const_data_ptr(), xr.stride(0), (const float*)pointer(row_sums),
                            norm_eps ? (float)*norm_eps : 0.f, w.packed.const_data_ptr(), w.scales.const_data_ptr(), w.scale_dtype,
                            (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
                            r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, K, dt,

@@ -8,6 +8,8 @@ counterpart there.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -19,10 +21,20 @@ __all__ = ["Weight4Bit", "linear_4bit", "Linear4Bit"]
 GROUP_SIZES = (32, 64, 128)
 
 
+@contextmanager
+def _buffers_on(device):
+    """Allocate a weight's buffers: on ``device``, and under inference mode too as tensors that count their writes
+    (which keeps the row sums in line with them)."""
+    with torch.cuda.device(device), torch.inference_mode(False), torch.no_grad():
+        yield
+
+
 class Weight4Bit:
     """A packed 4-bit weight: made once from codes (``from_codes``) or by rounding a weight
-    (``quantize``), then passed to linear_4bit.  Its buffers may be written in place (load_state_dict); a
-    recorded graph with norm_eps sees that after ``refresh``.
+    (``quantize``), then passed to linear_4bit.  Its buffers may be written in place (load_state_dict): the
+    row sums that norm_eps reads are formed again, with a wait of the host, by the next call with it.
+    Inside a recording that is refused: ``refresh`` first; a graph recorded before sees the new sums after
+    ``refresh`` too.
 
     ``shape`` (N, K), ``group_size``; ``packed`` uint8, ``scales`` (float32 or bfloat16) and ``zeros``
     (uint8 or None) in the layout of hdcm_w4_linear_fwd (include/hdcm.h)."""
@@ -65,7 +77,7 @@ class Weight4Bit:
         for name, t in (("codes", codes), ("zeros", zeros)):
             if t is not None and int(t.max()) > 15:
                 raise ValueError(f"{name} must be in 0..15, got {int(t.max())}")
-        with torch.cuda.device(codes.device):
+        with _buffers_on(codes.device):
             codes = codes.contiguous()
             packed = torch.empty(int(_ops.lib().hdcm_w4_packed_bytes(N, K)), dtype=torch.uint8, device=codes.device)
             _ops._check("hdcm_w4_pack", _ops.lib().hdcm_w4_pack(codes.data_ptr(), codes.stride(0), N, K, packed.data_ptr(),
@@ -97,7 +109,7 @@ class Weight4Bit:
         if not bool(torch.isfinite(weight).all()):
             raise ValueError("a weight with infinities or NaN cannot be rounded to 4 bits")
         dev = weight.device
-        with torch.cuda.device(dev):
+        with _buffers_on(dev):
             weight = weight.contiguous()
             packed = torch.empty(int(_ops.lib().hdcm_w4_packed_bytes(N, K)), dtype=torch.uint8, device=dev)
             scales = torch.empty(G, Np, dtype=scale_dtype, device=dev)

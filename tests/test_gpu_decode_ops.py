@@ -751,3 +751,84 @@ def test_graphs_share_no_workspace(dev):
         torch.cuda.synchronize()
         for ((token, logprob), y), ((t, p), z) in zip(outs, want):
             assert torch.equal(token, t) and torch.equal(logprob, p) and torch.equal(y, z)
+
+
+# ------------------------------------------------------------------------------- row sums of norm_eps
+def _norm_weights(dev):
+    """Rows with a mean, a weight and another of its shape, and the other's product behind a LayerNorm."""
+    one, two = (hm.Weight4Bit.quantize(torch.randn(96, 256, generator=_gen(s)).to(BF).to(dev), 64, True) for s in (1, 2))
+    x = (torch.randn(5, 256, generator=_gen(3)) + 2).to(BF).to(dev)
+    return x, one, two, hm.linear_4bit(x, two, norm_eps=1e-5)
+
+
+def _write(to, other):
+    for name in ("packed", "scales", "zeros"):
+        getattr(to, name).copy_(getattr(other, name))
+
+
+def test_row_sums_are_finished_for_every_stream(dev):
+    """A weight is written in place and both streams are past that: the first call forms the row sums behind a busy
+    stream, the second, on another one, must not read them unwritten.  The same for a module that was moved."""
+    x, w, other, want = _norm_weights(dev)
+    hm.linear_4bit(x, w, norm_eps=1e-5)
+    layer = hm.Linear4Bit(w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for moved in (False, True):
+        _write(w, other)
+        if moved:
+            layer.cpu().to(dev)
+        torch.cuda.synchronize()
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if i == 0:
+                    torch.cuda._sleep(20_000_000)
+                got.append(hm.linear_4bit(x, layer.weight4 if moved else w, norm_eps=1e-5))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want) and torch.equal(got[1], want), moved
+        w.scales.zero_()
+        hm.linear_4bit(x, w, norm_eps=1e-5)
+
+
+def test_row_sums_are_not_left_to_a_recording(dev):
+    """The first call after a write is one being recorded: refused, and no later call takes the sums for formed."""
+    x, w, other, want = _norm_weights(dev)
+    hm.linear_4bit(x, w, norm_eps=1e-5)
+    _write(w, other)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="recording"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        hm.linear_4bit(x, w, norm_eps=1e-5)
+    assert torch.equal(hm.linear_4bit(x, w, norm_eps=1e-5), want)
+    w.scales.mul_(2)
+    w.refresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hm.linear_4bit(x, w, norm_eps=1e-5)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, hm.linear_4bit(x, w, norm_eps=1e-5))
+        torch.cuda.synchronize()
+
+
+def test_row_sums_follow_writes_under_inference_mode(dev):
+    x, w, other, want = _norm_weights(dev)
+    with torch.inference_mode():
+        made = hm.Weight4Bit.quantize(torch.randn(96, 256, generator=_gen(1)).to(BF).to(dev), 64, True)
+        clones = hm.Weight4Bit(w.packed.clone(), w.scales.clone(), w.zeros.clone(), w.shape, w.group_size)
+        assert clones.packed.is_inference()
+        for v in (made, clones):
+            hm.linear_4bit(x, v, norm_eps=1e-5)
+            _write(v, other)
+            assert torch.equal(hm.linear_4bit(x, v, norm_eps=1e-5), want)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = hm.linear_4bit(x, clones, norm_eps=1e-5)
+        for factor in (1, 2, 4):  # scales by powers of two: the normalised product likewise
+            clones.scales.copy_(other.scales * factor)
+            graph.replay()
+            assert torch.equal(out, want * factor)
+            torch.cuda.synchronize()
+    made.scales.mul_(2)
+    assert torch.equal(hm.linear_4bit(x, made, norm_eps=1e-5), want * 2)
