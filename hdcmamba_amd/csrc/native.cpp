@@ -588,11 +588,14 @@ Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor& ref) {
 }
 Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
 
-// The operators below are inference only: one that autograd would have to differentiate is refused.
+// The operators below are inference only: one that autograd would have to differentiate, in either mode, is refused.
 void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : ts)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), op, " has no gradient: call it under torch.no_grad() or on detached tensors");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : ts) {
+    if (!t || !t->defined()) continue;
+    TORCH_CHECK(!(backward && t->requires_grad()) && !(forward && t->_fw_grad(0).defined()), op,
+                " has no gradient: call it under torch.no_grad() or on detached tensors");
+  }
 }
 const Tensor& or_none(const OptTensor& t) {
   static const Tensor none;
@@ -696,7 +699,7 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
                    std::optional<double> norm_eps) {
   const Tensor &bias = or_none(bias_), &residual = or_none(residual_), &given = or_none(out_);
   on_gpu(x);
-  no_gradient("linear_4bit", {&x, &bias, &residual, &given});
+  no_gradient("linear_4bit", {&x, &w.scales, &bias, &residual, &given});
   Entry entry;
   const c10::DeviceGuard guard(x.device());
   const int dt = dtype_of(x);
@@ -754,6 +757,7 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
 
 // ------------------------------------------------------------------------ logits and tokens
 using Penalty = std::optional<std::variant<double, Tensor>>;
+const Tensor* tensor_of(const Penalty& p) { return p ? std::get_if<Tensor>(&*p) : nullptr; }
 // The controls of B rows of V logits, and what has to stay alive for the call.
 struct Controls {
   hdcm_logits_controls c{};
@@ -785,6 +789,9 @@ std::pair<const void*, int64_t> shared_rows(const Tensor& t, int64_t B, int64_t 
   return {held.back().const_data_ptr(), shared ? 0 : held.back().stride(0)};
 }
 using ControlArgs = std::tuple<OptTensor, Penalty, Penalty, Penalty, OptTensor, OptTensor>;
+void no_gradient(const char* op, const ControlArgs& a) {
+  no_gradient(op, {tensor_of(std::get<1>(a)), tensor_of(std::get<2>(a)), tensor_of(std::get<3>(a)), &or_none(std::get<4>(a))});
+}
 Controls controls_of(const ControlArgs& a, const Tensor& logits) {
   const auto& [history, repetition, frequency, presence, bias, mask] = a;
   const int64_t B = logits.size(0), V = logits.size(1);
@@ -822,7 +829,8 @@ void logits_shape(const Tensor& logits, const char* op) {
 
 Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTensor& out_) {
   logits_shape(logits, "process_logits");
-  no_gradient("process_logits", {&logits, &or_none(std::get<4>(args)), &or_none(out_)});
+  no_gradient("process_logits", {&logits, &or_none(out_)});
+  no_gradient("process_logits", args);
   Entry entry;
   const c10::DeviceGuard guard(logits.device());
   const int dt = dtype_of(logits);
@@ -851,7 +859,8 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
 std::tuple<Tensor, Tensor> select_tokens(const Tensor& logits, const ControlArgs& args, const Penalty& temperature,
                                          const OptTensor& noise_) {
   logits_shape(logits, "select_tokens");
-  no_gradient("select_tokens", {&logits, &or_none(std::get<4>(args)), &or_none(noise_)});
+  no_gradient("select_tokens", {&logits, &or_none(noise_), tensor_of(temperature)});
+  no_gradient("select_tokens", args);
   Entry entry;
   const c10::DeviceGuard guard(logits.device());
   const int dt = dtype_of(logits);

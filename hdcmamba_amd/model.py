@@ -33,7 +33,7 @@ from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from . import _ops
-from .quant4 import Linear4Bit, linear_4bit
+from .quant4 import Linear4Bit, carries_tangent, linear_4bit
 
 __all__ = ["HdcMamba9v3Block", "HdcMamba9v3Model", "FusedNormConv1dFunction",
            "fused_norm_conv1d_trainable", "RowLayerNormFunction", "layer_norm", "SlotSsmMixerFunction",
@@ -447,9 +447,10 @@ class HdcMamba9v3Block(nn.Module):
         xp = _ops.native().pad_rows(x, pad, _ops._stream(x))
         return self._native_forward(xp, out=xp, train=train)[:, pad:, :]
 
-    def _no_grad_4bit(self):
-        if self.weights_4bit and (self.training or torch.is_grad_enabled()):
-            raise RuntimeError("a block with 4-bit weights is for inference: call eval() and run under torch.no_grad()")
+    def _no_grad_4bit(self, x):
+        if self.weights_4bit and (self.training or torch.is_grad_enabled() or carries_tangent(x)):
+            raise RuntimeError("a block with 4-bit weights is for inference: call eval() and run under torch.no_grad(), without "
+                               "forward-mode tangents")
 
     def _fused_out(self, x):
         """Whether out_proj runs as the GEMM with the LayerNorm folded in (bf16, no autograd).
@@ -528,7 +529,7 @@ class HdcMamba9v3Block(nn.Module):
     def _inner_forward(self, x, state=None):
         """Block body on a chunk-aligned [B,L,dm] input; returns x + out_proj(LN(combined))."""
         B, L, dm = x.shape
-        self._no_grad_4bit()
+        self._no_grad_4bit(x)
         if not torch.is_grad_enabled() and self._native_ok(x):
             return self._native_forward(x, state)
         if self._fused_out(x):
@@ -552,6 +553,7 @@ class HdcMamba9v3Block(nn.Module):
         """In-place variant for a model-owned residual stream r [B,L,dm] (chunk-aligned):
         r += out_proj(LN(combined)), with the GEMM accumulating straight into r."""
         B, L, dm = r.shape
+        self._no_grad_4bit(r)
         if not torch.is_grad_enabled() and self._native_ok(r) and r.is_contiguous():
             return self._native_forward(r, state, out=r)
         if self._fused_out(r):
@@ -649,7 +651,7 @@ class HdcMamba9v3Block(nn.Module):
     def _step_4bit(self, x, state, pos_dev):
         """step with 4-bit in_proj and out_proj: LayerNorm + conv of the token, in_proj, the mixer step, and out_proj
         with the row LayerNorm before it and the residual."""
-        self._no_grad_4bit()
+        self._no_grad_4bit(x)
         dm, ds, H, C = self.d_model, self.d_state, self.num_heads, self.chunk_size
         xc = _ops.norm_conv_step(x, self.norm.weight, self.norm.bias, self.conv1d.weight.squeeze(1), self.conv1d.bias,
                                  self.norm.eps, state.conv)
@@ -679,7 +681,7 @@ class HdcMamba9v3Block(nn.Module):
 
     def forward(self, x):
         _ops._on_gpu(x)
-        self._no_grad_4bit()
+        self._no_grad_4bit(x)
         B, L_in, _ = x.shape
         pad = (self.chunk_size - (L_in % self.chunk_size)) % self.chunk_size
         if self.training:

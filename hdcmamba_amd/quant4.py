@@ -13,12 +13,18 @@ from contextlib import contextmanager
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _ops
 
 __all__ = ["Weight4Bit", "linear_4bit", "Linear4Bit"]
 
 GROUP_SIZES = (32, 64, 128)
+
+
+def carries_tangent(x):
+    """Whether x is a dual tensor of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
 
 @contextmanager
@@ -153,7 +159,7 @@ def linear_4bit(x, weight, bias=None, residual=None, out=None, norm_eps=None):
     sums, one rounding.  ``out`` may be ``residual``.  ``norm_eps`` (bfloat16 rows of at least 8 columns):
     the product of the rows after a LayerNorm without affine, in the same launch; its variance is the
     difference of two fp32 sums, for rows whose mean is not far above their deviation.  A bf16 row
-    that holds an infinity becomes NaN.  No gradient: refused where one would be recorded."""
+    that holds an infinity becomes NaN.  No gradient: refused where one would be recorded or carried forward."""
     return _ops.native().linear_4bit(x, weight._handle, bias, residual, out, norm_eps)
 
 
@@ -197,7 +203,7 @@ class Linear4Bit(nn.Module):
             self.weight4.refresh()
 
     def forward(self, x):
-        if torch.is_grad_enabled() and x.requires_grad:
+        if (torch.is_grad_enabled() and x.requires_grad) or carries_tangent(x):
             raise RuntimeError("a Linear4Bit has no gradient: call it under torch.no_grad() or on detached tensors")
         rows = x.numel() // max(x.shape[-1], 1)
         if rows > self.direct_rows:

@@ -14,7 +14,8 @@ and in this order:
 ``repetition`` (> 0), ``frequency`` and ``presence`` are numbers or tensors of one value per
 sequence and need ``history``, an int16 table [B, V] (new_token_history): the sign bit marks the
 prompt's tokens, the low 15 bits count the token in the output (at most 32767).  ``bias`` is [V] or
-[B, V] (float32 or bfloat16), ``mask`` int32 [ceil(V / 32)] or [B, ceil(V / 32)].
+[B, V] (float32 or bfloat16), ``mask`` int32 [ceil(V / 32)] or [B, ceil(V / 32)].  No gradient: a
+tensor among all these that needs one, or carries a tangent, is refused.
 """
 from __future__ import annotations
 
@@ -27,7 +28,7 @@ __all__ = ["process_logits", "select_tokens", "new_token_history", "fill_token_h
 
 def process_logits(logits, history=None, repetition=None, frequency=None, presence=None, bias=None, mask=None, out=None):
     """logits [B, V] (float32 or bfloat16) under the controls, rounded once to their type; ``out`` may be
-    ``logits``.  No gradient."""
+    ``logits``."""
     return _ops.native().process_logits(logits, (history, repetition, frequency, presence, bias, mask), out)
 
 
@@ -41,7 +42,7 @@ def select_tokens(logits, history=None, repetition=None, frequency=None, presenc
     distribution (-log(-log(u)), u uniform in (0, 1)) it is a sample of softmax(t).  ``temperature`` is a
     number or one per sequence (1 by default); one that is not above 0 makes a greedy choice, without
     noise, from t = processed.  -inf and NaN are never chosen: a sequence with nothing else gets token -1
-    and -inf.  A NaN or +inf among the allowed logits makes the log-probability NaN.  No gradient."""
+    and -inf.  A NaN or +inf among the allowed logits makes the log-probability NaN."""
     return _ops.native().select_tokens(logits, (history, repetition, frequency, presence, bias, mask), temperature, noise)
 
 

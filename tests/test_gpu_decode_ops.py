@@ -832,3 +832,38 @@ def test_row_sums_follow_writes_under_inference_mode(dev):
             torch.cuda.synchronize()
     made.scales.mul_(2)
     assert torch.equal(hm.linear_4bit(x, made, norm_eps=1e-5), want * 2)
+
+
+# ------------------------------------------------------------------------------- gradients
+def test_controls_that_need_a_gradient_are_refused(dev):
+    B, V = 2, 40
+    l, h = torch.zeros(B, V, device=dev), hm.new_token_history(B, V, dev)
+    need = lambda *n: torch.ones(*n, device=dev, requires_grad=True)  # noqa: E731
+    for kw in (dict(history=h, repetition=need(B)), dict(history=h, frequency=need(B)), dict(history=h, presence=need(B)),
+               dict(bias=need(V)), dict(temperature=need(B)), dict(noise=need(B, V))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            hm.select_tokens(l, **kw)
+        with torch.no_grad():
+            hm.select_tokens(l, **kw)
+        if "temperature" not in kw and "noise" not in kw:
+            with pytest.raises(RuntimeError, match="no gradient"):
+                hm.process_logits(l, **kw)
+
+
+def test_tangents_are_refused(dev):
+    """Forward mode: no operator drops a tangent, whatever the number of rows and with backward mode off."""
+    from torch.autograd import forward_ad
+
+    B, V = 2, 40
+    l, h = torch.zeros(B, V, device=dev), hm.new_token_history(B, V, dev)
+    layer = hm.Linear4Bit.from_linear(torch.nn.Linear(64, V, device=dev), 32)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = lambda *n: forward_ad.make_dual(torch.ones(*n, device=dev), torch.ones(*n, device=dev))  # noqa: E731
+        for call in (lambda: hm.process_logits(dual(B, V)), lambda: hm.process_logits(l, history=h, presence=dual(B)),
+                     lambda: hm.select_tokens(l, temperature=dual(B)), lambda: hm.select_tokens(l, noise=dual(B, V)),
+                     lambda: hm.linear_4bit(dual(3, 64), layer.weight4),
+                     lambda: hm.linear_4bit(torch.ones(3, 64, device=dev), layer.weight4, residual=dual(3, V)),
+                     lambda: layer(dual(3, 64)), lambda: layer(dual(500, 64))):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        assert layer(torch.ones(500, 64, device=dev)).shape == (500, V)

@@ -237,3 +237,18 @@ def test_generate_with_nothing_allowed(dev):
     tokens, lp = lm.generate(ids, 6, mask=mask, presence=0.5)
     assert (tokens[0] == -1).all() and (lp[0] == -float("inf")).all()
     assert torch.equal(tokens[1], lm.generate(ids, 6, presence=0.5)[0][1])
+
+
+def test_quantized_block_refuses_tangents(dev):
+    from torch.autograd import forward_ad
+
+    lm = hm.quantize_4bit(_lm(256, 64, 4, 32, 1, 100, BF).to(dev))
+    blk = lm.backbone.layers[0]
+    x = torch.randn(2, 32, 256, device=dev).to(BF)
+    with forward_ad.dual_level(), torch.no_grad():
+        d = forward_ad.make_dual(x, x.clone())
+        for call in (lambda: blk(d), lambda: lm.backbone(d), lambda: lm.backbone.prefill(d),
+                     lambda: blk.step(forward_ad.make_dual(x[:, 0].clone(), x[:, 1].clone()), blk.new_state(2, dev, BF))):
+            with pytest.raises(RuntimeError, match="inference"):
+                call()
+        assert lm.backbone(x).shape == x.shape
