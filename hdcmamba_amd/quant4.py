@@ -170,7 +170,8 @@ class Linear4Bit(nn.Module):
     Up to ``direct_rows`` rows go through linear_4bit; more multiply by the weight brought back to x's
     type, which rounds it once more (measured at d_model 2048, us: in_proj with 256 rows 21 against 37,
     384 25 against 34, 768 44 against 46; the head with 768 198 against 185; in groups of 32 the in_proj
-    with 256 rows 28 against 36, 384 37 against 33)."""
+    with 256 rows 28 against 36, 384 37 against 33).  In an autocast region x is cast to its type first,
+    as nn.Linear does (float16, which the kernels do not take, is refused)."""
 
     direct_rows = 384
 
@@ -205,6 +206,8 @@ class Linear4Bit(nn.Module):
     def forward(self, x):
         if (torch.is_grad_enabled() and x.requires_grad) or carries_tangent(x):
             raise RuntimeError("a Linear4Bit has no gradient: call it under torch.no_grad() or on detached tensors")
+        if torch.is_autocast_enabled("cuda"):  # as nn.Linear's, one type for any number of rows
+            x = x.to(torch.get_autocast_dtype("cuda"))
         rows = x.numel() // max(x.shape[-1], 1)
         if rows > self.direct_rows:
             return F.linear(x, self.weight4.dequantize(x.dtype), None if self.bias is None else self.bias.to(x.dtype))

@@ -867,3 +867,20 @@ def test_tangents_are_refused(dev):
             with pytest.raises(RuntimeError, match="no gradient"):
                 call()
         assert layer(torch.ones(500, 64, device=dev)).shape == (500, V)
+
+
+def test_linear4bit_module_under_autocast(dev):
+    """One result type on both sides of direct_rows, nn.Linear's; values those of rows cast beforehand."""
+    linear = torch.nn.Linear(64, 40, device=dev)
+    layer = hm.Linear4Bit.from_linear(linear, 32)
+    x = torch.randn(layer.direct_rows + 1, 64, generator=_gen(1)).to(dev)
+    with torch.no_grad():
+        for rows in (1, layer.direct_rows, layer.direct_rows + 1):
+            want = layer(x[:rows].to(BF))
+            with torch.amp.autocast("cuda", dtype=BF):
+                got = layer(x[:rows])
+                assert got.dtype == linear(x[:rows]).dtype == BF and torch.equal(got, want)
+                with torch.amp.autocast("cuda", enabled=False):
+                    assert layer(x[:rows]).dtype == F32
+            with torch.amp.autocast("cuda", dtype=torch.float16), pytest.raises(TypeError, match="dtype"):
+                layer(x[:rows])
