@@ -24,6 +24,7 @@ defects that are not reproduced).  Only GPU tensors are accepted; there is no CP
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -38,6 +39,13 @@ from .quant4 import Linear4Bit, carries_tangent, linear_4bit
 __all__ = ["HdcMamba9v3Block", "HdcMamba9v3Model", "FusedNormConv1dFunction",
            "fused_norm_conv1d_trainable", "RowLayerNormFunction", "layer_norm", "SlotSsmMixerFunction",
            "set_differentiable_mixer", "set_fused_out_proj", "set_fused_step_front", "quantize_4bit", "BlockState"]
+
+
+def _products_in(dtype):
+    """Where library products between the kernels run: in an autocast region of another type they would return that
+    type, while the kernels around them are told ``dtype``."""
+    other = torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != dtype
+    return torch.amp.autocast("cuda", enabled=False) if other else nullcontext()
 
 
 @dataclass
@@ -309,7 +317,8 @@ class HdcMamba9v3Block(nn.Module):
         elif _ops.gemm_f32_preferred(B * L, x_conv, w_in, b_in):
             projs = _ops.gemm_f32(x_conv.view(B * L, dm), w_in, b_in).view(B, L, -1)
         else:
-            projs = F.linear(x_conv, w_in, b_in)
+            with _products_in(dtype):
+                projs = F.linear(x_conv, w_in, b_in)
         combined = torch.empty(B, L, ds + dm, device=x.device, dtype=dtype)
         # The SSM and the slot kernels read projs and write disjoint columns of `combined`,
         # so the SSM may run on a side stream beside some of the slot kernels (ssm_overlap:
@@ -547,7 +556,8 @@ class HdcMamba9v3Block(nn.Module):
         w = self._weights(x.dtype)[1].to(x.dtype)
         if not torch.is_grad_enabled() and forward_ad._current_level < 0 and _ops.gemm_f32_preferred(x.shape[0], c, w, x):
             return _ops.gemm_f32(c, w, res=x, out=out)
-        return torch.addmm(x, c, w.t()) if out is None else out.addmm_(c, w.t())
+        with nullcontext() if torch.is_grad_enabled() else _products_in(x.dtype):
+            return torch.addmm(x, c, w.t()) if out is None else out.addmm_(c, w.t())
 
     def _residual_step_(self, r, state=None):
         """In-place variant for a model-owned residual stream r [B,L,dm] (chunk-aligned):
@@ -630,7 +640,8 @@ class HdcMamba9v3Block(nn.Module):
             xc = _ops.norm_conv_step(x, self.norm.weight, self.norm.bias, conv_w, self.conv1d.bias, self.norm.eps,
                                      state.conv)
             # few rows: the weight-streaming skinny GEMM; otherwise the library GEMM
-            projs = _ops.skinny_linear(xc, w_in, b_in) if _ops.skinny_ok(xc, w_in) else F.linear(xc, w_in, b_in)
+            with _products_in(dtype):
+                projs = _ops.skinny_linear(xc, w_in, b_in) if _ops.skinny_ok(xc, w_in) else F.linear(xc, w_in, b_in)
         combined = torch.empty(B, ds + dm, device=x.device, dtype=dtype)
         _ops.mixer_step(projs, self.A_log, ds, 3 * ds, self.gamma_buf.to(dtype), self.group_norm.weight,
                         self.group_norm.bias, 1e-5, state.h, state.S_prev, state.S_intra, state.pos, C,
@@ -643,7 +654,8 @@ class HdcMamba9v3Block(nn.Module):
             if _ops.skinny_ok(combined, w_out):
                 y = _ops.skinny_linear(combined, w_out, residual=x)
             else:
-                y = torch.addmm(x, combined, w_out.t())
+                with _products_in(dtype):
+                    y = torch.addmm(x, combined, w_out.t())
         if pos_dev is None:
             state.pos = (state.pos + 1) % C
         return y

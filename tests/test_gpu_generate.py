@@ -252,3 +252,26 @@ def test_quantized_block_refuses_tangents(dev):
             with pytest.raises(RuntimeError, match="inference"):
                 call()
         assert lm.backbone(x).shape == x.shape
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_fp32_blocks_under_bf16_autocast(dev, quantized):
+    """Inference of an fp32 model in a bf16 autocast region: the blocks compute in their rows' type, as outside of it (a
+    product in another type would hand the kernels around it what they read as fp32)."""
+    _say("fp32 blocks under autocast", quantized)
+    lm = _lm(256, 64, 4, 32, 2, 300, F32).to(dev)
+    if quantized:
+        hm.quantize_4bit(lm, 64)
+    x = torch.randn(2, 70, 256, generator=torch.Generator().manual_seed(1)).to(dev)
+
+    def run():
+        y, states = lm.backbone.prefill(x[:, :40])
+        return [lm.backbone(x), y, *(lm.backbone.step(x[:, 40 + i].contiguous(), states) for i in range(3)), lm.backbone.layers[0](x)[0]]
+
+    with torch.no_grad():
+        want = run()
+        with torch.amp.autocast("cuda", dtype=BF):
+            got = run()
+    for a, b in zip(got, want):
+        assert a.dtype == F32
+        assert_close(a, b.cpu(), F32, "under autocast")
