@@ -310,7 +310,7 @@ class HdcMamba9v3Block(nn.Module):
         ds, H, C = self.d_state, self.num_heads, self.chunk_size
         dtype = x.dtype
         x_conv = fused_norm_conv1d_trainable(x, self.norm, self.conv1d)
-        w_in, b_in = self._weights(dtype)[0].to(dtype), self.in_proj.bias.to(dtype)
+        w_in, b_in = self._weight(self.in_proj, dtype).to(dtype), self.in_proj.bias.to(dtype)
         # the SSM and slot kernels are constants for autograd, so projs needs no graph either
         if _ops.gemm_preferred(x_conv, w_in, b_in):
             projs = _ops.gemm(x_conv, w_in, b_in)
@@ -411,11 +411,9 @@ class HdcMamba9v3Block(nn.Module):
         """Whether in_proj and out_proj hold 4-bit weights (quantize_4bit): inference only."""
         return isinstance(self.in_proj, Linear4Bit)
 
-    def _weights(self, dtype):
-        """in_proj's and out_proj's weights; 4-bit ones brought back to ``dtype`` for products of many rows."""
-        if self.weights_4bit:
-            return self.in_proj.weight4.dequantize(dtype), self.out_proj.weight4.dequantize(dtype)
-        return self.in_proj.weight, self.out_proj.weight
+    def _weight(self, linear, dtype):
+        """in_proj's or out_proj's weight for products of many rows: a 4-bit one brought back to ``dtype``."""
+        return linear.weight4.dequantize(dtype) if self.weights_4bit else linear.weight
 
     def _params(self, weights=None):
         """The parameters in the order the native host path takes them."""
@@ -440,7 +438,7 @@ class HdcMamba9v3Block(nn.Module):
         (two-pass variance, the weight as it is now: the folded form reads row sums kept until the
         weight's version changes, which a write through ``.data`` or a flat buffer does not do)."""
         fused = not train and self._fused_out(x)
-        weights = self._weights(x.dtype)
+        weights = self._weight(self.in_proj, x.dtype), self._weight(self.out_proj, x.dtype)
         sums = None
         if fused and _ops.rowln_stats_ok(x, self.d_model):
             sums = _ops.row_sums(weights[1]) if self.weights_4bit else self._out_weight_sums(x.dtype)
@@ -507,7 +505,7 @@ class HdcMamba9v3Block(nn.Module):
         row statistics to the GEMM (hdcm_rowln_gemm_stats_fwd); otherwise the GEMM takes them
         from its operands (hdcm_rowln_gemm_fwd)."""
         B, L, dm = x.shape
-        w = self._weights(x.dtype)[1].to(x.dtype)
+        w = self._weight(self.out_proj, x.dtype).to(x.dtype)
         x2 = x.reshape(B * L, dm)
         o2 = None if out is None else out.view(B * L, dm)
         if _ops.rowln_stats_ok(x2, dm):
@@ -553,7 +551,7 @@ class HdcMamba9v3Block(nn.Module):
 
     def _out_proj(self, x, c, out=None):
         """x + c @ out_proj.weight^T of rows x [M, dm], c [M, ds + dm], into ``out`` (which may be x) when given."""
-        w = self._weights(x.dtype)[1].to(x.dtype)
+        w = self._weight(self.out_proj, x.dtype).to(x.dtype)
         if not torch.is_grad_enabled() and forward_ad._current_level < 0 and _ops.gemm_f32_preferred(x.shape[0], c, w, x):
             return _ops.gemm_f32(c, w, res=x, out=out)
         with nullcontext() if torch.is_grad_enabled() else _products_in(x.dtype):

@@ -275,3 +275,21 @@ def test_fp32_blocks_under_bf16_autocast(dev, quantized):
     for a, b in zip(got, want):
         assert a.dtype == F32
         assert_close(a, b.cpu(), F32, "under autocast")
+
+
+def test_a_forward_brings_each_weight_back_once(dev, monkeypatch):
+    """The native path and the composition (with and without the folded LayerNorm): two weights a block, no more."""
+    blk = hm.quantize_4bit(_lm(256, 64, 4, 32, 1, 50, BF).to(dev)).backbone.layers[0]
+    calls, plain = [], hm.Weight4Bit.dequantize
+    monkeypatch.setattr(hm.Weight4Bit, "dequantize", lambda self, dtype: calls.append(self.shape) or plain(self, dtype))
+    x = torch.randn(1, 64, 256, device=dev).to(BF)
+    shapes = [blk.in_proj.weight4.shape, blk.out_proj.weight4.shape]
+    with torch.no_grad():
+        for native in (True, False):
+            if not native:
+                monkeypatch.setattr(blk, "_native_ok", lambda x: False)
+            for fused in (True, False):
+                hm.set_fused_out_proj(blk, fused)
+                calls.clear()
+                blk(x)
+                assert sorted(calls) == sorted(shapes), (native, fused)
