@@ -50,7 +50,8 @@ class Weight4Bit:
     def __init__(self, packed, scales, zeros, shape, group_size):
         self.packed, self.scales, self.zeros = packed, scales, zeros
         self.shape, self.group_size = tuple(int(n) for n in shape), int(group_size)
-        self._handle = _ops.native().Weight4(packed, scales, zeros, *self.shape, self.group_size)
+        # on the CPU it can be kept, copied and moved, no more
+        self._handle = _ops.native().Weight4(packed, scales, zeros, *self.shape, self.group_size) if packed.is_cuda else None
 
     def __reduce__(self):  # copies and pickles are made from the buffers
         return Weight4Bit, (self.packed, self.scales, self.zeros, self.shape, self.group_size)
@@ -146,6 +147,7 @@ class Weight4Bit:
 
     def refresh(self):
         """Bring what the weight keeps beside its buffers (the row sums of norm_eps) in line with them."""
+        _ops._on_gpu(self.packed)
         self._handle.refresh()
 
     def __repr__(self):
@@ -160,6 +162,8 @@ def linear_4bit(x, weight, bias=None, residual=None, out=None, norm_eps=None):
     the product of the rows after a LayerNorm without affine, in the same launch; its variance is the
     difference of two fp32 sums, for rows whose mean is not far above their deviation.  A bf16 row
     that holds an infinity becomes NaN.  No gradient: refused where one would be recorded or carried forward."""
+    if weight._handle is None:
+        _ops._on_gpu(weight.packed)
     return _ops.native().linear_4bit(x, weight._handle, bias, residual, out, norm_eps)
 
 
@@ -192,16 +196,29 @@ class Linear4Bit(nn.Module):
 
     @property
     def weight4(self) -> Weight4Bit:
-        """The packed weight (made anew after the buffers were moved)."""
+        """The buffers as the packed weight that linear_4bit takes."""
         w = self._weight4
-        if w.packed is not self.packed or w.scales is not self.scales or w.zeros is not self.zeros:
-            w = self._weight4 = Weight4Bit(self.packed, self.scales, self.zeros, w.shape, w.group_size)
+        if w is None or w.packed is not self.packed or w.scales is not self.scales or w.zeros is not self.zeros:
+            w = self._weight4 = Weight4Bit(self.packed, self.scales, self.zeros, (self.out_features, self.in_features),
+                                           self.group_size)
         return w
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._weight4 = None  # which holds the buffers from before
+        if self.packed.is_cuda and self.scales.dtype in _ops._DTYPES:
+            self.weight4
+        return self
+
+    def __getstate__(self):  # the buffers once
+        return dict(self.__dict__, _weight4=None)
 
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
         if self.packed.is_cuda:
             self.weight4.refresh()
+        else:
+            self._weight4 = None
 
     def forward(self, x):
         if (torch.is_grad_enabled() and x.requires_grad) or carries_tangent(x):

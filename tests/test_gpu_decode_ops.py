@@ -884,3 +884,51 @@ def test_linear4bit_module_under_autocast(dev):
                     assert layer(x[:rows]).dtype == F32
             with torch.amp.autocast("cuda", dtype=torch.float16), pytest.raises(TypeError, match="dtype"):
                 layer(x[:rows])
+
+
+# ------------------------------------------------------------------------------- where a weight is held
+def test_weight_and_module_on_the_cpu(dev):
+    """A weight and a module that were moved to the CPU hold no GPU memory, are copied, saved and loaded there (also what was
+    saved on the GPU), refuse to compute, and moved back give the same products."""
+    import io
+
+    N, K = 4096, 1024
+    x = torch.randn(3, K, generator=_gen(1)).to(BF).to(dev)
+    linear = torch.nn.Linear(K, N, device=dev, dtype=BF)
+    layer = hm.Linear4Bit.from_linear(linear, 64, zero_points=True)
+    want, normed = layer(x), hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+    torch.cuda.synchronize()
+    size = layer.packed.numel()
+    files = [io.BytesIO(), io.BytesIO()]
+    for f, thing in zip(files, (layer, layer.weight4)):
+        torch.save(thing, f)
+        assert size < f.tell() < 1.3 * size  # the buffers once
+        f.seek(0)
+    del thing
+    before = torch.cuda.memory_allocated(dev)
+    layer.cpu()
+    assert before - torch.cuda.memory_allocated(dev) >= size
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        layer(x.cpu())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        hm.linear_4bit(x, layer.weight4)
+    copies = [layer, copy.deepcopy(layer), pickle.loads(pickle.dumps(layer)), *(torch.load(f, map_location="cpu", weights_only=False) for f in files)]
+    state = hm.Linear4Bit.from_linear(linear, 64, zero_points=True).cpu()
+    state.packed.zero_()
+    state.load_state_dict(layer.state_dict())
+    for c in [*copies, state]:
+        assert c.packed.device.type == "cpu" and torch.equal(c.packed, layer.packed if c is not layer else c.packed)
+    layer.to(dev)
+    for c in copies[1:] + [state]:
+        c = c.to(dev)
+        w = c if isinstance(c, hm.Weight4Bit) else c.weight4
+        assert torch.equal(hm.linear_4bit(x, w, bias=linear.bias.detach()), want)
+        assert torch.equal(hm.linear_4bit(x, w, norm_eps=1e-5), normed)
+    assert torch.equal(layer(x), want)
+    layer.cpu().to(dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # the first product after a move
+        out = hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+    graph.replay()
+    assert torch.equal(out, normed)
