@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from . import _ops
 from .model import BlockState, HdcMamba9v3Model, layer_norm
+from .quant4 import Linear4Bit
 from .sampling import append_tokens, fill_token_history, new_token_history, select_tokens
 
 __all__ = ["HdcMambaLM", "DecodeGraph", "ForwardGraph", "SIZES"]
@@ -145,6 +146,14 @@ def _clone_state(st):
                       S_intra=st.S_intra.clone(), pos=st.pos)
 
 
+def _recorded_tensors(lm):
+    """What a recording of lm reads, to be held by it: the module may get other weights (quantize_4bit, a move) while
+    the recording goes on with these."""
+    held = [t.detach() for t in (*lm.parameters(), *lm.buffers())]
+    held += [m.weight4 for m in lm.modules() if isinstance(m, Linear4Bit)]
+    return held + [getattr(m, "_wsum", None) for m in lm.modules()]  # out_proj's row sums
+
+
 class DecodeGraph:
     """One decode step of an HdcMambaLM recorded once as a HIP graph and replayed per token.
 
@@ -155,7 +164,9 @@ class DecodeGraph:
     bf16: the LayerNorm + conv + in_proj front, the mixer step and out_proj) at once instead
     of launching each from Python.  The states passed in are the ones the replays
     update; ``step`` keeps their host-side ``pos`` in sync.  Replays of one DecodeGraph must
-    not overlap with other work on the same states.
+    not overlap with other work on the same states.  Weights are read at replay time; a model that was
+    rounded (quantize_4bit) or moved since has others, while the graph replays on, and holds, those it
+    was recorded with.
 
     With ``controls`` (the keyword arguments of sampling.select_tokens but for the logits) the recording goes on
     to choose the next token of every sequence, counts it in controls["history"] where there is one and
@@ -197,6 +208,7 @@ class DecodeGraph:
         with torch.cuda.graph(self.graph):
             self.logits = self._run(self.states, self.pos)
             self.tokens, self.logprobs = self._choose(self.logits, self.controls)
+        self._held = _recorded_tensors(lm) + [(st.conv, st.h, st.S_prev, st.S_intra) for st in states]
 
     def _run(self, states, pos):
         with torch.no_grad():
@@ -247,7 +259,8 @@ class ForwardGraph:
     weights are read at replay time (in place updates are seen: values derived from a
     weight and kept between forwards, the out_proj row sums, are refreshed in place before
     a replay when the weight's version changed); the recorded shapes, dtypes and buffers
-    are fixed.
+    are fixed: a model that was rounded (quantize_4bit) or moved since has other weights, while the
+    graph replays on, and holds, those it was recorded with.
     """
 
     def __init__(self, lm, input_ids, warmup=2):
@@ -268,6 +281,7 @@ class ForwardGraph:
         self.graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.logits = lm(self.ids)
+        self._held = _recorded_tensors(lm)
         self._refresh = [m for m in lm.modules() if hasattr(m, "refresh_derived_weights")]
 
     def forward(self, input_ids):

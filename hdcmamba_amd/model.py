@@ -474,13 +474,13 @@ class HdcMamba9v3Block(nn.Module):
 
     def _out_weight_sums(self, dtype):
         """Row sums of the out_proj weight as used (in ``dtype``), kept until the parameter changes (its
-        storage or its version counter).  A refresh writes into the same buffer, so a recorded graph
-        that reads it sees the new sums."""
+        storage or its version counter).  A refresh for the same storage writes into the same buffer, so
+        a recorded graph that reads both sees the new sums; another storage gets another buffer."""
         p = self.out_proj.weight
         key = (p.data_ptr(), p._version, dtype, p.device)
         if getattr(self, "_wsum_key", None) != key:
             old = getattr(self, "_wsum", None)
-            if old is not None and old.device == p.device and old.numel() == p.shape[0]:
+            if old is not None and key[0] == self._wsum_key[0] and old.device == p.device and old.numel() == p.shape[0]:
                 _ops.row_sums(p.to(dtype), out=old)
             else:
                 self._wsum = _ops.row_sums(p.to(dtype))
@@ -835,7 +835,8 @@ def quantize_4bit(module, group_size=128, zero_points=False, head=True):
     """Round in_proj and out_proj of every HdcMamba9v3Block inside ``module`` to 4 bits with group scales
     (Weight4Bit.quantize, scales in the weight's type), and with ``head`` every ``lm_head`` (the embedding
     that HdcMambaLM's shares its weight with keeps it); returns ``module``, on the GPU and for inference
-    only from then on.  A decode step then streams a quarter of the weights' bytes."""
+    only from then on.  A decode step then streams a quarter of the weights' bytes.  A DecodeGraph or
+    ForwardGraph recorded before goes on with the weights from before, whose memory it holds."""
     for m in module.modules():
         names = ("in_proj", "out_proj") if isinstance(m, HdcMamba9v3Block) else ("lm_head",) if head else ()
         for name in names:

@@ -293,3 +293,36 @@ def test_a_forward_brings_each_weight_back_once(dev, monkeypatch):
                 calls.clear()
                 blk(x)
                 assert sorted(calls) == sorted(shapes), (native, fused)
+
+
+@pytest.mark.parametrize("change", ["quantize", "move", "move a quantized"])
+def test_recordings_outlive_the_weights_of_the_module(dev, change):
+    """A model that gets other weights, and memory that is used again: earlier recordings replay on theirs."""
+    from hdcmamba_amd.lm import _clone_state
+
+    lm = _lm(256, 64, 4, 32, 2, 500, BF).to(dev)
+    if change == "move a quantized":
+        hm.quantize_4bit(lm)
+    ids = torch.randint(0, 500, (2, 64), generator=torch.Generator().manual_seed(3)).to(dev)
+    _, states = lm.prefill(ids)
+    start = [_clone_state(st) for st in states]
+    fg, dg = lm.capture_forward(ids), lm.capture_decode(states)
+    want = fg(ids).clone(), dg.step(ids[:, 0]).clone()
+    for a, b in zip(states, start):
+        for name in ("conv", "h", "S_prev", "S_intra"):
+            getattr(a, name).copy_(getattr(b, name))
+    dg.pos.fill_(start[0].pos)
+    torch.cuda.synchronize()
+    sizes = [t.numel() for m in (lm, lm.backbone) for t in (*m.parameters(), *m.buffers())]
+    if change == "quantize":
+        hm.quantize_4bit(lm)
+    else:
+        lm.cpu().to(dev)
+        with torch.no_grad():  # and other values, which a forward uses
+            for p in (*lm.parameters(), *(m.scales for m in lm.modules() if isinstance(m, hm.Linear4Bit))):
+                p.mul_(1.5)
+            assert not torch.equal(lm(ids), want[0])
+    junk = [torch.full((n,), float("nan"), device=dev, dtype=dt) for n in sizes for dt in (BF, F32) for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(fg(ids), want[0])
+    assert torch.equal(dg.step(ids[:, 0]), want[1]) and len(junk) == 4 * len(sizes)
