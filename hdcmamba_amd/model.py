@@ -475,15 +475,22 @@ class HdcMamba9v3Block(nn.Module):
     def _out_weight_sums(self, dtype):
         """Row sums of the out_proj weight as used (in ``dtype``), kept until the parameter changes (its
         storage or its version counter).  A refresh for the same storage writes into the same buffer, so
-        a recorded graph that reads both sees the new sums; another storage gets another buffer."""
+        a recorded graph that reads both sees the new sums; another storage gets another buffer.  The host
+        waits for them, once per change of the weight, so that they are finished for every stream; inside a
+        recording they are formed for it alone."""
         p = self.out_proj.weight
         key = (p.data_ptr(), p._version, dtype, p.device)
         if getattr(self, "_wsum_key", None) != key:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                return _ops.row_sums(p.to(dtype))
+            self._wsum_key, last = None, getattr(self, "_wsum_key", None)
             old = getattr(self, "_wsum", None)
-            if old is not None and key[0] == self._wsum_key[0] and old.device == p.device and old.numel() == p.shape[0]:
+            if old is not None and last is not None and key[0] == last[0] and old.device == p.device and old.numel() == p.shape[0]:
                 _ops.row_sums(p.to(dtype), out=old)
             else:
                 self._wsum = _ops.row_sums(p.to(dtype))
+            if p.is_cuda:
+                torch.cuda.current_stream(p.device).synchronize()
             self._wsum_key = key
         return self._wsum
 

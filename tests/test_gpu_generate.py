@@ -326,3 +326,39 @@ def test_recordings_outlive_the_weights_of_the_module(dev, change):
     torch.cuda.synchronize()
     assert torch.equal(fg(ids), want[0])
     assert torch.equal(dg.step(ids[:, 0]), want[1]) and len(junk) == 4 * len(sizes)
+
+
+def test_out_proj_row_sums_are_finished_for_every_reader(dev):
+    """An unquantised block's weight is written in place: two streams use it, the first one busy; then a recording is the
+    first to use it, and an eager forward comes before the first replay."""
+    blk, twin = (_lm(512, 64, 4, 32, 1, 50, BF).to(dev).backbone.layers[0] for _ in range(2))
+    x = torch.randn(2, 64, 512, generator=torch.Generator().manual_seed(2)).to(BF).to(dev)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    with torch.no_grad():
+        blk(x)
+        assert blk._wsum is not None
+        blk.out_proj.weight.mul_(-2)
+        twin.out_proj.weight.mul_(-2)
+        want = twin(x)[0]
+        torch.cuda.synchronize()
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if i == 0:
+                    torch.cuda._sleep(20_000_000)
+                got.append(blk(x)[0])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want) and torch.equal(got[1], want)
+        blk.out_proj.weight.mul_(4)
+        twin.out_proj.weight.mul_(4)
+        want = twin(x)[0]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = blk(x)[0]
+        assert torch.equal(blk(x)[0], want)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+            torch.cuda.synchronize()
