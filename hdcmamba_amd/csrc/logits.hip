@@ -217,7 +217,7 @@ __device__ __forceinline__ void write_pick(const Pick& a, int64_t* token, float*
   // nothing allowed (or only NaN): no token
   const bool none = a.at == kNoToken;
   *token = none ? -1 : a.at;
-  *logprob = none ? -kInf : a.t - (a.max + logf(a.sum));
+  *logprob = none ? -kInf : (a.t - a.max) - logf(a.sum);  // of large logits: no rounding at their magnitude
 }
 
 constexpr int kPickThreads = 512;

@@ -932,3 +932,20 @@ def test_weight_and_module_on_the_cpu(dev):
         out = hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
     graph.replay()
     assert torch.equal(out, normed)
+
+
+@pytest.mark.parametrize("V", [5, 3000, 50277])
+def test_log_probabilities_of_large_logits(dev, V):
+    """Logits far from 0, and small temperatures: the sum as in test_select_tokens, 320 2^-24 of it; the difference to the
+    largest logit and the result rounded once each.  Nothing is rounded at the logits' own magnitude."""
+    g = _gen(V)
+    l = torch.randn(4, V, generator=g) * 2 + torch.tensor([5000.0, -20000.0, 3.0, 1e6])[:, None]
+    noise = -torch.log(-torch.log(torch.rand(4, V, generator=g).clamp(1e-6, 1 - 1e-6)))
+    temp = torch.tensor([1.0, 0.9, 0.003, 2.0])
+    for n in (None, noise):
+        tok, lp = (t.cpu() for t in hm.select_tokens(l.to(dev), temperature=temp.to(dev), noise=None if n is None else n.to(dev)))
+        t = l / temp[:, None]
+        assert torch.equal(tok, (t if n is None else t + n).argmax(1))
+        want = t.double().log_softmax(1).gather(1, tok[:, None])[:, 0]
+        below = (t.amax(1) - t.gather(1, tok[:, None])[:, 0]).double()
+        assert ((lp.double() - want).abs() <= 320 * 2.0**-24 + 2.0**-23 * (below + want.abs())).all()
