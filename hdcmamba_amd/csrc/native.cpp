@@ -606,6 +606,11 @@ const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() :
 // torch's current stream on t's device (asked here: a call through Python costs 1.8 us)
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// A kernel wrote t through its pointer: counted as a write, so that autograd sees a saved tensor overwritten.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void same_device(const Tensor& t, const Tensor& ref, const char* name) {
   TORCH_CHECK(t.device() == ref.device(), name, " is on ", t.device(), ", expected ", ref.device());
 }
@@ -752,6 +757,7 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
                            (const uint8_t*)pointer(w.zeros), w.group, pointer(b), pointer(r),
                            r.defined() ? r.stride(0) : 0, o.mutable_data_ptr(), o.stride(0), o.size(0), w.N, K, dt,
                            stream_of(x)));
+  if (given.defined()) written(given);
   return out;
 }
 
@@ -853,6 +859,7 @@ Tensor process_logits(const Tensor& logits, const ControlArgs& args, const OptTe
   check("hdcm_logits_process",
         hdcm_logits_process(l.const_data_ptr(), l.stride(0), &k.c, out.mutable_data_ptr(), out.stride(0), l.size(0), l.size(1), dt,
                             stream_of(l)));
+  if (out_) written(out);
   return out;
 }
 
@@ -927,6 +934,7 @@ Tensor fill_token_history(Tensor table, const OptTensor& prompt, const OptTensor
   check("hdcm_token_history_fill",
         hdcm_token_history_fill(table.mutable_data_ptr<int16_t>(), table.stride(0), p.p, p.stride, p.n, p.width, o.p, o.stride,
                                 o.n, o.width, table.size(0), table.size(1), stream_of(table)));
+  written(table);
   return table;
 }
 
@@ -938,6 +946,7 @@ Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& length
   check("hdcm_token_history_append",
         hdcm_token_history_append(table.mutable_data_ptr<int16_t>(), table.stride(0), t.p, t.stride, t.n, t.width, table.size(0),
                                   table.size(1), stream_of(table)));
+  written(table);
   return table;
 }
 

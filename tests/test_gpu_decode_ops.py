@@ -949,3 +949,24 @@ def test_log_probabilities_of_large_logits(dev, V):
         want = t.double().log_softmax(1).gather(1, tok[:, None])[:, 0]
         below = (t.amax(1) - t.gather(1, tok[:, None])[:, 0]).double()
         assert ((lp.double() - want).abs() <= 320 * 2.0**-24 + 2.0**-23 * (below + want.abs())).all()
+
+
+def test_writes_into_given_memory_are_counted(dev):
+    """out= and the history table: a write is seen by autograd's check of the tensors it saved, as torch's own are."""
+    w = hm.Weight4Bit.quantize(torch.randn(40, 64, generator=_gen(5)).to(dev), 32)
+    x, leaf = torch.ones(3, 64, device=dev), torch.zeros(3, 40, device=dev, requires_grad=True)
+    for write in (lambda t: hm.process_logits(t, bias=torch.ones(40, device=dev), out=t), lambda t: hm.linear_4bit(x, w, out=t),
+                  lambda t: hm.linear_4bit(x, w, residual=t, out=t)):
+        y = leaf.exp()  # saved for its own gradient
+        with torch.no_grad():
+            assert write(y.detach()).data_ptr() == y.data_ptr()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    table = hm.new_token_history(3, 40, dev)
+    for write in (lambda: hm.fill_token_history(table), lambda: hm.append_tokens(table, torch.zeros(3, dtype=torch.long, device=dev))):
+        before = table._version
+        write()
+        assert table._version > before
+    with torch.inference_mode():
+        t = torch.zeros(3, 40, device=dev)
+        assert hm.process_logits(t, out=t) is t
