@@ -642,15 +642,15 @@ bool same_place(const Tensor& a, const Tensor& b) {
   return a.const_data_ptr() == b.const_data_ptr() && (a.size(0) <= 1 || a.stride(0) == b.stride(0));
 }
 
-// A packed weight, checked once (the handle of a Weight4Bit), and its row sums as the products give them: for
+// A packed weight (the handle of a Weight4Bit), and its row sums as the products give them: for
 // products behind a LayerNorm, formed again where a buffer was written since (load_state_dict).  The host
 // waits for them (a weight is made or written once), so a call on any stream, and any recording, reads finished sums.
 struct Weight4 {
   Tensor packed, scales, zeros, row_sums;
   int64_t N, K, group;
   int scale_dtype;
-  using Versions = std::array<uint32_t, 3>;
-  std::optional<Versions> versions{};  // of the buffers that row_sums belongs to
+  using Versions = std::array<std::pair<uint32_t, const void*>, 3>;
+  std::optional<Versions> versions{};  // and storages, of the buffers that row_sums belongs to
   // none where a buffer was made under inference mode: such a tensor does not count its writes
   std::optional<Versions> versions_now() const {
     Versions v{};
@@ -658,9 +658,21 @@ struct Weight4 {
     for (int i = 0; i < 3; ++i)
       if (ts[i]->defined()) {
         if (ts[i]->is_inference()) return std::nullopt;
-        v[i] = (uint32_t)ts[i]->_version();
+        v[i] = {(uint32_t)ts[i]->_version(), ts[i]->const_data_ptr()};
       }
     return v;
+  }
+  // with every use: a buffer's storage can be replaced under the tensor (t.data = other, set_, resize_)
+  void check() const {
+    const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
+    TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() &&
+                    (size_t)packed.numel() == hdcm_w4_packed_bytes(N, K) && scales.is_contiguous() && scales.numel() == per &&
+                    dtype_of(scales) == scale_dtype,
+                "the packed weight's buffers do not hold [", N, ", ", K, "] in groups of ", group);
+    same_device(scales, packed, "scales");
+    if (!zeros.defined()) return;
+    same_device(zeros, packed, "zeros");
+    TORCH_CHECK(zeros.scalar_type() == at::kByte && zeros.is_contiguous() && zeros.numel() == per, "zeros must hold one byte per scale");
   }
 };
 Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const OptTensor& residual_, const OptTensor& out_,
@@ -685,16 +697,7 @@ Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor
   Weight4 w{packed, scales, or_none(zeros), Tensor(), N, K, group, dtype_of(scales)};
   TORCH_CHECK(N > 0 && K > 0 && (group == 32 || group == 64 || group == 128), "a 4-bit weight [", N, ", ", K, "] in groups of ",
               group);
-  const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
-  same_device(scales, packed, "scales");
-  TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() &&
-                  (size_t)packed.numel() == hdcm_w4_packed_bytes(N, K) && scales.is_contiguous() && scales.numel() == per,
-              "the packed weight's buffers do not hold [", N, ", ", K, "] in groups of ", group);
-  if (w.zeros.defined()) {
-    same_device(w.zeros, packed, "zeros");
-    TORCH_CHECK(w.zeros.scalar_type() == at::kByte && w.zeros.is_contiguous() && w.zeros.numel() == per,
-                "zeros must hold one byte per scale");
-  }
+  w.check();
   w.row_sums = fp32({N}, packed);
   sum_rows(w);
   return w;
@@ -709,6 +712,7 @@ Tensor linear_4bit(const Tensor& x, Weight4& w, const OptTensor& bias_, const Op
   const c10::DeviceGuard guard(x.device());
   const int dt = dtype_of(x);
   same_device(w.packed, x, "the weight");
+  w.check();
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) == w.K, "linear_4bit: x ", x.sizes(), " does not end in the weight's ", w.K, " columns");
   auto shape = x.sizes().vec();
   shape.back() = w.N;
@@ -973,7 +977,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mixer_backward", &mixer_backward);
   m.def("norm_conv_forward", &norm_conv_forward);
   m.def("norm_conv_backward", &norm_conv_backward);
-  pybind11::class_<Weight4>(m, "Weight4").def(pybind11::init(&make_weight4)).def("refresh", &sum_rows);
+  pybind11::class_<Weight4>(m, "Weight4").def(pybind11::init(&make_weight4)).def("refresh", &sum_rows).def("check", &Weight4::check);
   m.def("linear_4bit", &linear_4bit);
   m.def("process_logits", &process_logits);
   m.def("select_tokens", &select_tokens);

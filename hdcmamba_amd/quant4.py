@@ -40,7 +40,7 @@ class Weight4Bit:
     (``quantize``), then passed to linear_4bit.  Its buffers may be written in place (load_state_dict): the
     row sums that norm_eps reads are formed again, with a wait of the host, by the next call with it.
     Inside a recording that is refused: ``refresh`` first; a graph recorded before sees the new sums after
-    ``refresh`` too.
+    ``refresh`` too, and so does any call after a write through ``.data``, which tensors do not count.
 
     ``shape`` (N, K), ``group_size``; ``packed`` uint8, ``scales`` (float32 or bfloat16) and ``zeros``
     (uint8 or None) in the layout of hdcm_w4_linear_fwd (include/hdcm.h)."""
@@ -131,6 +131,7 @@ class Weight4Bit:
         if dtype not in _ops._DTYPES:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
         _ops._on_gpu(self.packed)
+        self._handle.check()
         N, K = self.shape
         with torch.cuda.device(self.packed.device):
             out = torch.empty(N, K, dtype=dtype, device=self.packed.device)

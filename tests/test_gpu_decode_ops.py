@@ -970,3 +970,21 @@ def test_writes_into_given_memory_are_counted(dev):
     with torch.inference_mode():
         t = torch.zeros(3, 40, device=dev)
         assert hm.process_logits(t, out=t) is t
+
+
+def test_a_weight_whose_buffer_was_replaced_is_refused(dev):
+    """A buffer with another storage under it (t.data = other) is checked again at every use."""
+    x = torch.zeros(2, 128, device=dev, dtype=BF)
+    for name, other, match in (("packed", lambda t: t[:1024].clone(), "do not hold"), ("scales", lambda t: t[:1].clone(), "do not hold"),
+                               ("scales", lambda t: t.t().contiguous().t(), "do not hold"), ("zeros", lambda t: t[:1].clone(), "one byte"),
+                               ("packed", lambda t: t.cpu(), "cpu")):
+        w = hm.Weight4Bit.quantize(torch.randn(64, 128, generator=_gen(5)).to(dev), 32, True)
+        t = getattr(w, name)
+        t.data = other(t)
+        for call in (lambda: hm.linear_4bit(x, w), lambda: hm.linear_4bit(x, w, norm_eps=1e-5), lambda: w.dequantize(), w.refresh):
+            with pytest.raises(RuntimeError, match=match):
+                call()
+    x, w, other, want = _norm_weights(dev)
+    for name in ("packed", "scales", "zeros"):  # of the same size: the weight is the other, and so are its row sums
+        getattr(w, name).data = getattr(other, name).clone()
+    assert torch.equal(hm.linear_4bit(x, w, norm_eps=1e-5), want)
