@@ -844,10 +844,11 @@ def quantize_4bit(module, group_size=128, zero_points=False, head=True):
     that HdcMambaLM's shares its weight with keeps it); returns ``module``, on the GPU and for inference
     only from then on.  A decode step then streams a quarter of the weights' bytes.  A DecodeGraph or
     ForwardGraph recorded before goes on with the weights from before, whose memory it holds."""
-    for m in module.modules():
-        names = ("in_proj", "out_proj") if isinstance(m, HdcMamba9v3Block) else ("lm_head",) if head else ()
-        for name in names:
-            linear = getattr(m, name, None)
-            if isinstance(linear, nn.Linear):
-                setattr(m, name, Linear4Bit.from_linear(linear, group_size, zero_points))
+    found = [(m, name) for m in module.modules()
+             for name in (("in_proj", "out_proj") if isinstance(m, HdcMamba9v3Block) else ("lm_head",) if head else ())
+             if isinstance(getattr(m, name, None), nn.Linear)]
+    # all of them before the first is replaced: a weight that is refused leaves the module as it was
+    rounded = [Linear4Bit.from_linear(getattr(m, name), group_size, zero_points) for m, name in found]
+    for (m, name), linear in zip(found, rounded):
+        setattr(m, name, linear)
     return module

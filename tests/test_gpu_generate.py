@@ -362,3 +362,18 @@ def test_out_proj_row_sums_are_finished_for_every_reader(dev):
             graph.replay()
             assert torch.equal(out, want)
             torch.cuda.synchronize()
+
+
+def test_a_refused_weight_leaves_the_model_as_it_was(dev):
+    lm = _lm(256, 64, 4, 32, 2, 50, BF).to(dev)
+    ids = torch.randint(0, 50, (1, 32), device=dev)
+    with torch.no_grad():
+        want = lm(ids)
+        weight = lm.backbone.layers[1].out_proj.weight
+        kept = weight[3, 5].clone()
+        weight[3, 5] = float("nan")
+        with pytest.raises(ValueError, match="infinities"):
+            hm.quantize_4bit(lm)
+        weight[3, 5] = kept
+        assert not any(isinstance(m, hm.Linear4Bit) for m in lm.modules()) and torch.equal(lm(ids), want)
+        assert sum(isinstance(m, hm.Linear4Bit) for m in hm.quantize_4bit(lm).modules()) == 5
