@@ -667,7 +667,7 @@ class HdcMamba9v3Block(nn.Module):
 
     def _step_4bit(self, x, state, pos_dev):
         """step with 4-bit in_proj and out_proj: LayerNorm + conv of the token, in_proj, the mixer step, and out_proj
-        with the row LayerNorm before it and the residual."""
+        with the row LayerNorm before it (in the same launch with fused_out_proj, in bf16) and the residual."""
         self._no_grad_4bit(x)
         dm, ds, H, C = self.d_model, self.d_state, self.num_heads, self.chunk_size
         xc = _ops.norm_conv_step(x, self.norm.weight, self.norm.bias, self.conv1d.weight.squeeze(1), self.conv1d.bias,
@@ -678,7 +678,7 @@ class HdcMamba9v3Block(nn.Module):
                         self.group_norm.bias, 1e-5, state.h, state.S_prev, state.S_intra, state.pos, C, combined, dm, H,
                         pos_dev=pos_dev)
         eps = 1e-5
-        if x.dtype != torch.bfloat16:  # the product's own LayerNorm is for bfloat16
+        if not self.fused_out_proj or x.dtype != torch.bfloat16:  # the product's own LayerNorm is for bfloat16
             _ops.layer_norm(combined, eps=eps, out=combined)
             eps = None
         y = linear_4bit(combined, self.out_proj.weight4, residual=x, norm_eps=eps)

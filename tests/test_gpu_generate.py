@@ -377,3 +377,21 @@ def test_a_refused_weight_leaves_the_model_as_it_was(dev):
         weight[3, 5] = kept
         assert not any(isinstance(m, hm.Linear4Bit) for m in lm.modules()) and torch.equal(lm(ids), want)
         assert sum(isinstance(m, hm.Linear4Bit) for m in hm.quantize_4bit(lm).modules()) == 5
+
+
+def test_quantized_step_without_the_folded_layer_norm(dev, monkeypatch):
+    """set_fused_out_proj(False): the LayerNorm in a pass of its own, the same step within bf16."""
+    from hdcmamba_amd import model
+
+    eps, plain = [], model.linear_4bit
+    monkeypatch.setattr(model, "linear_4bit", lambda *a, norm_eps=None, **kw: eps.append(norm_eps) or plain(*a, norm_eps=norm_eps, **kw))
+    blk = hm.quantize_4bit(_lm(256, 64, 4, 32, 1, 50, BF).to(dev)).backbone.layers[0]
+    x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1)).to(BF).to(dev)
+    got = []
+    with torch.no_grad():
+        for fused in (True, False):
+            hm.set_fused_out_proj(blk, fused)
+            eps.clear()
+            got.append(blk.step(x, blk.new_state(3, dev, BF)))
+            assert eps == [None, 1e-5 if fused else None]
+    assert_close_normwise(got[0], got[1].cpu(), BF, "step")
