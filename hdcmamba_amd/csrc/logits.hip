@@ -1,6 +1,6 @@
 // From logits to the next tokens of a batch of sequences (no counterpart in the reference, whose
 // generate samples on the host side of torch, train.py:139-151):
-//   process:  z = seen ? (l > 0 ? l / r : l r) : l;  z -= f count;  z -= p [count > 0];  z += bias;
+//   process:  z = seen ? (l > 0 ? l / r : l r) : l;  count > 0: z -= f count, z -= p;  z += bias;
 //             out = allowed ? z : -inf
 //   select:   t = z / T, token = the lowest index of the largest t + noise, and
 //             logprob = t[token] - log sum exp t, in one read and without writing z
@@ -141,7 +141,7 @@ template <typename T> struct Eight {
       for (int e = 0; e < 8; ++e) {
         const uint32_t t = (h.v[0][e / 2] >> (16 * (e & 1))) & 0xffffu, count = t & 0x7fffu;
         if (t) z[e] = z[e] > 0.f ? z[e] / c.r : z[e] * c.r;
-        z[e] = z[e] - c.f * (float)count;
+        z[e] = z[e] - (count ? c.f * (float)count : 0.f);  // an infinite penalty bans what the output holds, no more
         z[e] = z[e] - (count ? c.p : 0.f);
       }
     }

@@ -6,10 +6,12 @@ Controls, shared by process_logits and select_tokens.  For logit l of token v of
 and in this order:
 
   repetition  l / repetition if l > 0, else l * repetition, for tokens of the prompt or the output
-  frequency   l - frequency * count, count = how often the output holds the token
+  frequency   l - frequency * count if count > 0, count = how often the output holds the token
   presence    l - presence if count > 0
   bias        l + bias[v]
   mask        -inf unless bit v % 32 of mask word v // 32 is set
+
+An infinite ``frequency`` or ``presence`` bans the output's tokens.
 
 ``repetition`` (> 0), ``frequency`` and ``presence`` are numbers or tensors of one value per
 sequence and need ``history``, an int16 table [B, V] (new_token_history): the sign bit marks the

@@ -577,7 +577,7 @@ int hdcm_w4_linear_fwd(const void* x, int64_t x_row_stride, const float* row_sum
  * 0 shares one row between all sequences, and a penalty is per row ([B] fp32) or, where its pointer is
  * NULL, the `_all` value.  For logit l of token v of a row, in fp32, each step rounded once:
  *   seen (its history entry is not 0):  l > 0 ? l / repetition : l * repetition
- *   l - frequency * count;  l - presence if count > 0;  l + bias;  -inf unless bit v % 32 of mask
+ *   count > 0: l - frequency * count, l - presence;  l + bias;  -inf unless bit v % 32 of mask
  *   word v / 32 is set.
  * history is an int16 table: the sign bit marks tokens of the prompt, the low 15 bits count the
  * token in the output.  A row with repetition 1 and frequency and presence 0 does not read it.

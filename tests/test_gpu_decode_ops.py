@@ -988,3 +988,19 @@ def test_a_weight_whose_buffer_was_replaced_is_refused(dev):
     for name in ("packed", "scales", "zeros"):  # of the same size: the weight is the other, and so are its row sums
         getattr(w, name).data = getattr(other, name).clone()
     assert torch.equal(hm.linear_4bit(x, w, norm_eps=1e-5), want)
+
+
+@pytest.mark.parametrize("which", ["frequency", "presence"])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_infinite_penalties_ban_the_output(dev, which, per_row):
+    """Tokens of the output become -inf; what lies beside them, prompt tokens among it, keeps its logit."""
+    B, V = 2, 40
+    l = torch.randn(B, V, generator=_gen(1))
+    l[:, 3] = 9
+    prompt, output = torch.tensor([[3, 4, 30], [3, 7, 31]]), torch.tensor([[5, 30, 30], [3, 5, 22]])
+    table = hm.fill_token_history(hm.new_token_history(B, V, dev), prompt.to(dev), None, output.to(dev))
+    kw = {"history": table, which: torch.full((B,), float("inf"), device=dev) if per_row else float("inf")}
+    want = l.scatter(1, output, float("-inf"))
+    assert torch.equal(hm.process_logits(l.to(dev), **kw).cpu(), want)
+    token, lp = hm.select_tokens(l.to(dev), **kw)
+    assert torch.equal(token.cpu(), want.argmax(1)) and lp.isfinite().all()
