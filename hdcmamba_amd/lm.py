@@ -205,7 +205,7 @@ class DecodeGraph:
         torch.cuda.synchronize(dev)
         del scratch, scratch_pos, scratch_controls
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with torch.cuda.graph(self.graph, stream=side):  # (the default stream for recordings is one device's)
             self.logits = self._run(self.states, self.pos)
             self.tokens, self.logprobs = self._choose(self.logits, self.controls)
         self._held = _recorded_tensors(lm) + [(st.conv, st.h, st.S_prev, st.S_intra) for st in states]
@@ -279,7 +279,7 @@ class ForwardGraph:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(self.graph):
+        with torch.no_grad(), torch.cuda.graph(self.graph, stream=side):
             self.logits = lm(self.ids)
         self._held = _recorded_tensors(lm)
         self._refresh = [m for m in lm.modules() if hasattr(m, "refresh_derived_weights")]

@@ -395,3 +395,23 @@ def test_quantized_step_without_the_folded_layer_norm(dev, monkeypatch):
             got.append(blk.step(x, blk.new_state(3, dev, BF)))
             assert eps == [None, 1e-5 if fused else None]
     assert_close_normwise(got[0], got[1].cpu(), BF, "step")
+
+
+def test_recordings_are_made_on_the_models_device(dev, monkeypatch):
+    """torch records on one stream of the process by default, which lies on the device that recorded first: the model's
+    recordings name a stream of its own device."""
+    plain, seen = torch.cuda.graph, []
+    monkeypatch.setattr(torch.cuda, "graph", lambda g, stream=None: seen.append(stream) or plain(g, stream=stream))
+    lm = _lm(256, 64, 4, 32, 1, 50, BF).to(dev)
+    ids = torch.randint(0, 50, (1, 32), device=dev)
+    lm.capture_forward(ids)
+    lm.generate(ids, 3)
+    assert len(seen) == 2 and all(s is not None and s.device == dev for s in seen)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_generate_on_another_device():
+    lm, ids = _lm(256, 64, 4, 32, 1, 50, BF), torch.randint(0, 50, (2, 32))
+    want = [t.cpu() for t in lm.to("cuda:0").generate(ids.to("cuda:0"), 5, presence=0.5)]
+    got = [t.cpu() for t in lm.to("cuda:1").generate(ids.to("cuda:1"), 5, presence=0.5)]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
