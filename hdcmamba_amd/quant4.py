@@ -159,9 +159,10 @@ class Weight4Bit:
 def linear_4bit(x, weight, bias=None, residual=None, out=None, norm_eps=None):
     """x [..., K] times a Weight4Bit [N, K], transposed, (+ bias [N]) (+ residual [..., N]) -> [..., N] in
     x's type (float32 or bfloat16): fp32 sums of exact code products, the scales applied to the groups'
-    sums, one rounding.  ``out`` may be ``residual``.  ``norm_eps`` (bfloat16 rows of at least 8 columns):
+    sums, one rounding.  At most 16 * 65535 rows.  ``out`` may be ``residual``.  ``norm_eps`` (bfloat16 rows of at least 8 columns):
     the product of the rows after a LayerNorm without affine, in the same launch; its variance is the
-    difference of two fp32 sums, for rows whose mean is not far above their deviation.  A bf16 row
+    difference of two fp32 sums, for rows whose mean is not far above their deviation.  bf16 rows hold
+    values up to 2^115 (4e34): larger ones may become infinite or NaN in the sums of x (16 + c), and a row
     that holds an infinity becomes NaN.  No gradient: refused where one would be recorded or carried forward."""
     if weight._handle is None:
         _ops._on_gpu(weight.packed)

@@ -550,7 +550,8 @@ int hdcm_rowln_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t
  * `dtype`, fp32 accumulation of exact code products, the scales applied to the groups' sums, one
  * rounding.  bias and res may be NULL; res may be out itself.  x, bias, res and out need only
  * their type's alignment; rows may have any stride of at least their width.  x's columns past K (row
- * padding) are not read.  K >= 8 (bf16) or 4 (fp32).  bf16 x: an infinity makes its row NaN.  For the decode
+ * padding) are not read.  K >= 8 (bf16) or 4 (fp32), M <= 16 * 65535.  bf16 x: values up to 2^115 (4e34; the sums are of
+ * x (16 + c), 128 columns at a time, and of -x (16 + z)); an infinity makes its row NaN.  For the decode
  * step's rows: the weight is read once per block of up to 64 bf16 rows (16 of fp32), the largest where
  * the output is wide.
  * row_sums [N] fp32 (sum_k w[n,k]; NULL: x as it is): the product of x's rows after a LayerNorm without

@@ -108,3 +108,22 @@ def test_layer_norm_of_whole_rows(dev, M, K, N, group, zeros):
     bad = ref_x.clone()
     bad[:, -(K % group or group):] = 0
     assert not (((bad * rstd) @ dense.t() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,largest", [(BF, 2.0**115), (F32, 2.0**120)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
+def test_range_of_rows(dev, dtype, largest, group, zeros):
+    """Rows at the ends of the documented range: the products of rows times a power of two are the products times it.  (fp32:
+    codes of at most 15 times 2^120 times 128 columns would not be finite; these rows' largest sums are 2^6 times smaller.)"""
+    K, N = 1000, 70
+    codes, scales, z, dense = _weight(N, K, group, zeros, F32, 3)
+    w = _pack(dev, codes, scales / 2**20, z, group)
+    x = torch.randint(-2, 3, (6, K), generator=_gen(4)).float()
+    x[2] = 2  # all of the largest
+    x[3, 1:] = 0
+    want = hm.linear_4bit(x.to(dtype).to(dev), w).cpu().double()
+    assert want.abs().max() > 0
+    up = largest / 2 if dtype == BF else largest / 2**7
+    assert torch.equal(hm.linear_4bit((x * up).to(dtype).to(dev), w).cpu().double(), want * up)
+    down = 2.0**-100
+    assert torch.equal(hm.linear_4bit((x * down).to(dtype).to(dev), w).cpu().double(), want * down)
