@@ -207,9 +207,10 @@ class Linear4Bit(nn.Module):
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self._weight4 = None  # which holds the buffers from before
         if self.packed.is_cuda and self.scales.dtype in _ops._DTYPES:
-            self.weight4
+            self.weight4  # the same one (which recordings read) where nothing was moved
+        else:
+            self._weight4 = None  # nothing holds the buffers from before
         return self
 
     def __getstate__(self):  # the buffers once

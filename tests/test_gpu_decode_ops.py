@@ -1004,3 +1004,18 @@ def test_infinite_penalties_ban_the_output(dev, which, per_row):
     assert torch.equal(hm.process_logits(l.to(dev), **kw).cpu(), want)
     token, lp = hm.select_tokens(l.to(dev), **kw)
     assert torch.equal(token.cpu(), want.argmax(1)) and lp.isfinite().all()
+
+
+def test_a_move_to_the_same_place_keeps_the_weight(dev):
+    """... which a recording reads: a state dict loaded after it reaches the recording."""
+    x, one, two, want = _norm_weights(dev)
+    layer = hm.Linear4Bit(one)
+    hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hm.linear_4bit(x, layer.weight4, norm_eps=1e-5)
+    assert layer.to(dev).weight4 is one
+    layer.load_state_dict(hm.Linear4Bit(two).state_dict())
+    graph.replay()
+    assert torch.equal(out, want)
