@@ -568,7 +568,8 @@ class HdcMamba9v3Block(nn.Module):
         """In-place variant for a model-owned residual stream r [B,L,dm] (chunk-aligned):
         r += out_proj(LN(combined)), with the GEMM accumulating straight into r."""
         B, L, dm = r.shape
-        self._no_grad_4bit(r)
+        if self.weights_4bit and carries_tangent(r):
+            self._no_grad_4bit(r)
         if not torch.is_grad_enabled() and self._native_ok(r) and r.is_contiguous():
             return self._native_forward(r, state, out=r)
         if self._fused_out(r):

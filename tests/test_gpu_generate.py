@@ -415,3 +415,11 @@ def test_generate_on_another_device():
     want = [t.cpu() for t in lm.to("cuda:0").generate(ids.to("cuda:0"), 5, presence=0.5)]
     got = [t.cpu() for t in lm.to("cuda:1").generate(ids.to("cuda:1"), 5, presence=0.5)]
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_prefill_of_a_quantized_model_in_training_mode(dev):
+    """A prefill is inference whatever the module's mode."""
+    lm = hm.quantize_4bit(_lm(256, 64, 4, 32, 1, 50, BF).to(dev))
+    ids = torch.randint(0, 50, (1, 40), device=dev)
+    want = lm.prefill(ids)[0]
+    assert torch.equal(lm.train().prefill(ids)[0], want)
