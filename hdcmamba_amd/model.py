@@ -497,13 +497,13 @@ class HdcMamba9v3Block(nn.Module):
     def refresh_derived_weights(self):
         """Bring the kept out_proj row sums up to date with the weight (a recorded forward
         graph calls this before each replay; it launches nothing when the weight is
-        unchanged)."""
+        unchanged, or another storage, which no recording reads)."""
         if getattr(self, "_wsum_key", None) is None:
             return
         if self.weights_4bit:
             return
         p = self.out_proj.weight
-        if (p.data_ptr(), p._version) != self._wsum_key[:2]:
+        if p.data_ptr() == self._wsum_key[0] and p._version != self._wsum_key[1]:
             self._out_weight_sums(self._wsum_key[2])
 
     def _fused_mixer_out(self, x, state, out=None):

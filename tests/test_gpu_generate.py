@@ -423,3 +423,17 @@ def test_prefill_of_a_quantized_model_in_training_mode(dev):
     ids = torch.randint(0, 50, (1, 40), device=dev)
     want = lm.prefill(ids)[0]
     assert torch.equal(lm.train().prefill(ids)[0], want)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_recording_replays_while_the_model_is_elsewhere(dev, quantized):
+    lm = _lm(512, 64, 4, 32, 1, 100, BF).to(dev)
+    if quantized:
+        hm.quantize_4bit(lm)
+    ids = torch.randint(0, 100, (2, 64), device=dev)
+    fg, dg = lm.capture_forward(ids), lm.capture_decode(lm.prefill(ids)[1])
+    want = fg(ids).clone()
+    lm.cpu()
+    assert torch.equal(fg(ids), want) and dg.step(ids[:, 0]).isfinite().all()
+    lm.to(dev)
+    assert torch.equal(fg(ids), want)
