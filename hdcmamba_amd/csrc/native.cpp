@@ -592,7 +592,7 @@ Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() ==
 void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
   const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : ts) {
-    if (!t || !t->defined()) continue;
+    if (!t || !t->defined() || !t->unsafeGetTensorImpl()->autograd_meta()) continue;  // most take part in nothing
     TORCH_CHECK(!(backward && t->requires_grad()) && !(forward && t->_fw_grad(0).defined()), op,
                 " has no gradient: call it under torch.no_grad() or on detached tensors");
   }
@@ -649,6 +649,7 @@ struct Weight4 {
   Tensor packed, scales, zeros, row_sums;
   int64_t N, K, group;
   int scale_dtype;
+  int64_t packed_bytes, per;  // of the buffers
   using Versions = std::array<std::pair<uint32_t, const void*>, 3>;
   std::optional<Versions> versions{};  // and storages, of the buffers that row_sums belongs to
   // none where a buffer was made under inference mode: such a tensor does not count its writes
@@ -664,9 +665,7 @@ struct Weight4 {
   }
   // with every use: a buffer's storage can be replaced under the tensor (t.data = other, set_, resize_)
   void check() const {
-    const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
-    TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() &&
-                    (size_t)packed.numel() == hdcm_w4_packed_bytes(N, K) && scales.is_contiguous() && scales.numel() == per &&
+    TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() && packed.numel() == packed_bytes && scales.is_contiguous() && scales.numel() == per &&
                     dtype_of(scales) == scale_dtype,
                 "the packed weight's buffers do not hold [", N, ", ", K, "] in groups of ", group);
     same_device(scales, packed, "scales");
@@ -694,9 +693,10 @@ void sum_rows(Weight4& w) {
 }
 Weight4 make_weight4(const Tensor& packed, const Tensor& scales, const OptTensor& zeros, int64_t N, int64_t K, int64_t group) {
   on_gpu(packed);
-  Weight4 w{packed, scales, or_none(zeros), Tensor(), N, K, group, dtype_of(scales)};
   TORCH_CHECK(N > 0 && K > 0 && (group == 32 || group == 64 || group == 128), "a 4-bit weight [", N, ", ", K, "] in groups of ",
               group);
+  const int64_t per = (K + 127) / 128 * 128 / group * ((N + 15) / 16 * 16);
+  Weight4 w{packed, scales, or_none(zeros), Tensor(), N, K, group, dtype_of(scales), (int64_t)hdcm_w4_packed_bytes(N, K), per};
   w.check();
   w.row_sums = fp32({N}, packed);
   sum_rows(w);
