@@ -252,7 +252,9 @@ template <typename T, bool NORM = false> struct Ending {
 // (split there a run of four is split once, and rows past M cost nothing: 3 x 3264 x 768 4.6 us, 5.6 with
 // the fragments split).
 // What a launch takes beyond its weight stream: about 2 us of launch, 1 of x, and the issue of ~40
-// instructions per wave and tile.
+// instructions per wave and tile.  Figures here and at the rules below are recorded calls with the weight in the caches;
+// from HBM, as a step reads it: 16 x 8576 x 2048 6.3 us (5.5), 16 x 50304 x 2048 15.3 (13.5), 33 x 50277 x 768 18.9 (16.5),
+// 128 x 8576 x 2048 14.0 (13.1), 16 x 2048 x 2176 4.4 (4.4).
 // NORM (bf16): out = rstd (x w - mean sum w) takes the row LayerNorm without affine behind the product.  The rows' sums
 // and sums of squares come from MFMAs on the fragments that are there (squares: the diagonal of x x'), so they cost no pass
 // and no barrier: 0.6 us at 16 x 2048 x 2176 (5.1 us, 4.5 without).  Normalising the rows on their way in, with two

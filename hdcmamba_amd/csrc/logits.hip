@@ -158,8 +158,9 @@ template <typename T> struct Eight {
   }
 };
 
-// Bound by its one pass: 64 x 50277 bf16 with history, a shared bias and masks (20 MB) 8.1 us, a launch included,
-// though odd rows start at 2-byte alignment; one sequence 3.4 us recorded, of which 2 are an empty kernel's.
+// Bound by its one pass: 64 x 50277 bf16 with history, a shared bias and masks (20 MB) 8.1 us (from HBM 9.6), of which 2
+// are a launch: 63 % of a copy's rate, since odd rows make the 16-byte accesses straddle their lines; one sequence 3.4 us
+// recorded.
 constexpr int kProcThreads = 256;
 
 template <typename T>
@@ -226,7 +227,7 @@ constexpr int kPickWaves = kPickThreads / kWave;
 // Workgroup (s, b) takes part s of gridDim.x of row b, in whole groups of eight columns.  One pass: the
 // eight values' maximum moves the running one, and only a maximum above the best so far is looked
 // up.  128 x 50304 fp32 with history, biases and noise (90 MB) 20.4 us: the read.  16 x 50304 bf16 with
-// history and masks 6.4 us recorded (7.5 with every input from HBM), two launches and their latency: a row on one
+// history and masks 6.4 us recorded (7.6 with every input from HBM), two launches and their latency: a row on one
 // workgroup of 1024 threads, without a join, takes 9.8 us at one sequence, in parts 4.9.
 template <typename T>
 __global__ __launch_bounds__(kPickThreads) void token_select_kernel(const T* logits, int64_t l_rs, hdcm_logits_controls ctl,
@@ -477,7 +478,10 @@ extern "C" int hdcm_token_history_append(int16_t* table, int64_t table_row_strid
   HDCM_CHECK_ARG(B == 1 || (table_row_stride >= V && tokens_row_stride >= T), HDCM_EINVAL);
   HDCM_CHECK_ARG(V <= kMaxVocab && B <= kMaxRows && T <= kMaxIds, HDCM_EUNSUPPORTED);
   hipStream_t s = (hipStream_t)stream;
-  // up to 16 tokens a row (a step, or a few accepted drafts) touch single entries; more are counted slice by slice
+  // Up to 16 tokens a row (a step, or a few accepted drafts) touch single entries, one round trip each; more are counted
+  // slice by slice, which reads and writes the whole table.  us recorded for 1, 8, 16 and 24 tokens of 50304, single and
+  // by slices: 1 row 1.8, 3.2, 5.1, 6.9 and 3.6; 16 rows 1.8, 3.4, 5.7, 7.8 and 3.9; 64 rows 1.8, 4.0, 6.7, 9.2 and 8.1;
+  // 256 rows 2.1, 4.1, 6.9, 9.3 and 22.
   if (T <= 16)
     HDCM_LAUNCH(token_append_kernel, dim3((unsigned)((B + kWave - 1) / kWave)), dim3(kWave), 0, s, table, table_row_stride,
                 tokens, tokens_row_stride, lengths, T, B, (int)V);
