@@ -16,7 +16,8 @@
 // bf16 x: a group's sum is formed as sum x (16 + c) - (16 + z) sum x, the second term started with:
 // all products are exact, so the roundings are those of the fp32 sums and the last one; the scale
 // multiplies the group's sum, not the weights.  (An infinity in x meets its negative there: that
-// row becomes NaN; 128 values of at most 2^115 times 31 stay finite.)  fp32 x, whose sums have no bits to spare for that: c - z is formed per weight.
+// row becomes NaN; 128 values of at most 2^115 times 31 stay finite.)  fp32 x, whose sums have no bits to spare
+// for that: c - z is formed per weight.
 #include "hdcm_common.h"
 
 using namespace hdcm;

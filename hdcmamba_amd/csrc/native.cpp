@@ -665,8 +665,8 @@ struct Weight4 {
   }
   // with every use: a buffer's storage can be replaced under the tensor (t.data = other, set_, resize_)
   void check() const {
-    TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() && packed.numel() == packed_bytes && scales.is_contiguous() && scales.numel() == per &&
-                    dtype_of(scales) == scale_dtype,
+    TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() && packed.numel() == packed_bytes &&
+                    scales.is_contiguous() && scales.numel() == per && dtype_of(scales) == scale_dtype,
                 "the packed weight's buffers do not hold [", N, ", ", K, "] in groups of ", group);
     same_device(scales, packed, "scales");
     if (!zeros.defined()) return;

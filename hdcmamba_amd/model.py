@@ -477,8 +477,11 @@ class HdcMamba9v3Block(nn.Module):
         storage or its version counter).  A refresh for the same storage writes into the same buffer, so
         a recorded graph that reads both sees the new sums; another storage gets another buffer.  The host
         waits for them, once per change of the weight, so that they are finished for every stream; inside a
-        recording they are formed for it alone."""
+        recording they are formed for it alone, and each time for a weight made under inference mode, which
+        does not count its writes."""
         p = self.out_proj.weight
+        if p.is_inference():
+            return _ops.row_sums(p.to(dtype))
         key = (p.data_ptr(), p._version, dtype, p.device)
         if getattr(self, "_wsum_key", None) != key:
             if p.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -503,7 +506,7 @@ class HdcMamba9v3Block(nn.Module):
         if self.weights_4bit:
             return
         p = self.out_proj.weight
-        if p.data_ptr() == self._wsum_key[0] and p._version != self._wsum_key[1]:
+        if not p.is_inference() and p.data_ptr() == self._wsum_key[0] and p._version != self._wsum_key[1]:
             self._out_weight_sums(self._wsum_key[2])
 
     def _fused_mixer_out(self, x, state, out=None):

@@ -437,3 +437,27 @@ def test_a_recording_replays_while_the_model_is_elsewhere(dev, quantized):
     assert torch.equal(fg(ids), want) and dg.step(ids[:, 0]).isfinite().all()
     lm.to(dev)
     assert torch.equal(fg(ids), want)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_models_made_under_inference_mode(dev, quantized):
+    """Construction, rounding, forward, generation and recordings under inference mode, and the forward outside of it; an
+    in-place write, which such tensors do not count, is seen."""
+    with torch.inference_mode():
+        lm = _lm(256, 64, 4, 32, 2, 300, BF).to(dev)
+        if quantized:
+            hm.quantize_4bit(lm)
+        ids = torch.randint(0, 300, (2, 64), device=dev)
+        want = lm(ids)
+        fg = lm.capture_forward(ids)
+        assert torch.equal(fg(ids), want)
+        assert lm.generate(ids, 4, temperature=0.7, presence=0.5)[0].shape == (2, 4)
+        out = lm.backbone.layers[0].out_proj
+        write = out.scales if quantized else out.weight
+        write.mul_(2)
+        changed = lm(ids)
+        assert not torch.equal(changed, want)
+        write.mul_(0.5)
+        assert torch.equal(lm(ids), want)
+    with torch.no_grad():
+        assert torch.equal(lm(ids), want)
