@@ -13,6 +13,8 @@ from .model import (
     set_fused_out_proj,
     set_fused_step_front,
 )
+from .embeddings import Embedding, embedding, embedding_grad
+from .grads import clip_grad_norm_, clip_grads_, grad_norm
 from .lm import DecodeGraph, ForwardGraph, HdcMambaLM
 from .quant4 import Linear4Bit, Weight4Bit, linear_4bit
 from .sampling import append_tokens, fill_token_history, new_token_history, process_logits, select_tokens
@@ -38,4 +40,10 @@ __all__ = [
     "new_token_history",
     "fill_token_history",
     "append_tokens",
+    "Embedding",
+    "embedding",
+    "embedding_grad",
+    "grad_norm",
+    "clip_grads_",
+    "clip_grad_norm_",
 ]

@@ -29,6 +29,11 @@ class LogitsControls(ctypes.Structure):
                 ("mask_row_stride", c_int64)]
 
 
+class TensorRef(ctypes.Structure):
+    """hdcm_tensor of include/hdcm.h."""
+    _fields_ = [("data", c_void_p), ("count", c_int64), ("dtype", c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/hdcm.h
 _PROTOS = {
     "hdcm_abi_version": (c_int, []),
@@ -139,6 +144,14 @@ _PROTOS = {
                                         c_int64, c_int64, c_int64, c_void_p]),
     "hdcm_token_history_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
                                           c_void_p]),
+    "hdcm_embedding_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float,
+                                   c_int, c_void_p]),
+    "hdcm_embedding_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int]),
+    "hdcm_embedding_grad": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_size_t,
+                                    c_int64, c_int64, c_int64, c_int64, c_float, c_int64, c_int, c_int, c_void_p]),
+    "hdcm_grad_norm_workspace_bytes": (c_size_t, [ctypes.POINTER(TensorRef), c_int64]),
+    "hdcm_grad_norm": (c_int, [ctypes.POINTER(TensorRef), c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "hdcm_grad_scale": (c_int, [ctypes.POINTER(TensorRef), c_int64, c_void_p, c_float, c_void_p]),
 }
 
 _lib = None

@@ -12,6 +12,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
 #include <variant>
@@ -954,6 +955,169 @@ Tensor append_tokens(Tensor table, const Tensor& tokens, const OptTensor& length
   return table;
 }
 
+// ------------------------------------------------------------------------ token rows and their gradient
+// Whether the ranges of memory that two tensors lie in meet
+bool meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (uintptr_t)t.const_data_ptr() + (last + 1) * t.element_size();
+  };
+  return (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
+}
+
+int id_bytes(const Tensor& ids) {
+  TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "token ids must be int64 or int32, got ",
+                   ids.scalar_type());
+  return (int)ids.element_size();
+}
+
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale) {
+  Entry entry;
+  on_gpu(weight);
+  on_gpu(ids);
+  const c10::DeviceGuard guard(weight.device());
+  same_device(ids, weight, "ids");
+  TORCH_CHECK(weight.dim() == 2, "embedding: the weight must be [tokens, width], got ", weight.sizes());
+  const int dt = dtype_of(weight), bytes_of = id_bytes(ids);
+  const Tensor w = rows(weight), i = ids.contiguous();
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(w.size(1));
+  Tensor out = fresh(shape, weight.scalar_type(), weight);
+  check("hdcm_embedding_fwd",
+        hdcm_embedding_fwd(i.const_data_ptr(), bytes_of, w.const_data_ptr(), w.stride(0), out.mutable_data_ptr(), w.size(1), i.numel(),
+                           w.size(0), w.size(1), (float)scale, dt, stream_of(w)));
+  return out;
+}
+
+Tensor embedding_grad(const Tensor& ids, const Tensor& grad, int64_t V, double scale, std::optional<int64_t> padding,
+                      const OptTensor& out_, bool accumulate) {
+  Entry entry;
+  on_gpu(grad);
+  on_gpu(ids);
+  const c10::DeviceGuard guard(grad.device());
+  same_device(ids, grad, "ids");
+  const int dt = dtype_of(grad), bytes_of = id_bytes(ids);
+  TORCH_CHECK(grad.dim() == ids.dim() + 1 && grad.sizes().slice(0, ids.dim()) == ids.sizes(), "embedding_grad: the gradient ",
+              grad.sizes(), " must hold a row for each of the ids ", ids.sizes());
+  TORCH_CHECK(V >= 0, "embedding_grad: ", V, " tokens");
+  TORCH_CHECK(!padding || (*padding >= 0 && *padding < V), "padding_idx ", padding.value_or(0), " is not one of ", V, " tokens");
+  TORCH_CHECK(out_ || !accumulate, "embedding_grad: accumulate needs out");
+  const int64_t D = grad.size(-1), L = ids.dim() ? ids.size(-1) : 1, B = L ? ids.numel() / L : 0;
+  const Tensor i = ids.contiguous();
+  // [B, L, D] in any batch stride, with rows that do not overlap (or one row for all positions)
+  Tensor g = grad.numel() ? grad.reshape({B, L, D}) : grad;
+  if (grad.numel() && ((D > 1 && g.stride(2) != 1) || (L > 1 && g.stride(1) != 0 && g.stride(1) < D))) g = g.contiguous();
+  Tensor out;
+  if (out_) {
+    out = *out_;
+    same_device(out, grad, "out");
+    dtype_of(out);
+    TORCH_CHECK(out.dim() == 2 && out.size(0) == V && out.size(1) == D && plain_rows(out), "embedding_grad: out must be [", V, ", ", D,
+                "] with contiguous rows, got ", out.sizes());
+    TORCH_CHECK(!meet(out, grad) && !meet(out, ids), "embedding_grad: out shares memory with the gradient or the ids");
+  } else {
+    out = fresh({V, D}, grad.scalar_type(), grad);
+  }
+  const size_t n = hdcm_embedding_grad_workspace_bytes(B, L, V, D, dt);
+  const c10::DataPtr ws = n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr();  // on the current stream
+  const bool any = grad.numel() > 0;
+  check("hdcm_embedding_grad",
+        hdcm_embedding_grad(i.const_data_ptr(), bytes_of, any ? g.const_data_ptr() : nullptr, any && B > 1 ? g.stride(0) : 0,
+                            any && L > 1 ? g.stride(1) : D, out.mutable_data_ptr(), V > 1 ? out.stride(0) : D, dtype_of(out), ws.get(), n,
+                            B, L, V, D, (float)scale, padding.value_or(-1), accumulate, dt, stream_of(grad)));
+  if (out_) written(out);
+  return out;
+}
+
+// ------------------------------------------------------------------------ the gradients' norm
+// A list of tensors on one device as the library's, copied to be dense where `copies` lets them.
+struct TensorList {
+  std::vector<hdcm_tensor> refs;
+  std::vector<Tensor> held;
+  TensorList(const std::vector<Tensor>& ts, const char* op, bool copies) {
+    refs.reserve(ts.size());
+    for (const Tensor& t : ts) {
+      TORCH_CHECK(t.layout() == at::kStrided, op, ": a tensor is ", t.layout(), "; the kernels take dense ones");
+      on_gpu(t);
+      same_device(t, ts[0], "a tensor");
+      const int dt = dtype_of(t);
+      const bool dense = t.is_non_overlapping_and_dense();
+      TORCH_CHECK(dense || copies, op, ": a tensor of shape ", t.sizes(), " and strides ", t.strides(),
+                  " has gaps or overlaps in memory and cannot be scaled in place");
+      if (!dense) held.push_back(t.contiguous());
+      refs.push_back({const_cast<void*>((dense ? t : held.back()).const_data_ptr()), t.numel(), dt});
+    }
+  }
+};
+
+void no_gradient(const char* op, const std::vector<Tensor>& ts) {
+  for (const Tensor& t : ts) no_gradient(op, {&t});
+}
+
+// Scaled tensors, and the norm that is read meanwhile, share no memory.
+void apart(const TensorList& l, const Tensor& norm, const char* op) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  spans.reserve(l.refs.size() + 1);
+  const auto add = [&](const void* p, int64_t bytes) {
+    if (bytes) spans.emplace_back((uintptr_t)p, (uintptr_t)p + bytes);
+  };
+  for (const hdcm_tensor& t : l.refs) add(t.data, t.count * (t.dtype == HDCM_F32 ? 4 : 2));
+  add(norm.const_data_ptr(), 4);
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i].first >= spans[i - 1].second, op, ": tensors share memory, with each other or with the norm");
+}
+
+Tensor norm_of(const TensorList& l, const Tensor& like, int kind) {
+  Tensor out = fresh({}, at::kFloat, like);
+  const size_t n = hdcm_grad_norm_workspace_bytes(l.refs.data(), (int64_t)l.refs.size());
+  const c10::DataPtr ws = n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr();  // on the current stream
+  check("hdcm_grad_norm", hdcm_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, out.mutable_data_ptr<float>(), ws.get(), n,
+                                         stream_of(out)));
+  return out;
+}
+void scale_by(const std::vector<Tensor>& ts, const TensorList& l, double max_norm, const Tensor& norm) {
+  check("hdcm_grad_scale", hdcm_grad_scale(l.refs.data(), (int64_t)l.refs.size(), norm.const_data_ptr<float>(), (float)max_norm,
+                                           stream_of(norm)));
+  for (const Tensor& t : ts) written(t);
+}
+
+Tensor grad_norm(const std::vector<Tensor>& ts, int kind) {
+  TORCH_CHECK(!ts.empty(), "grad_norm: no tensors");
+  no_gradient("grad_norm", ts);
+  Entry entry;
+  const c10::DeviceGuard guard(ts[0].device());
+  return norm_of(TensorList(ts, "grad_norm", true), ts[0], kind);
+}
+
+void clip_grads(const std::vector<Tensor>& ts, double max_norm, const Tensor& norm_) {
+  if (ts.empty()) return;
+  no_gradient("clip_grads_", ts);
+  Entry entry;
+  const c10::DeviceGuard guard(ts[0].device());
+  same_device(norm_, ts[0], "total_norm");
+  TORCH_CHECK(norm_.numel() == 1 && norm_.is_floating_point(), "total_norm must be one floating-point number, got ", norm_.scalar_type(),
+              " ", norm_.sizes());
+  const Tensor norm = as_type(norm_, at::kFloat);
+  const TensorList l(ts, "clip_grads_", false);
+  apart(l, norm, "clip_grads_");
+  scale_by(ts, l, max_norm, norm);
+}
+
+Tensor clip_grad_norm(const std::vector<Tensor>& ts, double max_norm, int kind) {
+  TORCH_CHECK(!ts.empty(), "clip_grad_norm_: no tensors");
+  no_gradient("clip_grad_norm_", ts);
+  Entry entry;
+  const c10::DeviceGuard guard(ts[0].device());
+  const TensorList l(ts, "clip_grad_norm_", false);
+  const Tensor norm = norm_of(l, ts[0], kind);
+  apart(l, norm, "clip_grad_norm_");
+  scale_by(ts, l, max_norm, norm);
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -983,4 +1147,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("select_tokens", &select_tokens);
   m.def("fill_token_history", &fill_token_history);
   m.def("append_tokens", &append_tokens);
+  m.def("embedding", &embedding);
+  m.def("embedding_grad", &embedding_grad);
+  m.def("grad_norm", &grad_norm);
+  m.def("clip_grads", &clip_grads);
+  m.def("clip_grad_norm", &clip_grad_norm);
+  m.attr("NORM_2") = (int)HDCM_NORM_2;
+  m.attr("NORM_MAX") = (int)HDCM_NORM_MAX;
 }

@@ -1,0 +1,109 @@
+"""Token rows of an embedding and the weight's gradient on the HIP kernels (csrc/embedding.hip): the first kernel of
+an HdcMambaLM's forward and the last of its backward.  The reference's model uses nn.Embedding
+(train_fineweb.py:49,87).
+
+An id outside 0..V-1 (a padding id -1, an ignored position) gives a row of zeros and no gradient.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd import forward_ad
+
+from . import _ops
+from .quant4 import carries_tangent
+
+__all__ = ["embedding", "embedding_grad", "Embedding"]
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """scale * weight[ids], rounded once: ids of any shape (int64 or int32), weight [V, D] (float32 or bfloat16) ->
+    [*ids.shape, D] of weight's type, differentiable in weight (and again in the gradient).  The rows of ``padding_idx``
+    (counted from the end where negative) are looked up as others are but give no gradient."""
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, weight.shape[0])
+    if (torch.is_grad_enabled() and weight.requires_grad) or carries_tangent(weight):
+        return EmbeddingFunction.apply(ids, weight, float(scale), padding_idx)
+    return _ops.native().embedding(ids, weight, scale)
+
+
+def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, out=None, accumulate=False):
+    """The gradient of ``embedding`` for its weight: row v is scale * the sum of grad's rows [*ids.shape, D] at the ids v,
+    in fp32 in an order that the ids alone fix, rounded once to grad's type -> [num_embeddings, D].
+
+    ``out`` ([num_embeddings, D], float32 or bfloat16, contiguous rows) is written instead; with ``accumulate`` the sums
+    are added to it, and rows without an id are not touched."""
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, num_embeddings)
+    needed = torch.is_grad_enabled() and (grad.requires_grad or (out is not None and out.requires_grad))
+    if needed or carries_tangent(grad):
+        if out is not None:
+            raise RuntimeError("embedding_grad with out has no gradient: call it under torch.no_grad() or on detached tensors")
+        return EmbeddingGradFunction.apply(ids, grad, int(num_embeddings), float(scale), padding_idx)
+    return _ops.native().embedding_grad(ids, grad, num_embeddings, scale, padding_idx, out, accumulate)
+
+
+def _padding(index, rows):
+    if not -rows <= index < rows:
+        raise ValueError(f"padding_idx {index} is not one of {rows} tokens")
+    return index % rows
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """``apply(ids, weight, scale, padding_idx)``: the lookup, whose backward is EmbeddingGradFunction."""
+
+    @staticmethod
+    def forward(ids, weight, scale, padding_idx):
+        return _ops.native().embedding(ids, weight, scale)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ids, weight, ctx.scale, ctx.padding_idx = inputs
+        ctx.rows = weight.shape[0]
+        ctx.save_for_backward(ids)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, EmbeddingGradFunction.apply(*ctx.saved_tensors, grad, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+
+
+class EmbeddingGradFunction(torch.autograd.Function):
+    """``apply(ids, grad, rows, scale, padding_idx)``: the weight's gradient, itself linear in grad."""
+
+    @staticmethod
+    def forward(ids, grad, rows, scale, padding_idx):
+        return _ops.native().embedding_grad(ids, grad, rows, scale, padding_idx, None, False)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ids, _, _, ctx.scale, ctx.padding_idx = inputs
+        ctx.save_for_backward(ids)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        if ctx.padding_idx is not None:
+            ids = ids.masked_fill(ids == ctx.padding_idx, -1)
+        return None, EmbeddingFunction.apply(ids, grad, ctx.scale, None), None, None, None
+
+
+class Embedding(nn.Embedding):
+    """nn.Embedding on these kernels, its rows times ``scale``: the same constructor, parameters and initial values.
+
+    What the kernels do not take goes through nn.Embedding's own forward: weights on the CPU or of other types, max_norm,
+    sparse and scale_grad_by_freq, and forward-mode differentiation."""
+
+    def __init__(self, *args, scale=1.0, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.scale = float(scale)
+
+    def forward(self, ids):
+        w = self.weight
+        if (not w.is_cuda or w.dtype not in _ops._DTYPES or self.max_norm is not None or self.sparse
+                or self.scale_grad_by_freq or forward_ad._current_level >= 0):
+            y = super().forward(ids)
+            return y if self.scale == 1.0 else y * self.scale
+        return embedding(ids, w, self.scale, self.padding_idx)
+
+    def extra_repr(self):
+        return super().extra_repr() + (f", scale={self.scale}" if self.scale != 1.0 else "")

@@ -15,6 +15,7 @@ import torch
 import torch.nn as nn
 
 from . import _ops
+from .embeddings import Embedding
 from .model import BlockState, HdcMamba9v3Model, layer_norm
 from .quant4 import Linear4Bit
 from .sampling import append_tokens, fill_token_history, new_token_history, select_tokens
@@ -34,7 +35,7 @@ class HdcMambaLM(nn.Module):
                  num_slots=32):
         super().__init__()
         self.d_model = d_model
-        self.embedding = nn.Embedding(vocab_size, d_model)
+        self.embedding = Embedding(vocab_size, d_model)
         self.backbone = HdcMamba9v3Model(d_model=d_model, n_layers=n_layers, d_state=d_state,
                                          num_slots=num_slots, num_heads=num_heads, chunk_size=chunk_size)
         self.norm_f = nn.LayerNorm(d_model)

@@ -628,6 +628,45 @@ int hdcm_token_history_append(int16_t* table, int64_t table_row_stride, const in
                               int64_t tokens_row_stride, const int64_t* lengths, int64_t T, int64_t B, int64_t V,
                               void* stream);
 
+/*
+ * Token rows of an embedding (csrc/embedding.hip; nn.Embedding and its autograd, train_fineweb.py:49,87).
+ * ids: `rows` (fwd) or B * L (grad) token ids of id_bytes 4 or 8, contiguous.  V <= 2^30 rows of D <= 2^24 columns, at
+ * most 2^30 ids.  Rows need only their type's alignment.
+ * hdcm_embedding_fwd: out[t] = scale * w[ids[t]], rounded once; zeros where ids[t] is not in 0..V-1.
+ * hdcm_embedding_grad: dw[v] = scale * sum of dy[b, l] over ids[b, l] = v, for all V rows (with accumulate: added to
+ * dw, whose other rows are not touched).  dy [B, L, D] of `dtype` with any batch stride and a row stride of at
+ * least D, or 0 (one row for all positions); dw of dw_dtype.  Ids outside 0..V-1 and padding_idx (-1: none)
+ * are passed over.  fp32 sums in an order that the ids alone fix, one rounding (so the same call gives the
+ * same bits).  ws: hdcm_embedding_grad_workspace_bytes(B, L, V, D, dtype) bytes, 16-byte aligned, not kept between
+ * calls.
+ */
+int hdcm_embedding_fwd(const void* ids, int id_bytes, const void* w, int64_t w_row_stride, void* out,
+                       int64_t out_row_stride, int64_t rows, int64_t V, int64_t D, float scale, int dtype, void* stream);
+size_t hdcm_embedding_grad_workspace_bytes(int64_t B, int64_t L, int64_t V, int64_t D, int dtype);
+int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride,
+                        void* dw, int64_t dw_row_stride, int dw_dtype, void* ws, size_t ws_bytes, int64_t B, int64_t L,
+                        int64_t V, int64_t D, float scale, int64_t padding_idx, int accumulate, int dtype, void* stream);
+
+/*
+ * The norm of many tensors together, and their scaling by it (csrc/grad_norm.hip; no counterpart in the reference,
+ * which trains without clipping).  A tensor is `count` elements, one behind the other, at its type's alignment;
+ * the array of n of them lies on the host and is read before the call returns.
+ * hdcm_grad_norm: *out (device) = sqrt(sum x^2) (HDCM_NORM_2; 64-bit sums, so that no square overflows) or max |x|
+ * (HDCM_NORM_MAX; NaN where there is one), 0 for no elements.  ws: hdcm_grad_norm_workspace_bytes(tensors, n) bytes,
+ * 8-byte aligned, not kept between calls.
+ * hdcm_grad_scale: x *= min(1, max_norm / (*norm + 1e-6)), the product rounded to the tensor's type; tensors are not
+ * touched where the factor is 1.  max_norm >= 0.  Tensors must not overlap.
+ */
+typedef struct {
+  void* data;
+  int64_t count;
+  int dtype;
+} hdcm_tensor;
+enum { HDCM_NORM_2 = 0, HDCM_NORM_MAX = 1 };
+size_t hdcm_grad_norm_workspace_bytes(const hdcm_tensor* tensors, int64_t n);
+int hdcm_grad_norm(const hdcm_tensor* tensors, int64_t n, int norm, float* out, void* ws, size_t ws_bytes, void* stream);
+int hdcm_grad_scale(const hdcm_tensor* tensors, int64_t n, const float* norm, float max_norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
