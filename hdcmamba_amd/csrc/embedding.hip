@@ -2,9 +2,10 @@
 // train_fineweb.py:49,87):
 //   lookup:    y[t] = scale w[id_t], zeros where id_t is no row of the weight
 //   gradient:  dw[v] = scale sum_{t: id_t = v} dy[t], fp32 sums in an order that the ids alone fix
-// The gradient sorts the positions by token (stable radix passes), cuts the sorted list into units of equal
-// length, so that a frequent token costs no more than many rare ones, sums each unit's runs of equal tokens
-// in registers and joins the runs that units share in a second launch.  No floating-point atomics.
+// The gradient of many positions sorts them by token (stable radix passes), cuts the sorted list into units of equal
+// length, so that a frequent token costs no more than many rare ones, sums each unit's runs of equal tokens in
+// registers, joins the runs that units share in LDS, and those that workgroups share in a last launch.  Few positions
+// need no sorting: every workgroup looks for its own tokens among all ids.  No floating-point atomics.
 #include "hdcm_common.h"
 
 using namespace hdcm;
@@ -115,117 +116,7 @@ void launch_lookup(const void* ids, const void* w, int64_t w_rs, void* out, int6
   else go(embedding_kernel<T, I, 4, true>, 4);
 }
 
-// ------------------------------------------------------------------ positions in the order of their tokens
-// Stable radix passes over digits of up to kDigitBits bits of the token, least significant first: a pass
-// counts the digits of each workgroup's stretch of the list, and scatters every stretch behind what the
-// counts put before it.  Ids outside the weight and the padding index become the key V, behind all tokens.
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave;
-constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
-constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
-constexpr int kMaxGroups = 128;  // workgroups of a pass, so that each may add all counts up by itself
-
-// A pass' input: the caller's ids (first pass) or the keys and positions of the pass before.
-struct SortIn {
-  const void* ids;  // null: keys, pos
-  const int *keys, *pos;
-  int id_bytes, V, padding;
-  __device__ __forceinline__ int key(int64_t i) const {
-    if (!ids) return keys[i];
-    const int64_t id = id_bytes == 8 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
-    return (uint64_t)id < (uint64_t)V && id != padding ? (int)id : V;
-  }
-  __device__ __forceinline__ int position(int64_t i) const { return ids ? (int)i : pos[i]; }
-};
-
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, int n, int stretch, int shift, int bits, int* counts) {
-  __shared__ int count[kBins];
-  const int tid = threadIdx.x, bins = 1 << bits;
-  if (tid < bins) count[tid] = 0;
-  __syncthreads();
-  const int64_t b = (int64_t)blockIdx.x * stretch, e = min(b + stretch, (int64_t)n);
-  for (int64_t i = b + tid; i < e; i += kSortThreads) atomicAdd(&count[(in.key(i) >> shift) & (bins - 1)], 1);
-  __syncthreads();
-  if (tid < bins) counts[blockIdx.x * bins + tid] = count[tid];
-}
-
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, int n, int stretch, int shift, int bits,
-                                                                    const int* counts, int* keys, int* pos) {
-  __shared__ int next[kBins];              // where the next key of a digit goes
-  __shared__ int sums[kSortWaves];
-  __shared__ int mine[kSortWaves][kBins];  // a wave's keys of a digit, then where its first goes
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, bins = 1 << bits;
-  // all keys of lower digits, and this digit's in the stretches before
-  int before = 0, total = 0;
-  if (tid < bins)
-    for (int g = 0; g < (int)gridDim.x; ++g) {
-      const int c = counts[g * bins + tid];
-      before += g < (int)blockIdx.x ? c : 0;
-      total += c;
-    }
-  int scan = total;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int up = __shfl_up(scan, o, kWave);
-    scan += lane >= o ? up : 0;
-  }
-  if (lane == kWave - 1) sums[w] = scan;
-  __syncthreads();
-  int lower = scan - total;
-  for (int i = 0; i < w; ++i) lower += sums[i];
-  next[tid] = lower + before;  // kBins == kSortThreads
-  const int64_t b = (int64_t)blockIdx.x * stretch, e = min(b + stretch, (int64_t)n);
-  for (int64_t t = b; t < e; t += kTile) {
-#pragma unroll
-    for (int i = 0; i < kSortWaves; ++i) mine[i][tid] = 0;
-    __syncthreads();
-    int key[kPer], at[kPer], digit[kPer], rank[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int64_t i = t + w * (kPer * kWave) + j * kWave + lane;
-      key[j] = i < e ? in.key(i) : 0;
-      at[j] = i < e ? in.position(i) : -1;
-      digit[j] = (key[j] >> shift) & (bins - 1);
-    }
-    // the wave's lanes with the same digit, found a bit at a time, rank themselves behind the wave's earlier ones
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      uint64_t same = __ballot(at[j] >= 0);
-      for (int k = 0; k < bits; ++k) {
-        const bool set = (digit[j] >> k) & 1;
-        const uint64_t with = __ballot(set);
-        same &= set ? with : ~with;
-      }
-      const int below = __popcll(same & ((1ull << lane) - 1));
-      const int had = mine[w][digit[j]];
-      rank[j] = had + below;
-      __builtin_amdgcn_wave_barrier();  // all lanes have read before one of them writes
-      if (at[j] >= 0 && below == 0) mine[w][digit[j]] = had + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
-    int run = next[tid];
-#pragma unroll
-    for (int i = 0; i < kSortWaves; ++i) {
-      const int c = mine[i][tid];
-      mine[i][tid] = run;
-      run += c;
-    }
-    next[tid] = run;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int to = mine[w][digit[j]] + rank[j];
-      if (at[j] >= 0 && (unsigned)to < (unsigned)n) keys[to] = key[j], pos[to] = at[j];  // (inside, whatever the ids became since)
-    }
-    __syncthreads();
-  }
-}
-
-// ------------------------------------------------------------------ sums of the sorted rows
-constexpr int kRowsAhead = 16;  // rows of dy in flight
-constexpr int kUnit = 32;       // sorted positions of a wave, a multiple of kRowsAhead
-constexpr int kSumThreads = 256, kSumWaves = kSumThreads / kWave;
-
+// ------------------------------------------------------------------ the gradient's rows
 // dy [.., L, D]: position p lies at (p / L) batch stride + (p % L) row stride.
 struct GradRows {
   const void* p;
@@ -233,16 +124,21 @@ struct GradRows {
   uint32_t L;
   __device__ __forceinline__ int64_t offset(uint32_t at) const { return (at / L) * batch + (at % L) * row; }
 };
-struct Sorted {
-  const int *keys, *pos;
-  int n, V;
+
+// The caller's ids as keys: what is no token of the weight, and the padding index, becomes V.
+struct Ids {
+  const void* p;
+  int bytes, V, padding;
+  __device__ __forceinline__ int key(int64_t i) const {
+    const int64_t id = bytes == 8 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+    return (uint64_t)id < (uint64_t)V && id != padding ? (int)id : V;
+  }
 };
 
-// Writes (or adds) a finished sum: v[0..E) at columns inside the row.
-template <typename TG, typename TO>
-__device__ __forceinline__ void put_row(TO* p, const float* sum, float scale, int n, bool add) {
+// Writes (or adds) a finished sum: E columns from p on, n of them inside the row.
+template <int E, typename TO> __device__ __forceinline__ void put_row(TO* p, const float* sum, float scale, int n, bool add) {
 #pragma unroll
-  for (int e0 = 0; e0 < kE<TG>; e0 += 4) {
+  for (int e0 = 0; e0 < E; e0 += 4) {
     if (e0 >= n) break;
     float v[4];
 #pragma unroll
@@ -273,96 +169,395 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// A wave takes one unit and 64 pieces of its rows.  A run of equal tokens that lies inside the unit is written
-// to dw at once; what the unit holds of a run that began before it goes to its partial row 0, of one that
-// begins in it and goes on behind it to its partial row 1.
+constexpr int kAhead = 16;                                      // rows of dy that a wave has in flight
+constexpr int kSumThreads = 512, kSumWaves = kSumThreads / kWave;  // of the kernels that add rows up
+
+// A wave's lanes hold the offsets of `count` (1..kAhead) rows: loads them all.
+template <typename T>
+__device__ __forceinline__ void load_rows(u32x4_t (&x)[kAhead], const T* rows, int64_t offs, int count, int n) {
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) x[j] = load_piece<T>(rows + lane_value(offs, min(j, count - 1)), n);
+}
+template <typename T> __device__ __forceinline__ void add_piece(float* sum, u32x4_t x) {
+  float v[kE<T>];
+  values<T>(x, v);
+#pragma unroll
+  for (int e = 0; e < kE<T>; ++e) sum[e] += v[e];
+}
+
+// ------------------------------------------------------------------ few positions: one launch
+// A workgroup takes R tokens and 64 pieces of their rows, finds its tokens among all ids (a bit for each position
+// and token in LDS), and writes all R rows, most of them zeros.  A token of up to kShort positions is a wave's; the
+// waves share the positions of a more frequent one.
+constexpr int kFewPositions = 32 * kWave;  // a word of bits for each lane
+constexpr int kMostTokens = 32, kShort = 2 * kAhead;
+
 template <typename TG, typename TO>
-__global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(Sorted s, GradRows g, TO* out, int64_t out_rs, float* part, int D,
-                                                                    int slices, float scale, bool add) {
+__global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int n, GradRows g, TO* out, int64_t out_rs, int D,
+                                                                    int slices, int R, float scale, bool add) {
   constexpr int E = kE<TG>;
-  const int lane = threadIdx.x % kWave;
-  const int64_t wave = (int64_t)blockIdx.x * kSumWaves + threadIdx.x / kWave;
-  const int64_t begin = wave / slices * kUnit;
-  if (begin >= s.n) return;
-  const int slice = (int)(wave % slices), col = (slice * kWave + lane) * E;
-  const int end = (int)min(begin + kUnit, (int64_t)s.n);
+  __shared__ uint32_t bits[kMostTokens][kWave];
+  __shared__ uint32_t frequent;
+  __shared__ uint16_t list[kFewPositions];  // a wave's part in turn, or a frequent token's positions
+  __shared__ __attribute__((aligned(16))) float part[kSumWaves][kWave * E];
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  const int v0 = blockIdx.x / slices * R, slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
   const TG* rows = static_cast<const TG*>(g.p) + col;
-  float* mine = part + (begin / kUnit * 2 * slices * kWave + slice * kWave + lane) * E;
-  const int64_t one = (int64_t)slices * kWave * E;
-  float sum[E];
+  int key[kFewPositions / kSumThreads];
 #pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = 0.f;
-  bool began = begin == 0 || s.keys[begin - 1] != s.keys[begin], open = false;
-  for (int b = (int)begin; b < end; b += kRowsAhead) {
-    const int at = min(b + lane, s.n - 1), count = min(kRowsAhead, end - b);
-    const int keys = b + lane < s.n ? s.keys[at] : -1;  // no token behind the last
-    const int64_t offs = g.offset((uint32_t)s.pos[at]);
-    u32x4_t x[kRowsAhead];
+  for (int j = 0; j < kFewPositions / kSumThreads; ++j) {
+    const int i = j * kSumThreads + tid;
+    key[j] = i < n ? ids.key(i) : ids.V;
+  }
+  for (int i = tid; i < R * kWave; i += kSumThreads) bits[i / kWave][i % kWave] = 0;
+  if (tid == 0) frequent = 0;
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kRowsAhead; ++j) x[j] = load_piece<TG>(rows + lane_value(offs, min(j, count - 1)), D - col);
+  for (int j = 0; j < kFewPositions / kSumThreads; ++j) {
+    const int i = j * kSumThreads + tid, r = key[j] - v0;
+    if (key[j] < ids.V && (unsigned)r < (unsigned)R) atomicOr(&bits[r][i / 32], 1u << (i % 32));
+  }
+  __syncthreads();
+  // the positions of token r, in order, to `to`; their number
+  const auto positions = [&](int r, uint16_t* to, int most) {
+    uint32_t word = bits[r][lane];
+    int before = __popc(word);
 #pragma unroll
-    for (int j = 0; j < kRowsAhead; ++j) {
-      const int key = __builtin_amdgcn_readlane(keys, j);
-      if (j < count && key < s.V) {
-        float v[E];
-        values<TG>(x[j], v);
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int up = __shfl_up(before, o, kWave);
+      before += lane >= o ? up : 0;
+    }
+    const int count = __builtin_amdgcn_readlane(before, kWave - 1);
+    before -= __popc(word);
+    if (count <= most)
+      for (; word; word &= word - 1) to[before++] = (uint16_t)(32 * lane + __builtin_ctz(word));
+    __builtin_amdgcn_wave_barrier();
+    return count;
+  };
+  const auto add_up = [&](float* sum, const uint16_t* at, int count) {
+    for (int b = 0; b < count; b += kAhead) {
+      u32x4_t x[kAhead];
+      load_rows<TG>(x, rows, g.offset(at[min(b + lane, count - 1)]), min(kAhead, count - b), D - col);
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += v[e];
-        open = __builtin_amdgcn_readlane(keys, j + 1) == key;
-        if (!open) {
-          if (began) {
-            if (col < D) put_row<TG, TO>(out + key * out_rs + col, sum, scale, D - col, add);
-          } else {
+      for (int j = 0; j < kAhead; ++j)
+        if (b + j < count) add_piece<TG>(sum, x[j]);
+    }
+  };
+  uint16_t* mine = list + w * kShort;
+  for (int r = w; r < R && v0 + r < ids.V; r += kSumWaves) {
+    float sum[E] = {};
+    const int count = positions(r, mine, kShort);
+    if (count > kShort) {
+      if (lane == 0) atomicOr(&frequent, 1u << r);
+      continue;
+    }
+    add_up(sum, mine, count);
+    if (col < D && (count || !add)) put_row<E, TO>(out + (v0 + r) * out_rs + col, sum, scale, D - col, add);
+  }
+  __syncthreads();
+  for (uint32_t rest = frequent; rest; rest &= rest - 1) {
+    const int r = __builtin_ctz(rest), count = positions(r, list, w == 0 ? kFewPositions : 0);
+    __syncthreads();
+    const int per = (count + kSumWaves - 1) / kSumWaves, b = min(w * per, count);
+    float sum[E] = {};
+    add_up(sum, list + b, min(per, count - b));
 #pragma unroll
-            for (int e = 0; e < E; ++e) mine[e] = sum[e];
-          }
+    for (int e = 0; e < E; ++e) part[w][lane * E + e] = sum[e];
+    __syncthreads();
+    if (w == 0 && col < D) {
+      for (int i = 1; i < kSumWaves; ++i)
 #pragma unroll
-          for (int e = 0; e < E; ++e) sum[e] = 0.f;
-          began = true;
-        }
-      }
+        for (int e = 0; e < E; ++e) sum[e] += part[i][lane * E + e];
+      put_row<E, TO>(out + (v0 + r) * out_rs + col, sum, scale, D - col, add);
     }
   }
-  if (open) {
+}
+
+// ------------------------------------------------------------------ positions in the order of their tokens
+// Stable radix passes over digits of up to kDigitBits bits of the token, least significant first: a pass
+// counts the digits of each workgroup's stretch of the list, and scatters every stretch behind what the
+// counts put before it.
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave;
+constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+constexpr int kMaxGroups = 128;  // workgroups of a pass, so that each may add all counts up by itself
+constexpr int kCountsAhead = 16;
+
+// A pass' input: the caller's ids (first pass) or the keys and positions of the pass before.
+struct SortIn {
+  Ids ids;
+  const int *keys, *pos;  // null: ids
+  __device__ __forceinline__ int key(int64_t i) const { return keys ? keys[i] : ids.key(i); }
+  __device__ __forceinline__ int position(int64_t i) const { return keys ? pos[i] : (int)i; }
+};
+struct Pass {
+  int n, stretch, groups, shift, bits;
+};
+
+// Zeros for the weight's gradient, written by the workgroups of a sorting launch that have nothing to sort: these
+// launches are short and leave most CUs idle.  Bytes [begin, end), kFillBytes a workgroup.
+constexpr int kFillAhead = 8, kFillBytes = kFillAhead * kSortThreads * 16;
+struct Fill {
+  char* p;
+  int64_t begin, end;
+};
+__device__ __forceinline__ void fill_part(const Fill& f, int64_t part) {
+  typedef u32x4_t loose_t __attribute__((aligned(2)));
+  const int64_t b = f.begin + part * kFillBytes;
 #pragma unroll
-    for (int e = 0; e < E; ++e) mine[(began ? one : 0) + e] = sum[e];
+  for (int u = 0; u < kFillAhead; ++u) {
+    const int64_t i = b + (u * kSortThreads + (int)threadIdx.x) * 16;
+    if (i + 16 <= f.end) *reinterpret_cast<loose_t*>(f.p + i) = u32x4_t{0, 0, 0, 0};
+    else
+      for (int64_t k = i; k < f.end; k += 2) *reinterpret_cast<uint16_t*>(f.p + k) = 0;
   }
 }
 
-// The runs that begin in a unit and end in a later one: the partial rows in the units' order.
-template <typename TG, typename TO>
-__global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, TO* out, int64_t out_rs, const float* part, int D,
-                                                                     int slices, float scale, bool add) {
-  constexpr int E = kE<TG>;
-  const int lane = threadIdx.x % kWave;
-  const int64_t wave = (int64_t)blockIdx.x * kSumWaves + threadIdx.x / kWave;
-  const int64_t unit = wave / slices, begin = unit * kUnit, end = begin + kUnit;
-  if (end >= s.n) return;
-  const int key = s.keys[end];
-  if (key >= s.V || s.keys[end - 1] != key) return;
-  if (begin > 0 && s.keys[begin - 1] == key) return;  // it began before
-  const int slice = (int)(wave % slices), col = (slice * kWave + lane) * E;
-  const int64_t one = (int64_t)slices * kWave * E;
-  const float* p = part + unit * 2 * one + (slice * kWave + lane) * E;
-  float sum[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) sum[e] = p[one + e];
-  for (int64_t u = unit + 1;; ++u) {
-    const float* q = p + (u - unit) * 2 * one;
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] += q[e];
-    if ((u + 1) * kUnit >= s.n || s.keys[(u + 1) * kUnit] != key) break;
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pass p, int* counts, Fill fill) {
+  __shared__ int count[kBins];
+  if ((int)blockIdx.x >= p.groups) {
+    fill_part(fill, (int)blockIdx.x - p.groups);
+    return;
   }
-  if (col < D) put_row<TG, TO>(out + key * out_rs + col, sum, scale, D - col, add);
+  const int tid = threadIdx.x, bins = 1 << p.bits;
+  count[tid] = 0;  // kBins == kSortThreads
+  __syncthreads();
+  const int64_t b = (int64_t)blockIdx.x * p.stretch, e = min(b + p.stretch, (int64_t)p.n);
+  for (int64_t t = b; t < e; t += kTile) {
+    int key[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t i = t + j * kSortThreads + tid;
+      key[j] = i < e ? in.key(i) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (t + j * kSortThreads + tid < e) atomicAdd(&count[(key[j] >> p.shift) & (bins - 1)], 1);
+  }
+  __syncthreads();
+  if (tid < bins) counts[blockIdx.x * bins + tid] = count[tid];
 }
 
-// Zeros in all V rows of D columns.
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, Pass p, const int* counts, int* keys, int* pos,
+                                                                    Fill fill) {
+  __shared__ int next[kBins];              // where the next key of a digit goes
+  __shared__ int sums[kSortWaves];
+  __shared__ int mine[kSortWaves][kBins];  // a wave's keys of a digit, then where its first goes
+  if ((int)blockIdx.x >= p.groups) {
+    fill_part(fill, (int)blockIdx.x - p.groups);
+    return;
+  }
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, bins = 1 << p.bits;
+  const int64_t b = (int64_t)blockIdx.x * p.stretch, e = min(b + p.stretch, (int64_t)p.n);
+  // all keys of lower digits, and this digit's in the stretches before
+  int before = 0, total = 0;
+  if (tid < bins)
+    for (int g0 = 0; g0 < p.groups; g0 += kCountsAhead) {
+      int c[kCountsAhead];
+#pragma unroll
+      for (int g = 0; g < kCountsAhead; ++g) c[g] = counts[min(g0 + g, p.groups - 1) * bins + tid];
+#pragma unroll
+      for (int g = 0; g < kCountsAhead; ++g) {
+        before += g0 + g < (int)blockIdx.x ? c[g] : 0;
+        total += g0 + g < p.groups ? c[g] : 0;
+      }
+    }
+  int scan = total;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int up = __shfl_up(scan, o, kWave);
+    scan += lane >= o ? up : 0;
+  }
+  if (lane == kWave - 1) sums[w] = scan;
+  __syncthreads();
+  int lower = scan - total;
+  for (int i = 0; i < w; ++i) lower += sums[i];
+  next[tid] = lower + before;
+  for (int64_t t = b; t < e; t += kTile) {
+#pragma unroll
+    for (int i = 0; i < kSortWaves; ++i) mine[i][tid] = 0;
+    __syncthreads();
+    int key[kPer], at[kPer], digit[kPer], rank[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t i = t + w * (kPer * kWave) + j * kWave + lane;
+      key[j] = i < e ? in.key(i) : 0;
+      at[j] = i < e ? in.position(i) : -1;
+      digit[j] = (key[j] >> p.shift) & (bins - 1);
+    }
+    // the wave's lanes with the same digit, found a bit at a time, rank themselves behind the wave's earlier ones
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      uint64_t same = __ballot(at[j] >= 0);
+      for (int k = 0; k < p.bits; ++k) {
+        const bool set = (digit[j] >> k) & 1;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
+      }
+      const int below = __popcll(same & ((1ull << lane) - 1));
+      const int had = mine[w][digit[j]];
+      rank[j] = had + below;
+      __builtin_amdgcn_wave_barrier();  // all lanes have read before one of them writes
+      if (at[j] >= 0 && below == 0) mine[w][digit[j]] = had + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    int run = next[tid];
+#pragma unroll
+    for (int i = 0; i < kSortWaves; ++i) {
+      const int c = mine[i][tid];
+      mine[i][tid] = run;
+      run += c;
+    }
+    next[tid] = run;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int to = mine[w][digit[j]] + rank[j];
+      if (at[j] >= 0 && (unsigned)to < (unsigned)p.n) keys[to] = key[j], pos[to] = at[j];  // (inside, whatever the ids became since)
+    }
+    __syncthreads();
+  }
+}
+
+// Zeros in all rows of a gradient whose rows are not adjacent.
 template <typename T>
 __global__ __launch_bounds__(256) void zero_rows_kernel(T* out, int64_t rs, int64_t rows, int D) {
   const uint32_t P = (D + kE<T> - 1) / kE<T>;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / P;
   const int col = kE<T> * (int)(i - row * P);
   if (row < rows) store_piece<T>(out + row * rs + col, u32x4_t{0, 0, 0, 0}, D - col);
+}
+
+// ------------------------------------------------------------------ sums of the sorted rows
+struct Sorted {
+  const int *keys, *pos;
+  int n, V, unit;  // unit: sorted positions of a wave, a multiple of kAhead
+};
+
+// A wave takes one unit, a workgroup kSumWaves units in a row, of 64 pieces of their rows.  A run of equal tokens
+// inside a unit is written to dw at once.  What a unit holds of a run that began before it (its head) or goes on behind it
+// (its tail) meets in LDS: the wave in which a run begins adds the heads behind it.  A run that goes on behind the
+// workgroup leaves the workgroup's part of it as partial row 1 where it began here, else as partial row 0.
+template <typename TG, typename TO>
+__global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(Sorted s, GradRows g, TO* out, int64_t out_rs, float* partial,
+                                                                    int D, int slices, float scale, bool add) {
+  constexpr int E = kE<TG>;
+  __shared__ __attribute__((aligned(16))) float head[kSumWaves][kWave * E];
+  __shared__ int passes[kSumWaves];  // whether a wave's unit is one run that began before it and goes on behind it
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
+  const int64_t group = blockIdx.x / slices, begin = (group * kSumWaves + w) * s.unit;
+  const int end = (int)min(begin + s.unit, (int64_t)s.n);
+  const TG* rows = static_cast<const TG*>(g.p) + col;
+  float sum[E] = {};
+  // before: the run at hand began before the unit; open: it goes on behind what was added
+  bool before = begin > 0 && begin < s.n && s.keys[begin - 1] == s.keys[begin], open = false;
+  const bool has_head = before;
+  int key = 0;
+  for (int64_t b = begin; b < end; b += kAhead) {
+    const int at = (int)min(b + lane, (int64_t)s.n - 1), count = (int)min((int64_t)kAhead, end - b);
+    const int keys = b + lane < s.n ? s.keys[at] : -1;  // no token behind the last
+    u32x4_t x[kAhead];
+    load_rows<TG>(x, rows, g.offset((uint32_t)s.pos[at]), count, D - col);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      key = __builtin_amdgcn_readlane(keys, j);
+      if (j < count && key < s.V) {
+        add_piece<TG>(sum, x[j]);
+        open = __builtin_amdgcn_readlane(keys, j + 1) == key;
+        if (!open) {
+          if (before) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) head[w][lane * E + e] = sum[e];
+          } else if (col < D) {
+            put_row<E, TO>(out + key * out_rs + col, sum, scale, D - col, add);
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum[e] = 0.f;
+          before = false;
+        }
+      }
+    }
+  }
+  if (open && before) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) head[w][lane * E + e] = sum[e];
+  }
+  if (lane == 0) passes[w] = open && before;
+  __syncthreads();
+  float* mine = partial + (group * 2 * slices * kWave + slice * kWave + lane) * E;
+  const int64_t one = (int64_t)slices * kWave * E;
+  // a run that came from before the workgroup
+  if (w == 0 && has_head && s.keys[begin] < s.V) {
+    float t[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) t[e] = head[0][lane * E + e];
+    for (int i = 0; i + 1 < kSumWaves && passes[i]; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) t[e] += head[i + 1][lane * E + e];
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine[e] = t[e];
+  }
+  if (open && !before) {
+    const int last = s.keys[end - 1];
+    int i = w;
+    do {
+      if (++i == kSumWaves) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] += head[i][lane * E + e];
+    } while (passes[i]);
+    if (i < kSumWaves) {
+      if (col < D) put_row<E, TO>(out + last * out_rs + col, sum, scale, D - col, add);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine[one + e] = sum[e];
+    }
+  }
+}
+
+// The runs that begin in one workgroup of the sums and end in a later one: the partial rows in their order.  The run's end is
+// found 64 workgroups at a time, and its partial rows are shared by the waves.
+template <typename TG, typename TO>
+__global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, TO* out, int64_t out_rs, const float* partial, int D,
+                                                                     int slices, float scale, bool add) {
+  constexpr int E = kE<TG>;
+  __shared__ __attribute__((aligned(16))) float part[kSumWaves][kWave * E];
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  const int64_t group = blockIdx.x / slices, per = (int64_t)s.unit * kSumWaves, begin = group * per, end = begin + per;
+  if (end >= s.n) return;
+  const int key = s.keys[end];
+  if (key >= s.V || s.keys[end - 1] != key) return;
+  if (begin > 0 && s.keys[begin - 1] == key) return;  // it began before
+  // groups behind this one that the run reaches
+  int64_t more = 1;
+  for (;; more += kWave) {
+    const int64_t at = end + (more + lane) * per;  // the first position behind the group that it may reach
+    const uint64_t ends = __ballot(at >= s.n || s.keys[min(at, (int64_t)s.n - 1)] != key);
+    if (ends) {
+      more += __builtin_ctzll(ends);
+      break;
+    }
+  }
+  const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
+  const int64_t one = (int64_t)slices * kWave * E, two = 2 * one;
+  const float* p = partial + group * two + (slice * kWave + lane) * E;
+  float sum[E] = {};
+  const int64_t share = (more + kSumWaves - 1) / kSumWaves, u0 = w * share + 1, u1 = min(u0 + share, more + 1);
+#pragma unroll 4
+  for (int64_t u = u0; u < u1; ++u)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] += p[u * two + e];
+#pragma unroll
+  for (int e = 0; e < E; ++e) part[w][lane * E + e] = sum[e];
+  __syncthreads();
+  if (w != 0 || col >= D) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = p[one + e];
+  for (int i = 0; i < kSumWaves; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] += part[i][lane * E + e];
+  put_row<E, TO>(out + key * out_rs + col, sum, scale, D - col, add);
 }
 
 // ------------------------------------------------------------------ host side
@@ -374,40 +569,62 @@ int bit_length(int64_t v) {
 
 // How a call's passes and workspace are cut.
 struct Plan {
-  int passes, bits, groups, stretch, slices;
-  int64_t units;
+  bool few;
+  int passes, bits, groups, stretch, slices, unit, tokens;
+  int64_t sum_groups;
   size_t list, counts, part;  // bytes of one list of n positions, of the counts, of the partial rows
-  size_t bytes() const { return 4 * list + counts + part; }
+  size_t bytes() const { return few ? 0 : 4 * list + counts + part; }
 };
 Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
-  Plan p;
+  Plan p{};
+  const int E = 16 / hdcm_elt_size(dtype);
+  p.slices = (int)((D + kWave * E - 1) / (kWave * E));
+  p.few = n <= kFewPositions;
+  // a wave for each token where that makes no more than four rounds of workgroups
+  p.tokens = kSumWaves;
+  while (p.tokens < kMostTokens && (V + p.tokens - 1) / p.tokens * p.slices > 4096) p.tokens *= 2;
   const int bits = bit_length(V);  // of the largest key, V
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.bits = (bits + p.passes - 1) / p.passes;
   const int64_t tiles = (n + kTile - 1) / kTile;
   p.stretch = (int)((tiles + kMaxGroups - 1) / kMaxGroups * kTile);
   p.groups = (int)((n + p.stretch - 1) / p.stretch);
-  const int E = 16 / hdcm_elt_size(dtype);
-  p.slices = (int)((D + kWave * E - 1) / (kWave * E));
-  p.units = (n + kUnit - 1) / kUnit;
+  p.unit = kAhead;
+  p.sum_groups = (n + p.unit * kSumWaves - 1) / (p.unit * kSumWaves);
   const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
   p.list = whole((size_t)n * 4);
   p.counts = whole((size_t)p.groups * kBins * 4);
-  p.part = whole((size_t)p.units * 2 * p.slices * kWave * E * 4);
+  p.part = whole((size_t)p.sum_groups * 2 * p.slices * kWave * E * 4);
   return p;
 }
 
 constexpr int64_t kMaxVocab = (int64_t)1 << 30, kMaxPositions = (int64_t)1 << 30, kMaxWidth = (int64_t)1 << 24;
 
 template <typename TG, typename TO>
+void launch_few(const Plan& p, const Ids& ids, int n, const GradRows& g, void* out, int64_t out_rs, int64_t D, float scale, bool add,
+                hipStream_t stream) {
+  const dim3 grid((unsigned)((ids.V + p.tokens - 1) / p.tokens * (int64_t)p.slices));
+  HDCM_LAUNCH((embedding_few_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, ids, n, g, (TO*)out, out_rs, (int)D, p.slices,
+              p.tokens, scale, add);
+}
+
+template <typename TG, typename TO>
 void launch_sums(const Plan& p, const Sorted& s, const GradRows& g, void* out, int64_t out_rs, float* part, int64_t D, float scale,
                  bool add, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.units * p.slices + kSumWaves - 1) / kSumWaves));
+  const dim3 grid((unsigned)(p.sum_groups * p.slices));
   HDCM_LAUNCH((embedding_sum_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, s, g, (TO*)out, out_rs, part, (int)D, p.slices,
               scale, add);
-  if (p.units > 1)
+  if (p.sum_groups > 1)
     HDCM_LAUNCH((embedding_join_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, s, (TO*)out, out_rs, (const float*)part, (int)D,
                 p.slices, scale, add);
+}
+
+// Zeros by a launch of their own: there is nothing to sort, or rows lie apart
+void launch_zeros(void* dw, int64_t rs, int64_t V, int64_t D, int dtype, hipStream_t s) {
+  const int E = 16 / hdcm_elt_size(dtype);
+  const dim3 grid((unsigned)((V * ((D + E - 1) / E) + 255) / 256));
+  if (dtype == HDCM_F32) HDCM_LAUNCH(zero_rows_kernel<float>, grid, dim3(256), 0, s, (float*)dw, rs, V, (int)D);
+  else HDCM_LAUNCH(zero_rows_kernel<bf16_t>, grid, dim3(256), 0, s, (bf16_t*)dw, rs, V, (int)D);
 }
 
 }  // namespace
@@ -452,32 +669,49 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   Plan p{};
   if (!none) {
     p = plan_of(B * L, V, D, dtype);
-    HDCM_CHECK_ARG(ws && ws_bytes >= p.bytes(), HDCM_EWORKSPACE);
+    HDCM_CHECK_ARG(p.bytes() == 0 || (ws && ws_bytes >= p.bytes()), HDCM_EWORKSPACE);
     HDCM_CHECK_ARG(hdcm_aligned16(ws), HDCM_EALIGN);
   }
-  if (!accumulate) {
-    const int64_t P = (D + 16 / hdcm_elt_size(dw_dtype) - 1) / (16 / hdcm_elt_size(dw_dtype));
-    const dim3 grid((unsigned)((V * P + 255) / 256));
-    if (dw_dtype == HDCM_F32) HDCM_LAUNCH(zero_rows_kernel<float>, grid, dim3(256), 0, s, (float*)dw, dw_row_stride, V, (int)D);
-    else HDCM_LAUNCH(zero_rows_kernel<bf16_t>, grid, dim3(256), 0, s, (bf16_t*)dw, dw_row_stride, V, (int)D);
+  if (none) {
+    launch_zeros(dw, dw_row_stride, V, D, dw_dtype, s);
+    return hdcm_launch_status();
   }
-  if (none) return hdcm_launch_status();
   const int n = (int)(B * L);
+  const Ids keys_of{ids, id_bytes, (int)V, (int)padding_idx};
+  const GradRows g{dy, dy_batch_stride, dy_row_stride, (uint32_t)L};
+  if (p.few) {
+    const auto go = [&](auto launch) { launch(p, keys_of, n, g, dw, dw_row_stride, D, scale, accumulate != 0, s); };
+    if (dtype == HDCM_F32) dw_dtype == HDCM_F32 ? go(launch_few<float, float>) : go(launch_few<float, bf16_t>);
+    else dw_dtype == HDCM_F32 ? go(launch_few<bf16_t, float>) : go(launch_few<bf16_t, bf16_t>);
+    return hdcm_launch_status();
+  }
   char* at = (char*)ws;
   int* lists[4];
   for (int i = 0; i < 4; ++i, at += p.list) lists[i] = (int*)at;
   int* counts = (int*)at;
   float* part = (float*)(at + p.counts);
-  SortIn in{ids, nullptr, nullptr, id_bytes, (int)V, (int)padding_idx};
+  // the zeros go with the sorting launches, a share for a count and two for a scatter
+  const bool apart = dw_row_stride != D && V > 1;
+  if (!accumulate && apart) launch_zeros(dw, dw_row_stride, V, D, dw_dtype, s);
+  const int64_t zeros = accumulate || apart ? 0 : V * D * hdcm_elt_size(dw_dtype);
+  int shares = 0;
+  const auto fill_share = [&](int share) {
+    const auto bytes = [&](int k) { return k == 3 * p.passes ? zeros : zeros / (3 * p.passes) * k / 16 * 16; };
+    const Fill f{(char*)dw, bytes(shares), bytes(shares + share)};
+    shares += share;
+    return f;
+  };
+  const auto grid = [&](const Fill& f) { return dim3((unsigned)(p.groups + (f.end - f.begin + kFillBytes - 1) / kFillBytes)); };
+  SortIn in{keys_of, nullptr, nullptr};
   for (int k = 0; k < p.passes; ++k) {
     int *keys = lists[2 * (k & 1)], *pos = lists[2 * (k & 1) + 1];
-    HDCM_LAUNCH(sort_count_kernel, dim3(p.groups), dim3(kSortThreads), 0, s, in, n, p.stretch, k * p.bits, p.bits, counts);
-    HDCM_LAUNCH(sort_scatter_kernel, dim3(p.groups), dim3(kSortThreads), 0, s, in, n, p.stretch, k * p.bits, p.bits,
-                (const int*)counts, keys, pos);
-    in = SortIn{nullptr, keys, pos, 4, (int)V, -1};
+    const Pass pass{n, p.stretch, p.groups, k * p.bits, p.bits};
+    const Fill first = fill_share(1), second = fill_share(2);
+    HDCM_LAUNCH(sort_count_kernel, grid(first), dim3(kSortThreads), 0, s, in, pass, counts, first);
+    HDCM_LAUNCH(sort_scatter_kernel, grid(second), dim3(kSortThreads), 0, s, in, pass, (const int*)counts, keys, pos, second);
+    in.keys = keys, in.pos = pos;
   }
-  const Sorted sorted{in.keys, in.pos, n, (int)V};
-  const GradRows g{dy, dy_batch_stride, dy_row_stride, (uint32_t)L};
+  const Sorted sorted{in.keys, in.pos, n, (int)V, p.unit};
   const auto go = [&](auto launch) { launch(p, sorted, g, dw, dw_row_stride, part, D, scale, accumulate != 0, s); };
   if (dtype == HDCM_F32) dw_dtype == HDCM_F32 ? go(launch_sums<float, float>) : go(launch_sums<float, bf16_t>);
   else dw_dtype == HDCM_F32 ? go(launch_sums<bf16_t, float>) : go(launch_sums<bf16_t, bf16_t>);

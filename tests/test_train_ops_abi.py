@@ -46,12 +46,12 @@ def test_embedding_fwd_validation():
 def test_embedding_grad_validation():
     lib = _ops.lib()
     f, need = lib.hdcm_embedding_grad, lib.hdcm_embedding_grad_workspace_bytes
-    n = need(2, 512, 50304, 1024, BF16)
+    n = need(2, 4096, 50304, 1024, BF16)
     assert 0 < n < 64 << 20
-    assert need(0, 512, 50304, 1024, BF16) == 0 and need(2, 512, 0, 1024, BF16) == 0
+    assert need(0, 4096, 50304, 1024, BF16) == 0 and need(2, 4096, 0, 1024, BF16) == 0
     assert need(1 << 20, 1 << 20, 50304, 1024, BF16) == 0  # more than the kernels take
     # ids, id_bytes, dy, dy_bs, dy_rs, dw, dw_rs, dw_dtype, ws, ws_bytes, B, L, V, D, scale, padding, accumulate, dtype, stream
-    base = [P16, 8, P16, 512 * 1024, 1024, P16, 1024, BF16, P16, n, 2, 512, 50304, 1024, 1.0, -1, 0, BF16, None]
+    base = [P16, 8, P16, 4096 * 1024, 1024, P16, 1024, BF16, P16, n, 2, 4096, 50304, 1024, 1.0, -1, 0, BF16, None]
     assert f(*with_(base, _17=5)) == EUNSUPPORTED
     assert f(*with_(base, _7=5)) == EUNSUPPORTED
     assert f(*with_(base, _1=1)) == EUNSUPPORTED
