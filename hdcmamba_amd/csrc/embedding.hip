@@ -185,103 +185,224 @@ template <typename T> __device__ __forceinline__ void add_piece(float* sum, u32x
   for (int e = 0; e < kE<T>; ++e) sum[e] += v[e];
 }
 
-// ------------------------------------------------------------------ few positions: one launch
-// A workgroup takes R tokens and 64 pieces of their rows, finds its tokens among all ids (a bit for each position
-// and token in LDS), and writes all R rows, most of them zeros.  A token of up to kShort positions is a wave's; the
-// waves share the positions of a more frequent one.
-constexpr int kFewPositions = 32 * kWave;  // a word of bits for each lane
-constexpr int kMostTokens = 32, kShort = 2 * kAhead;
+// Sums of the rows of a list that is sorted by token, by the kSumWaves waves of a workgroup, for 64 pieces of the
+// rows.  A wave takes `unit` positions in a row (a multiple of kAhead), the first from `first` on.  A run of equal
+// tokens inside a unit is written to dw at once.  What a unit holds of a run that began before it (its head) or goes on
+// behind it meets in LDS: the wave in which a run begins adds the heads behind it.  A run that goes on behind the
+// workgroup leaves the workgroup's part of it at partial + one where it began here, else at partial.
+struct List {  // of n positions; tokens from V on are none
+  int64_t first;
+  int n, V, unit;
+};
+template <typename TG, typename TO> struct Sums {
+  const TG* rows;  // at the lane's columns
+  GradRows g;
+  TO* out;
+  int64_t out_rs;
+  int col, D;
+  float scale;
+  bool add;
+  __device__ __forceinline__ void put(int64_t token, const float* sum) const {
+    if (col < D) put_row<kE<TG>, TO>(out + token * out_rs + col, sum, scale, D - col, add);
+  }
+};
+template <typename TG> struct Heads {
+  __attribute__((aligned(16))) float sum[kSumWaves][kWave * kE<TG>];
+  int passes[kSumWaves];  // whether a wave's unit is one run that began before it and goes on behind it
+};
 
-template <typename TG, typename TO>
-__global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int n, GradRows g, TO* out, int64_t out_rs, int D,
-                                                                    int slices, int R, float scale, bool add) {
+template <typename TG, typename TO, typename Key, typename Pos>
+__device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, const Sums<TG, TO>& o, Heads<TG>& head, float* partial,
+                                       int64_t one) {
   constexpr int E = kE<TG>;
-  __shared__ uint32_t bits[kMostTokens][kWave];
-  __shared__ uint32_t frequent;
-  __shared__ uint16_t list[kFewPositions];  // a wave's part in turn, or a frequent token's positions
-  __shared__ __attribute__((aligned(16))) float part[kSumWaves][kWave * E];
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
-  const int v0 = blockIdx.x / slices * R, slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
-  const TG* rows = static_cast<const TG*>(g.p) + col;
-  int key[kFewPositions / kSumThreads];
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  const int64_t begin = l.first + (int64_t)w * l.unit, end = min(begin + l.unit, (int64_t)l.n);
+  float sum[E] = {};
+  // before: the run at hand began before the unit; open: it goes on behind what was added
+  bool before = begin > 0 && begin < l.n && key_at(begin - 1) == key_at(begin), open = false;
+  const bool has_head = before;
+  int last = l.V;
+  for (int64_t b = begin; b < end; b += kAhead) {
+    const int64_t at = min(b + lane, (int64_t)l.n - 1);
+    const int count = (int)min((int64_t)kAhead, end - b);
+    const int keys = b + lane < l.n ? key_at(at) : -1;  // no token behind the last
+    u32x4_t x[kAhead];
+    load_rows<TG>(x, o.rows, o.g.offset((uint32_t)pos_at(at)), count, o.D - o.col);
 #pragma unroll
-  for (int j = 0; j < kFewPositions / kSumThreads; ++j) {
-    const int i = j * kSumThreads + tid;
-    key[j] = i < n ? ids.key(i) : ids.V;
-  }
-  for (int i = tid; i < R * kWave; i += kSumThreads) bits[i / kWave][i % kWave] = 0;
-  if (tid == 0) frequent = 0;
-  __syncthreads();
+    for (int j = 0; j < kAhead; ++j) {
+      const int key = __builtin_amdgcn_readlane(keys, j);
+      if (j < count && key < l.V) {
+        add_piece<TG>(sum, x[j]);
+        open = __builtin_amdgcn_readlane(keys, j + 1) == key;
+        last = key;
+        if (!open) {
+          if (before) {
 #pragma unroll
-  for (int j = 0; j < kFewPositions / kSumThreads; ++j) {
-    const int i = j * kSumThreads + tid, r = key[j] - v0;
-    if (key[j] < ids.V && (unsigned)r < (unsigned)R) atomicOr(&bits[r][i / 32], 1u << (i % 32));
-  }
-  __syncthreads();
-  // the positions of token r, in order, to `to`; their number
-  const auto positions = [&](int r, uint16_t* to, int most) {
-    uint32_t word = bits[r][lane];
-    int before = __popc(word);
+            for (int e = 0; e < E; ++e) head.sum[w][lane * E + e] = sum[e];
+          } else {
+            o.put(key, sum);
+          }
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int up = __shfl_up(before, o, kWave);
-      before += lane >= o ? up : 0;
+          for (int e = 0; e < E; ++e) sum[e] = 0.f;
+          before = false;
+        }
+      }
     }
-    const int count = __builtin_amdgcn_readlane(before, kWave - 1);
-    before -= __popc(word);
-    if (count <= most)
-      for (; word; word &= word - 1) to[before++] = (uint16_t)(32 * lane + __builtin_ctz(word));
-    __builtin_amdgcn_wave_barrier();
-    return count;
-  };
-  const auto add_up = [&](float* sum, const uint16_t* at, int count) {
-    for (int b = 0; b < count; b += kAhead) {
-      u32x4_t x[kAhead];
-      load_rows<TG>(x, rows, g.offset(at[min(b + lane, count - 1)]), min(kAhead, count - b), D - col);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (b + j < count) add_piece<TG>(sum, x[j]);
-    }
-  };
-  uint16_t* mine = list + w * kShort;
-  for (int r = w; r < R && v0 + r < ids.V; r += kSumWaves) {
-    float sum[E] = {};
-    const int count = positions(r, mine, kShort);
-    if (count > kShort) {
-      if (lane == 0) atomicOr(&frequent, 1u << r);
-      continue;
-    }
-    add_up(sum, mine, count);
-    if (col < D && (count || !add)) put_row<E, TO>(out + (v0 + r) * out_rs + col, sum, scale, D - col, add);
   }
+  if (open && before) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) head.sum[w][lane * E + e] = sum[e];
+  }
+  if (lane == 0) head.passes[w] = open && before;
   __syncthreads();
-  for (uint32_t rest = frequent; rest; rest &= rest - 1) {
-    const int r = __builtin_ctz(rest), count = positions(r, list, w == 0 ? kFewPositions : 0);
-    __syncthreads();
-    const int per = (count + kSumWaves - 1) / kSumWaves, b = min(w * per, count);
-    float sum[E] = {};
-    add_up(sum, list + b, min(per, count - b));
+  if (w == 0 && has_head && key_at(begin) < l.V) {  // a run that came from before the workgroup
+    float t[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) part[w][lane * E + e] = sum[e];
-    __syncthreads();
-    if (w == 0 && col < D) {
-      for (int i = 1; i < kSumWaves; ++i)
+    for (int e = 0; e < E; ++e) t[e] = head.sum[0][lane * E + e];
+    for (int i = 0; i + 1 < kSumWaves && head.passes[i]; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += part[i][lane * E + e];
-      put_row<E, TO>(out + (v0 + r) * out_rs + col, sum, scale, D - col, add);
+      for (int e = 0; e < E; ++e) t[e] += head.sum[i + 1][lane * E + e];
+#pragma unroll
+    for (int e = 0; e < E; ++e) partial[e] = t[e];
+  }
+  if (open && !before) {
+    int i = w;
+    do {
+      if (++i == kSumWaves) break;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] += head.sum[i][lane * E + e];
+    } while (head.passes[i]);
+    if (i < kSumWaves) {
+      o.put(last, sum);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) partial[one + e] = sum[e];
     }
   }
 }
 
-// ------------------------------------------------------------------ positions in the order of their tokens
-// Stable radix passes over digits of up to kDigitBits bits of the token, least significant first: a pass
-// counts the digits of each workgroup's stretch of the list, and scatters every stretch behind what the
-// counts put before it.
-constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave;
-constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
+// ------------------------------------------------------------------ the order of tokens within a workgroup
+// Ranks keys by digit, stably: thread `lane` of wave w holds the keys (w rounds + j) 64 + lane, j < rounds <= PER.  rank[j] becomes
+// how many earlier keys of the wave have the same digit; mine[w][d] the wave's keys of digit d.  The wave's lanes with
+// the same digit are found a bit at a time.
+template <int PER> __device__ __forceinline__ void rank_digits(const int (&digit)[PER], const bool (&there)[PER], int rounds, int bits,
+                                                               int* mine, int (&rank)[PER]) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (j >= rounds) break;
+    uint64_t same = __ballot(there[j]);
+    for (int k = 0; k < bits; ++k) {
+      const bool set = (digit[j] >> k) & 1;
+      const uint64_t with = __ballot(set);
+      same &= set ? with : ~with;
+    }
+    const int below = __popcll(same & ((1ull << lane) - 1)), had = mine[digit[j]];
+    rank[j] = had + below;
+    __builtin_amdgcn_wave_barrier();  // all lanes have read before one of them writes
+    if (there[j] && below == 0) mine[digit[j]] = had + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+// Exclusive sum of v over the workgroup's threads; sums: an int for each wave, free afterwards.
+template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums) {
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  int scan = v;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int up = __shfl_up(scan, o, kWave);
+    scan += lane >= o ? up : 0;
+  }
+  if (lane == kWave - 1) sums[w] = scan;
+  __syncthreads();
+  int before = scan - v;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) before += i < w ? sums[i] : 0;
+  __syncthreads();
+  return before;
+}
+
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
-constexpr int kMaxGroups = 128;  // workgroups of a pass, so that each may add all counts up by itself
-constexpr int kCountsAhead = 16;
+
+// ------------------------------------------------------------------ few positions: one launch
+// Workgroup g of G (for each 64 pieces of the rows) takes the tokens g, g + G, .. (up to kBins of them: frequent
+// tokens are often neighbours), finds their positions among all ids, orders them by token in LDS, writes zeros
+// to the rows of those that it has not found and adds up the others'.
+constexpr int kFewPositions = 1024, kFewPer = kFewPositions / kSumThreads;
+
+template <typename TG, typename TO>
+__global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int n, GradRows g, TO* out, int64_t out_rs, int D,
+                                                                    int slices, int bits, float scale, bool add) {
+  constexpr int E = kE<TG>;
+  __shared__ Heads<TG> head;
+  __shared__ int mine[kSumWaves][kBins];
+  __shared__ int sums[kSumWaves];
+  __shared__ uint16_t token[kFewPositions], at[kFewPositions];  // the found positions, by token
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  const uint32_t G = gridDim.x / slices, group = blockIdx.x / slices;
+  const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
+  int digit[kFewPer], rank[kFewPer];
+  bool there[kFewPer];
+#pragma unroll
+  for (int j = 0; j < kFewPer; ++j) {
+    const int i = (w * kFewPer + j) * kWave + lane;
+    digit[j] = i < n ? ids.key(i) : ids.V;
+  }
+#pragma unroll
+  for (int i = 0; i < kSumWaves; ++i) mine[i][tid] = 0;  // kBins == kSumThreads
+#pragma unroll
+  for (int j = 0; j < kFewPer; ++j) {
+    const uint32_t key = digit[j], r = key / G;
+    there[j] = key < (uint32_t)ids.V && key - r * G == group;
+    digit[j] = there[j] ? (int)r : 0;
+  }
+  __syncthreads();
+  rank_digits<kFewPer>(digit, there, kFewPer, bits, mine[w], rank);
+  __syncthreads();
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kSumWaves; ++i) count += mine[i][tid];
+  int run = sum_before<kSumWaves>(count, sums);
+#pragma unroll
+  for (int i = 0; i < kSumWaves; ++i) {
+    const int c = mine[i][tid];
+    mine[i][tid] = run;
+    run += c;
+  }
+  if (tid == kBins - 1) sums[0] = run;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kFewPer; ++j) {
+    if (!there[j]) continue;
+    const int to = mine[w][digit[j]] + rank[j];
+    token[to] = (uint16_t)digit[j], at[to] = (uint16_t)((w * kFewPer + j) * kWave + lane);
+  }
+  const int found = sums[0];
+  __syncthreads();
+  mine[0][tid] = count;
+  __syncthreads();
+  const Sums<TG, TO> o{static_cast<const TG*>(g.p) + col, g, out, out_rs, col, D, scale, add};
+  if (!add) {
+    const float zeros[E] = {};
+    const int tokens = (int)((ids.V - group + G - 1) / G);
+    for (int r = w; r < tokens; r += kSumWaves)
+      if (mine[0][r] == 0) o.put((int64_t)r * G + group, zeros);
+  }
+  const int unit = (found + kSumWaves * kAhead - 1) / (kSumWaves * kAhead) * kAhead;
+  add_up<TG, TO>(List{0, found, ids.V, unit}, [&](int64_t i) { return (int)(token[i] * G + group); }, [&](int64_t i) { return at[i]; }, o,
+                 head, nullptr, 0);
+}
+
+// ------------------------------------------------------------------ many positions in the order of their tokens
+// Stable radix passes over digits of up to kDigitBits bits of the token, least significant first.  A workgroup
+// scatters its stretch of the list behind the keys of lower digits and those of the same digit in the stretches
+// before, which a launch before has counted.  Up to kOneGroup positions are one workgroup's work: all passes in LDS, in one
+// launch.
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
+constexpr int kMaxGroups = 128;                           // workgroups of a pass, so that each may add all counts up by itself
+constexpr int kCountAhead = 16;                           // keys or counts of a thread in flight
+constexpr int kOnePer = 8, kOneGroup = kOnePer * kSortThreads;
 
 // A pass' input: the caller's ids (first pass) or the keys and positions of the pass before.
 struct SortIn {
@@ -296,7 +417,7 @@ struct Pass {
 
 // Zeros for the weight's gradient, written by the workgroups of a sorting launch that have nothing to sort: these
 // launches are short and leave most CUs idle.  Bytes [begin, end), kFillBytes a workgroup.
-constexpr int kFillAhead = 8, kFillBytes = kFillAhead * kSortThreads * 16;
+constexpr int kFillAhead = 4, kFillBytes = kFillAhead * kSortThreads * 16;
 struct Fill {
   char* p;
   int64_t begin, end;
@@ -313,14 +434,75 @@ __device__ __forceinline__ void fill_part(const Fill& f, int64_t part) {
   }
 }
 
+__global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids ids, int n, int passes, int bits, int* keys, int* pos, Fill fill) {
+  __shared__ int sums[kSortWaves];
+  __shared__ int mine[kSortWaves][kBins];  // a wave's keys of a digit, then where its first goes
+  __shared__ int list[kOneGroup];
+  __shared__ uint16_t place[kOneGroup];
+  if (blockIdx.x > 0) {
+    fill_part(fill, (int)blockIdx.x - 1);
+    return;
+  }
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  const int per = (n + kSortThreads - 1) / kSortThreads;  // rounds of the keys that there are
+  int key[kOnePer], at[kOnePer], digit[kOnePer], rank[kOnePer];
+  bool there[kOnePer];
+#pragma unroll
+  for (int j = 0; j < kOnePer; ++j) {
+    at[j] = (w * per + j) * kWave + lane;
+    there[j] = j < per && at[j] < n;
+    key[j] = there[j] ? ids.key(at[j]) : 0;
+  }
+  for (int k = 0; k < passes; ++k) {
+    for (int i = tid; i < kSortWaves * kBins; i += kSortThreads) mine[i / kBins][i % kBins] = 0;
+#pragma unroll
+    for (int j = 0; j < kOnePer; ++j) digit[j] = (key[j] >> (k * bits)) & ((1 << bits) - 1);
+    __syncthreads();
+    rank_digits<kOnePer>(digit, there, per, bits, mine[w], rank);
+    __syncthreads();
+    int total = 0;
+    if (tid < kBins)
+#pragma unroll
+      for (int i = 0; i < kSortWaves; ++i) total += mine[i][tid];
+    int run = sum_before<kSortWaves>(total, sums);
+    if (tid < kBins)
+#pragma unroll
+      for (int i = 0; i < kSortWaves; ++i) {
+        const int c = mine[i][tid];
+        mine[i][tid] = run;
+        run += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOnePer; ++j)
+      if (there[j]) {
+        const int to = mine[w][digit[j]] + rank[j];
+        list[to] = key[j], place[to] = (uint16_t)at[j];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOnePer; ++j)
+      if (there[j]) {
+        const int i = (w * per + j) * kWave + lane;
+        key[j] = list[i], at[j] = place[i];
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < kOnePer; ++j)
+    if (there[j]) {
+      const int i = (w * per + j) * kWave + lane;
+      keys[i] = key[j], pos[i] = at[j];
+    }
+}
+
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pass p, int* counts, Fill fill) {
   __shared__ int count[kBins];
   if ((int)blockIdx.x >= p.groups) {
     fill_part(fill, (int)blockIdx.x - p.groups);
     return;
   }
-  const int tid = threadIdx.x, bins = 1 << p.bits;
-  count[tid] = 0;  // kBins == kSortThreads
+  const int tid = threadIdx.x;
+  if (tid < kBins) count[tid] = 0;
   __syncthreads();
   const int64_t b = (int64_t)blockIdx.x * p.stretch, e = min(b + p.stretch, (int64_t)p.n);
   for (int64_t t = b; t < e; t += kTile) {
@@ -332,10 +514,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pas
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (t + j * kSortThreads + tid < e) atomicAdd(&count[(key[j] >> p.shift) & (bins - 1)], 1);
+      if (t + j * kSortThreads + tid < e) atomicAdd(&count[(key[j] >> p.shift) & ((1 << p.bits) - 1)], 1);
   }
   __syncthreads();
-  if (tid < bins) counts[blockIdx.x * bins + tid] = count[tid];
+  if (tid < kBins) counts[blockIdx.x * kBins + tid] = count[tid];
 }
 
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, Pass p, const int* counts, int* keys, int* pos,
@@ -347,75 +529,59 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, P
     fill_part(fill, (int)blockIdx.x - p.groups);
     return;
   }
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, bins = 1 << p.bits;
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
   const int64_t b = (int64_t)blockIdx.x * p.stretch, e = min(b + p.stretch, (int64_t)p.n);
-  // all keys of lower digits, and this digit's in the stretches before
-  int before = 0, total = 0;
-  if (tid < bins)
-    for (int g0 = 0; g0 < p.groups; g0 += kCountsAhead) {
-      int c[kCountsAhead];
+  int key[kPer], at[kPer];
+  const auto load = [&](int64_t t) {
 #pragma unroll
-      for (int g = 0; g < kCountsAhead; ++g) c[g] = counts[min(g0 + g, p.groups - 1) * bins + tid];
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t i = t + (w * kPer + j) * kWave + lane;
+      key[j] = i < e ? in.key(i) : 0;
+      at[j] = i < e ? in.position(i) : -1;
+    }
+  };
+  load(b);
+  int before = 0, total = 0;  // keys of digit `tid`: in the stretches before, in all
+  if (tid < kBins) {
+    for (int g0 = 0; g0 < p.groups; g0 += kCountAhead) {
+      int c[kCountAhead];
 #pragma unroll
-      for (int g = 0; g < kCountsAhead; ++g) {
+      for (int g = 0; g < kCountAhead; ++g) c[g] = counts[min(g0 + g, p.groups - 1) * kBins + tid];
+#pragma unroll
+      for (int g = 0; g < kCountAhead; ++g) {
         before += g0 + g < (int)blockIdx.x ? c[g] : 0;
         total += g0 + g < p.groups ? c[g] : 0;
       }
     }
-  int scan = total;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int up = __shfl_up(scan, o, kWave);
-    scan += lane >= o ? up : 0;
   }
-  if (lane == kWave - 1) sums[w] = scan;
-  __syncthreads();
-  int lower = scan - total;
-  for (int i = 0; i < w; ++i) lower += sums[i];
-  next[tid] = lower + before;
+  const int lower = sum_before<kSortWaves>(total, sums);
+  if (tid < kBins) next[tid] = lower + before;
   for (int64_t t = b; t < e; t += kTile) {
-#pragma unroll
-    for (int i = 0; i < kSortWaves; ++i) mine[i][tid] = 0;
+    for (int i = tid; i < kSortWaves * kBins; i += kSortThreads) mine[i / kBins][i % kBins] = 0;
     __syncthreads();
-    int key[kPer], at[kPer], digit[kPer], rank[kPer];
+    int digit[kPer], rank[kPer];
+    bool there[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int64_t i = t + w * (kPer * kWave) + j * kWave + lane;
-      key[j] = i < e ? in.key(i) : 0;
-      at[j] = i < e ? in.position(i) : -1;
-      digit[j] = (key[j] >> p.shift) & (bins - 1);
-    }
-    // the wave's lanes with the same digit, found a bit at a time, rank themselves behind the wave's earlier ones
+    for (int j = 0; j < kPer; ++j) there[j] = at[j] >= 0, digit[j] = (key[j] >> p.shift) & ((1 << p.bits) - 1);
+    rank_digits<kPer>(digit, there, kPer, p.bits, mine[w], rank);
+    __syncthreads();
+    if (tid < kBins) {
+      int run = next[tid];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      uint64_t same = __ballot(at[j] >= 0);
-      for (int k = 0; k < p.bits; ++k) {
-        const bool set = (digit[j] >> k) & 1;
-        const uint64_t with = __ballot(set);
-        same &= set ? with : ~with;
+      for (int i = 0; i < kSortWaves; ++i) {
+        const int c = mine[i][tid];
+        mine[i][tid] = run;
+        run += c;
       }
-      const int below = __popcll(same & ((1ull << lane) - 1));
-      const int had = mine[w][digit[j]];
-      rank[j] = had + below;
-      __builtin_amdgcn_wave_barrier();  // all lanes have read before one of them writes
-      if (at[j] >= 0 && below == 0) mine[w][digit[j]] = had + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
+      next[tid] = run;
     }
-    __syncthreads();
-    int run = next[tid];
-#pragma unroll
-    for (int i = 0; i < kSortWaves; ++i) {
-      const int c = mine[i][tid];
-      mine[i][tid] = run;
-      run += c;
-    }
-    next[tid] = run;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int to = mine[w][digit[j]] + rank[j];
-      if (at[j] >= 0 && (unsigned)to < (unsigned)p.n) keys[to] = key[j], pos[to] = at[j];  // (inside, whatever the ids became since)
+      if (there[j] && (unsigned)to < (unsigned)p.n) keys[to] = key[j], pos[to] = at[j];  // (inside, whatever the ids became since)
     }
+    load(t + kTile);
     __syncthreads();
   }
 }
@@ -432,88 +598,20 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(T* out, int64_t rs, int6
 // ------------------------------------------------------------------ sums of the sorted rows
 struct Sorted {
   const int *keys, *pos;
-  int n, V, unit;  // unit: sorted positions of a wave, a multiple of kAhead
+  int n, V, unit;
 };
 
-// A wave takes one unit, a workgroup kSumWaves units in a row, of 64 pieces of their rows.  A run of equal tokens
-// inside a unit is written to dw at once.  What a unit holds of a run that began before it (its head) or goes on behind it
-// (its tail) meets in LDS: the wave in which a run begins adds the heads behind it.  A run that goes on behind the
-// workgroup leaves the workgroup's part of it as partial row 1 where it began here, else as partial row 0.
 template <typename TG, typename TO>
 __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(Sorted s, GradRows g, TO* out, int64_t out_rs, float* partial,
                                                                     int D, int slices, float scale, bool add) {
   constexpr int E = kE<TG>;
-  __shared__ __attribute__((aligned(16))) float head[kSumWaves][kWave * E];
-  __shared__ int passes[kSumWaves];  // whether a wave's unit is one run that began before it and goes on behind it
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
-  const int64_t group = blockIdx.x / slices, begin = (group * kSumWaves + w) * s.unit;
-  const int end = (int)min(begin + s.unit, (int64_t)s.n);
-  const TG* rows = static_cast<const TG*>(g.p) + col;
-  float sum[E] = {};
-  // before: the run at hand began before the unit; open: it goes on behind what was added
-  bool before = begin > 0 && begin < s.n && s.keys[begin - 1] == s.keys[begin], open = false;
-  const bool has_head = before;
-  int key = 0;
-  for (int64_t b = begin; b < end; b += kAhead) {
-    const int at = (int)min(b + lane, (int64_t)s.n - 1), count = (int)min((int64_t)kAhead, end - b);
-    const int keys = b + lane < s.n ? s.keys[at] : -1;  // no token behind the last
-    u32x4_t x[kAhead];
-    load_rows<TG>(x, rows, g.offset((uint32_t)s.pos[at]), count, D - col);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      key = __builtin_amdgcn_readlane(keys, j);
-      if (j < count && key < s.V) {
-        add_piece<TG>(sum, x[j]);
-        open = __builtin_amdgcn_readlane(keys, j + 1) == key;
-        if (!open) {
-          if (before) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) head[w][lane * E + e] = sum[e];
-          } else if (col < D) {
-            put_row<E, TO>(out + key * out_rs + col, sum, scale, D - col, add);
-          }
-#pragma unroll
-          for (int e = 0; e < E; ++e) sum[e] = 0.f;
-          before = false;
-        }
-      }
-    }
-  }
-  if (open && before) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) head[w][lane * E + e] = sum[e];
-  }
-  if (lane == 0) passes[w] = open && before;
-  __syncthreads();
-  float* mine = partial + (group * 2 * slices * kWave + slice * kWave + lane) * E;
-  const int64_t one = (int64_t)slices * kWave * E;
-  // a run that came from before the workgroup
-  if (w == 0 && has_head && s.keys[begin] < s.V) {
-    float t[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) t[e] = head[0][lane * E + e];
-    for (int i = 0; i + 1 < kSumWaves && passes[i]; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) t[e] += head[i + 1][lane * E + e];
-#pragma unroll
-    for (int e = 0; e < E; ++e) mine[e] = t[e];
-  }
-  if (open && !before) {
-    const int last = s.keys[end - 1];
-    int i = w;
-    do {
-      if (++i == kSumWaves) break;
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum[e] += head[i][lane * E + e];
-    } while (passes[i]);
-    if (i < kSumWaves) {
-      if (col < D) put_row<E, TO>(out + last * out_rs + col, sum, scale, D - col, add);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine[one + e] = sum[e];
-    }
-  }
+  __shared__ Heads<TG> head;
+  const int lane = threadIdx.x % kWave, slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
+  const int64_t group = blockIdx.x / slices, one = (int64_t)slices * kWave * E;
+  add_up<TG, TO>(List{group * kSumWaves * s.unit, s.n, s.V, s.unit}, [&](int64_t i) { return s.keys[i]; },
+                 [&](int64_t i) { return s.pos[i]; },
+                 Sums<TG, TO>{static_cast<const TG*>(g.p) + col, g, out, out_rs, col, D, scale, add}, head,
+                 partial + group * 2 * one + (slice * kWave + lane) * E, one);
 }
 
 // The runs that begin in one workgroup of the sums and end in a later one: the partial rows in their order.  The run's end is
@@ -544,7 +642,7 @@ __global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, T
   const float* p = partial + group * two + (slice * kWave + lane) * E;
   float sum[E] = {};
   const int64_t share = (more + kSumWaves - 1) / kSumWaves, u0 = w * share + 1, u1 = min(u0 + share, more + 1);
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t u = u0; u < u1; ++u)
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] += p[u * two + e];
@@ -570,7 +668,9 @@ int bit_length(int64_t v) {
 // How a call's passes and workspace are cut.
 struct Plan {
   bool few;
-  int passes, bits, groups, stretch, slices, unit, tokens;
+  int few_groups, few_bits;                   // few positions
+  int passes, bits, groups, stretch;          // sorting
+  int slices, unit;
   int64_t sum_groups;
   size_t list, counts, part;  // bytes of one list of n positions, of the counts, of the partial rows
   size_t bytes() const { return few ? 0 : 4 * list + counts + part; }
@@ -580,9 +680,11 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   const int E = 16 / hdcm_elt_size(dtype);
   p.slices = (int)((D + kWave * E - 1) / (kWave * E));
   p.few = n <= kFewPositions;
-  // a wave for each token where that makes no more than four rounds of workgroups
-  p.tokens = kSumWaves;
-  while (p.tokens < kMostTokens && (V + p.tokens - 1) / p.tokens * p.slices > 4096) p.tokens *= 2;
+  // a round of workgroups, as far as their tokens are kSumWaves at least and kBins at most
+  int64_t tokens = V * p.slices / 512;
+  tokens = tokens < kSumWaves ? kSumWaves : tokens > kBins ? kBins : tokens;
+  p.few_groups = (int)((V + tokens - 1) / tokens);
+  p.few_bits = bit_length((V + p.few_groups - 1) / p.few_groups - 1);
   const int bits = bit_length(V);  // of the largest key, V
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.bits = (bits + p.passes - 1) / p.passes;
@@ -593,7 +695,7 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   p.sum_groups = (n + p.unit * kSumWaves - 1) / (p.unit * kSumWaves);
   const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
   p.list = whole((size_t)n * 4);
-  p.counts = whole((size_t)p.groups * kBins * 4);
+  p.counts = (size_t)p.groups * kBins * 4;
   p.part = whole((size_t)p.sum_groups * 2 * p.slices * kWave * E * 4);
   return p;
 }
@@ -603,9 +705,9 @@ constexpr int64_t kMaxVocab = (int64_t)1 << 30, kMaxPositions = (int64_t)1 << 30
 template <typename TG, typename TO>
 void launch_few(const Plan& p, const Ids& ids, int n, const GradRows& g, void* out, int64_t out_rs, int64_t D, float scale, bool add,
                 hipStream_t stream) {
-  const dim3 grid((unsigned)((ids.V + p.tokens - 1) / p.tokens * (int64_t)p.slices));
+  const dim3 grid((unsigned)((int64_t)p.few_groups * p.slices));
   HDCM_LAUNCH((embedding_few_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, ids, n, g, (TO*)out, out_rs, (int)D, p.slices,
-              p.tokens, scale, add);
+              p.few_bits, scale, add);
 }
 
 template <typename TG, typename TO>
@@ -690,26 +792,33 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   for (int i = 0; i < 4; ++i, at += p.list) lists[i] = (int*)at;
   int* counts = (int*)at;
   float* part = (float*)(at + p.counts);
-  // the zeros go with the sorting launches, a share for a count and two for a scatter
+  // the zeros go with the sorting launches: a share for a count, two for a scatter
   const bool apart = dw_row_stride != D && V > 1;
   if (!accumulate && apart) launch_zeros(dw, dw_row_stride, V, D, dw_dtype, s);
   const int64_t zeros = accumulate || apart ? 0 : V * D * hdcm_elt_size(dw_dtype);
-  int shares = 0;
+  const int shares = 3 * p.passes;
+  int shared = 0;
   const auto fill_share = [&](int share) {
-    const auto bytes = [&](int k) { return k == 3 * p.passes ? zeros : zeros / (3 * p.passes) * k / 16 * 16; };
-    const Fill f{(char*)dw, bytes(shares), bytes(shares + share)};
-    shares += share;
+    const auto bytes = [&](int k) { return k == shares ? zeros : zeros / shares * k / 16 * 16; };
+    const Fill f{(char*)dw, bytes(shared), bytes(shared + share)};
+    shared += share;
     return f;
   };
-  const auto grid = [&](const Fill& f) { return dim3((unsigned)(p.groups + (f.end - f.begin + kFillBytes - 1) / kFillBytes)); };
+  const auto grid = [&](int groups, const Fill& f) { return dim3((unsigned)(groups + (f.end - f.begin + kFillBytes - 1) / kFillBytes)); };
   SortIn in{keys_of, nullptr, nullptr};
-  for (int k = 0; k < p.passes; ++k) {
-    int *keys = lists[2 * (k & 1)], *pos = lists[2 * (k & 1) + 1];
-    const Pass pass{n, p.stretch, p.groups, k * p.bits, p.bits};
-    const Fill first = fill_share(1), second = fill_share(2);
-    HDCM_LAUNCH(sort_count_kernel, grid(first), dim3(kSortThreads), 0, s, in, pass, counts, first);
-    HDCM_LAUNCH(sort_scatter_kernel, grid(second), dim3(kSortThreads), 0, s, in, pass, (const int*)counts, keys, pos, second);
-    in.keys = keys, in.pos = pos;
+  if (n <= kOneGroup) {
+    const Fill f = fill_share(shares);
+    HDCM_LAUNCH(sort_one_kernel, grid(1, f), dim3(kSortThreads), 0, s, keys_of, n, p.passes, p.bits, lists[0], lists[1], f);
+    in.keys = lists[0], in.pos = lists[1];
+  } else {
+    for (int k = 0; k < p.passes; ++k) {
+      int *keys = lists[2 * (k & 1)], *pos = lists[2 * (k & 1) + 1];
+      const Pass pass{n, p.stretch, p.groups, k * p.bits, p.bits};
+      const Fill first = fill_share(1), second = fill_share(2);
+      HDCM_LAUNCH(sort_count_kernel, grid(p.groups, first), dim3(kSortThreads), 0, s, in, pass, counts, first);
+      HDCM_LAUNCH(sort_scatter_kernel, grid(p.groups, second), dim3(kSortThreads), 0, s, in, pass, (const int*)counts, keys, pos, second);
+      in.keys = keys, in.pos = pos;
+    }
   }
   const Sorted sorted{in.keys, in.pos, n, (int)V, p.unit};
   const auto go = [&](auto launch) { launch(p, sorted, g, dw, dw_row_stride, part, D, scale, accumulate != 0, s); };
