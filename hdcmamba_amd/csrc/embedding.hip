@@ -25,7 +25,8 @@ template <> struct Loose<float> {
   typedef u32x4_t type __attribute__((aligned(4)));
 };
 // The first n of them (all from E on), zero bits behind
-template <typename T> __device__ __forceinline__ u32x4_t load_piece(const T* p, int n) {
+template <typename T, bool STREAM = false> __device__ __forceinline__ u32x4_t load_piece(const T* p, int n) {
+  if (STREAM && n >= kE<T>) return __builtin_nontemporal_load(reinterpret_cast<const typename Loose<T>::type*>(p));
   if (n >= kE<T>) return *reinterpret_cast<const typename Loose<T>::type*>(p);
   u32x4_t r = {0, 0, 0, 0};
 #pragma unroll
@@ -117,12 +118,16 @@ void launch_lookup(const void* ids, const void* w, int64_t w_rs, void* out, int6
 }
 
 // ------------------------------------------------------------------ the gradient's rows
-// dy [.., L, D]: position p lies at (p / L) batch stride + (p % L) row stride.
+// dy [.., L, D]: position p lies at (p / L) batch stride + (p % L) row stride; L 0: one batch.
 struct GradRows {
   const void* p;
   int64_t batch, row;
   uint32_t L;
-  __device__ __forceinline__ int64_t offset(uint32_t at) const { return (at / L) * batch + (at % L) * row; }
+  __device__ __forceinline__ int64_t offset(uint32_t at) const {
+    if (!L) return at * row;
+    const uint32_t b = at / L;
+    return b * batch + (at - b * L) * row;
+  }
 };
 
 // The caller's ids as keys: what is no token of the weight, and the padding index, becomes V.
@@ -143,23 +148,25 @@ template <int E, typename TO> __device__ __forceinline__ void put_row(TO* p, con
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = sum[e0 + e] * scale;
-    if (add) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e0 + e < n) v[e] += to_f<TO>(p[e0 + e]);
-    }
     if (e0 + 4 <= n) {
       if constexpr (sizeof(TO) == 2) {
         typedef uint32_t pair_t __attribute__((ext_vector_type(2), aligned(2)));
+        if (add) {
+          const pair_t old = *reinterpret_cast<const pair_t*>(p + e0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) v[2 * i] += __uint_as_float(old[i] << 16), v[2 * i + 1] += __uint_as_float(old[i] & 0xffff0000u);
+        }
         *reinterpret_cast<pair_t*>(p + e0) = pair_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
       } else {
         typedef float quad_t __attribute__((ext_vector_type(4), aligned(4)));
-        *reinterpret_cast<quad_t*>(p + e0) = quad_t{v[0], v[1], v[2], v[3]};
+        quad_t q = {v[0], v[1], v[2], v[3]};
+        if (add) q += *reinterpret_cast<const quad_t*>(p + e0);
+        *reinterpret_cast<quad_t*>(p + e0) = q;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e0 + e < n) p[e0 + e] = from_f<TO>(v[e]);
+        if (e0 + e < n) p[e0 + e] = from_f<TO>(v[e] + (add ? to_f<TO>(p[e0 + e]) : 0.f));
     }
   }
 }
@@ -169,14 +176,14 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-constexpr int kAhead = 16;                                      // rows of dy that a wave has in flight
+constexpr int kAhead = 8;                                       // rows of dy that a wave has in flight
 constexpr int kSumThreads = 512, kSumWaves = kSumThreads / kWave;  // of the kernels that add rows up
 
 // A wave's lanes hold the offsets of `count` (1..kAhead) rows: loads them all.
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void load_rows(u32x4_t (&x)[kAhead], const T* rows, int64_t offs, int count, int n) {
 #pragma unroll
-  for (int j = 0; j < kAhead; ++j) x[j] = load_piece<T>(rows + lane_value(offs, min(j, count - 1)), n);
+  for (int j = 0; j < kAhead; ++j) x[j] = load_piece<T, STREAM>(rows + lane_value(offs, min(j, count - 1)), n);
 }
 template <typename T> __device__ __forceinline__ void add_piece(float* sum, u32x4_t x) {
   float v[kE<T>];
@@ -211,7 +218,7 @@ template <typename TG> struct Heads {
   int passes[kSumWaves];  // whether a wave's unit is one run that began before it and goes on behind it
 };
 
-template <typename TG, typename TO, typename Key, typename Pos>
+template <bool STREAM, typename TG, typename TO, typename Key, typename Pos>
 __device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, const Sums<TG, TO>& o, Heads<TG>& head, float* partial,
                                        int64_t one) {
   constexpr int E = kE<TG>;
@@ -219,15 +226,16 @@ __device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, co
   const int64_t begin = l.first + (int64_t)w * l.unit, end = min(begin + l.unit, (int64_t)l.n);
   float sum[E] = {};
   // before: the run at hand began before the unit; open: it goes on behind what was added
-  bool before = begin > 0 && begin < l.n && key_at(begin - 1) == key_at(begin), open = false;
-  const bool has_head = before;
+  bool before = false, open = false, has_head = false;
   int last = l.V;
   for (int64_t b = begin; b < end; b += kAhead) {
-    const int64_t at = min(b + lane, (int64_t)l.n - 1);
+    // lanes up to kAhead: the batch and the key behind it; the last lane: the key before it
+    const int64_t mine = lane < kWave - 1 ? b + lane : b - 1, at = max(min(mine, (int64_t)l.n - 1), (int64_t)0);
     const int count = (int)min((int64_t)kAhead, end - b);
-    const int keys = b + lane < l.n ? key_at(at) : -1;  // no token behind the last
+    const int found = key_at(at), keys = mine >= 0 && mine < l.n ? found : -1;  // no token before the first or behind the last
     u32x4_t x[kAhead];
-    load_rows<TG>(x, o.rows, o.g.offset((uint32_t)pos_at(at)), count, o.D - o.col);
+    load_rows<STREAM, TG>(x, o.rows, o.g.offset((uint32_t)pos_at(at)), count, o.D - o.col);
+    if (b == begin) has_head = before = __builtin_amdgcn_readlane(keys, kWave - 1) == __builtin_amdgcn_readlane(keys, 0);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int key = __builtin_amdgcn_readlane(keys, j);
@@ -282,6 +290,8 @@ __device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, co
 }
 
 // ------------------------------------------------------------------ the order of tokens within a workgroup
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+
 // Ranks keys by digit, stably: thread `lane` of wave w holds the keys (w rounds + j) 64 + lane, j < rounds <= PER.  rank[j] becomes
 // how many earlier keys of the wave have the same digit; mine[w][d] the wave's keys of digit d.  The wave's lanes with
 // the same digit are found a bit at a time.
@@ -304,8 +314,18 @@ template <int PER> __device__ __forceinline__ void rank_digits(const int (&digit
     __builtin_amdgcn_wave_barrier();
   }
 }
-// Exclusive sum of v over the workgroup's threads; sums: an int for each wave, free afterwards.
-template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums) {
+// The waves' keys of digit d, mine[w][d], become where the first of them goes, `next` being where the digit's first
+// goes; returns where its next one will.
+template <int WAVES> __device__ __forceinline__ int place_digit(int (*mine)[kBins], const int (&count)[WAVES], int d, int next) {
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    mine[i][d] = next;
+    next += count[i];
+  }
+  return next;
+}
+// Exclusive sum of v over the workgroup's threads, and the whole sum; sums: an int for each wave.
+template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums, int& all) {
   const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
   int scan = v;
 #pragma unroll
@@ -316,13 +336,14 @@ template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums)
   if (lane == kWave - 1) sums[w] = scan;
   __syncthreads();
   int before = scan - v;
+  all = 0;
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) before += i < w ? sums[i] : 0;
-  __syncthreads();
+  for (int i = 0; i < WAVES; ++i) {
+    before += i < w ? sums[i] : 0;
+    all += sums[i];
+  }
   return before;
 }
-
-constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 
 // ------------------------------------------------------------------ few positions: one launch
 // Workgroup g of G (for each 64 pieces of the rows) takes the tokens g, g + G, .. (up to kBins of them: frequent
@@ -338,6 +359,7 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
   __shared__ int mine[kSumWaves][kBins];
   __shared__ int sums[kSumWaves];
   __shared__ uint16_t token[kFewPositions], at[kFewPositions];  // the found positions, by token
+  __shared__ bool none[kBins];                                   // tokens that were not found
   const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
   const uint32_t G = gridDim.x / slices, group = blockIdx.x / slices;
   const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
@@ -359,17 +381,11 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
   __syncthreads();
   rank_digits<kFewPer>(digit, there, kFewPer, bits, mine[w], rank);
   __syncthreads();
-  int count = 0;
+  int each[kSumWaves], count = 0, found;
 #pragma unroll
-  for (int i = 0; i < kSumWaves; ++i) count += mine[i][tid];
-  int run = sum_before<kSumWaves>(count, sums);
-#pragma unroll
-  for (int i = 0; i < kSumWaves; ++i) {
-    const int c = mine[i][tid];
-    mine[i][tid] = run;
-    run += c;
-  }
-  if (tid == kBins - 1) sums[0] = run;
+  for (int i = 0; i < kSumWaves; ++i) count += each[i] = mine[i][tid];
+  place_digit<kSumWaves>(mine, each, tid, sum_before<kSumWaves>(count, sums, found));
+  none[tid] = count == 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kFewPer; ++j) {
@@ -377,19 +393,16 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
     const int to = mine[w][digit[j]] + rank[j];
     token[to] = (uint16_t)digit[j], at[to] = (uint16_t)((w * kFewPer + j) * kWave + lane);
   }
-  const int found = sums[0];
-  __syncthreads();
-  mine[0][tid] = count;
-  __syncthreads();
   const Sums<TG, TO> o{static_cast<const TG*>(g.p) + col, g, out, out_rs, col, D, scale, add};
   if (!add) {
     const float zeros[E] = {};
     const int tokens = (int)((ids.V - group + G - 1) / G);
     for (int r = w; r < tokens; r += kSumWaves)
-      if (mine[0][r] == 0) o.put((int64_t)r * G + group, zeros);
+      if (none[r]) o.put((int64_t)r * G + group, zeros);
   }
+  __syncthreads();
   const int unit = (found + kSumWaves * kAhead - 1) / (kSumWaves * kAhead) * kAhead;
-  add_up<TG, TO>(List{0, found, ids.V, unit}, [&](int64_t i) { return (int)(token[i] * G + group); }, [&](int64_t i) { return at[i]; }, o,
+  add_up<false, TG, TO>(List{0, found, ids.V, unit}, [&](int64_t i) { return (int)(token[i] * G + group); }, [&](int64_t i) { return at[i]; }, o,
                  head, nullptr, 0);
 }
 
@@ -460,18 +473,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids ids, int n, 
     __syncthreads();
     rank_digits<kOnePer>(digit, there, per, bits, mine[w], rank);
     __syncthreads();
-    int total = 0;
+    int each[kSortWaves] = {}, total = 0, all;
     if (tid < kBins)
 #pragma unroll
-      for (int i = 0; i < kSortWaves; ++i) total += mine[i][tid];
-    int run = sum_before<kSortWaves>(total, sums);
-    if (tid < kBins)
-#pragma unroll
-      for (int i = 0; i < kSortWaves; ++i) {
-        const int c = mine[i][tid];
-        mine[i][tid] = run;
-        run += c;
-      }
+      for (int i = 0; i < kSortWaves; ++i) total += each[i] = mine[i][tid];
+    const int lower = sum_before<kSortWaves>(total, sums, all);
+    if (tid < kBins) place_digit<kSortWaves>(mine, each, tid, lower);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kOnePer; ++j)
@@ -522,7 +529,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pas
 
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, Pass p, const int* counts, int* keys, int* pos,
                                                                     Fill fill) {
-  __shared__ int next[kBins];              // where the next key of a digit goes
   __shared__ int sums[kSortWaves];
   __shared__ int mine[kSortWaves][kBins];  // a wave's keys of a digit, then where its first goes
   if ((int)blockIdx.x >= p.groups) {
@@ -554,8 +560,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, P
       }
     }
   }
-  const int lower = sum_before<kSortWaves>(total, sums);
-  if (tid < kBins) next[tid] = lower + before;
+  int all;
+  int next = sum_before<kSortWaves>(total, sums, all) + before;  // where the next key of digit `tid` goes
   for (int64_t t = b; t < e; t += kTile) {
     for (int i = tid; i < kSortWaves * kBins; i += kSortThreads) mine[i / kBins][i % kBins] = 0;
     __syncthreads();
@@ -566,14 +572,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, P
     rank_digits<kPer>(digit, there, kPer, p.bits, mine[w], rank);
     __syncthreads();
     if (tid < kBins) {
-      int run = next[tid];
+      int each[kSortWaves];
 #pragma unroll
-      for (int i = 0; i < kSortWaves; ++i) {
-        const int c = mine[i][tid];
-        mine[i][tid] = run;
-        run += c;
-      }
-      next[tid] = run;
+      for (int i = 0; i < kSortWaves; ++i) each[i] = mine[i][tid];
+      next = place_digit<kSortWaves>(mine, each, tid, next);
     }
     __syncthreads();
 #pragma unroll
@@ -601,14 +603,14 @@ struct Sorted {
   int n, V, unit;
 };
 
-template <typename TG, typename TO>
+template <bool STREAM, typename TG, typename TO>
 __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(Sorted s, GradRows g, TO* out, int64_t out_rs, float* partial,
                                                                     int D, int slices, float scale, bool add) {
   constexpr int E = kE<TG>;
   __shared__ Heads<TG> head;
   const int lane = threadIdx.x % kWave, slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
   const int64_t group = blockIdx.x / slices, one = (int64_t)slices * kWave * E;
-  add_up<TG, TO>(List{group * kSumWaves * s.unit, s.n, s.V, s.unit}, [&](int64_t i) { return s.keys[i]; },
+  add_up<STREAM, TG, TO>(List{group * kSumWaves * s.unit, s.n, s.V, s.unit}, [&](int64_t i) { return s.keys[i]; },
                  [&](int64_t i) { return s.pos[i]; },
                  Sums<TG, TO>{static_cast<const TG*>(g.p) + col, g, out, out_rs, col, D, scale, add}, head,
                  partial + group * 2 * one + (slice * kWave + lane) * E, one);
@@ -665,12 +667,18 @@ int bit_length(int64_t v) {
   return n;
 }
 
+// Rows of dy, each read once, are read past the caches where they and dw are more than the caches hold of them anyway.  us a
+// call, three sets of inputs in turn, cached and past the caches: bf16, 50304 tokens, 32768 x 768 (121 MiB) 44.9 and 47.1,
+// 32768 x 1024 (162) 52.7 and 50.0, 131072 x 1024 (354) 115 and 100, 131072 x 2048 (708) 205 and 160.
+constexpr int64_t kStreamBytes = (int64_t)128 << 20;
+
 // How a call's passes and workspace are cut.
 struct Plan {
   bool few;
   int few_groups, few_bits;                   // few positions
   int passes, bits, groups, stretch;          // sorting
   int slices, unit;
+  bool stream;
   int64_t sum_groups;
   size_t list, counts, part;  // bytes of one list of n positions, of the counts, of the partial rows
   size_t bytes() const { return few ? 0 : 4 * list + counts + part; }
@@ -691,7 +699,10 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   const int64_t tiles = (n + kTile - 1) / kTile;
   p.stretch = (int)((tiles + kMaxGroups - 1) / kMaxGroups * kTile);
   p.groups = (int)((n + p.stretch - 1) / p.stretch);
-  p.unit = kAhead;
+  // two workgroups a CU at least; where there are many, longer units leave fewer partial rows
+  const int64_t groups = (n + kAhead * kSumWaves - 1) / (kAhead * kSumWaves) * p.slices;
+  p.unit = kAhead * (groups < 512 ? 1 : groups < 8192 ? 2 : 4);
+  p.stream = (n + V) * D * hdcm_elt_size(dtype) > kStreamBytes;
   p.sum_groups = (n + p.unit * kSumWaves - 1) / (p.unit * kSumWaves);
   const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
   p.list = whole((size_t)n * 4);
@@ -714,8 +725,8 @@ template <typename TG, typename TO>
 void launch_sums(const Plan& p, const Sorted& s, const GradRows& g, void* out, int64_t out_rs, float* part, int64_t D, float scale,
                  bool add, hipStream_t stream) {
   const dim3 grid((unsigned)(p.sum_groups * p.slices));
-  HDCM_LAUNCH((embedding_sum_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, s, g, (TO*)out, out_rs, part, (int)D, p.slices,
-              scale, add);
+  const auto sums = p.stream ? embedding_sum_kernel<true, TG, TO> : embedding_sum_kernel<false, TG, TO>;
+  HDCM_LAUNCH(sums, grid, dim3(kSumThreads), 0, stream, s, g, (TO*)out, out_rs, part, (int)D, p.slices, scale, add);
   if (p.sum_groups > 1)
     HDCM_LAUNCH((embedding_join_kernel<TG, TO>), grid, dim3(kSumThreads), 0, stream, s, (TO*)out, out_rs, (const float*)part, (int)D,
                 p.slices, scale, add);
@@ -780,7 +791,7 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   }
   const int n = (int)(B * L);
   const Ids keys_of{ids, id_bytes, (int)V, (int)padding_idx};
-  const GradRows g{dy, dy_batch_stride, dy_row_stride, (uint32_t)L};
+  const GradRows g{dy, dy_batch_stride, dy_row_stride, (uint32_t)(B > 1 ? L : 0)};
   if (p.few) {
     const auto go = [&](auto launch) { launch(p, keys_of, n, g, dw, dw_row_stride, D, scale, accumulate != 0, s); };
     if (dtype == HDCM_F32) dw_dtype == HDCM_F32 ? go(launch_few<float, float>) : go(launch_few<float, bf16_t>);
