@@ -152,6 +152,7 @@ _PROTOS = {
     "hdcm_grad_norm_workspace_bytes": (c_size_t, [ctypes.POINTER(TensorRef), c_int64]),
     "hdcm_grad_norm": (c_int, [ctypes.POINTER(TensorRef), c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "hdcm_grad_scale": (c_int, [ctypes.POINTER(TensorRef), c_int64, c_void_p, c_float, c_void_p]),
+    "hdcm_clip_grad_norm": (c_int, [ctypes.POINTER(TensorRef), c_int64, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

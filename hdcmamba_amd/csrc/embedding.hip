@@ -349,7 +349,7 @@ template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums,
 // Workgroup g of G (for each 64 pieces of the rows) takes the tokens g, g + G, .. (up to kBins of them: frequent
 // tokens are often neighbours), finds their positions among all ids, orders them by token in LDS, writes zeros
 // to the rows of those that it has not found and adds up the others'.
-constexpr int kFewPositions = 1024, kFewPer = kFewPositions / kSumThreads;
+constexpr int kFewPositions = 512, kFewPer = kFewPositions / kSumThreads;
 
 template <typename TG, typename TO>
 __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int n, GradRows g, TO* out, int64_t out_rs, int D,
@@ -667,6 +667,11 @@ int bit_length(int64_t v) {
   return n;
 }
 
+// Few positions beside little to fill with zeros: one launch, whose workgroups wait for all ids before they write.  us
+// recorded, in one launch and sorted: 512 positions of text with 8 MiB of zeros 7.4 and 15.1, 32 MiB 13.9 and 17.2, 64 MiB 20.0 and
+// 19.5, 98 MiB 25.2 and 23.6; of one token, whose rows one workgroup adds up, 18.6 and 14.2 with 8 MiB (1024: 40 and 14).
+bool few_of(int64_t n, int64_t zeros) { return n <= kFewPositions && zeros <= (int64_t)48 << 20; }
+
 // Rows of dy, each read once, are read past the caches where they and dw are more than the caches hold of them anyway.  us a
 // call, three sets of inputs in turn, cached and past the caches: bf16, 50304 tokens, 32768 x 768 (121 MiB) 44.9 and 47.1,
 // 32768 x 1024 (162) 52.7 and 50.0, 131072 x 1024 (354) 115 and 100, 131072 x 2048 (708) 205 and 160.
@@ -674,20 +679,18 @@ constexpr int64_t kStreamBytes = (int64_t)128 << 20;
 
 // How a call's passes and workspace are cut.
 struct Plan {
-  bool few;
   int few_groups, few_bits;                   // few positions
   int passes, bits, groups, stretch;          // sorting
   int slices, unit;
   bool stream;
   int64_t sum_groups;
   size_t list, counts, part;  // bytes of one list of n positions, of the counts, of the partial rows
-  size_t bytes() const { return few ? 0 : 4 * list + counts + part; }
+  size_t bytes() const { return 4 * list + counts + part; }
 };
 Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   Plan p{};
   const int E = 16 / hdcm_elt_size(dtype);
   p.slices = (int)((D + kWave * E - 1) / (kWave * E));
-  p.few = n <= kFewPositions;
   // a round of workgroups, as far as their tokens are kSumWaves at least and kBins at most
   int64_t tokens = V * p.slices / 512;
   tokens = tokens < kSumWaves ? kSumWaves : tokens > kBins ? kBins : tokens;
@@ -760,7 +763,7 @@ extern "C" int hdcm_embedding_fwd(const void* ids, int id_bytes, const void* w, 
 
 extern "C" size_t hdcm_embedding_grad_workspace_bytes(int64_t B, int64_t L, int64_t V, int64_t D, int dtype) {
   if (B <= 0 || L <= 0 || V <= 0 || D <= 0 || L > kMaxPositions / B || V > kMaxVocab || D > kMaxWidth) return 0;
-  return plan_of(B * L, V, D, dtype).bytes();
+  return few_of(B * L, V * D * 4) ? 0 : plan_of(B * L, V, D, dtype).bytes();
 }
 
 extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride,
@@ -780,9 +783,10 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   HDCM_CHECK_ARG(V <= kMaxVocab && D <= kMaxWidth && (none || L <= kMaxPositions / B), HDCM_EUNSUPPORTED);
   hipStream_t s = (hipStream_t)stream;
   Plan p{};
-  if (!none) {
-    p = plan_of(B * L, V, D, dtype);
-    HDCM_CHECK_ARG(p.bytes() == 0 || (ws && ws_bytes >= p.bytes()), HDCM_EWORKSPACE);
+  const bool few = !none && few_of(B * L, accumulate ? 0 : V * D * hdcm_elt_size(dw_dtype));
+  if (!none) p = plan_of(B * L, V, D, dtype);
+  if (!none && !few) {
+    HDCM_CHECK_ARG(ws && ws_bytes >= p.bytes(), HDCM_EWORKSPACE);
     HDCM_CHECK_ARG(hdcm_aligned16(ws), HDCM_EALIGN);
   }
   if (none) {
@@ -792,7 +796,7 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   const int n = (int)(B * L);
   const Ids keys_of{ids, id_bytes, (int)V, (int)padding_idx};
   const GradRows g{dy, dy_batch_stride, dy_row_stride, (uint32_t)(B > 1 ? L : 0)};
-  if (p.few) {
+  if (few) {
     const auto go = [&](auto launch) { launch(p, keys_of, n, g, dw, dw_row_stride, D, scale, accumulate != 0, s); };
     if (dtype == HDCM_F32) dw_dtype == HDCM_F32 ? go(launch_few<float, float>) : go(launch_few<float, bf16_t>);
     else dw_dtype == HDCM_F32 ? go(launch_few<bf16_t, float>) : go(launch_few<bf16_t, bf16_t>);

@@ -1032,13 +1032,28 @@ Tensor embedding_grad(const Tensor& ids, const Tensor& grad, int64_t V, double s
 }
 
 // ------------------------------------------------------------------------ the gradients' norm
-// A list of tensors on one device as the library's, copied to be dense where `copies` lets them.
+// The tensors of a Python list, or (of parameters) their gradients.  A caster to a vector would take 0.1 us for each, and a
+// parameter's .grad in Python as much.
+std::vector<Tensor> listed(const pybind11::list& list, bool grads) {
+  std::vector<Tensor> ts;
+  ts.reserve(list.size());
+  for (const pybind11::handle item : list) {
+    TORCH_CHECK_TYPE(THPVariable_Check(item.ptr()), "a list of tensors is expected, got a ", Py_TYPE(item.ptr())->tp_name);
+    const Tensor& t = THPVariable_Unpack(item.ptr());
+    if (!grads) ts.push_back(t);
+    else if (t.grad().defined()) ts.push_back(t.grad());
+  }
+  return ts;
+}
+
+// Tensors on one device as the library's, copied to be dense where `copies` lets them.
 struct TensorList {
   std::vector<hdcm_tensor> refs;
   std::vector<Tensor> held;
   TensorList(const std::vector<Tensor>& ts, const char* op, bool copies) {
     refs.reserve(ts.size());
     for (const Tensor& t : ts) {
+      no_gradient(op, {&t});
       TORCH_CHECK(t.layout() == at::kStrided, op, ": a tensor is ", t.layout(), "; the kernels take dense ones");
       on_gpu(t);
       same_device(t, ts[0], "a tensor");
@@ -1046,76 +1061,83 @@ struct TensorList {
       const bool dense = t.is_non_overlapping_and_dense();
       TORCH_CHECK(dense || copies, op, ": a tensor of shape ", t.sizes(), " and strides ", t.strides(),
                   " has gaps or overlaps in memory and cannot be scaled in place");
-      if (!dense) held.push_back(t.contiguous());
+      if (!dense) held.push_back(t.detach().contiguous());
       refs.push_back({const_cast<void*>((dense ? t : held.back()).const_data_ptr()), t.numel(), dt});
     }
   }
+  // Whether no two of them, and not the norm that is read while they are scaled, share memory
+  bool apart(const Tensor* norm) const {
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    spans.reserve(refs.size() + 1);
+    const auto add = [&](const void* p, int64_t bytes) {
+      if (bytes) spans.emplace_back((uintptr_t)p, (uintptr_t)p + bytes);
+    };
+    for (const hdcm_tensor& t : refs) add(t.data, t.count * (t.dtype == HDCM_F32 ? 4 : 2));
+    if (norm) add(norm->const_data_ptr(), norm->element_size());
+    if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+      if (spans[i].first < spans[i - 1].second) return false;
+    return true;
+  }
+};
+constexpr const char* kNotApart = ": tensors share memory, with each other or with the norm";
+
+// Device memory that the library may use in this call, on the current stream
+struct NormWorkspace {
+  size_t n;
+  c10::DataPtr p;
+  explicit NormWorkspace(const TensorList& l)
+      : n(hdcm_grad_norm_workspace_bytes(l.refs.data(), (int64_t)l.refs.size())),
+        p(n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr()) {}
 };
 
-void no_gradient(const char* op, const std::vector<Tensor>& ts) {
-  for (const Tensor& t : ts) no_gradient(op, {&t});
-}
-
-// Scaled tensors, and the norm that is read meanwhile, share no memory.
-void apart(const TensorList& l, const Tensor& norm, const char* op) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  spans.reserve(l.refs.size() + 1);
-  const auto add = [&](const void* p, int64_t bytes) {
-    if (bytes) spans.emplace_back((uintptr_t)p, (uintptr_t)p + bytes);
-  };
-  for (const hdcm_tensor& t : l.refs) add(t.data, t.count * (t.dtype == HDCM_F32 ? 4 : 2));
-  add(norm.const_data_ptr(), 4);
-  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK(spans[i].first >= spans[i - 1].second, op, ": tensors share memory, with each other or with the norm");
-}
-
-Tensor norm_of(const TensorList& l, const Tensor& like, int kind) {
-  Tensor out = fresh({}, at::kFloat, like);
-  const size_t n = hdcm_grad_norm_workspace_bytes(l.refs.data(), (int64_t)l.refs.size());
-  const c10::DataPtr ws = n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr();  // on the current stream
-  check("hdcm_grad_norm", hdcm_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, out.mutable_data_ptr<float>(), ws.get(), n,
+Tensor grad_norm(const pybind11::list& list, int kind) {
+  const std::vector<Tensor> ts = listed(list, false);
+  TORCH_CHECK(!ts.empty(), "grad_norm: no tensors");
+  const c10::DeviceGuard guard(ts[0].device());
+  const TensorList l(ts, "grad_norm", true);
+  Tensor out = fresh({}, at::kFloat, ts[0]);
+  const NormWorkspace ws(l);
+  check("hdcm_grad_norm", hdcm_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, out.mutable_data_ptr<float>(), ws.p.get(), ws.n,
                                          stream_of(out)));
   return out;
 }
-void scale_by(const std::vector<Tensor>& ts, const TensorList& l, double max_norm, const Tensor& norm) {
+
+void clip_grads(const pybind11::list& list, double max_norm, const Tensor& norm_) {
+  const std::vector<Tensor> ts = listed(list, false);
+  if (ts.empty()) return;
+  const c10::DeviceGuard guard(ts[0].device());
+  const TensorList l(ts, "clip_grads_", false);
+  same_device(norm_, ts[0], "total_norm");
+  TORCH_CHECK(norm_.numel() == 1 && norm_.is_floating_point(), "total_norm must be one floating-point number, got ", norm_.scalar_type(),
+              " ", norm_.sizes());
+  TORCH_CHECK(l.apart(&norm_), "clip_grads_", kNotApart);
+  const Tensor norm = as_type(norm_.detach(), at::kFloat);
   check("hdcm_grad_scale", hdcm_grad_scale(l.refs.data(), (int64_t)l.refs.size(), norm.const_data_ptr<float>(), (float)max_norm,
                                            stream_of(norm)));
   for (const Tensor& t : ts) written(t);
 }
 
-Tensor grad_norm(const std::vector<Tensor>& ts, int kind) {
-  TORCH_CHECK(!ts.empty(), "grad_norm: no tensors");
-  no_gradient("grad_norm", ts);
-  Entry entry;
+// None where no parameter has a gradient
+OptTensor clip_grad_norm(const pybind11::list& params, double max_norm, int kind) {
+  std::vector<Tensor> ts = listed(params, true);
+  if (ts.empty()) return std::nullopt;
   const c10::DeviceGuard guard(ts[0].device());
-  return norm_of(TensorList(ts, "grad_norm", true), ts[0], kind);
-}
-
-void clip_grads(const std::vector<Tensor>& ts, double max_norm, const Tensor& norm_) {
-  if (ts.empty()) return;
-  no_gradient("clip_grads_", ts);
-  Entry entry;
-  const c10::DeviceGuard guard(ts[0].device());
-  same_device(norm_, ts[0], "total_norm");
-  TORCH_CHECK(norm_.numel() == 1 && norm_.is_floating_point(), "total_norm must be one floating-point number, got ", norm_.scalar_type(),
-              " ", norm_.sizes());
-  const Tensor norm = as_type(norm_, at::kFloat);
-  const TensorList l(ts, "clip_grads_", false);
-  apart(l, norm, "clip_grads_");
-  scale_by(ts, l, max_norm, norm);
-}
-
-Tensor clip_grad_norm(const std::vector<Tensor>& ts, double max_norm, int kind) {
-  TORCH_CHECK(!ts.empty(), "clip_grad_norm_: no tensors");
-  no_gradient("clip_grad_norm_", ts);
-  Entry entry;
-  const c10::DeviceGuard guard(ts[0].device());
-  const TensorList l(ts, "clip_grad_norm_", false);
-  const Tensor norm = norm_of(l, ts[0], kind);
-  apart(l, norm, "clip_grad_norm_");
-  scale_by(ts, l, max_norm, norm);
-  return norm;
+  TensorList l(ts, "clip_grad_norm_", false);
+  if (!l.apart(nullptr)) {  // a parameter that is given twice counts once
+    std::vector<Tensor> once;
+    for (const Tensor& t : ts)
+      if (std::none_of(once.begin(), once.end(), [&](const Tensor& o) { return o.is_same(t); })) once.push_back(t);
+    ts = std::move(once);
+    l = TensorList(ts, "clip_grad_norm_", false);
+    TORCH_CHECK(l.apart(nullptr), "clip_grad_norm_", kNotApart);
+  }
+  Tensor out = fresh({}, at::kFloat, ts[0]);
+  const NormWorkspace ws(l);
+  check("hdcm_clip_grad_norm", hdcm_clip_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, (float)max_norm,
+                                                   out.mutable_data_ptr<float>(), ws.p.get(), ws.n, stream_of(out)));
+  for (const Tensor& t : ts) written(t);
+  return out;
 }
 
 }  // namespace
@@ -1152,6 +1174,4 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grad_norm", &grad_norm);
   m.def("clip_grads", &clip_grads);
   m.def("clip_grad_norm", &clip_grad_norm);
-  m.attr("NORM_2") = (int)HDCM_NORM_2;
-  m.attr("NORM_MAX") = (int)HDCM_NORM_MAX;
 }

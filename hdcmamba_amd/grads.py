@@ -15,6 +15,8 @@ from . import _ops
 
 __all__ = ["grad_norm", "clip_grads_", "clip_grad_norm_"]
 
+_NORM_2, _NORM_MAX = 0, 1  # HDCM_NORM_2, HDCM_NORM_MAX
+
 
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all elements of a list of tensors together, as a float32 number on their GPU: ``norm_type`` 2, or
@@ -41,21 +43,16 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """torch.nn.utils.clip_grad_norm_ on these kernels: clip_grads_ on the gradients of ``parameters`` (an iterable, or
     one) by their own grad_norm, which is returned.  A parameter given twice counts once.  ``error_if_nonfinite`` waits
     for the norm, and raises with the gradients as they were where it is not finite."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
-    kind, max_norm = _kind(norm_type), _limit(max_norm)
-    if not grads:
-        return torch.zeros(())
-    if not error_if_nonfinite:
-        return _ops.native().clip_grad_norm(grads, max_norm, kind)
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("error_if_nonfinite waits for the norm, which a recording cannot")
-    norm = _ops.native().grad_norm(grads, kind)
-    if not math.isfinite(norm.item()):
-        raise RuntimeError(f"the gradients' norm is {norm.item()}, not finite: they are not clipped")
-    _ops.native().clip_grads(grads, max_norm, norm)
-    return norm
+    parameters, kind, max_norm = _listed(parameters), _kind(norm_type), _limit(max_norm)
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("error_if_nonfinite waits for the norm, which a recording cannot")
+        grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
+        norm = grad_norm(grads, norm_type).item()
+        if not math.isfinite(norm):
+            raise RuntimeError(f"the gradients' norm is {norm}, not finite: they are not clipped")
+    norm = _ops.native().clip_grad_norm(parameters, max_norm, kind)
+    return torch.zeros(()) if norm is None else norm
 
 
 def _listed(tensors):
@@ -66,7 +63,7 @@ def _kind(norm_type):
     p = float(norm_type)
     if p not in (2.0, math.inf):
         raise ValueError(f"norm_type must be 2 or math.inf, got {norm_type}")
-    return _ops.native().NORM_2 if p == 2.0 else _ops.native().NORM_MAX
+    return _NORM_2 if p == 2.0 else _NORM_MAX
 
 
 def _limit(max_norm):

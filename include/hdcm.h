@@ -656,6 +656,7 @@ int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy, int64_t d
  * 8-byte aligned, not kept between calls.
  * hdcm_grad_scale: x *= min(1, max_norm / (*norm + 1e-6)), the product rounded to the tensor's type; tensors are not
  * touched where the factor is 1.  max_norm >= 0.  Tensors must not overlap.
+ * hdcm_clip_grad_norm: both, the norm of the tensors to *out and their scaling by it (ws as for the norm).
  */
 typedef struct {
   void* data;
@@ -666,6 +667,8 @@ enum { HDCM_NORM_2 = 0, HDCM_NORM_MAX = 1 };
 size_t hdcm_grad_norm_workspace_bytes(const hdcm_tensor* tensors, int64_t n);
 int hdcm_grad_norm(const hdcm_tensor* tensors, int64_t n, int norm, float* out, void* ws, size_t ws_bytes, void* stream);
 int hdcm_grad_scale(const hdcm_tensor* tensors, int64_t n, const float* norm, float max_norm, void* stream);
+int hdcm_clip_grad_norm(const hdcm_tensor* tensors, int64_t n, int norm, float max_norm, float* out, void* ws,
+                        size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -99,6 +99,14 @@ def test_grad_norm_validation():
                       ((P17, 10, BF16), EALIGN)):
         t = tensors(bad)
         assert f(*with_(base, _0=t, _1=1)) == code and need(t, 1) == 0
+    h = lib.hdcm_clip_grad_norm  # tensors, n, norm, max_norm, out, ws, ws_bytes, stream
+    both = [good, 3, 0, 1.0, P16, P16, n, None]
+    assert h(*with_(both, _2=2)) == EUNSUPPORTED
+    assert h(*with_(both, _3=-1.0)) == EINVAL
+    assert h(*with_(both, _3=float("nan"))) == EINVAL
+    assert h(*with_(both, _4=None)) == EINVAL
+    assert h(*with_(both, _6=n - 8)) == EWORKSPACE
+    assert h(*with_(both, _5=P18)) == EALIGN
     g = lib.hdcm_grad_scale  # tensors, n, norm, max_norm, stream
     assert g(good, 3, None, 1.0, None) == EINVAL
     assert g(good, 3, P16, -1.0, None) == EINVAL
