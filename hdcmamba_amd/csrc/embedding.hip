@@ -37,9 +37,10 @@ template <typename T, bool STREAM = false> __device__ __forceinline__ u32x4_t lo
     }
   return r;
 }
-template <typename T> __device__ __forceinline__ void store_piece(T* p, u32x4_t r, int n) {
+template <typename T, bool STREAM = false> __device__ __forceinline__ void store_piece(T* p, u32x4_t r, int n) {
   if (n >= kE<T>) {
-    *reinterpret_cast<typename Loose<T>::type*>(p) = r;
+    if constexpr (STREAM) __builtin_nontemporal_store(r, reinterpret_cast<typename Loose<T>::type*>(p));
+    else *reinterpret_cast<typename Loose<T>::type*>(p) = r;
     return;
   }
 #pragma unroll
@@ -63,12 +64,22 @@ template <typename T> __device__ __forceinline__ u32x4_t packed(const float* v) 
   return u32x4_t{r.x, r.y, r.z, r.w};
 }
 
+// What is read or written once goes past the caches where it is more than they hold of it until it is used again.  us
+// a call, three sets of inputs in turn, cached and past the caches.  Rows of dy (bf16, 50304 tokens, dy and dw together):
+// 32768 x 768 (121 MiB) 44.9 and 47.1, 32768 x 1024 (162) 52.7 and 50.0, 131072 x 1024 (354) 115 and 100, 131072 x 2048
+// (708) 205 and 160.  Rows looked up: 131072 x 2048 (512 MiB) 157 and 113; 32768 x 1024 (64) 16.7 and 16.2, but there the next
+// kernel finds them in the caches.
+constexpr int64_t kStreamBytes = (int64_t)128 << 20;
+
 // ------------------------------------------------------------------ lookup
 // A thread copies U pieces of 16 bytes, 256 pieces apart in the order of the output, so that all lanes work at any
 // width; every piece's id, then every piece's row, is in flight before the first is used.
+// us recorded with 1, 2 and 4: 16 x 2048 bf16 1.9, 2.0, 2.7; 1024 x 1024 2.1, 2.3, 3.0; 8192 x 1024 6.1, 5.7, 6.7; 32768 x 1024
+// 16.8, 16.7, 17.0 (4 TB/s of writes, 5 in all).
 constexpr int kLookThreads = 256;
+constexpr int64_t kLookSmall = 1 << 18;
 
-template <typename T, typename I, int U, bool SCALED>
+template <typename T, typename I, int U, bool SCALED, bool STREAM>
 __global__ __launch_bounds__(kLookThreads) void embedding_kernel(const I* __restrict__ ids, const T* __restrict__ w, int64_t w_rs,
                                                                  T* __restrict__ out, int64_t out_rs, int64_t rows, int V, int D,
                                                                  float scale) {
@@ -101,7 +112,7 @@ __global__ __launch_bounds__(kLookThreads) void embedding_kernel(const I* __rest
       x[u] = packed<T>(v);
       if ((uint64_t)id[u] >= (uint64_t)V) x[u] = u32x4_t{0, 0, 0, 0};  // of an infinite or negative scale too
     }
-    store_piece<T>(out + row[u] * out_rs + col[u], x[u], D - col[u]);
+    store_piece<T, STREAM>(out + row[u] * out_rs + col[u], x[u], D - col[u]);
   }
 }
 
@@ -113,8 +124,10 @@ void launch_lookup(const void* ids, const void* w, int64_t w_rs, void* out, int6
     HDCM_LAUNCH(kernel, dim3((unsigned)((pieces + U * kLookThreads - 1) / (U * kLookThreads))), dim3(kLookThreads), 0, s,
                 (const I*)ids, (const T*)w, w_rs, (T*)out, out_rs, rows, (int)V, (int)D, scale);
   };
-  if (scale == 1.f) go(embedding_kernel<T, I, 4, false>, 4);
-  else go(embedding_kernel<T, I, 4, true>, 4);
+  const bool scaled = scale != 1.f;
+  if (pieces <= kLookSmall) scaled ? go(embedding_kernel<T, I, 1, true, false>, 1) : go(embedding_kernel<T, I, 1, false, false>, 1);
+  else if (pieces * 16 <= kStreamBytes) scaled ? go(embedding_kernel<T, I, 2, true, false>, 2) : go(embedding_kernel<T, I, 2, false, false>, 2);
+  else scaled ? go(embedding_kernel<T, I, 2, true, true>, 2) : go(embedding_kernel<T, I, 2, false, true>, 2);
 }
 
 // ------------------------------------------------------------------ the gradient's rows
@@ -197,9 +210,13 @@ template <typename T> __device__ __forceinline__ void add_piece(float* sum, u32x
 // tokens inside a unit is written to dw at once.  What a unit holds of a run that began before it (its head) or goes on
 // behind it meets in LDS: the wave in which a run begins adds the heads behind it.  A run that goes on behind the
 // workgroup leaves the workgroup's part of it at partial + one where it began here, else at partial.
-struct List {  // of n positions; tokens from V on are none
+struct List {
   int64_t first;
-  int n, V, unit;
+  int n, V, unit;  // of n positions; keys from V on are no tokens
+  uint32_t last;   // the largest position
+  // Nor are negative ones, which a caller that writes its ids meanwhile could leave in the sorted list, and positions are
+  // taken into the list: nothing outside the buffers is read or written then either.
+  __device__ __forceinline__ bool token(int key) const { return (unsigned)key < (unsigned)V; }
 };
 template <typename TG, typename TO> struct Sums {
   const TG* rows;  // at the lane's columns
@@ -234,12 +251,12 @@ __device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, co
     const int count = (int)min((int64_t)kAhead, end - b);
     const int found = key_at(at), keys = mine >= 0 && mine < l.n ? found : -1;  // no token before the first or behind the last
     u32x4_t x[kAhead];
-    load_rows<STREAM, TG>(x, o.rows, o.g.offset((uint32_t)pos_at(at)), count, o.D - o.col);
+    load_rows<STREAM, TG>(x, o.rows, o.g.offset(min((uint32_t)pos_at(at), l.last)), count, o.D - o.col);
     if (b == begin) has_head = before = __builtin_amdgcn_readlane(keys, kWave - 1) == __builtin_amdgcn_readlane(keys, 0);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int key = __builtin_amdgcn_readlane(keys, j);
-      if (j < count && key < l.V) {
+      if (j < count && l.token(key)) {
         add_piece<TG>(sum, x[j]);
         open = __builtin_amdgcn_readlane(keys, j + 1) == key;
         last = key;
@@ -263,7 +280,7 @@ __device__ __forceinline__ void add_up(const List& l, Key key_at, Pos pos_at, co
   }
   if (lane == 0) head.passes[w] = open && before;
   __syncthreads();
-  if (w == 0 && has_head && key_at(begin) < l.V) {  // a run that came from before the workgroup
+  if (w == 0 && has_head && l.token(key_at(begin))) {  // a run that came from before the workgroup
     float t[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) t[e] = head.sum[0][lane * E + e];
@@ -348,7 +365,9 @@ template <int WAVES> __device__ __forceinline__ int sum_before(int v, int* sums,
 // ------------------------------------------------------------------ few positions: one launch
 // Workgroup g of G (for each 64 pieces of the rows) takes the tokens g, g + G, .. (up to kBins of them: frequent
 // tokens are often neighbours), finds their positions among all ids, orders them by token in LDS, writes zeros
-// to the rows of those that it has not found and adds up the others'.
+// to the rows of those that it has not found and adds up the others'.  384 x 256 of 1024 tokens 6.0 us: a chain of the ids'
+// arrival, four barriers, the rows' arrival and a join (0.7 MB moved).  With each workgroup's tokens adjacent and its
+// frequent ones one after the other it took 11.
 constexpr int kFewPositions = 512, kFewPer = kFewPositions / kSumThreads;
 
 template <typename TG, typename TO>
@@ -398,12 +417,12 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
     const float zeros[E] = {};
     const int tokens = (int)((ids.V - group + G - 1) / G);
     for (int r = w; r < tokens; r += kSumWaves)
-      if (none[r]) o.put((int64_t)r * G + group, zeros);
+      if (none[r] && col < D) put_row<E, TO>(out + ((int64_t)r * G + group) * out_rs + col, zeros, 1.f, D - col, false);
   }
   __syncthreads();
   const int unit = (found + kSumWaves * kAhead - 1) / (kSumWaves * kAhead) * kAhead;
-  add_up<false, TG, TO>(List{0, found, ids.V, unit}, [&](int64_t i) { return (int)(token[i] * G + group); }, [&](int64_t i) { return at[i]; }, o,
-                 head, nullptr, 0);
+  add_up<false, TG, TO>(List{0, found, ids.V, unit, (uint32_t)n - 1}, [&](int64_t i) { return (int)(token[i] * G + group); }, [&](int64_t i) { return at[i]; }, o,
+                              head, nullptr, 0);
 }
 
 // ------------------------------------------------------------------ many positions in the order of their tokens
@@ -411,6 +430,9 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
 // scatters its stretch of the list behind the keys of lower digits and those of the same digit in the stretches
 // before, which a launch before has counted.  Up to kOneGroup positions are one workgroup's work: all passes in LDS, in one
 // launch.
+// Bound by latency: without zeros to write a count takes 3.4 us and a scatter 6.1 at 32768 positions (launch, ids, counts,
+// stores), with a third of 98 MiB of zeros each pass 14, where the zeros alone would take 5.  4096 positions of two passes: 19
+// us a call sorted by one workgroup, 30 in four launches; 8192 25 and 30; 16384 (16 keys a thread) 44 and 28.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
 constexpr int kMaxGroups = 128;                           // workgroups of a pass, so that each may add all counts up by itself
@@ -581,7 +603,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, P
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int to = mine[w][digit[j]] + rank[j];
-      if (there[j] && (unsigned)to < (unsigned)p.n) keys[to] = key[j], pos[to] = at[j];  // (inside, whatever the ids became since)
+      if (there[j] && (unsigned)to < (unsigned)p.n) keys[to] = key[j], pos[to] = at[j];  // (whatever the ids became since the count)
     }
     load(t + kTile);
     __syncthreads();
@@ -598,6 +620,10 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(T* out, int64_t rs, int6
 }
 
 // ------------------------------------------------------------------ sums of the sorted rows
+// Bound by the rows of dy, each read once where it lies: 32768 x 1024 bf16 17.9 us (67 MB of rows and 20 of sums, 4.9 TB/s),
+// 131072 x 2048 108 (537 MB, 5.2 with the sums; 149 with loads through the caches).  Eight rows ahead leave 6 waves a SIMD;
+// 16 rows ahead 19.0.  Units of 8, 16 and 32 positions: 32768 x 1024 18.5, 17.9, 21.1; 131072 x 2048 and the join behind it
+// 113 + 22, 112 + 14, 108 + 8.  A contiguous part of the groups for each XCD: 181 for 149.
 struct Sorted {
   const int *keys, *pos;
   int n, V, unit;
@@ -610,14 +636,15 @@ __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(Sorted s, Gr
   __shared__ Heads<TG> head;
   const int lane = threadIdx.x % kWave, slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
   const int64_t group = blockIdx.x / slices, one = (int64_t)slices * kWave * E;
-  add_up<STREAM, TG, TO>(List{group * kSumWaves * s.unit, s.n, s.V, s.unit}, [&](int64_t i) { return s.keys[i]; },
+  add_up<STREAM, TG, TO>(List{group * kSumWaves * s.unit, s.n, s.V, s.unit, (uint32_t)s.n - 1}, [&](int64_t i) { return s.keys[i]; },
                  [&](int64_t i) { return s.pos[i]; },
                  Sums<TG, TO>{static_cast<const TG*>(g.p) + col, g, out, out_rs, col, D, scale, add}, head,
                  partial + group * 2 * one + (slice * kWave + lane) * E, one);
 }
 
 // The runs that begin in one workgroup of the sums and end in a later one: the partial rows in their order.  The run's end is
-// found 64 workgroups at a time, and its partial rows are shared by the waves.
+// found 64 workgroups at a time, and its partial rows are shared by the waves: 4 us at 32768 positions of text, 8 where
+// a quarter of 131072 is one token (726 when one wave added its partial rows one after the other).
 template <typename TG, typename TO>
 __global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, TO* out, int64_t out_rs, const float* partial, int D,
                                                                      int slices, float scale, bool add) {
@@ -627,7 +654,7 @@ __global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, T
   const int64_t group = blockIdx.x / slices, per = (int64_t)s.unit * kSumWaves, begin = group * per, end = begin + per;
   if (end >= s.n) return;
   const int key = s.keys[end];
-  if (key >= s.V || s.keys[end - 1] != key) return;
+  if ((unsigned)key >= (unsigned)s.V || s.keys[end - 1] != key) return;
   if (begin > 0 && s.keys[begin - 1] == key) return;  // it began before
   // groups behind this one that the run reaches
   int64_t more = 1;
@@ -671,11 +698,6 @@ int bit_length(int64_t v) {
 // recorded, in one launch and sorted: 512 positions of text with 8 MiB of zeros 7.4 and 15.1, 32 MiB 13.9 and 17.2, 64 MiB 20.0 and
 // 19.5, 98 MiB 25.2 and 23.6; of one token, whose rows one workgroup adds up, 18.6 and 14.2 with 8 MiB (1024: 40 and 14).
 bool few_of(int64_t n, int64_t zeros) { return n <= kFewPositions && zeros <= (int64_t)48 << 20; }
-
-// Rows of dy, each read once, are read past the caches where they and dw are more than the caches hold of them anyway.  us a
-// call, three sets of inputs in turn, cached and past the caches: bf16, 50304 tokens, 32768 x 768 (121 MiB) 44.9 and 47.1,
-// 32768 x 1024 (162) 52.7 and 50.0, 131072 x 1024 (354) 115 and 100, 131072 x 2048 (708) 205 and 160.
-constexpr int64_t kStreamBytes = (int64_t)128 << 20;
 
 // How a call's passes and workspace are cut.
 struct Plan {

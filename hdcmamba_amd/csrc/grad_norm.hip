@@ -146,6 +146,8 @@ template <typename T, bool STREAM, typename A> __device__ __forceinline__ void n
   if (i < s.count) a.take(to_f<T>(p[i]));
 }
 
+// Bound by its one read: 2.06 GB of bf16 303 us (6.8 TB/s; 342 through the caches), 0.38 GB 58.  The conversions to 64 bits and
+// the multiply-adds fit beside it (128 KB a workgroup: the same).
 template <bool MAX, bool STREAM, int N>
 __global__ __launch_bounds__(kThreads) void norm_parts_kernel(Table<N> t, int bits, double* parts) {
   const Stretch s = stretch_of(t, bits, blockIdx.x);
@@ -174,6 +176,7 @@ template <bool MAX, int THREADS> __device__ __forceinline__ float join_parts(con
   return a.norm();
 }
 
+// 31000 parts 9 us, 5800 4.7: a chain of their arrival and two reductions.
 constexpr int kJoinThreads = 1024;
 template <bool MAX> __global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(const double* parts, int64_t n, float* norm) {
   const float v = join_parts<MAX, kJoinThreads>(parts, n);
@@ -209,7 +212,8 @@ template <typename T, bool STREAM> __device__ __forceinline__ void scale_of(cons
 // Where the norm comes from: given, or joined from its parts by every workgroup (the first writes it).
 enum From { kGiven, kParts2, kPartsMax };
 
-// Nothing is read or written where the factor is 1.
+// Nothing is read or written where the factor is 1 (3.9 us for 5800 workgroups).  0.76 GB of fp32 285 us: 5.3 TB/s of reads and
+// writes (315 through the caches); 4.2 MB 4.3.
 template <int FROM, bool STREAM, int N>
 __global__ __launch_bounds__(kThreads) void scale_kernel(Table<N> t, int bits, float* norm, const double* parts, int n_parts,
                                                          float max_norm) {
@@ -238,6 +242,7 @@ int check_tensors(const hdcm_tensor* t, int64_t n) {
   return HDCM_OK;
 }
 
+// Small lists are cut finer, into more workgroups: 4.2 MB scaled in 4.3 us instead of 7.2, its norm's parts 3.8 for 4.4.
 constexpr int64_t kSmallBytes = (int64_t)16 << 20;
 
 // What a list comes to.  Elements that are read (and written) once go past the caches where they are more than the

@@ -1120,6 +1120,7 @@ void clip_grads(const pybind11::list& list, double max_norm, const Tensor& norm_
 
 // None where no parameter has a gradient
 OptTensor clip_grad_norm(const pybind11::list& params, double max_norm, int kind) {
+  const at::NoGradGuard no_grad;  // as torch's clip_grad_norm_
   std::vector<Tensor> ts = listed(params, true);
   if (ts.empty()) return std::nullopt;
   const c10::DeviceGuard guard(ts[0].device());

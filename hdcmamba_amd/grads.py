@@ -2,8 +2,8 @@
 does between its backward and its optimizer.  The reference trains without clipping (train_fineweb.py:161-179).
 
 Tensors are float32 or bfloat16, mixed as they come, on one GPU.  Squares are added in 64 bits, so that no gradient is
-too large or too small for the norm, in a fixed order; nothing waits for the host.  No gradient of their own: a tensor
-that needs one (a backward with create_graph) is refused.
+too large or too small for the norm, in a fixed order; nothing waits for the host.  None has a gradient of its own:
+clip_grad_norm_ runs without autograd, as torch's, the others refuse a tensor that needs one.
 """
 from __future__ import annotations
 
@@ -48,7 +48,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("error_if_nonfinite waits for the norm, which a recording cannot")
         grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
-        norm = grad_norm(grads, norm_type).item()
+        with torch.no_grad():
+            norm = grad_norm(grads, norm_type).item()
         if not math.isfinite(norm):
             raise RuntimeError(f"the gradients' norm is {norm}, not finite: they are not clipped")
     norm = _ops.native().clip_grad_norm(parameters, max_norm, kind)

@@ -194,6 +194,45 @@ def test_gradient_layouts(dev, dtype):
     check_grad(hm.embedding_grad(ids[0, 0].to(dev), dy[0, 0].to(dev), V), *grad64(ids[0, 0], dy[0, 0], V))
 
 
+@pytest.mark.parametrize("T", [511, 512, 513, 8191, 8192, 8193])
+@pytest.mark.parametrize("V", [511, 512, 50304])
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_gradient_on_either_side_of_its_ways(dev, T, V, dtype):
+    """Sizes around the last call that is one launch and the last that one workgroup sorts; the zeros of tokens that do not occur are
+    zeros under any scale; accumulating in every way."""
+    _say("gradient ways", T, V, dtype)
+    D = 520
+    ids = make_ids("text", T, V, seed=T)
+    dy = torch.randn(T, D, generator=gen(T)).to(dtype)
+    for scale in (1.0, -0.5, float("inf")):
+        got = hm.embedding_grad(ids.to(dev), dy.to(dev), V, scale=scale).cpu()
+        absent = torch.bincount(ids, minlength=V) == 0
+        zeros = got[absent]
+        assert torch.equal(zeros.view(torch.int32 if dtype == FP else torch.int16), torch.zeros_like(zeros, dtype=torch.int32 if dtype == FP else torch.int16))
+        if scale != float("inf"):
+            check_grad(got, *grad64(ids, dy, V, scale))
+    old = torch.randn(V, D, generator=gen(1)).to(dtype)
+    out = old.to(dev)
+    hm.embedding_grad(ids.to(dev), dy.to(dev), V, out=out, accumulate=True)
+    ref, off = grad64(ids, dy, V)
+    assert torch.equal(out.cpu()[absent], old[absent])
+    check_grad(out, ref + old.double(), off + U * (ref.abs() + old.double().abs() + off))
+
+
+def test_rows_past_the_caches(dev):
+    """Lookups and gradients of more than the caches hold, and units of 32 positions."""
+    T, D, V = 70000, 1030, 40000
+    ids, w = make_ids("text", T, V).to(dev), torch.randn(V, D, generator=gen(1)).to(BF).to(dev)
+    assert torch.equal(hm.embedding(ids, w), w[ids])
+    dy = torch.randn(T, D, generator=gen(2)).to(BF)
+    check_grad(hm.embedding_grad(ids, dy.to(dev), V), *grad64(ids.cpu(), dy, V))
+    T, D = 540000, 8
+    ids = make_ids("two", T, V)
+    ids[::3] = make_ids("text", T, V)[::3]
+    dy = torch.randn(T, D, generator=gen(3))
+    check_grad(hm.embedding_grad(ids.to(dev), dy.to(dev), V), *grad64(ids, dy, V))
+
+
 def test_gradient_of_nothing(dev):
     none = torch.zeros(3, 0, dtype=torch.long, device=dev)
     for dtype in (FP, BF):
@@ -481,6 +520,11 @@ def test_norm_refusals(dev):
         hm.grad_norm([x.clone().requires_grad_()])
     with torch.no_grad():
         hm.grad_norm([x.clone().requires_grad_()])
+    p = nn.Parameter(x.clone())
+    p.pow(3).sum().backward(create_graph=True)  # a gradient that needs one: clipped without autograd, as by torch
+    assert p.grad.requires_grad and abs(hm.clip_grad_norm_(p, 1.0).item() - 360 ** 0.5) < 1e-4
+    assert abs(p.grad.norm().item() - 1) < 1e-5
+    p.grad = None
     for bad in (x[::2], x[:1].expand(9)):
         with pytest.raises(RuntimeError, match="gaps or overlaps"):
             hm.clip_grads_([bad], 1.0, 2.0)
