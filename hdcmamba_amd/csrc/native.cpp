@@ -1032,39 +1032,50 @@ Tensor embedding_grad(const Tensor& ids, const Tensor& grad, int64_t V, double s
 }
 
 // ------------------------------------------------------------------------ the gradients' norm
-// The tensors of a Python list, or (of parameters) their gradients.  A caster to a vector would take 0.1 us for each, and a
-// parameter's .grad in Python as much.
-std::vector<Tensor> listed(const pybind11::list& list, bool grads) {
-  std::vector<Tensor> ts;
-  ts.reserve(list.size());
-  for (const pybind11::handle item : list) {
-    TORCH_CHECK_TYPE(THPVariable_Check(item.ptr()), "a list of tensors is expected, got a ", Py_TYPE(item.ptr())->tp_name);
-    const Tensor& t = THPVariable_Unpack(item.ptr());
-    if (!grads) ts.push_back(t);
-    else if (t.grad().defined()) ts.push_back(t.grad());
-  }
-  return ts;
-}
-
-// Tensors on one device as the library's, copied to be dense where `copies` lets them.
+// The tensors of a Python list, or (of parameters) their gradients, on one device, as the library's; tensors with gaps are
+// copied where nothing is written.  The list may hold hundreds: they are taken as they lie in it, without a caster, a
+// reference or a .grad in Python for each (0.1 us apiece).
 struct TensorList {
   std::vector<hdcm_tensor> refs;
+  std::vector<const Tensor*> ts;  // the list's, which outlives the call
   std::vector<Tensor> held;
-  TensorList(const std::vector<Tensor>& ts, const char* op, bool copies) {
-    refs.reserve(ts.size());
-    for (const Tensor& t : ts) {
-      no_gradient(op, {&t});
-      TORCH_CHECK(t.layout() == at::kStrided, op, ": a tensor is ", t.layout(), "; the kernels take dense ones");
-      on_gpu(t);
-      same_device(t, ts[0], "a tensor");
-      const int dt = dtype_of(t);
-      const bool dense = t.is_non_overlapping_and_dense();
-      TORCH_CHECK(dense || copies, op, ": a tensor of shape ", t.sizes(), " and strides ", t.strides(),
-                  " has gaps or overlaps in memory and cannot be scaled in place");
-      if (!dense) held.push_back(t.detach().contiguous());
-      refs.push_back({const_cast<void*>((dense ? t : held.back()).const_data_ptr()), t.numel(), dt});
+  const char* op;
+
+  static const Tensor& item(const pybind11::list& list, size_t i) {
+    PyObject* const o = PyList_GET_ITEM(list.ptr(), i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "a list of tensors is expected, got a ", Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+  }
+  TensorList(const pybind11::list& list, const char* name, bool grads) : op(name) {
+    ts.reserve(list.size());
+    for (size_t i = 0; i < list.size(); ++i) {
+      const Tensor& t = item(list, i);
+      if (!grads) ts.push_back(&t);
+      else if (t.grad().defined()) ts.push_back(&t.grad());
     }
   }
+  bool empty() const { return ts.empty(); }
+  const Tensor& first() const { return *ts[0]; }
+  void refer(bool write) {
+    const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    const auto device = first().device();
+    on_gpu(first());
+    refs.clear();
+    refs.reserve(ts.size());
+    for (const Tensor* p : ts) {
+      const Tensor& t = *p;
+      if (t.unsafeGetTensorImpl()->autograd_meta() && ((backward && t.requires_grad()) || forward)) no_gradient(op, {p});
+      TORCH_CHECK(t.layout() == at::kStrided, op, ": a tensor is ", t.layout(), "; the kernels take dense ones");
+      if (t.device() != device) on_gpu(t), same_device(t, first(), "a tensor");
+      const int dt = dtype_of(t);
+      const bool dense = t.is_non_overlapping_and_dense();
+      TORCH_CHECK(dense || !write, op, ": a tensor of shape ", t.sizes(), " and strides ", t.strides(),
+                  " has gaps or overlaps in memory and cannot be scaled in place");
+      if (!dense) held.push_back(t.detach().contiguous());
+      refs.push_back({write ? t.mutable_data_ptr() : const_cast<void*>((dense ? t : held.back()).const_data_ptr()), t.numel(), dt});
+    }
+  }
+  int64_t size() const { return (int64_t)refs.size(); }
   // Whether no two of them, and not the norm that is read while they are scaled, share memory
   bool apart(const Tensor* norm) const {
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
@@ -1079,6 +1090,9 @@ struct TensorList {
       if (spans[i].first < spans[i - 1].second) return false;
     return true;
   }
+  void all_written() const {
+    for (const Tensor* t : ts) written(*t);
+  }
 };
 constexpr const char* kNotApart = ": tensors share memory, with each other or with the norm";
 
@@ -1087,57 +1101,57 @@ struct NormWorkspace {
   size_t n;
   c10::DataPtr p;
   explicit NormWorkspace(const TensorList& l)
-      : n(hdcm_grad_norm_workspace_bytes(l.refs.data(), (int64_t)l.refs.size())),
+      : n(hdcm_grad_norm_workspace_bytes(l.refs.data(), l.size())),
         p(n ? c10::hip::HIPCachingAllocator::get()->allocate(n) : c10::DataPtr()) {}
 };
 
 Tensor grad_norm(const pybind11::list& list, int kind) {
-  const std::vector<Tensor> ts = listed(list, false);
-  TORCH_CHECK(!ts.empty(), "grad_norm: no tensors");
-  const c10::DeviceGuard guard(ts[0].device());
-  const TensorList l(ts, "grad_norm", true);
-  Tensor out = fresh({}, at::kFloat, ts[0]);
+  TensorList l(list, "grad_norm", false);
+  TORCH_CHECK(!l.empty(), "grad_norm: no tensors");
+  const c10::DeviceGuard guard(l.first().device());
+  l.refer(false);
+  Tensor out = fresh({}, at::kFloat, l.first());
   const NormWorkspace ws(l);
-  check("hdcm_grad_norm", hdcm_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, out.mutable_data_ptr<float>(), ws.p.get(), ws.n,
-                                         stream_of(out)));
+  check("hdcm_grad_norm",
+        hdcm_grad_norm(l.refs.data(), l.size(), kind, out.mutable_data_ptr<float>(), ws.p.get(), ws.n, stream_of(out)));
   return out;
 }
 
 void clip_grads(const pybind11::list& list, double max_norm, const Tensor& norm_) {
-  const std::vector<Tensor> ts = listed(list, false);
-  if (ts.empty()) return;
-  const c10::DeviceGuard guard(ts[0].device());
-  const TensorList l(ts, "clip_grads_", false);
-  same_device(norm_, ts[0], "total_norm");
+  TensorList l(list, "clip_grads_", false);
+  if (l.empty()) return;
+  const c10::DeviceGuard guard(l.first().device());
+  l.refer(true);
+  same_device(norm_, l.first(), "total_norm");
   TORCH_CHECK(norm_.numel() == 1 && norm_.is_floating_point(), "total_norm must be one floating-point number, got ", norm_.scalar_type(),
               " ", norm_.sizes());
   TORCH_CHECK(l.apart(&norm_), "clip_grads_", kNotApart);
   const Tensor norm = as_type(norm_.detach(), at::kFloat);
-  check("hdcm_grad_scale", hdcm_grad_scale(l.refs.data(), (int64_t)l.refs.size(), norm.const_data_ptr<float>(), (float)max_norm,
-                                           stream_of(norm)));
-  for (const Tensor& t : ts) written(t);
+  check("hdcm_grad_scale",
+        hdcm_grad_scale(l.refs.data(), l.size(), norm.const_data_ptr<float>(), (float)max_norm, stream_of(norm)));
+  l.all_written();
 }
 
 // None where no parameter has a gradient
 OptTensor clip_grad_norm(const pybind11::list& params, double max_norm, int kind) {
   const at::NoGradGuard no_grad;  // as torch's clip_grad_norm_
-  std::vector<Tensor> ts = listed(params, true);
-  if (ts.empty()) return std::nullopt;
-  const c10::DeviceGuard guard(ts[0].device());
-  TensorList l(ts, "clip_grad_norm_", false);
+  TensorList l(params, "clip_grad_norm_", true);
+  if (l.empty()) return std::nullopt;
+  const c10::DeviceGuard guard(l.first().device());
+  l.refer(true);
   if (!l.apart(nullptr)) {  // a parameter that is given twice counts once
-    std::vector<Tensor> once;
-    for (const Tensor& t : ts)
-      if (std::none_of(once.begin(), once.end(), [&](const Tensor& o) { return o.is_same(t); })) once.push_back(t);
-    ts = std::move(once);
-    l = TensorList(ts, "clip_grad_norm_", false);
+    std::vector<const Tensor*> once;
+    for (const Tensor* t : l.ts)
+      if (std::none_of(once.begin(), once.end(), [&](const Tensor* o) { return o->is_same(*t); })) once.push_back(t);
+    l.ts = std::move(once);
+    l.refer(true);
     TORCH_CHECK(l.apart(nullptr), "clip_grad_norm_", kNotApart);
   }
-  Tensor out = fresh({}, at::kFloat, ts[0]);
+  Tensor out = fresh({}, at::kFloat, l.first());
   const NormWorkspace ws(l);
-  check("hdcm_clip_grad_norm", hdcm_clip_grad_norm(l.refs.data(), (int64_t)l.refs.size(), kind, (float)max_norm,
-                                                   out.mutable_data_ptr<float>(), ws.p.get(), ws.n, stream_of(out)));
-  for (const Tensor& t : ts) written(t);
+  check("hdcm_clip_grad_norm", hdcm_clip_grad_norm(l.refs.data(), l.size(), kind, (float)max_norm, out.mutable_data_ptr<float>(),
+                                                   ws.p.get(), ws.n, stream_of(out)));
+  l.all_written();
   return out;
 }
 
