@@ -616,16 +616,18 @@ def train_bench(args, torch, cfg, make_lm, lm_input, dev):
     """Training steps of the headline LM as the reference's trainer runs them
     (train_fineweb.py:161-179): bf16 model under autocast, cross-entropy on fp32 logits,
     backward, AdamW step.  `--differentiable-mixer` also trains in_proj, the LN+conv, A_log
-    and the GroupNorm (the reference's kernels have no backward)."""
+    and the GroupNorm (the reference's kernels have no backward); `--max-grad-norm` clips the
+    gradients' norm before the AdamW step (the reference does not)."""
     import torch.nn.functional as F
-    from hdcmamba_amd import set_differentiable_mixer
+    from hdcmamba_amd import clip_grad_norm_, set_differentiable_mixer
 
     L = cfg["L"]
     steps = args.steps if args.steps != 10 else 3
     warm = max(args.warmup if args.warmup != 3 else 2, 1)
     lm = make_lm("lm_c4").to(torch.bfloat16).to(dev).train()
     set_differentiable_mixer(lm, args.differentiable_mixer)
-    opt = torch.optim.AdamW(lm.parameters(), lr=1e-4, betas=(0.9, 0.95), weight_decay=0.1)
+    params = list(lm.parameters())
+    opt = torch.optim.AdamW(params, lr=1e-4, betas=(0.9, 0.95), weight_decay=0.1)
     ids = lm_input("lm_c4", B=cfg["B"], L=L + 1).to(dev)
 
     def step():
@@ -634,6 +636,8 @@ def train_bench(args, torch, cfg, make_lm, lm_input, dev):
             logits = lm(ids[:, :-1])
             loss = F.cross_entropy(logits.view(-1, logits.size(-1)).float(), ids[:, 1:].reshape(-1))
         loss.backward()
+        if args.max_grad_norm:
+            clip_grad_norm_(params, args.max_grad_norm)
         opt.step()
         return loss
 
@@ -653,6 +657,7 @@ def train_bench(args, torch, cfg, make_lm, lm_input, dev):
         "vs_baseline": None, "dtype": "bf16", "data": "synthetic: uniform random token ids, random-init weights",
         "config": {"workload": "24-layer d_model=1024 HdcMamba LM training step, B=1, L=32768",
                    "differentiable_mixer": bool(args.differentiable_mixer), "optimizer": "AdamW",
+                   **({"max_grad_norm": args.max_grad_norm} if args.max_grad_norm else {}),
                    "loss": "cross-entropy on fp32 logits (train_fineweb.py:170-171)"},
         "loss": round(float(loss), 4),
         "peak_memory_GiB": round(torch.cuda.max_memory_allocated() / 2 ** 30, 1),
@@ -668,6 +673,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--differentiable-mixer", action="store_true",
                     help="lm_c4_train: train the SSM, slot and gate parameters too")
+    ap.add_argument("--max-grad-norm", type=float, default=0.0,
+                    help="lm_c4_train: clip the gradients' norm to this before the AdamW step (0: no clipping)")
     ap.add_argument("--workload", default="lm_c4",
                     choices=["lm_c4", "lm_c3", "block_c1", "block_c2", "lm_c5_decode", "lm_c4_train"],
                     help="lm_c5_decode: 48-layer d_model=2048 LM, prefill B=16 x 8192, then timed "
