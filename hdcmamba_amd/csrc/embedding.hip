@@ -653,18 +653,20 @@ __global__ __launch_bounds__(kSumThreads) void embedding_join_kernel(Sorted s, T
   const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
   const int64_t group = blockIdx.x / slices, per = (int64_t)s.unit * kSumWaves, begin = group * per, end = begin + per;
   if (end >= s.n) return;
-  const int key = s.keys[end];
-  if ((unsigned)key >= (unsigned)s.V || s.keys[end - 1] != key) return;
-  if (begin > 0 && s.keys[begin - 1] == key) return;  // it began before
-  // groups behind this one that the run reaches
-  int64_t more = 1;
-  for (;; more += kWave) {
-    const int64_t at = end + (more + lane) * per;  // the first position behind the group that it may reach
-    const uint64_t ends = __ballot(at >= s.n || s.keys[min(at, (int64_t)s.n - 1)] != key);
+  // all keys that most groups need at once: the run at the group's end, where it begins, how far it reaches
+  const int key = s.keys[end], at_end = s.keys[end - 1], at_begin = begin > 0 ? s.keys[begin - 1] : -1;
+  int64_t more = 1;  // groups behind this one that the run reaches
+  const auto reach = [&] { return end + (more + lane) * per; };  // the first position behind the group that it may reach
+  int reached = s.keys[min(reach(), (int64_t)s.n - 1)];
+  if ((unsigned)key >= (unsigned)s.V || at_end != key || at_begin == key) return;  // none, or it began before
+  for (;;) {
+    const uint64_t ends = __ballot(reach() >= s.n || reached != key);
     if (ends) {
       more += __builtin_ctzll(ends);
       break;
     }
+    more += kWave;
+    reached = s.keys[min(reach(), (int64_t)s.n - 1)];
   }
   const int slice = blockIdx.x % slices, col = (slice * kWave + lane) * E;
   const int64_t one = (int64_t)slices * kWave * E, two = 2 * one;
