@@ -91,7 +91,7 @@ class Embedding(nn.Embedding):
     """nn.Embedding on these kernels, its rows times ``scale``: the same constructor, parameters and initial values.
 
     What the kernels do not take goes through nn.Embedding's own forward: weights on the CPU or of other types, max_norm,
-    sparse and scale_grad_by_freq, and forward-mode differentiation."""
+    sparse and scale_grad_by_freq, forward-mode differentiation and torch.func's transforms (vmap)."""
 
     def __init__(self, *args, scale=1.0, **kwargs):
         super().__init__(*args, **kwargs)
@@ -100,7 +100,8 @@ class Embedding(nn.Embedding):
     def forward(self, ids):
         w = self.weight
         if (not w.is_cuda or w.dtype not in _ops._DTYPES or self.max_norm is not None or self.sparse
-                or self.scale_grad_by_freq or forward_ad._current_level >= 0):
+                or self.scale_grad_by_freq or forward_ad._current_level >= 0
+                or torch._C._functorch.maybe_current_level() is not None):
             y = super().forward(ids)
             return y if self.scale == 1.0 else y * self.scale
         return embedding(ids, w, self.scale, self.padding_idx)

@@ -233,6 +233,21 @@ def test_rows_past_the_caches(dev):
     check_grad(hm.embedding_grad(ids.to(dev), dy.to(dev), V), *grad64(ids, dy, V))
 
 
+@pytest.mark.parametrize("L", [301, 3001])
+def test_gradient_layouts_of_many(dev, L):
+    """Behind a left padding, broadcast over sequences or positions, added to a given fp32 gradient: sorted by one workgroup and by many."""
+    B, D, V = 3, 72, 500
+    ids = make_ids("text", B * L, V).view(B, L)
+    base = torch.randn(B, L + 9, D + 8, generator=gen(1)).to(BF)
+    views = lambda t: (t[:, 9:, :D], t[:1, 9:, 3:D + 3].expand(B, L, D), t[:, :1, :D].expand(B, L, D))  # noqa: E731
+    for dy, on in zip(views(base), views(base.to(dev))):
+        ref, off = grad64(ids, dy, V)
+        check_grad(hm.embedding_grad(ids.to(dev), on, V), ref, off)
+        old = torch.randn(V, D, generator=gen(2))
+        total = hm.embedding_grad(ids.to(dev), on, V, out=old.to(dev), accumulate=True)
+        check_grad(total, ref + old.double(), off + U * (ref.abs() + old.double().abs() + off))
+
+
 def test_gradient_of_nothing(dev):
     none = torch.zeros(3, 0, dtype=torch.long, device=dev)
     for dtype in (FP, BF):
@@ -310,8 +325,11 @@ def test_embedding_module(dev):
     h = hm.Embedding(20, 6, scale=2.0).to(dev)
     y, dy = torch.func.jvp(lambda w: torch.func.functional_call(h, {"weight": w}, (ids % 20,)), (h.weight.detach(),), (torch.ones(20, 6, device=dev),))
     assert torch.equal(y, h(ids % 20)) and bool(dy.eq(2).all())
-    g = torch.func.grad(lambda w: torch.func.functional_call(h, {"weight": w}, (ids % 20,)).sum())(h.weight.detach())
-    assert torch.equal(g, 2 * F.one_hot(ids.flatten() % 20, 20).sum(0).float()[:, None].expand(20, 6))
+    want = 2 * F.one_hot(ids.flatten() % 20, 20).sum(0).float()[:, None].expand(20, 6)
+    for lookup in (lambda w, i: torch.func.functional_call(h, {"weight": w}, (i,)), lambda w, i: hm.embedding(i, w, 2.0)):
+        assert torch.equal(torch.func.grad(lambda w: lookup(w, ids % 20).sum())(h.weight.detach()), want)
+    per = torch.func.vmap(torch.func.grad(lambda w, i: torch.func.functional_call(h, {"weight": w}, (i,)).sum()), (None, 0))
+    assert torch.equal(per(h.weight.detach(), ids % 20).sum(0), want)  # a gradient for each sequence
 
 
 def test_ids_written_between_forward_and_backward(dev):
@@ -588,7 +606,7 @@ def test_recorded(dev):
             hm.clip_grads_([dw, more], 1.0, norm)
             return y, dw, more, norm
 
-    recs = [Rec(3000), Rec(90)]
+    recs = [Rec(3000), Rec(90), Rec(9000)]
     for turn in range(4):
         for k, r in enumerate(recs):
             r.ids.copy_(make_ids("text" if turn % 2 else "same", r.ids.numel(), V, seed=turn))
@@ -597,6 +615,48 @@ def test_recorded(dev):
             r.graph.replay()
         for r in recs:
             assert all(torch.equal(a, b) for a, b in zip(r.out, r.run()))
+
+
+def test_recorded_step(dev):
+    """Forward, backward and clipping of an embedding with a tied head in one recording, replayed with new ids, against the same
+    step run eagerly on a copy."""
+    V, D, T = 600, 128, 1500
+
+    def make():
+        e = hm.Embedding(V, D, scale=2.0).to(BF).to(dev)
+        torch.nn.init.normal_(e.weight, std=0.1)
+        return e
+
+    torch.manual_seed(3)
+    e = make()
+    ids = torch.zeros(T, dtype=torch.long, device=dev)
+
+    def step(m, i):
+        m.weight.grad = None
+        y = m(i)
+        (y.float() @ m.weight.float().t()).logsumexp(1).mean().backward()
+        return y.detach(), hm.clip_grad_norm_(m.parameters(), 1e-3)
+
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(e, ids)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    torch.cuda.synchronize()
+    e.weight.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y, norm = step(e, ids)
+    grad = e.weight.grad
+    for turn in range(4):
+        ids.copy_(make_ids("text" if turn % 2 else "wild", T, V, seed=turn))
+        graph.replay()
+        other = make()
+        other.weight.data.copy_(e.weight)
+        y2, norm2 = step(other, ids)
+        assert torch.equal(y, y2) and torch.equal(norm, norm2) and torch.equal(grad, other.weight.grad)
+        assert norm > 1e-3
 
 
 def _lm(dev, dtype=BF, mixer=True):
