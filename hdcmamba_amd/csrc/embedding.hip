@@ -430,12 +430,14 @@ __global__ __launch_bounds__(kSumThreads) void embedding_few_kernel(Ids ids, int
 // scatters its stretch of the list behind the keys of lower digits and those of the same digit in the stretches
 // before, which a launch before has counted.  Up to kOneGroup positions are one workgroup's work: all passes in LDS, in one
 // launch.
-// Bound by latency: without zeros to write a count takes 3.4 us and a scatter 6.1 at 32768 positions (launch, ids, counts,
-// stores), with a third of 98 MiB of zeros each pass 14, where the zeros alone would take 5.  4096 positions of two passes: 19
-// us a call sorted by one workgroup, 30 in four launches; 8192 25 and 30; 16384 (16 keys a thread) 44 and 28.
+// Bound by latency: without zeros to write a count takes 3 us and a scatter 5 at 32768 positions (launch, ids, counts,
+// stores); 98 MiB of zeros, which alone take 15, make two passes 9 us longer (all with the scatters; a third of them with the
+// counts 11).  us a call of 32768 x 1024, 131072 x 1024 and 1048576 x 64 of 50304 tokens: one key a thread 45.1, 99, 223 (64
+// groups), two 47.5, 97, 177, in up to 256 groups 169, in 512 229.  4096 positions of two passes: 19 us a call sorted by one
+// workgroup, 27 in four launches; 8192 24 and 27; 16384 (16 keys a thread) 44 and 27.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kTile = 2048, kPer = kTile / kSortThreads;  // keys of a workgroup's round, and of a thread in it
-constexpr int kMaxGroups = 128;                           // workgroups of a pass, so that each may add all counts up by itself
+constexpr int kMaxGroups = 256;    // workgroups of a pass, so that each may add all counts up by itself
+constexpr int kOneKeyGroups = 64;  // up to so many take one key a thread in a round, more take two
 constexpr int kCountAhead = 16;                           // keys or counts of a thread in flight
 constexpr int kOnePer = 8, kOneGroup = kOnePer * kSortThreads;
 
@@ -524,12 +526,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids ids, int n, 
     }
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pass p, int* counts, Fill fill) {
+template <int kPer> __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pass p, int* counts) {
+  constexpr int kTile = kPer * kSortThreads;
   __shared__ int count[kBins];
-  if ((int)blockIdx.x >= p.groups) {
-    fill_part(fill, (int)blockIdx.x - p.groups);
-    return;
-  }
   const int tid = threadIdx.x;
   if (tid < kBins) count[tid] = 0;
   __syncthreads();
@@ -549,8 +548,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortIn in, Pas
   if (tid < kBins) counts[blockIdx.x * kBins + tid] = count[tid];
 }
 
+template <int kPer>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortIn in, Pass p, const int* counts, int* keys, int* pos,
                                                                     Fill fill) {
+  constexpr int kTile = kPer * kSortThreads;
   __shared__ int sums[kSortWaves];
   __shared__ int mine[kSortWaves][kBins];  // a wave's keys of a digit, then where its first goes
   if ((int)blockIdx.x >= p.groups) {
@@ -704,7 +705,7 @@ bool few_of(int64_t n, int64_t zeros) { return n <= kFewPositions && zeros <= (i
 // How a call's passes and workspace are cut.
 struct Plan {
   int few_groups, few_bits;                   // few positions
-  int passes, bits, groups, stretch;          // sorting
+  int passes, bits, keys, groups, stretch;    // sorting
   int slices, unit;
   bool stream;
   int64_t sum_groups;
@@ -723,8 +724,9 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   const int bits = bit_length(V);  // of the largest key, V
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.bits = (bits + p.passes - 1) / p.passes;
-  const int64_t tiles = (n + kTile - 1) / kTile;
-  p.stretch = (int)((tiles + kMaxGroups - 1) / kMaxGroups * kTile);
+  p.keys = n <= kOneKeyGroups * kSortThreads ? 1 : 2;
+  const int64_t tile = p.keys * kSortThreads, tiles = (n + tile - 1) / tile;
+  p.stretch = (int)((tiles + kMaxGroups - 1) / kMaxGroups * tile);
   p.groups = (int)((n + p.stretch - 1) / p.stretch);
   // two workgroups a CU at least; where there are many, longer units leave fewer partial rows
   const int64_t groups = (n + kAhead * kSumWaves - 1) / (kAhead * kSumWaves) * p.slices;
@@ -831,31 +833,29 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   for (int i = 0; i < 4; ++i, at += p.list) lists[i] = (int*)at;
   int* counts = (int*)at;
   float* part = (float*)(at + p.counts);
-  // the zeros go with the sorting launches: a share for a count, two for a scatter
+  // the zeros go with the sorting launches: with all scatters alike
   const bool apart = dw_row_stride != D && V > 1;
   if (!accumulate && apart) launch_zeros(dw, dw_row_stride, V, D, dw_dtype, s);
   const int64_t zeros = accumulate || apart ? 0 : V * D * hdcm_elt_size(dw_dtype);
-  const int shares = 3 * p.passes;
-  int shared = 0;
-  const auto fill_share = [&](int share) {
-    const auto bytes = [&](int k) { return k == shares ? zeros : zeros / shares * k / 16 * 16; };
-    const Fill f{(char*)dw, bytes(shared), bytes(shared + share)};
-    shared += share;
-    return f;
+  const auto fill_of = [&](int k, int n) {
+    const auto upto = [&](int i) { return i == n ? zeros : zeros / n * i / 16 * 16; };
+    return Fill{(char*)dw, upto(k), upto(k + 1)};
   };
   const auto grid = [&](int groups, const Fill& f) { return dim3((unsigned)(groups + (f.end - f.begin + kFillBytes - 1) / kFillBytes)); };
   SortIn in{keys_of, nullptr, nullptr};
   if (n <= kOneGroup) {
-    const Fill f = fill_share(shares);
+    const Fill f = fill_of(0, 1);
     HDCM_LAUNCH(sort_one_kernel, grid(1, f), dim3(kSortThreads), 0, s, keys_of, n, p.passes, p.bits, lists[0], lists[1], f);
     in.keys = lists[0], in.pos = lists[1];
   } else {
+    const auto count = p.keys == 1 ? sort_count_kernel<1> : sort_count_kernel<2>;
+    const auto scatter = p.keys == 1 ? sort_scatter_kernel<1> : sort_scatter_kernel<2>;
     for (int k = 0; k < p.passes; ++k) {
       int *keys = lists[2 * (k & 1)], *pos = lists[2 * (k & 1) + 1];
       const Pass pass{n, p.stretch, p.groups, k * p.bits, p.bits};
-      const Fill first = fill_share(1), second = fill_share(2);
-      HDCM_LAUNCH(sort_count_kernel, grid(p.groups, first), dim3(kSortThreads), 0, s, in, pass, counts, first);
-      HDCM_LAUNCH(sort_scatter_kernel, grid(p.groups, second), dim3(kSortThreads), 0, s, in, pass, (const int*)counts, keys, pos, second);
+      const Fill f = fill_of(k, p.passes);
+      HDCM_LAUNCH(count, dim3(p.groups), dim3(kSortThreads), 0, s, in, pass, counts);
+      HDCM_LAUNCH(scatter, grid(p.groups, f), dim3(kSortThreads), 0, s, in, pass, (const int*)counts, keys, pos, f);
       in.keys = keys, in.pos = pos;
     }
   }
