@@ -728,9 +728,9 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
   const int64_t tile = p.keys * kSortThreads, tiles = (n + tile - 1) / tile;
   p.stretch = (int)((tiles + kMaxGroups - 1) / kMaxGroups * tile);
   p.groups = (int)((n + p.stretch - 1) / p.stretch);
-  // two workgroups a CU at least; where there are many, longer units leave fewer partial rows
+  // two workgroups a CU at least (32768 x 256: 32.8 us a call for 34.8); where there are many, longer units leave fewer partial rows
   const int64_t groups = (n + kAhead * kSumWaves - 1) / (kAhead * kSumWaves) * p.slices;
-  p.unit = kAhead * (groups < 512 ? 1 : groups < 8192 ? 2 : 4);
+  p.unit = kAhead * (groups <= 512 ? 1 : groups < 8192 ? 2 : 4);
   p.stream = (n + V) * D * hdcm_elt_size(dtype) > kStreamBytes;
   p.sum_groups = (n + p.unit * kSumWaves - 1) / (p.unit * kSumWaves);
   const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
