@@ -22,7 +22,9 @@ constexpr int64_t kMaxCount = (int64_t)1 << 30;  // elements of an entry; a long
 // Entry i: `size` elements (and, in the highest bit, their type) at the address hi[i] : lo[i].  Arrays of words, for the
 // lanes of a wave to read.
 template <int N> struct Table {
+  static constexpr int kRows = (N + kWave - 1) / kWave;
   uint32_t lo[N], hi[N], size[N];  // entries behind the last have size 0
+  uint32_t before[kRows];          // workgroups of the entries before every kWave-th; all bits behind the last
 };
 
 // A workgroup's stretch: `count` elements from `data` on.
@@ -34,34 +36,32 @@ struct Stretch {
 // log2 of the elements in a stretch of 2^bits bytes
 __host__ __device__ __forceinline__ int stretch_shift(int bits, bool f32) { return f32 ? bits - 2 : bits - 1; }
 
-// Every wave looks its workgroup's entry up: the entries' workgroups are added up over the lanes, 64 entries at a time.
+// Every wave looks its workgroup's entry up: the workgroups of the kWave entries among which it is are added up over the
+// lanes.
 template <int N> __device__ __forceinline__ Stretch stretch_of(const Table<N>& t, int bits, uint32_t group) {
   const int lane = threadIdx.x % kWave;
-  uint32_t done = 0;  // workgroups of the entries before
-  Stretch s{nullptr, 0, false};
-  for (int i0 = 0; i0 < N; i0 += kWave) {
-    const int i = i0 + lane;
-    const uint32_t size = i < N ? t.size[i] : 0;
-    const int shift = stretch_shift(bits, size & kIsF32);
-    const uint32_t groups = ((size & ~kIsF32) + (1u << shift) - 1) >> shift;
-    uint32_t up_to = groups;  // of the lanes up to this one
+  int row = 0;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const uint32_t up = __shfl_up(up_to, o, kWave);
-      up_to += lane >= o ? up : 0;
-    }
-    const uint64_t behind = __ballot(group < done + up_to);
-    if (behind) {  // its first lane has the entry
-      const int at = __builtin_ctzll(behind);
-      const uint32_t first = __builtin_amdgcn_readlane(done + up_to - groups, at), whole = __builtin_amdgcn_readlane(size, at);
-      s.f32 = whole & kIsF32;
-      const uint32_t begin = (group - first) << stretch_shift(bits, s.f32);
-      s.data = (char*)((uint64_t)t.hi[i0 + at] << 32 | t.lo[i0 + at]) + ((uint64_t)begin << (s.f32 ? 2 : 1));
-      s.count = min((whole & ~kIsF32) - begin, 1u << stretch_shift(bits, s.f32));
-      return s;
-    }
-    done += __builtin_amdgcn_readlane(up_to, kWave - 1);
+  for (int r = 1; r < Table<N>::kRows; ++r) row = group >= t.before[r] ? r : row;
+  const int i = row * kWave + lane;
+  const uint32_t size = i < N ? t.size[i] : 0;
+  const int shift = stretch_shift(bits, size & kIsF32);
+  const uint32_t groups = ((size & ~kIsF32) + (1u << shift) - 1) >> shift;
+  uint32_t up_to = groups;  // of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t up = __shfl_up(up_to, o, kWave);
+    up_to += lane >= o ? up : 0;
   }
+  const uint64_t behind = __ballot(group - t.before[row] < up_to);  // its first lane has the entry
+  Stretch s{nullptr, 0, false};
+  if (!behind) return s;
+  const int at = __builtin_ctzll(behind);
+  const uint32_t first = __builtin_amdgcn_readlane(up_to - groups, at), whole = __builtin_amdgcn_readlane(size, at);
+  s.f32 = whole & kIsF32;
+  const uint32_t begin = (group - t.before[row] - first) << stretch_shift(bits, s.f32);
+  s.data = (char*)((uint64_t)t.hi[row * kWave + at] << 32 | t.lo[row * kWave + at]) + ((uint64_t)begin << (s.f32 ? 2 : 1));
+  s.count = min((whole & ~kIsF32) - begin, 1u << stretch_shift(bits, s.f32));
   return s;
 }
 
@@ -212,12 +212,11 @@ template <typename T, bool STREAM> __device__ __forceinline__ void scale_of(cons
 // Where the norm comes from: given, or joined from its parts by every workgroup (the first writes it).
 enum From { kGiven, kParts2, kPartsMax };
 
-// Nothing is read or written where the factor is 1 (3.9 us for 5800 workgroups).  0.76 GB of fp32 285 us: 5.3 TB/s of reads and
+// Nothing is read or written where the factor is 1 (4.4 us for 5800 workgroups; 7.0 with the table's entry looked up first).  0.76 GB of fp32 285 us: 5.3 TB/s of reads and
 // writes (315 through the caches); 4.2 MB 4.3.
 template <int FROM, bool STREAM, int N>
 __global__ __launch_bounds__(kThreads) void scale_kernel(Table<N> t, int bits, float* norm, const double* parts, int n_parts,
                                                          float max_norm) {
-  const Stretch s = stretch_of(t, bits, blockIdx.x);  // while the norm arrives
   float total;
   if constexpr (FROM == kGiven) {
     total = *norm;
@@ -227,6 +226,7 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table<N> t, int bits, f
   }
   const float ratio = max_norm / (total + 1e-6f), factor = ratio > 1.f ? 1.f : ratio;  // a NaN stays one
   if (factor == 1.f) return;
+  const Stretch s = stretch_of(t, bits, blockIdx.x);
   if (s.f32) scale_of<float, STREAM>(s, factor);
   else scale_of<bf16_t, STREAM>(s, factor);
 }
@@ -272,6 +272,7 @@ template <int N, typename F> void each_table(const hdcm_tensor* t, int64_t n, in
   uint32_t groups = 0;
   const auto flush = [&] {
     for (int i = held; i < N; ++i) table.lo[i] = table.hi[i] = table.size[i] = 0;
+    for (int r = (held + kWave - 1) / kWave; r < Table<N>::kRows; ++r) table.before[r] = ~0u;
     if (groups) launch(table, groups);
     held = 0, groups = 0;
   };
@@ -280,6 +281,7 @@ template <int N, typename F> void each_table(const hdcm_tensor* t, int64_t n, in
     uint64_t data = (uint64_t)(uintptr_t)t[i].data;
     for (int64_t left = t[i].count; left > 0; left -= kMaxCount, data += (uint64_t)kMaxCount << (f32 ? 2 : 1)) {
       const uint32_t count = (uint32_t)(left < kMaxCount ? left : kMaxCount);
+      if (held % kWave == 0) table.before[held / kWave] = groups;
       table.lo[held] = (uint32_t)data, table.hi[held] = (uint32_t)(data >> 32);
       table.size[held] = count | (f32 ? kIsF32 : 0);
       groups += (count + (1u << stretch_shift(bits, f32)) - 1) >> stretch_shift(bits, f32);
