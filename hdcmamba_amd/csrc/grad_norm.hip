@@ -212,8 +212,8 @@ template <typename T, bool STREAM> __device__ __forceinline__ void scale_of(cons
 // Where the norm comes from: given, or joined from its parts by every workgroup (the first writes it).
 enum From { kGiven, kParts2, kPartsMax };
 
-// Nothing is read or written where the factor is 1 (4.4 us for 5800 workgroups; 7.0 with the table's entry looked up first).  0.76 GB of fp32 285 us: 5.3 TB/s of reads and
-// writes (315 through the caches); 4.2 MB 4.3.
+// Nothing is read or written where the factor is 1 (4.4 us for 5800 workgroups; 7.0 with the table's entry looked up
+// first).  0.76 GB of fp32 285 us: 5.3 TB/s of reads and writes (315 through the caches); 4.2 MB 4.3.
 template <int FROM, bool STREAM, int N>
 __global__ __launch_bounds__(kThreads) void scale_kernel(Table<N> t, int bits, float* norm, const double* parts, int n_parts,
                                                          float max_norm) {

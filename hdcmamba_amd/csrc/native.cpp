@@ -1123,6 +1123,7 @@ void clip_grads(const pybind11::list& list, double max_norm, const Tensor& norm_
   const c10::DeviceGuard guard(l.first().device());
   l.refer(true);
   same_device(norm_, l.first(), "total_norm");
+  no_gradient("clip_grads_", {&norm_});
   TORCH_CHECK(norm_.numel() == 1 && norm_.is_floating_point(), "total_norm must be one floating-point number, got ", norm_.scalar_type(),
               " ", norm_.sizes());
   TORCH_CHECK(l.apart(&norm_), "clip_grads_", kNotApart);

@@ -557,6 +557,8 @@ def test_norm_refusals(dev):
         hm.clip_grads_([x], 1.0, torch.ones(()))
     with pytest.raises(RuntimeError, match="total_norm"):
         hm.clip_grads_([x], 1.0, torch.ones((), dtype=torch.long, device=dev))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        hm.clip_grads_([x], 1.0, torch.full((), 2.0, device=dev, requires_grad=True))
     assert bool(x.eq(1).all())
     hm.clip_grads_([x[:20], x[20:]], 1.0, 2.0)
     assert bool(x.lt(1).all())
