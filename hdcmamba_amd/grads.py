@@ -45,9 +45,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     for the norm, and raises with the gradients as they were where it is not finite."""
     parameters, kind, max_norm = _listed(parameters), _kind(norm_type), _limit(max_norm)
     if error_if_nonfinite:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("error_if_nonfinite waits for the norm, which a recording cannot")
         grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
+        if grads and grads[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("error_if_nonfinite waits for the norm, which a recording cannot")
         with torch.no_grad():
             norm = grad_norm(grads, norm_type).item()
         if not math.isfinite(norm):

@@ -155,6 +155,7 @@ def test_nothing_to_clip():
     assert hm.grad_norm([]).item() == 0.0
     assert hm.clip_grad_norm_([nn.Parameter(torch.zeros(3))], 1.0).item() == 0.0
     assert hm.clip_grads_([], 1.0, 2.0) is None
+    assert hm.clip_grad_norm_([nn.Parameter(torch.zeros(3))], 1.0, error_if_nonfinite=True).item() == 0.0
 
 
 def test_embedding_module_is_nn_embedding_on_the_cpu():
