@@ -15,7 +15,7 @@ import torch
 import torch.nn as nn
 
 from . import _ops
-from .embeddings import Embedding
+from .embeddings import Embedding, embedding
 from .model import BlockState, HdcMamba9v3Model, layer_norm
 from .quant4 import Linear4Bit
 from .sampling import append_tokens, fill_token_history, new_token_history, select_tokens
@@ -84,10 +84,11 @@ class HdcMambaLM(nn.Module):
         """One token per batch row: input_ids [B] -> logits [B,V]; states advance in place."""
         _ops._on_gpu(input_ids)
         with torch.no_grad():
-            # the embedding rows by indexing (PyTorch's gather kernel: ~2 us for 16 rows against
-            # ~7 us for nn.Embedding's index_select kernel, the same rows); norm_final and norm_f
-            # in one pass, then the tied head
-            x = self.embedding.weight[input_ids]
+            # the lookup of forward and prefill, so that an id means the same here (an nn.Embedding in the module's place
+            # has none for ids outside the vocabulary, which a sequence without an allowed token hands on); norm_final and
+            # norm_f in one pass, then the tied head
+            emb = self.embedding
+            x = emb(input_ids) if isinstance(emb, Embedding) else embedding(input_ids, emb.weight)
             return self.lm_head(self.backbone.step(x, states, pos_dev, then=self.norm_f))
 
     def capture_decode(self, states, controls=None):
@@ -236,7 +237,7 @@ class DecodeGraph:
     def next(self):
         """One token further from the tokens chosen last (at first those that ``ids`` was given): (tokens [B],
         log-probabilities [B]), static buffers that the next replay overwrites.  A sequence without an
-        allowed token has -1, which as the next input reads the embedding's last row."""
+        allowed token has -1, which as the next input is a row of zeros."""
         if self.controls is None:
             raise RuntimeError("next needs a DecodeGraph captured with controls")
         self._replay()
