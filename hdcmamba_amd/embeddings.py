@@ -87,11 +87,22 @@ class EmbeddingGradFunction(torch.autograd.Function):
         return None, EmbeddingFunction.apply(ids, grad, ctx.scale, None), None, None, None
 
 
+def _within(lookup, ids, weight):
+    """lookup(ids), with zeros for ids outside 0..V-1: PyTorch's own kernels read wherever such an id points (their
+    assertions are compiled out on ROCm)."""
+    V = weight.shape[0]
+    if V == 0:
+        return weight.new_zeros(*ids.shape, weight.shape[1])
+    return lookup(ids.clamp(0, V - 1)).masked_fill(((ids < 0) | (ids >= V)).unsqueeze(-1), 0)
+
+
 class Embedding(nn.Embedding):
     """nn.Embedding on these kernels, its rows times ``scale``: the same constructor, parameters and initial values.
 
     What the kernels do not take goes through nn.Embedding's own forward: weights on the CPU or of other types, max_norm,
-    sparse and scale_grad_by_freq, forward-mode differentiation and torch.func's transforms (vmap)."""
+    sparse and scale_grad_by_freq, forward-mode differentiation and torch.func's transforms (vmap).  On a GPU an id outside
+    0..V-1 is a row of zeros without a gradient there too (max_norm, and the frequencies and rows of a sparse gradient, count
+    it as the nearest token); on the CPU nn.Embedding refuses it."""
 
     def __init__(self, *args, scale=1.0, **kwargs):
         super().__init__(*args, **kwargs)
@@ -102,7 +113,7 @@ class Embedding(nn.Embedding):
         if (not w.is_cuda or w.dtype not in _ops._DTYPES or self.max_norm is not None or self.sparse
                 or self.scale_grad_by_freq or forward_ad._current_level >= 0
                 or torch._C._functorch.maybe_current_level() is not None):
-            y = super().forward(ids)
+            y = _within(super().forward, ids, w) if w.is_cuda else super().forward(ids)
             return y if self.scale == 1.0 else y * self.scale
         return embedding(ids, w, self.scale, self.padding_idx)
 

@@ -58,3 +58,47 @@ def test_an_id_outside_the_vocabulary_is_a_row_of_zeros_everywhere(dev, dtype, p
         for _ in range(3):
             assert torch.equal(a.step(wild[:, 11]), b.step(tame[:, 11]))
             assert torch.equal(a.step(ids[:, 0]), b.step(ids[:, 0]))
+
+
+WILD = [4, -1, 2, 20, 4, 2 ** 40, 9, -(2 ** 63), 0, 19, 21, 4]
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=torch.float64), dict(dtype=torch.half), dict(max_norm=0.7), dict(sparse=True),
+                                dict(scale_grad_by_freq=True), dict(scale_grad_by_freq=True, padding_idx=4)])
+def test_ids_outside_past_the_kernels(dev, kw):
+    """Where Embedding goes through nn.Embedding's forward an id that is no token is a row of zeros without a gradient too.
+    The rows are sums of at most three small whole numbers: exact in every type."""
+    _say("ids outside, past the kernels", kw)
+    ids = torch.tensor(WILD)
+    there = (ids >= 0) & (ids < 20)
+    w = torch.randint(-8, 9, (20, 6), generator=gen(1)).to(kw.get("dtype", FP))
+    m = hm.Embedding(20, 6, _weight=w.to(dev), scale=2.0, **kw)
+    ref = nn.Embedding(20, 6, _weight=w.clone(), **kw)
+    near = ids.clamp(0, 19)
+    y = m(ids.view(3, 4).to(dev))
+    want = ref(near) * 2 * there[:, None]
+    tol = 1e-6 if "max_norm" in kw else 0
+    torch.testing.assert_close(y.cpu().view(12, 6), want.detach(), rtol=tol, atol=0)
+    torch.testing.assert_close(m.weight.detach().cpu(), ref.weight.detach(), rtol=tol, atol=0)
+    R = torch.randint(-3, 4, (12, 6), generator=gen(2)).to(w.dtype)
+    (y.view(12, 6) * R.to(dev)).sum().backward()
+    (want * R).sum().backward()
+    assert m.weight.grad.is_sparse == kw.get("sparse", False)
+    assert torch.equal(m.weight.grad.to_dense().cpu(), ref.weight.grad.to_dense())
+    assert not hm.Embedding(0, 6, device=dev, dtype=torch.float64)(ids.to(dev)).any()
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_ids_outside_under_transforms(dev, dtype):
+    """Tangents and gradients for each sequence of a batch that is padded with ids that are no token."""
+    ids = torch.tensor(WILD, device=dev).view(3, 4)
+    there = (ids >= 0) & (ids < 20)
+    m = hm.Embedding(20, 6, device=dev, dtype=dtype, scale=2.0)
+    w = m.weight.detach()
+    call = lambda w, i: torch.func.functional_call(m, {"weight": w}, (i,))  # noqa: E731
+    y, dy = torch.func.jvp(lambda w: call(w, ids), (w,), (torch.ones_like(w),))
+    assert torch.equal(y, m(ids)) and torch.equal(dy, 2 * there[..., None].expand_as(dy).to(dtype))
+    per = torch.func.vmap(torch.func.grad(lambda w, i: call(w, i).sum()), (None, 0))(w, ids)
+    for i, t, g in zip(ids, there, per):
+        count = torch.bincount(i[t], minlength=20)
+        assert torch.equal(g, 2 * count[:, None].expand(20, 6).to(dtype))
