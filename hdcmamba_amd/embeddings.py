@@ -96,13 +96,23 @@ def _within(lookup, ids, weight):
     return lookup(ids.clamp(0, V - 1)).masked_fill(((ids < 0) | (ids >= V)).unsqueeze(-1), 0)
 
 
+_PLAIN = (torch.Tensor, nn.Parameter)
+
+
+def _traced():
+    """Whether PyTorch's operations are looked at rather than only run (a compiler or a tracer, a mode with a __torch_dispatch__),
+    which the kernels' calls would pass by."""
+    return torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or torch.jit.is_tracing()
+
+
 class Embedding(nn.Embedding):
     """nn.Embedding on these kernels, its rows times ``scale``: the same constructor, parameters and initial values.
 
     What the kernels do not take goes through nn.Embedding's own forward: weights on the CPU or of other types, max_norm,
-    sparse and scale_grad_by_freq, forward-mode differentiation and torch.func's transforms (vmap).  On a GPU an id outside
-    0..V-1 is a row of zeros without a gradient there too (max_norm, and the frequencies and rows of a sparse gradient, count
-    it as the nearest token); on the CPU nn.Embedding refuses it."""
+    sparse and scale_grad_by_freq, forward-mode differentiation and torch.func's transforms (vmap), tracing and compiling,
+    dispatch modes, and tensors of a class of their own (sharded, quantized, fake).  On a GPU an id outside 0..V-1 is a row
+    of zeros without a gradient there too (max_norm, and the frequencies and rows of a sparse gradient, count it as the
+    nearest token); on the CPU nn.Embedding refuses it, and a tensor's class does what it does."""
 
     def __init__(self, *args, scale=1.0, **kwargs):
         super().__init__(*args, **kwargs)
@@ -110,7 +120,10 @@ class Embedding(nn.Embedding):
 
     def forward(self, ids):
         w = self.weight
-        if (not w.is_cuda or w.dtype not in _ops._DTYPES or self.max_norm is not None or self.sparse
+        if type(w) not in _PLAIN or type(ids) is not torch.Tensor:
+            y = super().forward(ids)
+            return y if self.scale == 1.0 else y * self.scale
+        if (not w.is_cuda or w.dtype not in _ops._DTYPES or self.max_norm is not None or self.sparse or _traced()
                 or self.scale_grad_by_freq or forward_ad._current_level >= 0
                 or torch._C._functorch.maybe_current_level() is not None):
             y = _within(super().forward, ids, w) if w.is_cuda else super().forward(ids)

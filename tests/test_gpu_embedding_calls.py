@@ -102,3 +102,23 @@ def test_ids_outside_under_transforms(dev, dtype):
     for i, t, g in zip(ids, there, per):
         count = torch.bincount(i[t], minlength=20)
         assert torch.equal(g, 2 * count[:, None].expand(20, 6).to(dtype))
+
+
+def test_traced_compiled_and_seen_by_a_mode(dev):
+    """What follows the lookup's operations finds PyTorch's: no constant in a trace, one graph, an operation that a mode sees."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    m = hm.Embedding(20, 6, device=dev, scale=2.0)
+    ids, other = (torch.randint(0, 20, (2, 9), generator=gen(s)).to(dev) for s in (1, 2))
+    with torch.no_grad():
+        traced = torch.jit.trace(m, (ids,))
+        assert torch.equal(traced(other), m(other))
+    compiled = torch.compile(m, backend="eager", fullgraph=True)
+    for i in (ids, other):
+        y = compiled(i)
+        assert torch.equal(y, m(i))
+        y.sum().backward()
+        assert torch.equal(m.weight.grad, 2.0 * torch.bincount(i.flatten(), minlength=20)[:, None].expand(20, 6))
+        m.weight.grad = None
+    with FlopCounterMode(display=False):
+        assert torch.equal(m(other), traced(other))
