@@ -35,10 +35,13 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, out=N
     are added to it, and rows without an id are not touched."""
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, num_embeddings)
-    needed = torch.is_grad_enabled() and (grad.requires_grad or (out is not None and out.requires_grad))
-    if needed or carries_tangent(grad):
+    if accumulate and out is None:
+        raise RuntimeError("embedding_grad: accumulate needs out")
+    given = () if out is None else (out,)
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in (grad, *given))) or any(carries_tangent(t) for t in (grad, *given)):
         if out is not None:
-            raise RuntimeError("embedding_grad with out has no gradient: call it under torch.no_grad() or on detached tensors")
+            raise RuntimeError("embedding_grad with out has no gradient and no tangent: call it under torch.no_grad() or on detached "
+                               "tensors")
         return EmbeddingGradFunction.apply(ids, grad, int(num_embeddings), float(scale), padding_idx)
     return _ops.native().embedding_grad(ids, grad, num_embeddings, scale, padding_idx, out, accumulate)
 

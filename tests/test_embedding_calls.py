@@ -3,6 +3,7 @@ import pytest
 import torch
 import torch.nn as nn
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import hdcmamba_amd as hm
@@ -72,3 +73,19 @@ def test_traced_and_compiled_on_the_cpu():
     assert torch.equal(traced(other), m(other))
     compiled = torch.compile(m, backend="eager", fullgraph=True)
     assert torch.equal(compiled(other), m(other))
+
+
+def test_gradient_refusals_before_the_kernels():
+    ids, dy = torch.zeros(3, dtype=torch.long), torch.zeros(3, 4)
+    for g in (dy, dy.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="accumulate needs out"):
+            hm.embedding_grad(ids, g, 8, accumulate=True)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(dy, torch.ones_like(dy))
+        with pytest.raises(RuntimeError, match="accumulate needs out"):
+            hm.embedding_grad(ids, dual, 8, accumulate=True)
+        out = forward_ad.make_dual(torch.zeros(8, 4), torch.ones(8, 4))
+        for accumulate in (False, True):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no tangent"):
+                hm.embedding_grad(ids, dy, 8, out=out, accumulate=accumulate)
+        assert out.eq(0).all()
