@@ -22,9 +22,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     (counted from the end where negative) are looked up as others are but give no gradient."""
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
-    if (torch.is_grad_enabled() and weight.requires_grad) or carries_tangent(weight):
-        return EmbeddingFunction.apply(ids, weight, float(scale), padding_idx)
-    return _ops.native().embedding(ids, weight, scale)
+    return _ops.native().embedding(ids, weight, scale, padding_idx)
 
 
 def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, out=None, accumulate=False):
@@ -37,12 +35,9 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, out=N
         padding_idx = _padding(padding_idx, num_embeddings)
     if accumulate and out is None:
         raise RuntimeError("embedding_grad: accumulate needs out")
-    given = () if out is None else (out,)
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in (grad, *given))) or any(carries_tangent(t) for t in (grad, *given)):
-        if out is not None:
-            raise RuntimeError("embedding_grad with out has no gradient and no tangent: call it under torch.no_grad() or on detached "
-                               "tensors")
-        return EmbeddingGradFunction.apply(ids, grad, int(num_embeddings), float(scale), padding_idx)
+    if out is not None and ((torch.is_grad_enabled() and (grad.requires_grad or out.requires_grad))
+                            or carries_tangent(grad) or carries_tangent(out)):
+        raise RuntimeError("embedding_grad with out has no gradient and no tangent: call it under torch.no_grad() or on detached tensors")
     return _ops.native().embedding_grad(ids, grad, num_embeddings, scale, padding_idx, out, accumulate)
 
 
@@ -50,44 +45,6 @@ def _padding(index, rows):
     if not -rows <= index < rows:
         raise ValueError(f"padding_idx {index} is not one of {rows} tokens")
     return index % rows
-
-
-class EmbeddingFunction(torch.autograd.Function):
-    """``apply(ids, weight, scale, padding_idx)``: the lookup, whose backward is EmbeddingGradFunction."""
-
-    @staticmethod
-    def forward(ids, weight, scale, padding_idx):
-        return _ops.native().embedding(ids, weight, scale)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        ids, weight, ctx.scale, ctx.padding_idx = inputs
-        ctx.rows = weight.shape[0]
-        ctx.save_for_backward(ids)
-
-    @staticmethod
-    def backward(ctx, grad):
-        return None, EmbeddingGradFunction.apply(*ctx.saved_tensors, grad, ctx.rows, ctx.scale, ctx.padding_idx), None, None
-
-
-class EmbeddingGradFunction(torch.autograd.Function):
-    """``apply(ids, grad, rows, scale, padding_idx)``: the weight's gradient, itself linear in grad."""
-
-    @staticmethod
-    def forward(ids, grad, rows, scale, padding_idx):
-        return _ops.native().embedding_grad(ids, grad, rows, scale, padding_idx, None, False)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        ids, _, _, ctx.scale, ctx.padding_idx = inputs
-        ctx.save_for_backward(ids)
-
-    @staticmethod
-    def backward(ctx, grad):
-        (ids,) = ctx.saved_tensors
-        if ctx.padding_idx is not None:
-            ids = ids.masked_fill(ids == ctx.padding_idx, -1)
-        return None, EmbeddingFunction.apply(ids, grad, ctx.scale, None), None, None, None
 
 
 def _within(lookup, ids, weight):

@@ -122,3 +122,62 @@ def test_traced_compiled_and_seen_by_a_mode(dev):
         m.weight.grad = None
     with FlopCounterMode(display=False):
         assert torch.equal(m(other), traced(other))
+
+
+# ------------------------------------------------------------------ gradients of every kind
+def _sums(ids, dy, V, scale, padding=None):
+    """The gradient in 64 bits: whole numbers, exact in every type."""
+    i = ids.flatten()
+    ok = (i >= 0) & (i < V)
+    if padding is not None:
+        ok &= i != padding
+    return scale * torch.zeros(V, dy.shape[-1], dtype=torch.float64).index_add_(0, i[ok], dy.double().reshape(-1, dy.shape[-1])[ok])
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("padding_idx", [None, 4])
+def test_batched_gradients_and_transforms(dev, dtype, padding_idx):
+    """vmap over a backward's gradients, and both operators under torch.func: ids that are no token among the others."""
+    V, D = 20, 6
+    ids = torch.tensor(WILD).view(3, 4)
+    on = ids.to(dev)
+    w = torch.randint(-8, 9, (V, D), generator=gen(1)).to(dtype).to(dev)
+    Rs = torch.randint(-3, 4, (5, 3, 4, D), generator=gen(2)).to(dtype)
+    want = torch.stack([_sums(ids, R, V, 2.0, padding_idx) for R in Rs])
+    m = hm.Embedding(V, D, padding_idx=padding_idx, _weight=w.clone(), scale=2.0)
+    for y, leaf in ((m(on), m.weight), (hm.embedding(on, w.requires_grad_(), 2.0, padding_idx), w)):
+        (got,) = torch.autograd.grad(y, leaf, Rs.to(dev), is_grads_batched=True)
+        assert torch.equal(got.double().cpu(), want)
+    w = w.detach()
+    call = lambda w, i=on: hm.embedding(i, w, 2.0, padding_idx)  # noqa: E731
+    y, pull = torch.func.vjp(call, w)
+    assert torch.equal(y, call(w))
+    assert torch.equal(torch.func.vmap(lambda R: pull(R)[0])(Rs.to(dev)).double().cpu(), want)
+    y, dy = torch.func.jvp(call, (w,), (w + 1,))
+    rows = call(w + 1)
+    if padding_idx is not None:  # its rows are constants for the derivative
+        rows = rows.masked_fill((on == padding_idx)[..., None], 0)
+    assert torch.equal(y, call(w)) and torch.equal(dy, rows)
+    assert torch.equal(torch.func.vmap(call, (None, 0))(w, on), call(w))
+    grads = lambda R: hm.embedding_grad(on, R, V, 2.0, padding_idx)  # noqa: E731
+    assert torch.equal(torch.func.vmap(grads)(Rs.to(dev)).double().cpu(), want)
+    back = torch.func.grad(lambda R: (grads(R) * w).sum())(Rs[0].to(dev))
+    ref = 2 * w.cpu()[ids.clamp(0, V - 1)].masked_fill(((ids < 0) | (ids >= V) | (ids == padding_idx))[..., None], 0)
+    assert torch.equal(back.cpu(), ref)
+    with pytest.raises(RuntimeError, match="transforms"):
+        torch.func.vmap(lambda R: hm.embedding_grad(on, R, V, out=w))(Rs.to(dev))
+
+
+def test_gradients_are_formed_without_python(dev):
+    """Neither direction runs Python, which the host of a step of few tokens would wait for."""
+    w = torch.zeros(9, 4, device=dev, requires_grad=True)
+    y = hm.embedding(torch.zeros(3, dtype=torch.long, device=dev), w)
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y, requires_grad=True), create_graph=True)
+    for t in (y, dw):
+        assert t.grad_fn is not None and not isinstance(t.grad_fn, torch.autograd.function.BackwardCFunction)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.ones(3, 4, device=dev), torch.ones(3, 4, device=dev))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            hm.embedding_grad(torch.zeros(3, dtype=torch.long, device=dev), dual, 9)
+    with torch.inference_mode():
+        assert not hm.embedding(torch.zeros(3, dtype=torch.long, device=dev), w).any()
