@@ -741,6 +741,9 @@ Plan plan_of(int64_t n, int64_t V, int64_t D, int dtype) {
 }
 
 constexpr int64_t kMaxVocab = (int64_t)1 << 30, kMaxPositions = (int64_t)1 << 30, kMaxWidth = (int64_t)1 << 24;
+// A launch has fewer than 2^32 threads.
+bool fits(int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; }
+int64_t pieces_of(int64_t rows, int64_t D, int dtype) { return rows * ((D * hdcm_elt_size(dtype) + 15) / 16); }
 
 template <typename TG, typename TO>
 void launch_few(const Plan& p, const Ids& ids, int n, const GradRows& g, void* out, int64_t out_rs, int64_t D, float scale, bool add,
@@ -780,6 +783,7 @@ extern "C" int hdcm_embedding_fwd(const void* ids, int id_bytes, const void* w, 
   HDCM_CHECK_ARG(ids && out && (w || V == 0), HDCM_EINVAL);
   HDCM_CHECK_ARG((w_row_stride >= D || V <= 1) && (out_row_stride >= D || rows <= 1), HDCM_EINVAL);
   HDCM_CHECK_ARG(V <= kMaxVocab && D <= kMaxWidth && rows <= kMaxPositions, HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(fits(pieces_of(rows, D, dtype) / (2 * kLookThreads) + 1, kLookThreads), HDCM_EUNSUPPORTED);
   hipStream_t s = (hipStream_t)stream;
   const auto go = [&](auto launch) { launch(ids, w, w_row_stride, out, out_row_stride, rows, V, D, scale, s); };
   if (dtype == HDCM_F32) id_bytes == 8 ? go(launch_lookup<float, int64_t>) : go(launch_lookup<float, int32_t>);
@@ -811,6 +815,12 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   Plan p{};
   const bool few = !none && few_of(B * L, accumulate ? 0 : V * D * hdcm_elt_size(dw_dtype));
   if (!none) p = plan_of(B * L, V, D, dtype);
+  const bool apart = dw_row_stride != D && V > 1;  // rows of dw are not adjacent
+  const int64_t zeros = accumulate || apart ? 0 : V * D * hdcm_elt_size(dw_dtype);
+  HDCM_CHECK_ARG(none || (few ? fits((int64_t)p.few_groups * p.slices, kSumThreads)
+                              : fits(p.sum_groups * p.slices, kSumThreads) && fits(p.groups + zeros / kFillBytes + 1, kSortThreads)),
+                 HDCM_EUNSUPPORTED);
+  HDCM_CHECK_ARG(few || accumulate || !(none || apart) || fits(pieces_of(V, D, dw_dtype) / 256 + 1, 256), HDCM_EUNSUPPORTED);
   if (!none && !few) {
     HDCM_CHECK_ARG(ws && ws_bytes >= p.bytes(), HDCM_EWORKSPACE);
     HDCM_CHECK_ARG(hdcm_aligned16(ws), HDCM_EALIGN);
@@ -834,9 +844,7 @@ extern "C" int hdcm_embedding_grad(const void* ids, int id_bytes, const void* dy
   int* counts = (int*)at;
   float* part = (float*)(at + p.counts);
   // the zeros go with the sorting launches: with all scatters alike
-  const bool apart = dw_row_stride != D && V > 1;
   if (!accumulate && apart) launch_zeros(dw, dw_row_stride, V, D, dw_dtype, s);
-  const int64_t zeros = accumulate || apart ? 0 : V * D * hdcm_elt_size(dw_dtype);
   const auto fill_of = [&](int k, int n) {
     const auto upto = [&](int i) { return i == n ? zeros : zeros / n * i / 16 * 16; };
     return Fill{(char*)dw, upto(k), upto(k + 1)};

@@ -631,7 +631,8 @@ int hdcm_token_history_append(int16_t* table, int64_t table_row_stride, const in
 /*
  * Token rows of an embedding (csrc/embedding.hip; nn.Embedding and its autograd, train_fineweb.py:49,87).
  * ids: `rows` (fwd) or B * L (grad) token ids of id_bytes 4 or 8, contiguous.  V <= 2^30 rows of D <= 2^24 columns, at
- * most 2^30 ids.  Rows need only their type's alignment.
+ * most 2^30 ids, and sizes whose launches stay below 2^32 threads: at most 128 GiB looked up, 64 GiB of a dw whose rows
+ * are not adjacent (HDCM_EUNSUPPORTED above).  Rows need only their type's alignment.
  * hdcm_embedding_fwd: out[t] = scale * w[ids[t]], rounded once; zeros where ids[t] is not in 0..V-1.
  * hdcm_embedding_grad: dw[v] = scale * sum of dy[b, l] over ids[b, l] = v, for all V rows (with accumulate: added to
  * dw, whose other rows are not touched).  dy [B, L, D] of `dtype` with any batch stride and a row stride of at

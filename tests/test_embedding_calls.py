@@ -1,4 +1,6 @@
 """Calls of Embedding and its gradient that end before any kernel runs: tensors of other classes, modes, refusals."""
+import ctypes
+
 import pytest
 import torch
 import torch.nn as nn
@@ -7,6 +9,7 @@ from torch.autograd import forward_ad
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import hdcmamba_amd as hm
+from hdcmamba_amd import _ops
 
 
 class Held(torch.Tensor):
@@ -89,3 +92,23 @@ def test_gradient_refusals_before_the_kernels():
             with torch.no_grad(), pytest.raises(RuntimeError, match="no tangent"):
                 hm.embedding_grad(ids, dy, 8, out=out, accumulate=accumulate)
         assert out.eq(0).all()
+
+
+P16 = ctypes.c_void_p(16 * 1024)  # never dereferenced: every call is refused
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    lib, U = _ops.lib(), -3  # HDCM_EUNSUPPORTED
+    # ids, id_bytes, w, w_rs, out, out_rs, rows, V, D, scale, dtype, stream
+    f = lambda rows, D, dtype: lib.hdcm_embedding_fwd(P16, 4, P16, D, P16, D, rows, 100, D, 1.0, dtype, None)  # noqa: E731
+    assert f(1 << 30, 64, _ops.HDCM_BF16) == U  # 2^33 pieces, two a thread
+    assert f((1 << 30) - 3, 33, _ops.HDCM_F32) == U
+    # ids, id_bytes, dy, dy_bs, dy_rs, dw, dw_rs, dw_dtype, ws, ws_bytes, B, L, V, D, scale, padding, accumulate, dtype, stream
+    def g(L, V, D, rs, accumulate=0, dtype=_ops.HDCM_BF16):
+        return lib.hdcm_embedding_grad(P16, 4, P16, 0, 0, P16, rs, dtype, P16, 1 << 62, 1, L, V, D, 1.0, -1, accumulate, dtype, None)
+
+    assert g(1 << 30, 100, 513, 513) == U            # sums: 2^23 workgroups of 512 threads
+    assert g(0, 1 << 28, 128, 200) == U              # zeros of rows apart
+    assert g(9000, 1 << 28, 128, 200) == U
+    assert g(9000, 1 << 28, 520, 520) == U           # zeros beside the sorting: more than 2^38 bytes
+    assert g(9000, 1 << 28, 520, 520, dtype=_ops.HDCM_F32) == U
