@@ -285,7 +285,7 @@ template <int N, typename F> void each_table(const hdcm_tensor* t, int64_t n, in
       table.lo[held] = (uint32_t)data, table.hi[held] = (uint32_t)(data >> 32);
       table.size[held] = count | (f32 ? kIsF32 : 0);
       groups += (count + (1u << stretch_shift(bits, f32)) - 1) >> stretch_shift(bits, f32);
-      if (++held == N || groups >= 1u << 24) flush();
+      if (++held == N || groups >= 1u << 23) flush();  // (a launch has fewer than 2^32 threads)
     }
   }
   flush();

@@ -181,3 +181,10 @@ def test_gradients_are_formed_without_python(dev):
             hm.embedding_grad(torch.zeros(3, dtype=torch.long, device=dev), dual, 9)
     with torch.inference_mode():
         assert not hm.embedding(torch.zeros(3, dtype=torch.long, device=dev), w).any()
+
+
+# ------------------------------------------------------------------ the largest lists
+def test_norm_of_more_than_2_to_the_24_stretches(dev):
+    """One tensor of 4 GiB 260 times over, more workgroups than a launch takes; 260 * 2^30 ones, whose sum is exact."""
+    t = torch.ones(2 ** 30, device=dev)
+    assert hm.grad_norm([t] * 260).item() == torch.tensor(260.0 * 2 ** 30, dtype=torch.float64).sqrt().to(FP).item()
