@@ -1,6 +1,12 @@
 """Calls around the token rows, the gradients' norm and clipping that the operators' own tests leave out: ids outside the
-vocabulary through the whole model, lookups that go past the kernels, gradients of every kind, and the largest lists."""
+vocabulary through the whole model, lookups that go past the kernels, gradients of every kind, and the largest lists.
+
+Tolerances.  A product or sum in fp32 is off by at most 2^-24 of its value, a sum of m terms in any order by m 2^-24 of the
+sum of their magnitudes, and a result rounded to its type by half a step, finfo.eps / 2 of its value.  Squares are
+added in 64 bits, so a norm is off by its own rounding.
+"""
 import copy
+import math
 
 import pytest
 import torch
@@ -10,6 +16,7 @@ import hdcmamba_amd as hm
 from cfgs import reinit_block_
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
 BF, FP = torch.bfloat16, torch.float32
 
 
@@ -19,6 +26,10 @@ def _say(*a):
 
 def gen(seed):
     return torch.Generator().manual_seed(seed)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
 
 
 def _lm(dev, dtype=BF, V=300):
@@ -188,3 +199,72 @@ def test_norm_of_more_than_2_to_the_24_stretches(dev):
     """One tensor of 4 GiB 260 times over, more workgroups than a launch takes; 260 * 2^30 ones, whose sum is exact."""
     t = torch.ones(2 ** 30, device=dev)
     assert hm.grad_norm([t] * 260).item() == torch.tensor(260.0 * 2 ** 30, dtype=torch.float64).sqrt().to(FP).item()
+
+
+@pytest.mark.parametrize("dtypes", [(FP,), (BF,), (BF, FP, FP)], ids=["fp32", "bf16", "mixed"])
+@pytest.mark.parametrize("MiB", [70, 150])
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+def test_clip_of_large_lists(dev, kind, MiB, dtypes):
+    """More than 1024 stretches, whose norm is joined by a launch of its own; 400 tensors, more than one table; above 128 MiB past
+    the caches.  Bit for bit what the formula gives in fp32 operations."""
+    _say("clip of large lists", kind, MiB, dtypes)
+    g = torch.Generator(device=dev).manual_seed(MiB)
+    count = (MiB << 20) // sum(4 if dtypes[i % len(dtypes)] == FP else 2 for i in range(400))
+    ts = [torch.empty(count + i % 7, device=dev).normal_(generator=g).to(dtypes[i % len(dtypes)]) for i in range(400)]
+    ts[399][-1] = 9.0  # the largest, a tensor's last
+    if kind == 2.0:
+        ref = torch.stack([t.double().square().sum() for t in ts]).sum().sqrt()
+    else:
+        ref = torch.stack([t.abs().max().double() for t in ts]).max()
+    for share in (0.3, 1.5):
+        params = [nn.Parameter(torch.empty_like(t)) for t in ts]
+        for p, t in zip(params, ts):
+            p.grad = t.clone()
+        limit = float(ref) * share
+        norm = hm.clip_grad_norm_(params, limit, kind)
+        assert abs(norm.double() - ref) <= (U + 1e-9) * ref
+        assert torch.equal(norm, hm.grad_norm(ts, kind))
+        factor = (torch.tensor(limit, dtype=FP) / (norm.cpu() + 1e-6)).clamp(max=1.0).to(dev)
+        assert all(torch.equal(p.grad, (t.float() * factor).to(t.dtype)) for p, t in zip(params, ts))
+        on = [t.clone() for t in ts]
+        hm.clip_grads_(on, limit, norm)
+        assert all(torch.equal(a, p.grad) for a, p in zip(on, params))
+
+
+def _ids(T, V, seed, dev):
+    """Token ids as text has them, a sixth of them one token, and some that are none."""
+    u = torch.rand(T, generator=gen(seed), dtype=torch.float64)
+    ids = (torch.exp(u * math.log(V + 1)).long() - 1).clamp(0, V - 1)
+    ids[::6], ids[5::97] = V // 3, -1
+    return ids.to(dev)
+
+
+@pytest.mark.parametrize("dtype,T,D", [(FP, 110000, 1030), (FP, 50000, 700), (BF, 180000, 1030), (BF, 90000, 1030)])
+def test_gradient_past_the_caches(dev, dtype, T, D):
+    """Units of 16 and of 32 positions whose rows go past the caches, in both types."""
+    _say("gradient past the caches", dtype, T, D)
+    V = 3000
+    ids = _ids(T, V, T, dev)
+    dy = torch.empty(T, D, device=dev, dtype=dtype).normal_(generator=torch.Generator(device=dev).manual_seed(1))
+    got = hm.embedding_grad(ids, dy, V, scale=0.7)
+    there = ids >= 0
+    s = torch.tensor(0.7, dtype=FP).double().item()
+    ref, mag = torch.zeros(V, D, device=dev, dtype=torch.float64), torch.zeros(V, D, device=dev, dtype=torch.float64)
+    ref.index_add_(0, ids[there], dy[there].double()).mul_(s)
+    mag.index_add_(0, ids[there], dy[there].double().abs()).mul_(s)
+    terms = torch.bincount(ids[there], minlength=V).double()[:, None]
+    before = (terms + 1) * U * mag
+    assert bool(((got.double() - ref).abs() <= before + half_step(dtype) * (ref.abs() + before) + 1e-40).all())
+    assert torch.equal(got, hm.embedding_grad(ids.int(), dy, V, scale=0.7))
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("idt", [torch.int64, torch.int32])
+def test_lookup_past_the_caches(dev, dtype, idt):
+    """Outputs of more than 128 MiB, scaled and not, ids that are no token among them."""
+    T, D, V = 70000, 1030, 3000
+    ids = _ids(T, V, 1, dev).to(idt)
+    w = torch.empty(V, D, device=dev, dtype=dtype).normal_(generator=torch.Generator(device=dev).manual_seed(2))
+    rows = w[ids.clamp(min=0).long()].masked_fill((ids < 0)[:, None], 0)
+    assert torch.equal(hm.embedding(ids, w), rows)
+    assert torch.equal(hm.embedding(ids, w, scale=2.7), (rows.float() * 2.7).to(dtype))
