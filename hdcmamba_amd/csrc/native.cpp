@@ -1036,9 +1036,9 @@ Tensor lookup_by_ops(const Tensor& ids, const Tensor& weight, double scale, std:
     return at::zeros(shape, weight.options());
   }
   const Tensor no_token = at::logical_or(ids.lt(0), ids.ge(V)).unsqueeze(-1);
-  const Tensor at = ids.clamp(0, V - 1);
-  Tensor y = at::embedding(weight, at).masked_fill(no_token, 0);
-  if (padding) y = at::where(ids.eq(*padding).unsqueeze(-1), at::embedding(weight.detach(), at), y);  // constants, forward too
+  const Tensor near = ids.clamp(0, V - 1);
+  Tensor y = at::embedding(weight, near).masked_fill(no_token, 0);
+  if (padding) y = at::where(ids.eq(*padding).unsqueeze(-1), at::embedding(weight.detach(), near), y);  // constants, forward too
   return scale == 1.0 ? y : y * scale;
 }
 Tensor lookup_grad_by_ops(const Tensor& ids, const Tensor& grad, int64_t V, double scale, std::optional<int64_t> padding) {
@@ -1070,7 +1070,7 @@ template <typename F> Tensor in_backward(F f) {
 
 Tensor token_rows(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding);
 Tensor token_rows_grad(const Tensor& ids, const Tensor& grad, int64_t V, double scale, std::optional<int64_t> padding,
-                        const OptTensor& out, bool accumulate);
+                       const OptTensor& out, bool accumulate);
 
 struct Lookup : torch::autograd::Function<Lookup> {
   static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding) {
@@ -1085,7 +1085,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
     const Tensor ids = ctx->get_saved_variables()[0];
     return {Tensor(), in_backward([&] {
               return token_rows_grad(ids, grads[0], d["tokens"].toInt(), d["scale"].toDouble(), d["padding"].toOptional<int64_t>(), {},
-                                    false);
+                                     false);
             }),
             Tensor(), Tensor()};
   }
@@ -1120,7 +1120,7 @@ Tensor token_rows(const Tensor& ids, const Tensor& weight, double scale, std::op
 }
 
 Tensor token_rows_grad(const Tensor& ids, const Tensor& grad, int64_t V, double scale, std::optional<int64_t> padding,
-                        const OptTensor& out, bool accumulate) {
+                       const OptTensor& out, bool accumulate) {
   on_gpu(grad);
   on_gpu(ids);
   same_device(ids, grad, "ids");

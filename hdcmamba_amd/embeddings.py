@@ -17,7 +17,7 @@ __all__ = ["embedding", "embedding_grad", "Embedding"]
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
-    """scale * weight[ids], rounded once: ids of any shape (int64 or int32), weight [V, D] (float32 or bfloat16) ->
+    """scale * weight[ids] in fp32, rounded to weight's type: ids of any shape (int64 or int32), weight [V, D] (float32 or bfloat16) ->
     [*ids.shape, D] of weight's type, differentiable in weight (and again in the gradient).  The rows of ``padding_idx``
     (counted from the end where negative) are looked up as others are but give no gradient."""
     if padding_idx is not None:
@@ -27,7 +27,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
 
 def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, out=None, accumulate=False):
     """The gradient of ``embedding`` for its weight: row v is scale * the sum of grad's rows [*ids.shape, D] at the ids v,
-    in fp32 in an order that the ids alone fix, rounded once to grad's type -> [num_embeddings, D].
+    summed and scaled in fp32, rounded to grad's type -> [num_embeddings, D].  The ids and the call's sizes and types fix the
+    order of every sum: the same call gives the same bits.
 
     ``out`` ([num_embeddings, D], float32 or bfloat16, contiguous rows) is written instead; with ``accumulate`` the sums
     are added to it, and rows without an id are not touched."""

@@ -31,6 +31,9 @@ SIZES = {
 
 
 class HdcMambaLM(nn.Module):
+    """Token ids are not checked against the vocabulary (they are on the GPU, and nothing waits for it): one outside of it is a row
+    of zeros, without a gradient, in forward, prefill and step alike."""
+
     def __init__(self, d_model, n_layers, d_state, num_heads, vocab_size=50277, chunk_size=256,
                  num_slots=32):
         super().__init__()

@@ -633,12 +633,12 @@ int hdcm_token_history_append(int16_t* table, int64_t table_row_stride, const in
  * ids: `rows` (fwd) or B * L (grad) token ids of id_bytes 4 or 8, contiguous.  V <= 2^30 rows of D <= 2^24 columns, at
  * most 2^30 ids, and sizes whose launches stay below 2^32 threads: at most 128 GiB looked up, 64 GiB of a dw whose rows
  * are not adjacent (HDCM_EUNSUPPORTED above).  Rows need only their type's alignment.
- * hdcm_embedding_fwd: out[t] = scale * w[ids[t]], rounded once; zeros where ids[t] is not in 0..V-1.
+ * hdcm_embedding_fwd: out[t] = scale * w[ids[t]], the product in fp32, then rounded to dtype; zeros where ids[t] is not in 0..V-1.
  * hdcm_embedding_grad: dw[v] = scale * sum of dy[b, l] over ids[b, l] = v, for all V rows (with accumulate: added to
  * dw, whose other rows are not touched).  dy [B, L, D] of `dtype` with any batch stride and a row stride of at
  * least D, or 0 (one row for all positions); dw of dw_dtype.  Ids outside 0..V-1 and padding_idx (-1: none)
- * are passed over.  fp32 sums in an order that the ids alone fix, one rounding (so the same call gives the
- * same bits).  ws: hdcm_embedding_grad_workspace_bytes(B, L, V, D, dtype) bytes, 16-byte aligned, not kept between
+ * are passed over.  fp32 sums, times scale, then rounded to dw_dtype, in an order that the ids and the call's sizes,
+ * types and accumulate fix (so the same call gives the same bits).  ws: hdcm_embedding_grad_workspace_bytes(B, L, V, D, dtype) bytes, 16-byte aligned, not kept between
  * calls.
  */
 int hdcm_embedding_fwd(const void* ids, int id_bytes, const void* w, int64_t w_row_stride, void* out,
