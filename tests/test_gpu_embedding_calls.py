@@ -268,3 +268,60 @@ def test_lookup_past_the_caches(dev, dtype, idt):
     rows = w[ids.clamp(min=0).long()].masked_fill((ids < 0)[:, None], 0)
     assert torch.equal(hm.embedding(ids, w), rows)
     assert torch.equal(hm.embedding(ids, w, scale=2.7), (rows.float() * 2.7).to(dtype))
+
+
+# ------------------------------------------------------------------ what a trainer wraps a lookup in
+def test_gradient_in_a_trainers_wrappers(dev):
+    """Checkpointing, saved tensors on the host, anomaly detection, an autocast region, vectorized Jacobians, threads, and an id
+    tensor that was written between forward and backward: the gradient is that of the plain call, or the call is refused."""
+    import threading
+
+    from torch.utils.checkpoint import checkpoint
+
+    V, D = 50, 24
+    ids = torch.randint(-1, V, (4, 33), generator=gen(3)).to(dev)[:, 1:]
+    R = torch.randint(-3, 4, (4, 32, D), generator=gen(4)).float().to(dev)
+    m = hm.Embedding(V, D, device=dev, padding_idx=7)
+    want = _sums(ids.cpu(), R.cpu(), V, 1.0, 7).float().to(dev)
+
+    def backward(call):
+        m.weight.grad = None
+        (call(ids) * R).sum().backward()
+        assert torch.equal(m.weight.grad, want)
+
+    backward(m)
+    for reentrant in (False, True):
+        backward(lambda i: checkpoint(lambda i, w: hm.embedding(i, w, padding_idx=7), i, m.weight, use_reentrant=reentrant))
+    with torch.autograd.graph.save_on_cpu():
+        backward(m)
+    with torch.autograd.set_detect_anomaly(True):
+        backward(m)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = m(ids)
+        assert y.dtype == FP
+        backward(m)
+    for vectorize in (False, True):
+        J = torch.autograd.functional.jacobian(lambda w: hm.embedding(ids[0, :3], w, 2.0).sum(1), m.weight.detach(), vectorize=vectorize)
+        ref = torch.zeros(3, V, D, device=dev)
+        for k, i in enumerate(ids[0, :3].tolist()):
+            if i >= 0:
+                ref[k, i] = 2
+        assert torch.equal(J, ref)
+    got = [None] * 4
+
+    def work(k):
+        w = m.weight.detach().clone().requires_grad_()
+        for _ in range(20):
+            (got[k],) = torch.autograd.grad(hm.embedding(ids, w, padding_idx=7), w, R)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    y = m(ids)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.sum().backward()
